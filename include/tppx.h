@@ -677,6 +677,63 @@ int tppx_attn_prefill(const void* q, const void* kcache, const void* vcache,
                       void* out, int64_t B, int64_t S, int64_t Nq, int64_t Nkv,
                       int64_t H, int64_t Smax, tppx_stream_t stream);
 
+/* ---- MXFP4 key/value cache, sequences of different lengths, packed prompts ----
+ * No counterpart in the reference, whose cache is bf16 / fp32 and whose batches share one length.  Head sizes H: 64, 96,
+ * 128, 192, 256 (others TPPX_EUNSUPPORTED).
+ * Packed tokens: rows of q, k, v, out; sequence b owns rows cu[b] .. cu[b + 1] - 1 (cu: device i32 [B + 1], ascending;
+ * NULL: one token per sequence, T == B); it held past[b] (device i32 [B]) keys before them.  Row strides *_ld in elements
+ * (multiples of 8), heads of a row contiguous.  Rows of T behind cu[B] are neither read nor written.  Values in cu and
+ * past that do not fit are clamped on the device.
+ * A cache layer: codes u8 [B][Nkv][Smax][H/2] (E2M1, channel 2i in the low half of byte i; 16-byte aligned) and scales u8
+ * [B][Nkv][Smax][H/32] (E8M0) of the keys and of the values.  A block of 32 channels has the scale byte
+ * floor(log2 max) + 125; nearest, ties to the even code, 6 at most.  A block whose maximum is below 2^-124 is zero (byte 0), one
+ * that holds an infinity or a NaN gets byte 255 and stands for NaN. */
+
+/* Per-head RMSNorm of q [T][Nq][H] and k [T][Nkv][H] (bf16; gamma_q / gamma_k f32 or bf16 [H], each may be NULL: no norm)
+ * followed by the rotation at pos (i64 [T]; positions outside the table are left unrotated): emb_pos f32 [2][MP][HR] cos / sin
+ * on pairs (i, HR/2 + i), or with gptj [MP][HR] sin | cos on adjacent pairs, or NULL.  fp32 inside, one rounding;
+ * q_out [T][Nq][H], k_out [T][Nkv][H] contiguous (may be q and k where those are). */
+int tppx_qk_norm_rotary(const void* q, const void* k, const void* gamma_q,
+                        const void* gamma_k, int gamma_dtype, float eps,
+                        const void* emb_pos, int gptj, const void* pos,
+                        void* q_out, void* k_out, int64_t T, int64_t Nq,
+                        int64_t Nkv, int64_t H, int64_t q_ld, int64_t k_ld,
+                        int64_t MP, int64_t HR, tppx_stream_t stream);
+
+/* The same for packed tokens, with the keys (rounded once, from fp64, to their codes) and the values written to the cache
+ * at slots past[b], past[b] + 1, ... of their sequence (those at Smax and beyond are dropped).  q may be NULL; pos NULL:
+ * the slot.  k_out / v_out [T][Nkv][H] bf16 or NULL: the values that the codes stand for. */
+int tppx_append_mx4(const void* q, const void* k, const void* v,
+                    const void* gamma_q, const void* gamma_k, int gamma_dtype,
+                    float eps, const void* emb_pos, int gptj, const void* pos,
+                    void* k_codes, void* k_scales, void* v_codes,
+                    void* v_scales, const void* past, const void* cu,
+                    void* q_out, void* k_out, void* v_out, int64_t T, int64_t B,
+                    int64_t Nq, int64_t Nkv, int64_t H, int64_t Smax,
+                    int64_t q_ld, int64_t k_ld, int64_t v_ld, int64_t MP,
+                    int64_t HR, tppx_stream_t stream);
+
+/* Attention over the cache, after the tokens' own keys went to it: token i of sequence b sees the keys 0 .. past[b] + i.
+ * softmax(q K^T / sqrt(H) + mask) V; mask bf16 [B][mask_ld] over key positions or NULL (0 past mask_ld); a key under -inf is not
+ * looked at; rows that see nothing are zeros.  Few tokens per sequence: keys split over workgroups where ws
+ * (256-byte aligned scratch, no state) holds the partial results and counters (u32 words 256 bytes apart, zero before the
+ * first launch, left zero) has one per 16 (token, query head) pairs of a K/V head; otherwise unsplit.  Launches that share
+ * either must be ordered. */
+int tppx_attn_mx4(const void* q, const void* k_codes, const void* k_scales,
+                  const void* v_codes, const void* v_scales, const void* past,
+                  const void* cu, const void* mask, int64_t mask_ld, void* out,
+                  int64_t T, int64_t B, int64_t Nq, int64_t Nkv, int64_t H,
+                  int64_t Smax, int64_t q_ld, void* ws, int64_t ws_bytes,
+                  void* counters, int64_t counter_bytes, tppx_stream_t stream);
+
+/* Causal attention of packed prompts over their own bf16 keys and values: token i of a sequence sees its tokens 0 .. i;
+ * mask [B][mask_ld] over these, as above. */
+int tppx_attn_packed(const void* q, const void* k, const void* v,
+                     const void* cu, const void* mask, int64_t mask_ld,
+                     void* out, int64_t T, int64_t B, int64_t Nq, int64_t Nkv,
+                     int64_t H, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                     tppx_stream_t stream);
+
 /* The element-type switch of fc_plain_wrap (src/csrc/llm/fused_llm_infer.cpp:
  * 1526-1545) for QINT8-family weights and float / half activations, or a
  * pre-quantized qint8 input whose compute type is float

@@ -1,0 +1,92 @@
+"""What the operators of the MXFP4 cache and of packed prompts refuse, before anything is launched, and their 64-bit plain
+forms against known values."""
+import math
+
+import pytest
+import torch
+
+import mx4_ref as R
+
+
+def _mods():
+    import tpp_pytorch_extension  # noqa: F401
+    from tpp_pytorch_extension import _lib
+    from tpp_pytorch_extension._C import _tpp_attn
+    return _lib, _lib.lib(), _tpp_attn
+
+
+A = 1 << 20  # a fake, aligned "device pointer": refused before it is touched
+
+
+def test_c_refusals():
+    _lib, L, _ = _mods()
+
+    def rotary(q=A, k=A, gq=A, gk=A, gdt=0, emb=A, pos=A, qo=A, ko=A, T=3, Nq=4, Nkv=2, H=128, q_ld=512, k_ld=256, MP=10, HR=128):
+        return L.tppx_qk_norm_rotary(q, k, gq, gk, gdt, 1e-6, emb, 0, pos, qo, ko, T, Nq, Nkv, H, q_ld, k_ld, MP, HR, None)
+
+    assert rotary(q=None) == rotary(k=None) == rotary(qo=None) == rotary(ko=None) == rotary(pos=None) == _lib.EINVAL
+    assert rotary(q=A + 8) == rotary(gk=A + 4) == rotary(emb=A + 4) == rotary(gdt=2) == _lib.EINVAL
+    assert rotary(H=80) == rotary(H=32) == rotary(H=512) == _lib.EUNSUPPORTED
+    assert rotary(HR=24) == rotary(HR=144) == rotary(MP=0) == rotary(q_ld=504) == rotary(k_ld=260) == rotary(T=-1) == rotary(Nkv=0) == _lib.ESHAPE
+    assert rotary(T=0) == _lib.OK
+
+    def append(q=A, k=A, v=A, kc=A, ks=A, vc=A, vs=A, past=A, cu=A, qo=A, ko=A, vo=A, T=3, B=2, Nkv=2, H=128, Smax=9, v_ld=256):
+        return L.tppx_append_mx4(q, k, v, None, None, 0, 1e-6, None, 0, None, kc, ks, vc, vs, past, cu, qo, ko, vo, T, B, 4, Nkv, H, Smax,
+                                 512, 256, v_ld, 0, 0, None)
+
+    for name in ("k", "v", "kc", "ks", "vc", "vs", "past", "qo"):
+        assert append(**{name: None}) == _lib.EINVAL
+    assert append(kc=A + 8) == append(vo=A + 2) == _lib.EINVAL
+    assert append(H=48) == _lib.EUNSUPPORTED
+    assert append(cu=None) == append(Smax=0) == append(B=0) == append(v_ld=128) == append(Nkv=-1) == _lib.ESHAPE
+    assert append(T=0) == append(T=0, q=None, qo=None) == _lib.OK
+
+    def attn(q=A, kc=A, vs=A, past=A, cu=A, mask=None, mask_ld=0, out=A, T=3, B=2, Nq=4, Nkv=2, H=128, Smax=9, q_ld=512, ws=None, wb=0, ct=None, cb=0):
+        return L.tppx_attn_mx4(q, kc, A, A, vs, past, cu, mask, mask_ld, out, T, B, Nq, Nkv, H, Smax, q_ld, ws, wb, ct, cb, None)
+
+    for name in ("q", "kc", "vs", "past", "out"):
+        assert attn(**{name: None}) == _lib.EINVAL
+    assert attn(q=A + 4) == attn(vs=A + 2) == attn(mask=A) == attn(wb=64) == attn(cb=64) == attn(ct=A + 1, cb=64) == _lib.EINVAL
+    assert attn(H=160) == _lib.EUNSUPPORTED
+    assert attn(Nq=5) == attn(Smax=1 << 30) == attn(cu=None) == attn(q_ld=500) == attn(B=0) == attn(T=-1) == _lib.ESHAPE
+    assert attn(T=0) == _lib.OK
+
+    def packed(q=A, k=A, v=A, cu=A, out=A, T=3, B=2, Nq=4, Nkv=2, H=128, k_ld=256, v_ld=256):
+        return L.tppx_attn_packed(q, k, v, cu, None, 0, out, T, B, Nq, Nkv, H, 512, k_ld, v_ld, None)
+
+    for name in ("q", "k", "v", "cu", "out"):
+        assert packed(**{name: None}) == _lib.EINVAL
+    assert packed(k=A + 8) == _lib.EINVAL and packed(H=100) == _lib.EUNSUPPORTED
+    assert packed(Nq=3) == packed(k_ld=250) == packed(v_ld=100) == packed(T=1 << 31) == _lib.ESHAPE
+    assert packed(T=0) == _lib.OK
+
+
+def test_python_refuses_tensors_off_the_gpu():
+    _lib, _, at = _mods()
+    q, k = torch.zeros((3, 4, 128), dtype=torch.bfloat16), torch.zeros((3, 2, 128), dtype=torch.bfloat16)
+    i = torch.zeros(3, dtype=torch.int32)
+    layer = at.Mx4Layer(*(torch.zeros((3, 2, 8, w), dtype=torch.uint8) for w in (64, 4, 64, 4)))
+    for call in (lambda: at.qk_norm_rotary(q, k), lambda: at.append_mx4(q, k, k, layer, i), lambda: at.attn_mx4(q, layer, i),
+                 lambda: at.attn_packed(q, k, k, i)):
+        with pytest.raises(_lib.TppxError) as e:
+            call()
+        assert e.value.code == _lib.EINVAL
+
+
+def test_plain_forms():
+    grid = torch.tensor([0.0, 0.25, 0.26, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.9, -0.25, -0.75, -3.49, 4.0, 6.0, -6.0] * 2)
+    codes, scales = R.encode(grid)
+    assert scales.tolist() == [127]
+    want = torch.tensor([0.0, 0.0, 0.5, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0, 0.0, -1.0, -3.0, 4.0, 6.0, -6.0] * 2).double()
+    assert torch.equal(R.decode(codes, scales), want)
+    _, s = R.encode(torch.tensor([[2.0 ** -125] * 32, [2.0 ** -124] * 32, [3.0e38] * 32, [math.inf] * 32]))
+    assert s[:, 0].tolist() == [0, 1, 252, 255]
+    # a rotation keeps the length of its pairs; equal keys give the mean of the values
+    x = R.randn((2, 1, 64), 1.0, 1)
+    for style, table in (("llama", R.llama_table(9, 32)), ("gptj", R.gptj_table(9, 32))):
+        y, _ = R.turn(x, None, 0.0, table, torch.tensor([3, 8]), style)
+        assert torch.allclose(y.norm(dim=-1), x.double().norm(dim=-1), rtol=1e-6)
+        assert torch.equal(y[..., 32:], x[..., 32:].double())
+    v = torch.randn((1, 5, 64), dtype=torch.float64)
+    out, _ = R.attend(x, torch.zeros((1, 5, 64), dtype=torch.float64), v, 3)
+    assert torch.allclose(out[:, 0], torch.stack((v[0, :4].mean(0), v[0].mean(0))))

@@ -1,0 +1,774 @@
+// Key/value cache in MXFP4 (E2M1 codes, one E8M0 scale per 32 channels of a head) for sequences of different lengths, and
+// attention of packed prompts: per-head norms with the rotation and the append, single and few tokens over the cache with
+// the keys split over workgroups, and causal attention of prompts over packed bf16 rows or over the cache.
+//
+// Cache of a layer: codes [B][Nkv][Smax][H/2] (channel 2i of a byte in its low half), scales [B][Nkv][Smax][H/32], for the
+// keys and for the values.  Tokens are packed: sequence b owns rows cu[b] .. cu[b + 1] - 1 of q, k, v and out, and held past[b]
+// keys before them; cu null: one token per sequence.  Both arrays live on the device and are clamped there, so that no value in
+// them leads out of a buffer.
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+
+#include "tppx_mx4.h"
+
+namespace tppx {
+
+// ---------------------------------------------------------------------------
+// Norm, rotation and append.  A workgroup works on one token; G lanes take a head's row, 8 channels each: the mean square is
+// a sum over the G lanes, the rotation's partner channels come from the lane that holds them, an MX block is four lanes.
+//   y = x * (1 / sqrt(mean(x^2) + eps)) * gamma;  y' = y cos -+ partner sin
+// A query is computed in fp32 and rounded once, to bf16.  A key that goes to the cache is computed in fp64: its code is a step
+// function of the value, and in fp32 one in some 10^6 falls on the other side of a border than the formula's (a few hundred
+// thousand fp64 operations on a card that does 10^13 a second).  Codes: scale 2^(floor(log2 max) - 2), nearest, ties to the
+// even code, 6 at most, as the MXFP4 weights; a block whose maximum is below 2^-124 is zero, one that holds an infinity or a NaN
+// has scale byte 255 and reads back as NaN.
+// ---------------------------------------------------------------------------
+struct Mx4RowsParams {
+  const uint16_t *q, *k, *v; // [T][heads][H], rows q_ld, k_ld, v_ld elements apart; q or v may be null
+  uint16_t *qo, *ko, *vo;    // [T][heads][H] contiguous; with the cache ko, vo may be null (the values that the codes stand for)
+  uint8_t *kq, *ks, *vq, *vs;
+  const void *gq, *gk;       // [H] f32 or bf16, or null
+  const float* emb;          // [2][MP][HR] cos / sin, or with gptj [MP][HR] sin | cos, or null
+  const int64_t* pos;        // [T], or null: the slot in the cache
+  const int32_t *past, *cu;
+  int64_t q_ld, k_ld, v_ld;
+  int T, B, Nq, Nkv, H, MP, HR, Smax;
+  int gptj, gamma_f32;
+  float eps;
+};
+
+__device__ __forceinline__ double shfl_xor_t(double v, int d) { return __shfl_xor(v, d); }
+__device__ __forceinline__ float shfl_xor_t(float v, int d) { return __shfl_xor(v, d); }
+
+// channels u * 8 .. + 7 of a head's row, normalised and rotated; w holds them, all G lanes of the row take part
+template <int G, typename A>
+__device__ __forceinline__ void mx4_turn(const Mx4RowsParams& p, const uint4& w, int u, const void* gamma, int64_t at, A (&y)[8]) {
+  float f[8];
+  unpack8(w, f);
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+    y[e] = f[e];
+  A r = 1;
+  auto scale_of = [&](int c, A (&g)[8]) { // gamma of chunk c
+    if (p.gamma_f32) {
+      const f32x4* s = reinterpret_cast<const f32x4*>(gamma) + c * 2;
+      const f32x4 a = s[0], b = s[1];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        g[e] = a[e];
+        g[4 + e] = b[e];
+      }
+    } else {
+      float h[8];
+      unpack8(reinterpret_cast<const uint4*>(gamma)[c], h);
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        g[e] = h[e];
+    }
+  };
+  const bool live = u * 8 < p.H;
+  if (gamma) {
+    A ss = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      ss += y[e] * y[e];
+#pragma unroll
+    for (int d = 1; d < G; d *= 2)
+      ss += shfl_xor_t(ss, d);
+    r = (A)1 / sqrt(ss / (A)p.H + (A)p.eps);
+    A g[8];
+    scale_of(live ? u : 0, g);
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      y[e] = y[e] * r * g[e];
+  }
+  const bool rotate = p.emb && at >= 0 && at < p.MP; // positions outside the table are left unrotated
+  if (p.gptj) {
+    if (rotate && u * 8 < p.HR) {
+      const float* sn = p.emb + at * p.HR + u * 4;
+      const float* cs = sn + (p.HR >> 1);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const A a = y[2 * e], b = y[2 * e + 1], c = cs[e], s = sn[e];
+        if constexpr (std::is_same_v<A, float>) {
+          y[2 * e] = rotate_first(a, b, c, s);
+          y[2 * e + 1] = rotate_second(a, b, c, s);
+        } else {
+          y[2 * e] = a * c - b * s;
+          y[2 * e + 1] = b * c + a * s;
+        }
+      }
+    }
+    return;
+  }
+  const int half = p.HR >> 4; // chunks of the first half
+  const int mate = u < half ? u + half : u < 2 * half ? u - half : u;
+  const int lane = threadIdx.x & 63, src = (lane & ~(G - 1)) + mate;
+  const uint4 m = make_uint4(__shfl(w.x, src), __shfl(w.y, src), __shfl(w.z, src), __shfl(w.w, src));
+  if (rotate && u < 2 * half) {
+    unpack8(m, f);
+    A o[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      o[e] = f[e];
+    if (gamma) {
+      A g[8];
+      scale_of(mate, g);
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        o[e] = o[e] * r * g[e];
+    }
+    const f32x4* cp = reinterpret_cast<const f32x4*>(p.emb + at * p.HR + u * 8);
+    const f32x4* sp = reinterpret_cast<const f32x4*>(p.emb + ((int64_t)p.MP + at) * p.HR + u * 8);
+    const f32x4 c4[2] = {cp[0], cp[1]}, s4[2] = {sp[0], sp[1]};
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const A c = c4[e >> 2][e & 3], s = s4[e >> 2][e & 3];
+      if constexpr (std::is_same_v<A, float>)
+        y[e] = u < half ? rotate_first(y[e], o[e], c, s) : rotate_second(o[e], y[e], c, s);
+      else
+        y[e] = u < half ? y[e] * c - o[e] * s : y[e] * c + o[e] * s;
+    }
+  }
+}
+
+// codes of a lane's 8 values (a dword) and the block's scale byte; a block is four adjacent lanes
+template <typename A>
+__device__ __forceinline__ uint32_t mx4_encode(const A (&y)[8], int& byte) {
+  constexpr int TOP = std::is_same_v<A, double> ? 0x7ff : 0xff, BIAS = std::is_same_v<A, double> ? 1023 : 127;
+  int top = 0; // biased exponent of the largest magnitude
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    if constexpr (std::is_same_v<A, double>)
+      top = max(top, (__double2hiint(y[e]) >> 20) & 0x7ff);
+    else
+      top = max(top, (int)((__float_as_uint(y[e]) >> 23) & 0xffu));
+  }
+  top = max(top, __builtin_amdgcn_update_dpp(0, top, 0xB1, 0xf, 0xf, true)); // quad_perm [1,0,3,2]
+  top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x4E, 0xf, 0xf, true)); // quad_perm [2,3,0,1]
+  byte = top == TOP ? 255 : min(max(top - BIAS + 125, 0), 254);
+  uint32_t codes = 0;
+  if (byte != 0 && byte != 255) {
+    A by;
+    if constexpr (std::is_same_v<A, double>)
+      by = __hiloint2double((1023 + 127 - byte) << 20, 0);
+    else
+      by = ldexpf(1.0f, 127 - byte);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const A a = fabs(y[e] * by);
+      uint32_t c = (a > (A)0.25) + (a >= (A)0.75) + (a > (A)1.25) + (a >= (A)1.75) + (a > (A)2.5) + (a >= (A)3.5) + (a > (A)5);
+      c |= c != 0 && y[e] < 0 ? 8u : 0u;
+      codes |= c << (4 * e);
+    }
+  }
+  return codes;
+}
+
+template <int G, bool CACHE>
+__global__ void __launch_bounds__(256)
+mx4_rows_kernel(const Mx4RowsParams p) {
+  const int tok = blockIdx.x;
+  int b = 0, slot = 0;
+  if (CACHE) {
+    int first = tok;
+    b = tok;
+    if (p.cu) {
+      b = sequence_of(p.cu, p.B, tok);
+      if (b >= p.B || tok < p.cu[0])
+        return; // rows behind the last sequence
+      first = p.cu[b];
+    }
+    slot = p.past[b] + (tok - first);
+  }
+  const int64_t at = p.pos ? p.pos[tok] : (int64_t)slot;
+  const bool room = slot >= 0 && slot < p.Smax;
+  const int nq = p.q ? p.Nq : 0, nk = p.Nkv, nv = p.v ? p.Nkv : 0;
+  int i = (int)blockIdx.y * (256 / G) + (int)threadIdx.x / G;
+  const int u = threadIdx.x % G;
+  if (i >= nq + nk + nv)
+    return; // (whole groups of G lanes)
+  const bool live = u * 8 < p.H;
+  const int kind = i < nq ? 0 : i < nq + nk ? 1 : 2;
+  i -= kind == 0 ? 0 : kind == 1 ? nq : nq + nk;
+  const uint16_t* src = kind == 0 ? p.q + (int64_t)tok * p.q_ld : kind == 1 ? p.k + (int64_t)tok * p.k_ld : p.v + (int64_t)tok * p.v_ld;
+  const uint4 w = live ? *reinterpret_cast<const uint4*>(src + (int64_t)i * p.H + u * 8) : make_uint4(0, 0, 0, 0);
+  if (kind == 0 || !CACHE) {
+    float y[8];
+    mx4_turn<G>(p, w, u, kind == 0 ? p.gq : p.gk, at, y);
+    if (live)
+      *reinterpret_cast<uint4*>((kind == 0 ? p.qo + ((int64_t)tok * p.Nq + i) * p.H : p.ko + ((int64_t)tok * p.Nkv + i) * p.H) + u * 8) = pack8(y);
+    return;
+  }
+  uint32_t codes;
+  int byte;
+  if (kind == 1) {
+    double y[8];
+    mx4_turn<G>(p, w, u, p.gk, at, y);
+    codes = mx4_encode(y, byte);
+  } else {
+    float y[8];
+    unpack8(w, y);
+    codes = mx4_encode(y, byte);
+  }
+  if (!live)
+    return;
+  const int64_t row = ((int64_t)b * p.Nkv + i) * p.Smax + slot;
+  if (room) {
+    *reinterpret_cast<uint32_t*>((kind == 1 ? p.kq : p.vq) + row * (p.H >> 1) + u * 4) = codes;
+    if ((u & 3) == 0)
+      (kind == 1 ? p.ks : p.vs)[row * (p.H >> 5) + (u >> 2)] = (uint8_t)byte;
+  }
+  uint16_t* held = kind == 1 ? p.ko : p.vo;
+  if (held) {
+    typedef __attribute__((ext_vector_type(2))) float f32x2;
+    const float s = e8m0_to_f32((uint32_t)byte);
+    const f32x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1);
+    const f32x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3);
+    const float y[8] = {v0[0] * s, v0[1] * s, v1[0] * s, v1[1] * s, v2[0] * s, v2[1] * s, v3[0] * s, v3[1] * s};
+    *reinterpret_cast<uint4*>(held + ((int64_t)tok * p.Nkv + i) * p.H + u * 8) = pack8(y);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens over the cache, keys split over workgroups.  The columns of a sequence's K/V head are its (token, query head)
+// pairs; a workgroup takes 16 of them, the columns of a 16 x 16 x 32 MFMA, so that a cached row is read once for all of them
+// and with one token per sequence and up to 16 heads per K/V head once in all.  Both products run transposed:
+//   scores^T[key][col] = K Q^T,  out^T[channel][col] += V^T P^T,
+// the score tile's register layout being the second operand's of the V product.
+// A wave works by itself on tiles of 64 keys.  Keys: lane (g, c) holds channels g * H/4 .. of key c of a run of 16: whole blocks
+// (or parts of one), 4 H/32 bytes of codes loaded where they lie, no LDS; the channels an MFMA step sums over are the same
+// permutation for the query.  Values: a row's codes go to the wave's own LDS and come back by the transposing read for 4-bit
+// elements: of 16 lanes, lane i fetches 16 channels (8 bytes) of key i and gets the 16 keys of channel i.
+// A value's scale belongs to (key, block), in the transposed operand it differs from slot to slot, so it multiplies the
+// probability instead: P is rounded to bf16 and the exponent of each block's scale is added to it as an integer (exact; what
+// falls below bf16's range is zero), the codes enter unscaled.  A probability of zero stays zero whatever the scale, so a key that a
+// column does not see adds nothing, also where its block is NaN; blocks of seen keys that are NaN (scale byte 255) are found
+// by their bytes and put into the result.
+// Scores, maximum and sums in fp32; the probabilities' sum is that of the bf16 ones, taken by an MFMA with ones.
+// ---------------------------------------------------------------------------
+// maximum over the four 16-lane groups
+__device__ __forceinline__ float max_of_groups(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+template <int NJ>
+constexpr int mx4_scale_bytes() { // scale bytes of a lane's channels of a key: whole blocks, or one that they lie in
+  return NJ % 4 == 0 ? NJ / 4 : NJ <= 2 ? 1 : NJ;
+}
+
+template <int NJ, int W, bool MASK>
+__global__ void __launch_bounds__(W * 64)
+mx4_split_kernel(const Mx4AttnParams p) {
+  constexpr int H = 32 * NJ, RB = 16 * NJ;          // bytes of a row's codes
+  constexpr int PITCH = RB + 16;                     // of a row in LDS: 16 rows of a group on different banks
+  constexpr int SD = NJ > 4 ? 2 : 1;                 // dwords of a row's scales in LDS
+  constexpr int WAVE_LDS = 64 * PITCH + 64 * SD * 4; // per wave
+  constexpr int OP = H + 4;                          // pitch of a merged output row in floats
+  constexpr int MERGE = (W * 16 * OP + W * 32) * 4, LDS = W * WAVE_LDS > MERGE ? W * WAVE_LDS : MERGE;
+  constexpr int NS = mx4_scale_bytes<NJ>();
+  __shared__ __align__(16) uint8_t lds[LDS];
+  __shared__ float merged[16][33]; // weights of the splits, then the sum
+  __shared__ int arrived_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  const int hk = (int)blockIdx.x % p.Nkv;
+  Block o;
+  if (!locate(p.cu, p.B, p.T, p.R, 16, (int)blockIdx.x / p.Nkv, o))
+    return;
+  const int S = p.splits;
+  const int ncol = min(16, o.n * p.R - o.at * 16); // of this workgroup
+  const int col = o.at * 16 + min(c, ncol - 1), tok = col / p.R, r0 = col - tok * p.R;
+  const int past = p.past[o.b];
+  const int limit = min(max(past + tok + 1, 0), p.Smax); // keys this lane's column sees
+  const int L = min(max(past + (o.at * 16 + ncol - 1) / p.R + 1, 0), p.Smax);
+
+  const int64_t head = ((int64_t)o.b * p.Nkv + hk) * p.Smax;
+  const uint8_t* const kq = p.kq + head * RB;
+  const uint8_t* const ks = p.ks + head * NJ;
+  const uint8_t* const vq = p.vq + head * RB;
+  const uint8_t* const vs = p.vs + head * NJ;
+  const uint16_t* mrow = MASK ? p.mask + (int64_t)o.b * p.mask_ld : nullptr;
+
+  bf16x8 q[NJ];
+  {
+    const uint16_t* qrow = p.q + (int64_t)(o.start + tok) * p.q_ld + (hk * p.R + r0) * H + g * (8 * NJ);
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+      q[j] = *reinterpret_cast<const bf16x8*>(qrow + j * 8);
+  }
+  uint32_t kc[4][NJ], kb[4][NS]; // keys of the tile: codes and scale bytes
+  i32x4 vc[NJ];                  // values: 16-byte chunks i * 64 + lane of the tile's rows
+  uint32_t vb[SD];               // scales of the value of key `lane`
+  const int64_t vend = (int64_t)p.Smax * RB - 16;
+  auto request_k = [&](int base) { // rows past the cache's end repeat its last one
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      const int key = min(base + t * 16 + c, p.Smax - 1);
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(kq + (int64_t)key * RB + g * (4 * NJ));
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+        kc[t][j] = src[j];
+      const uint8_t* sb = ks + (int64_t)key * NJ;
+#pragma unroll
+      for (int j = 0; j < NS; j++)
+        kb[t][j] = sb[NJ % 4 == 0 ? g * NS + j : (g * NJ + j) >> 2];
+    }
+  };
+  auto request_v = [&](int base) {
+    const int64_t at = (int64_t)base * RB + lane * 16;
+#pragma unroll
+    for (int i = 0; i < NJ; i++)
+      vc[i] = *reinterpret_cast<const i32x4*>(vq + min(at + i * 1024, vend));
+    const uint8_t* sb = vs + (int64_t)min(base + lane, p.Smax - 1) * NJ;
+    if constexpr (NJ == 4) {
+      vb[0] = *reinterpret_cast<const uint32_t*>(sb);
+    } else if constexpr (NJ == 8) {
+      const i32x2 w = *reinterpret_cast<const i32x2*>(sb);
+      vb[0] = w[0];
+      vb[1] = w[1];
+    } else if constexpr (NJ == 2) {
+      vb[0] = *reinterpret_cast<const uint16_t*>(sb);
+    } else {
+#pragma unroll
+      for (int j = 0; j < SD; j++)
+        vb[j] = 0;
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+        vb[j >> 2] |= (uint32_t)sb[j] << (8 * (j & 3));
+    }
+  };
+
+  uint8_t* const mine = lds + wave * WAVE_LDS;
+  // key t * 16 + g * 4 + r of the tile lies at row g * 16 + t * 4 + r: the order in which lane group g holds its probabilities
+  auto place = [](int key) { return ((key >> 2) & 3) * 16 + (key >> 4) * 4 + (key & 3); };
+  float m = LOWEST;
+  f32x4 acc[2 * NJ], sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int dt = 0; dt < 2 * NJ; dt++)
+    acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const bf16x8 ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
+  const float scale2 = p.scale * LOG2E;
+
+  const int step = S * W * 64;
+  int base = ((int)blockIdx.y * W + wave) * 64;
+  if (base < L) {
+    request_k(base);
+    request_v(base);
+  }
+  for (; base < L; base += step) {
+    f32x4 sc[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        const uint32_t byte = kb[t][NJ % 4 == 0 ? j >> 2 : NS == 1 ? 0 : j];
+        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx4_to_bf16(kc[t][j], e8m0_to_f32(byte)), q[j], sc[t], 0, 0, 0);
+      }
+    }
+    const bool more = base + step < L; // wave-uniform
+    if (more)
+      request_k(base + step);
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      x[i] = sc[i >> 2][i & 3] * (MASK ? p.scale : scale2);
+    if (MASK) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int key = base + (i >> 2) * 16 + g * 4 + (i & 3);
+        const float mv = key < p.mask_ld ? bf16_bits_to_f32(mrow[min(key, p.mask_ld - 1)]) : 0.f;
+        x[i] = mv == -INFINITY ? -INFINITY : x[i] + mv; // (a key that is not looked at may be NaN)
+      }
+    }
+    if (base + 64 > min(past + 1, p.Smax)) { // wave-uniform: some column may not see some key
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        x[i] = base + (i >> 2) * 16 + g * 4 + (i & 3) < limit ? x[i] : -INFINITY;
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      mx = fmaxf(mx, x[i]);
+    if (__builtin_amdgcn_ballot_w64(mx > m) != 0) { // some column's maximum moves
+      mx = max_of_groups(mx);
+      const float alpha = __builtin_amdgcn_exp2f(MASK ? (m - mx) * LOG2E : m - mx);
+#pragma unroll
+      for (int dt = 0; dt < 2 * NJ; dt++)
+        acc[dt] *= alpha;
+      sum *= alpha;
+      m = mx;
+    }
+    uint32_t pr[8]; // bf16 pairs, slots 2 e, 2 e + 1
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      float f[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        f[h] = __builtin_amdgcn_exp2f(MASK ? (x[2 * e + h] - m) * LOG2E : x[2 * e + h] - m);
+      pr[e] = f32x2_to_bf16_bits(f[0], f[1]);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const i32x4 w = {(int)pr[4 * u], (int)pr[4 * u + 1], (int)pr[4 * u + 2], (int)pr[4 * u + 3]};
+      sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, __builtin_bit_cast(bf16x8, w), sum, 0, 0, 0);
+    }
+    // the values' codes and scales through LDS (the wave's own: its accesses to LDS stay in order)
+    const bool odd = base + lane < L && [&] {
+      uint32_t any = 0;
+#pragma unroll
+      for (int j = 0; j < SD; j++)
+        any |= ((vb[j] & 0x7f7f7f7fu) + 0x01010101u) & vb[j] & 0x80808080u;
+      return any != 0;
+    }();
+#pragma unroll
+    for (int i = 0; i < NJ; i++) {
+      const int ch = i * 64 + lane;
+      *reinterpret_cast<i32x4*>(mine + place(ch / NJ) * PITCH + (ch % NJ) * 16) = vc[i];
+    }
+#pragma unroll
+    for (int j = 0; j < SD; j++) // (rows past the keys may hold anything)
+      reinterpret_cast<uint32_t*>(mine + 64 * PITCH)[place(lane) * SD + j] = base + lane < L ? vb[j] : 0u;
+    if (more)
+      request_v(base + step);
+    uint32_t sd[16][SD];
+    {
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(mine + 64 * PITCH) + g * 16 * SD;
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+#pragma unroll
+        for (int j = 0; j < SD; j++)
+          sd[i][j] = src[i * SD + j];
+    }
+    if (__builtin_amdgcn_ballot_w64(odd) != 0) { // a block of NaN: into the columns that see its key
+#pragma unroll
+      for (int bl = 0; bl < NJ; bl++) {
+        int bad = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          bad |= ((sd[i][bl >> 2] >> (8 * (bl & 3))) & 0xffu) == 255u && x[i] != -INFINITY;
+        bad |= __shfl_xor(bad, 16);
+        bad |= __shfl_xor(bad, 32);
+        if (bad)
+          acc[2 * bl] = acc[2 * bl + 1] = f32x4{NAN, NAN, NAN, NAN};
+      }
+    }
+    i16x2 pe[8], nz[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      pe[e] = __builtin_bit_cast(i16x2, pr[e]) - (short)(127 * 128);
+      nz[e] = __builtin_bit_cast(i16x2, pr[e]) != i16x2{0, 0};
+    }
+    const uint8_t* const vrow = mine + (g * 16 + c) * PITCH;
+#pragma unroll
+    for (int bl = 0; bl < NJ; bl++) {
+      i32x4 w[2];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        constexpr uint32_t SEL = 0x0c040c00u;
+        const uint32_t s = __builtin_amdgcn_perm(sd[2 * e + 1][bl >> 2], sd[2 * e][bl >> 2], SEL + 0x00010001u * (bl & 3));
+        const i16x2 t = __builtin_elementwise_max(__builtin_bit_cast(i16x2, s) * (short)128 + pe[e], i16x2{0, 0});
+        w[e >> 2][e & 3] = __builtin_bit_cast(int, t & nz[e]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int dt = 2 * bl + h;
+        const i32x2 codes = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2*)(vrow + dt * 8));
+        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx4_to_bf16((uint32_t)codes[0], 1.0f), __builtin_bit_cast(bf16x8, w[0]), acc[dt], 0, 0, 0);
+        acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(mx4_to_bf16((uint32_t)codes[1], 1.0f), __builtin_bit_cast(bf16x8, w[1]), acc[dt], 0, 0, 0);
+      }
+    }
+  }
+  if (!MASK)
+    m *= 1.0f / LOG2E; // natural units, as with a mask
+
+  // the waves' states through LDS
+  __syncthreads();
+  float* const mo = reinterpret_cast<float*>(lds); // [wave][col][OP]
+  float* const sm = mo + W * 16 * OP;              // [wave][col] maximum, then sum
+#pragma unroll
+  for (int dt = 0; dt < 2 * NJ; dt++)
+    *reinterpret_cast<f32x4*>(mo + (wave * 16 + c) * OP + dt * 16 + g * 4) = acc[dt];
+  if (g == 0) {
+    sm[wave * 16 + c] = m;
+    sm[W * 16 + wave * 16 + c] = sum[0];
+  }
+  __syncthreads();
+  float* const part_o = p.part;
+  float* const part_ml = p.part + (int64_t)gridDim.x * S * p.cols * H;
+  const int64_t unit = blockIdx.x;
+  auto store4 = [&](int cc, int d4, f32x4 v, float Ls) {
+    const int cl = o.at * 16 + cc, tk = cl / p.R, rr = cl - tk * p.R;
+    uint32_t w[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) // (nothing seen: zeros; a NaN sum is kept)
+      w[e] = f32x2_to_bf16_bits(Ls != 0.f ? v[2 * e] / Ls : 0.f, Ls != 0.f ? v[2 * e + 1] / Ls : 0.f);
+    *reinterpret_cast<uint2*>(p.out + ((int64_t)(o.start + tk) * p.Nq + hk * p.R + rr) * H + d4 * 4) = make_uint2(w[0], w[1]);
+  };
+  for (int i = tid; i < ncol * (H / 4); i += W * 64) {
+    const int cc = i / (H / 4), d4 = i % (H / 4);
+    float M = sm[cc];
+#pragma unroll
+    for (int w = 1; w < W; w++)
+      M = fmaxf(M, sm[w * 16 + cc]);
+    float Ls = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+      const float wt = __builtin_amdgcn_exp2f((sm[w * 16 + cc] - M) * LOG2E);
+      Ls = fmaf(wt, sm[W * 16 + w * 16 + cc], Ls);
+      const f32x4 ow = *reinterpret_cast<const f32x4*>(mo + (w * 16 + cc) * OP + d4 * 4);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        v[e] = fmaf(wt, ow[e], v[e]);
+    }
+    if (S == 1) {
+      store4(cc, d4, v, Ls);
+      continue;
+    }
+    // device-scope stores: written through to the level that all XCDs share
+    const int64_t at = (unit * S + blockIdx.y) * p.cols + cc;
+    uint64_t* const dst = reinterpret_cast<uint64_t*>(part_o + at * H + d4 * 4);
+    __hip_atomic_store(dst, __builtin_bit_cast(uint64_t, make_float2(v[0], v[1])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(dst + 1, __builtin_bit_cast(uint64_t, make_float2(v[2], v[3])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (d4 == 0)
+      __hip_atomic_store(reinterpret_cast<uint64_t*>(part_ml + at * 2), __builtin_bit_cast(uint64_t, make_float2(M, Ls)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (S == 1)
+    return;
+  // The split that arrives last merges all of them, in split order (the same sums whichever that is).  Every thread waits until
+  // its own stores are acknowledged, then the barrier, the arrival, and the device-scope loads; nobody waits for another workgroup.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0)
+    arrived_last = atomicInc(p.counters + unit * MX4_COUNTER_STRIDE, (unsigned)S - 1) == (unsigned)S - 1;
+  __syncthreads();
+  if (!arrived_last)
+    return;
+  auto load2 = [](const float* src) {
+    return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(src), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  };
+  for (int i = tid; i < ncol * 32; i += W * 64) { // 32 lanes per column, one split each
+    const int cc = i >> 5, s = i & 31;
+    float2 ml = {LOWEST, 0.f};
+    if (s < S)
+      ml = load2(part_ml + ((unit * S + s) * p.cols + cc) * 2);
+    float M = ml.x;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2)
+      M = fmaxf(M, __shfl_xor(M, d));
+    const float wt = __builtin_amdgcn_exp2f((ml.x - M) * LOG2E);
+    float Ls = wt * ml.y;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2)
+      Ls += __shfl_xor(Ls, d);
+    merged[cc][s] = wt;
+    if (s == 0)
+      merged[cc][32] = Ls;
+  }
+  __syncthreads();
+  for (int i = tid; i < ncol * (H / 4); i += W * 64) {
+    const int cc = i / (H / 4), d4 = i % (H / 4);
+    const float* src = part_o + (unit * S * p.cols + cc) * H + d4 * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < S; s0 += 8) { // eight splits' loads in flight
+      float2 a[8][2];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const float* at = src + (int64_t)min(s0 + u, S - 1) * p.cols * H;
+        a[u][0] = load2(at);
+        a[u][1] = load2(at + 2);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        if (s0 + u < S) {
+          const float wt = merged[cc][s0 + u];
+          v[0] = fmaf(wt, a[u][0].x, v[0]);
+          v[1] = fmaf(wt, a[u][0].y, v[1]);
+          v[2] = fmaf(wt, a[u][1].x, v[2]);
+          v[3] = fmaf(wt, a[u][1].y, v[3]);
+        }
+    }
+    store4(cc, d4, v, merged[cc][32]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+static int rows_launch(const char* who, Mx4RowsParams& p, bool cache, hipStream_t stream) {
+  TPPX_REQUIRE(mx4_has_head(p.H), TPPX_EUNSUPPORTED, "%s: head size %d (64, 96, 128, 192 and 256 are built)", who, p.H);
+  TPPX_REQUIRE(p.T >= 0 && p.B > 0 && p.Nkv > 0 && (!p.q || p.Nq > 0) && p.Nq <= (1 << 20) && p.Nkv <= (1 << 20), TPPX_ESHAPE,
+               "%s: bad shape T=%d B=%d Nq=%d Nkv=%d", who, p.T, p.B, p.Nq, p.Nkv);
+  TPPX_REQUIRE(!p.emb || (p.MP > 0 && p.HR > 0 && p.HR <= p.H && p.HR % 16 == 0), TPPX_ESHAPE,
+               "%s: rotary_dim=%d must be a multiple of 16 and <= H=%d", who, p.HR, p.H);
+  TPPX_REQUIRE((!p.q || p.q_ld >= (int64_t)p.Nq * p.H) && p.k_ld >= (int64_t)p.Nkv * p.H && (!p.v || p.v_ld >= (int64_t)p.Nkv * p.H) &&
+                   (p.q_ld | p.k_ld | p.v_ld) % 8 == 0,
+               TPPX_ESHAPE, "%s: row strides must be multiples of 8 elements and hold a row", who);
+  if (p.T == 0)
+    return TPPX_OK;
+  if (!p.emb)
+    p.HR = 0;
+  const int G = p.H <= 64 ? 8 : p.H <= 128 ? 16 : 32;
+  const int64_t heads = (p.q ? p.Nq : 0) + p.Nkv + (p.v ? p.Nkv : 0), wgs = (heads * G + 255) / 256;
+  TPPX_REQUIRE(wgs <= 65535, TPPX_ESHAPE, "%s: too many heads", who);
+  const dim3 grid((unsigned)p.T, (unsigned)wgs);
+  auto go = [&](auto g) {
+    constexpr int GG = decltype(g)::value;
+    if (cache)
+      mx4_rows_kernel<GG, true><<<grid, dim3(256), 0, stream>>>(p);
+    else
+      mx4_rows_kernel<GG, false><<<grid, dim3(256), 0, stream>>>(p);
+  };
+  if (G == 8)
+    go(std::integral_constant<int, 8>{});
+  else if (G == 16)
+    go(std::integral_constant<int, 16>{});
+  else
+    go(std::integral_constant<int, 32>{});
+  return check_hip(hipGetLastError(), who);
+}
+
+static int split_launch(const char* who, Mx4AttnParams& p, int H, void* ws, int64_t ws_bytes, void* counters, int64_t counter_bytes,
+                        hipStream_t stream) {
+  constexpr int W = 4;
+  const int64_t blocks = p.cu ? ((int64_t)p.T * p.R + (int64_t)p.B * 15) / 16 : (int64_t)p.B * ((p.R + 15) / 16);
+  const int64_t units = blocks * p.Nkv;
+  TPPX_REQUIRE(units < ((int64_t)1 << 31), TPPX_ESHAPE, "%s: problem too large", who);
+  p.cols = p.cu ? 16 : std::min(16, p.R);
+  const int64_t trips = ((int64_t)p.Smax + W * 64 - 1) / (W * 64);
+  int64_t S = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(trips, 32), 768 / units));
+  if (!ws || units * S * p.cols * (H + 2) * (int64_t)sizeof(float) > ws_bytes || units * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) > counter_bytes)
+    S = 1;
+  p.splits = (int)S;
+  p.part = (float*)ws;
+  p.counters = (unsigned int*)counters;
+  const dim3 grid((unsigned)units, (unsigned)S);
+  mx4_for_head(H, [&](auto nj) {
+    constexpr int NJ = decltype(nj)::value;
+    if (p.mask)
+      mx4_split_kernel<NJ, W, true><<<grid, dim3(W * 64), 0, stream>>>(p);
+    else
+      mx4_split_kernel<NJ, W, false><<<grid, dim3(W * 64), 0, stream>>>(p);
+  });
+  return check_hip(hipGetLastError(), who);
+}
+
+static int attn_checks(const char* who, int64_t T, int64_t B, int64_t Nq, int64_t Nkv, int64_t H, int64_t q_ld, const void* mask, int64_t mask_ld) {
+  TPPX_REQUIRE(mx4_has_head(H), TPPX_EUNSUPPORTED, "%s: head size %ld (64, 96, 128, 192 and 256 are built)", who, (long)H);
+  TPPX_REQUIRE(T >= 0 && T < ((int64_t)1 << 30) && B > 0 && B < ((int64_t)1 << 24) && Nq > 0 && Nkv > 0 && Nq % Nkv == 0 && Nq <= (1 << 16) &&
+                   T * (Nq / Nkv) < ((int64_t)1 << 31),
+               TPPX_ESHAPE, "%s: bad shape T=%ld B=%ld Nq=%ld Nkv=%ld", who, (long)T, (long)B, (long)Nq, (long)Nkv);
+  TPPX_REQUIRE(q_ld >= Nq * H && q_ld % 8 == 0, TPPX_ESHAPE, "%s: row strides must be multiples of 8 elements and hold a row", who);
+  TPPX_REQUIRE(!mask || (mask_ld > 0 && mask_ld < ((int64_t)1 << 31)), TPPX_EINVAL, "%s: mask given with mask_ld=%ld", who, (long)mask_ld);
+  return TPPX_OK;
+}
+
+} // namespace tppx
+
+using namespace tppx;
+
+extern "C" int tppx_qk_norm_rotary(const void* q, const void* k, const void* gamma_q, const void* gamma_k, int gamma_dtype, float eps,
+                                   const void* emb_pos, int gptj, const void* pos, void* q_out, void* k_out, int64_t T, int64_t Nq,
+                                   int64_t Nkv, int64_t H, int64_t q_ld, int64_t k_ld, int64_t MP, int64_t HR, tppx_stream_t stream) {
+  const char* who = "tppx_qk_norm_rotary";
+  TPPX_REQUIRE(q && k && q_out && k_out && (pos || !emb_pos), TPPX_EINVAL, "%s: null pointer", who);
+  TPPX_REQUIRE(aligned16(q) && aligned16(k) && aligned16(q_out) && aligned16(k_out) && aligned16(gamma_q) && aligned16(gamma_k) && aligned16(emb_pos),
+               TPPX_EINVAL, "%s: pointer not 16-byte aligned", who);
+  TPPX_REQUIRE(gamma_dtype == TPPX_DT_F32 || gamma_dtype == TPPX_DT_BF16, TPPX_EINVAL, "%s: gamma dtype %d", who, gamma_dtype);
+  TPPX_REQUIRE(T < ((int64_t)1 << 31) && MP < ((int64_t)1 << 31) && Nq < (1 << 30) && Nkv < (1 << 30) && H < (1 << 30) && HR < (1 << 30), TPPX_ESHAPE, "%s: problem too large", who);
+  Mx4RowsParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.qo = (uint16_t*)q_out; p.ko = (uint16_t*)k_out;
+  p.gq = gamma_q; p.gk = gamma_k; p.gamma_f32 = gamma_dtype == TPPX_DT_F32; p.eps = eps;
+  p.emb = (const float*)emb_pos; p.gptj = gptj != 0; p.pos = (const int64_t*)pos;
+  p.q_ld = q_ld; p.k_ld = k_ld;
+  p.T = (int)T; p.B = 1; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.H = (int)H; p.MP = (int)MP; p.HR = (int)HR;
+  return rows_launch(who, p, false, (hipStream_t)stream);
+}
+
+extern "C" int tppx_append_mx4(const void* q, const void* k, const void* v, const void* gamma_q, const void* gamma_k, int gamma_dtype,
+                               float eps, const void* emb_pos, int gptj, const void* pos, void* k_codes, void* k_scales, void* v_codes,
+                               void* v_scales, const void* past, const void* cu, void* q_out, void* k_out, void* v_out, int64_t T,
+                               int64_t B, int64_t Nq, int64_t Nkv, int64_t H, int64_t Smax, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                               int64_t MP, int64_t HR, tppx_stream_t stream) {
+  const char* who = "tppx_append_mx4";
+  TPPX_REQUIRE(k && v && k_codes && k_scales && v_codes && v_scales && past && (!q || q_out), TPPX_EINVAL, "%s: null pointer", who);
+  TPPX_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) && aligned16(k_out) && aligned16(v_out) && aligned16(gamma_q) &&
+                   aligned16(gamma_k) && aligned16(emb_pos) && aligned16(k_codes) && aligned16(v_codes),
+               TPPX_EINVAL, "%s: pointer not 16-byte aligned", who);
+  TPPX_REQUIRE(gamma_dtype == TPPX_DT_F32 || gamma_dtype == TPPX_DT_BF16, TPPX_EINVAL, "%s: gamma dtype %d", who, gamma_dtype);
+  TPPX_REQUIRE(T < ((int64_t)1 << 31) && B < ((int64_t)1 << 31) && MP < ((int64_t)1 << 31) && Nq < (1 << 30) && Nkv < (1 << 30) && H < (1 << 30) && HR < (1 << 30),
+               TPPX_ESHAPE, "%s: problem too large", who);
+  TPPX_REQUIRE(Smax > 0 && Smax < ((int64_t)1 << 30), TPPX_ESHAPE, "%s: capacity %ld", who, (long)Smax);
+  TPPX_REQUIRE(cu || T == B, TPPX_ESHAPE, "%s: %ld tokens of %ld sequences need their bounds", who, (long)T, (long)B);
+  Mx4RowsParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.v = (const uint16_t*)v;
+  p.qo = (uint16_t*)q_out; p.ko = (uint16_t*)k_out; p.vo = (uint16_t*)v_out;
+  p.kq = (uint8_t*)k_codes; p.ks = (uint8_t*)k_scales; p.vq = (uint8_t*)v_codes; p.vs = (uint8_t*)v_scales;
+  p.gq = gamma_q; p.gk = gamma_k; p.gamma_f32 = gamma_dtype == TPPX_DT_F32; p.eps = eps;
+  p.emb = (const float*)emb_pos; p.gptj = gptj != 0; p.pos = (const int64_t*)pos;
+  p.past = (const int32_t*)past; p.cu = (const int32_t*)cu;
+  p.q_ld = q ? q_ld : 0; p.k_ld = k_ld; p.v_ld = v_ld;
+  p.T = (int)T; p.B = (int)B; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.H = (int)H; p.MP = (int)MP; p.HR = (int)HR; p.Smax = (int)Smax;
+  return rows_launch(who, p, true, (hipStream_t)stream);
+}
+
+extern "C" int tppx_attn_mx4(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                             const void* past, const void* cu, const void* mask, int64_t mask_ld, void* out, int64_t T, int64_t B,
+                             int64_t Nq, int64_t Nkv, int64_t H, int64_t Smax, int64_t q_ld, void* ws, int64_t ws_bytes, void* counters,
+                             int64_t counter_bytes, tppx_stream_t stream) {
+  const char* who = "tppx_attn_mx4";
+  TPPX_REQUIRE(q && k_codes && k_scales && v_codes && v_scales && past && out, TPPX_EINVAL, "%s: null pointer", who);
+  TPPX_REQUIRE(aligned16(q) && aligned16(k_codes) && aligned16(v_codes) && aligned16(out) && aligned16(ws), TPPX_EINVAL, "%s: pointer not 16-byte aligned", who);
+  if (int rc = attn_checks(who, T, B, Nq, Nkv, H, q_ld, mask, mask_ld))
+    return rc;
+  TPPX_REQUIRE(H % 128 != 0 || (((uintptr_t)k_scales | (uintptr_t)v_scales) & (H / 32 - 1)) == 0, TPPX_EINVAL, "%s: scales not aligned to a row of them", who);
+  TPPX_REQUIRE(H != 64 || ((uintptr_t)v_scales & 1) == 0, TPPX_EINVAL, "%s: scales not aligned to a row of them", who);
+  TPPX_REQUIRE(Smax > 0 && Smax < ((int64_t)1 << 30), TPPX_ESHAPE, "%s: capacity %ld", who, (long)Smax);
+  TPPX_REQUIRE(cu || T == B, TPPX_ESHAPE, "%s: %ld tokens of %ld sequences need their bounds", who, (long)T, (long)B);
+  TPPX_REQUIRE(ws_bytes >= 0 && (ws_bytes == 0 || ws) && counter_bytes >= 0 && (counter_bytes == 0 || counters), TPPX_EINVAL,
+               "%s: size given with a null pointer", who);
+  TPPX_REQUIRE(((uintptr_t)counters & 3u) == 0, TPPX_EINVAL, "%s: counters not 4-byte aligned", who);
+  if (T == 0)
+    return TPPX_OK;
+  Mx4AttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = (const uint16_t*)q; p.q_ld = q_ld;
+  p.kq = (const uint8_t*)k_codes; p.ks = (const uint8_t*)k_scales; p.vq = (const uint8_t*)v_codes; p.vs = (const uint8_t*)v_scales;
+  p.past = (const int32_t*)past; p.cu = (const int32_t*)cu; p.mask = (const uint16_t*)mask; p.mask_ld = (int)mask_ld; p.out = (uint16_t*)out;
+  p.T = (int)T; p.B = (int)B; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.R = (int)(Nq / Nkv); p.Smax = (int)Smax;
+  p.scale = 1.0f / sqrtf((float)H);
+  if (!cu || T * p.R <= 128 * B)
+    return split_launch(who, p, (int)H, ws, ws_bytes, counters, counter_bytes, (hipStream_t)stream);
+  return mx4_prompt_launch(who, p, (int)H, true, (hipStream_t)stream);
+}
+
+extern "C" int tppx_attn_packed(const void* q, const void* k, const void* v, const void* cu, const void* mask, int64_t mask_ld, void* out,
+                                int64_t T, int64_t B, int64_t Nq, int64_t Nkv, int64_t H, int64_t q_ld, int64_t k_ld, int64_t v_ld,
+                                tppx_stream_t stream) {
+  const char* who = "tppx_attn_packed";
+  TPPX_REQUIRE(q && k && v && cu && out, TPPX_EINVAL, "%s: null pointer", who);
+  TPPX_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), TPPX_EINVAL, "%s: pointer not 16-byte aligned", who);
+  if (int rc = attn_checks(who, T, B, Nq, Nkv, H, q_ld, mask, mask_ld))
+    return rc;
+  TPPX_REQUIRE(k_ld >= Nkv * H && v_ld >= Nkv * H && (k_ld | v_ld) % 8 == 0, TPPX_ESHAPE,
+               "%s: row strides must be multiples of 8 elements and hold a row", who);
+  if (T == 0)
+    return TPPX_OK;
+  Mx4AttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = (const uint16_t*)q; p.k = (const uint16_t*)k; p.v = (const uint16_t*)v; p.q_ld = q_ld; p.k_ld = k_ld; p.v_ld = v_ld;
+  p.cu = (const int32_t*)cu; p.mask = (const uint16_t*)mask; p.mask_ld = (int)mask_ld; p.out = (uint16_t*)out;
+  p.T = (int)T; p.B = (int)B; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.R = (int)(Nq / Nkv);
+  p.scale = 1.0f / sqrtf((float)H);
+  return mx4_prompt_launch(who, p, (int)H, false, (hipStream_t)stream);
+}

@@ -1,0 +1,310 @@
+// Attention of prompts, causal, over packed bf16 rows or over the MXFP4 cache.
+#include "tppx_mx4.h"
+
+namespace tppx {
+
+// ---------------------------------------------------------------------------
+// Prompts: W waves of 32 queries of one head share K and V tiles of 64 keys, bf16 in LDS in two stages, from packed rows or
+// from the cache (its codes expanded once per workgroup on the way to LDS).  Both products run transposed on the 32 x 32 x 16
+// MFMA: scores^T[key][query] = K Q^T, out^T[channel][query] += V^T P^T; a lane holds 16 keys of one query in the score tile, and
+// those, rounded to bf16, are the second operand of the V product as they lie; V's operand is read by the transposing LDS read.
+// 32 queries per wave: an operand read from LDS feeds 32 columns, with 16 the LDS (128 bytes per cycle) would take twice the
+// MFMAs' time.  Scores in fp32, running maximum and sum per query, rescaled only in tiles where some maximum moves.
+// A key that a query does not see (a later token, a mask of -inf) adds nothing whatever it holds: its score is replaced, and
+// values that are infinite or NaN in tiles where some query misses a key go a way of their own, element by element.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ bool mx4_non_finite(uint32_t pair) {
+  return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
+}
+// the pair with what is not finite set to zero
+__device__ __forceinline__ uint32_t mx4_finite(uint32_t pair) {
+  return ((pair & 0x7f80u) == 0x7f80u ? 0u : pair & 0xffffu) | ((pair & 0x7f800000u) == 0x7f800000u ? 0u : pair & 0xffff0000u);
+}
+
+template <int NJ, int W, bool CACHE>
+__global__ void __launch_bounds__(W * 64, NJ <= 4 ? 2 : 1)
+mx4_prompt_kernel(const Mx4AttnParams p) {
+  constexpr int H = 32 * NJ, PITCH = 2 * H + 16, STAGE = 2 * 64 * PITCH; // K rows, then V rows
+  constexpr int QB = 32 * W, TH = 64 * W;
+  constexpr int CH = 64 * 4 * NJ;              // 16-byte chunks of a tile of K or of V
+  constexpr int NC = CACHE ? (128 * NJ + TH - 1) / TH : 2 * CH / TH; // items of K and V a thread brings per tile
+  extern __shared__ __align__(16) uint8_t lds[]; // 2 stages
+  __shared__ int flags[2];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5;
+  // heads go round the XCDs, those of one K/V head to the same one
+  const int hr = (int)blockIdx.x % p.Nq, hk = hr % p.Nkv, hq = hk * p.R + hr / p.Nkv;
+  Block o;
+  if (!locate(p.cu, p.B, p.T, 1, QB, (int)blockIdx.x / p.Nq, o))
+    return;
+  const int qblk = (o.n + QB - 1) / QB - 1 - o.at; // the last queries see the most keys: first
+  const int past = CACHE ? max(p.past[o.b], 0) : 0;
+  const int total = CACHE ? min(past + o.n, p.Smax) : o.n; // keys of the sequence
+  const int q0 = qblk * QB + wave * 32;
+  const int qi = min(q0 + c, o.n - 1);
+  const int limit = min(past + qi + 1, total); // keys this lane's query sees
+  const int64_t head = ((int64_t)o.b * p.Nkv + hk) * p.Smax;
+  const uint8_t* const kq = CACHE ? p.kq + head * (16 * NJ) : nullptr;
+  const uint8_t* const vq = CACHE ? p.vq + head * (16 * NJ) : nullptr;
+  const uint8_t* const ks = CACHE ? p.ks + head * NJ : nullptr;
+  const uint8_t* const vs = CACHE ? p.vs + head * NJ : nullptr;
+  const uint16_t* const kr = CACHE ? nullptr : p.k + (int64_t)o.start * p.k_ld + hk * H;
+  const uint16_t* const vr = CACHE ? nullptr : p.v + (int64_t)o.start * p.v_ld + hk * H;
+  const uint16_t* const mrow = p.mask ? p.mask + (int64_t)o.b * p.mask_ld : nullptr;
+
+  bf16x8 q[2 * NJ];
+  {
+    const uint16_t* qrow = p.q + (int64_t)(o.start + qi) * p.q_ld + (int64_t)hq * H + h * 8;
+#pragma unroll
+    for (int j = 0; j < 2 * NJ; j++)
+      q[j] = *reinterpret_cast<const bf16x8*>(qrow + j * 16);
+  }
+  // keys that some query of this workgroup sees
+  const int keys = min(past + min(qblk * QB + QB, o.n), total), tiles = (keys + 63) / 64;
+  const int first_limit = min(past + qblk * QB + 1, total); // keys that all of them see
+
+  // item i of thread tid: 16 bytes of a row, K items before V's; rows past the keys: zeros
+  i32x4 item[NC];
+  uint32_t byte[CACHE ? NC : 1];
+  auto request = [&](int kb) {
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+      const int at = i * TH + tid;
+      if constexpr (CACHE) {
+        const bool is_v = at >= 64 * NJ;
+        const int row = (at - (is_v ? 64 * NJ : 0)) / NJ, bl = (at - (is_v ? 64 * NJ : 0)) % NJ;
+        const int key = kb * 64 + row;
+        item[i] = i32x4{0, 0, 0, 0};
+        byte[i] = 0;
+        if (at < 128 * NJ && key < keys) {
+          item[i] = *reinterpret_cast<const i32x4*>((is_v ? vq : kq) + (int64_t)key * (16 * NJ) + bl * 16);
+          byte[i] = (is_v ? vs : ks)[(int64_t)key * NJ + bl];
+        }
+      } else {
+        const bool is_v = at >= CH;
+        const int row = (at - (is_v ? CH : 0)) / (4 * NJ), ch = (at - (is_v ? CH : 0)) % (4 * NJ);
+        const int key = kb * 64 + row;
+        item[i] = key < keys ? *reinterpret_cast<const i32x4*>((is_v ? vr + (int64_t)key * p.v_ld : kr + (int64_t)key * p.k_ld) + ch * 8) : i32x4{0, 0, 0, 0};
+      }
+    }
+  };
+  auto deliver = [&](int kb, int stage) {
+    uint8_t* const st = lds + stage * STAGE;
+    const bool partial = mrow || kb * 64 + 64 > first_limit; // (uniform)
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+      const int at = i * TH + tid;
+      if constexpr (CACHE) {
+        const bool is_v = at >= 64 * NJ;
+        const int row = (at - (is_v ? 64 * NJ : 0)) / NJ, bl = (at - (is_v ? 64 * NJ : 0)) % NJ;
+        uint8_t* const dst = st + (is_v ? 64 * PITCH : 0) + row * PITCH + bl * 64;
+        const float s = byte[i] == 255u ? NAN : e8m0_to_f32(byte[i]);
+        if ((128 * NJ) % TH == 0 || at < 128 * NJ) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const bf16x8 w = mx4_to_bf16((uint32_t)item[i][j], s);
+            *reinterpret_cast<bf16x8*>(dst + j * 16) = byte[i] == 255u ? __builtin_bit_cast(bf16x8, i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0}) : w;
+          }
+          odd |= is_v && byte[i] == 255u;
+        }
+      } else {
+        const bool is_v = at >= CH;
+        const int row = (at - (is_v ? CH : 0)) / (4 * NJ), ch = (at - (is_v ? CH : 0)) % (4 * NJ);
+        *reinterpret_cast<i32x4*>(st + (is_v ? 64 * PITCH : 0) + row * PITCH + ch * 16) = item[i];
+        if (partial && is_v)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            odd |= mx4_non_finite((uint32_t)item[i][j]);
+      }
+    }
+    if (partial && __builtin_amdgcn_ballot_w64(odd) != 0)
+      flags[stage] = kb; // (every wave that writes writes the same)
+  };
+
+  float m = LOWEST, l = 0.f;
+  f32x16 acc[NJ];
+#pragma unroll
+  for (int dt = 0; dt < NJ; dt++)
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      acc[dt][i] = 0.f;
+  const float scale2 = p.scale * LOG2E;
+  const int wave_limit = min(past + min(q0 + 32, o.n), total); // keys that some query of this wave sees
+  const bool idle = q0 >= o.n;
+
+  if (tid < 2)
+    flags[tid] = -1;
+  request(0);
+  __syncthreads();
+  deliver(0, 0);
+  for (int kb = 0; kb < tiles; kb++) {
+    const int stage = kb & 1;
+    __syncthreads(); // this tile has been written, the other stage has been read
+    if (kb + 1 < tiles)
+      request(kb + 1);
+    if (!idle && kb * 64 < wave_limit) {
+      const uint8_t* const st = lds + stage * STAGE;
+      f32x16 sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          sc[t][i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2 * NJ; j++)
+          sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(st + (t * 32 + c) * PITCH + j * 32 + h * 16), q[j], sc[t], 0, 0, 0);
+      }
+      // key of score i of run t
+      auto key_of = [&](int t, int i) { return kb * 64 + t * 32 + (i & 3) + 8 * (i >> 2) + 4 * h; };
+      if (mrow) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int key = key_of(t, i);
+            const float mv = key < p.mask_ld ? bf16_bits_to_f32(mrow[min(key, p.mask_ld - 1)]) : 0.f;
+            sc[t][i] = mv == -INFINITY ? -INFINITY : fmaf(sc[t][i], p.scale, mv);
+          }
+      }
+      const bool partial = kb * 64 + 64 > min(past + q0 + 1, total); // (wave-uniform)
+      if (partial) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            sc[t][i] = key_of(t, i) < limit ? sc[t][i] : -INFINITY;
+      }
+      float mx = m;
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          mx = fmaxf(mx, sc[t][i]);
+      const float unit = mrow ? LOG2E : scale2;
+      float alpha = 1.f;
+      if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        alpha = __builtin_amdgcn_exp2f((m - mx) * unit);
+#pragma unroll
+        for (int dt = 0; dt < NJ; dt++)
+          acc[dt] *= alpha;
+        m = mx;
+      }
+      l *= alpha;
+      bf16x8 pb[4];
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const float pr = __builtin_amdgcn_exp2f((sc[t][i] - m) * unit);
+          l += pr;
+          pb[t * 2 + (i >> 3)][i & 7] = (__bf16)pr;
+        }
+      // V operand of 16 keys (step u) and 32 channels: two transposing reads of 4 keys each for this lane's half
+      const uint8_t* const vt = st + 64 * PITCH + (4 * h + ((lane & 15) >> 2)) * PITCH + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+      auto operand = [&](int dt, int u, int e) {
+        return __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+            (__attribute__((address_space(3))) bf16x4*)(vt + (u * 16 + e * 8) * PITCH + dt * 64)));
+      };
+      if (__builtin_expect(flags[stage] == kb, 0)) { // values that are not finite where some query misses a key
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+          for (int dt = 0; dt < NJ; dt++) {
+            const i32x2 a = operand(dt, u, 0), b = operand(dt, u, 1);
+            const i32x4 w = {(int)mx4_finite((uint32_t)a[0]), (int)mx4_finite((uint32_t)a[1]), (int)mx4_finite((uint32_t)b[0]), (int)mx4_finite((uint32_t)b[1])};
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[dt], 0, 0, 0);
+          }
+        // the probabilities through the stage that nobody reads now, 32 keys at a time; -1: not seen
+        uint16_t* const mine = reinterpret_cast<uint16_t*>(lds + (stage ^ 1) * STAGE) + wave * 1024;
+#pragma unroll 1
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float x = t ? sc[1][i] : sc[0][i];
+            mine[((i & 3) + 8 * (i >> 2) + 4 * h) * 32 + c] = (uint16_t)f32_to_bf16_bits(x == -INFINITY ? -1.f : __builtin_amdgcn_exp2f((x - m) * unit));
+          }
+#pragma unroll 1
+          for (int key = 0; key < 32; key++) {
+            const float pv = bf16_bits_to_f32(mine[key * 32 + c]);
+            const uint16_t* vrow = reinterpret_cast<const uint16_t*>(st + 64 * PITCH + (t * 32 + key) * PITCH);
+#pragma unroll
+            for (int dt = 0; dt < NJ; dt++)
+#pragma unroll
+              for (int k = 0; k < 16; k++) {
+                const uint32_t w = vrow[dt * 32 + (k & 3) + 8 * (k >> 2) + 4 * h];
+                if ((w & 0x7f80u) == 0x7f80u && !(pv < 0.f))
+                  acc[dt][k] += pv * bf16_bits_to_f32(w);
+              }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+          for (int dt = 0; dt < NJ; dt++) {
+            const i32x2 a = operand(dt, u, 0), b = operand(dt, u, 1);
+            const i32x4 w = {a[0], a[1], b[0], b[1]};
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[dt], 0, 0, 0);
+          }
+      }
+    }
+    if (kb + 1 < tiles) {
+      if (__builtin_expect(flags[stage] == kb, 0))
+        __syncthreads(); // (the other stage was used)
+      deliver(kb + 1, stage ^ 1);
+    }
+  }
+  if (idle)
+    return;
+  l += __shfl_xor(l, 32);
+  if (q0 + c < o.n) {
+    uint16_t* orow = p.out + ((int64_t)(o.start + q0 + c) * p.Nq + hq) * H;
+    const float inv = l != 0.f ? 1.0f / l : 0.f; // (nothing seen: zeros)
+#pragma unroll
+    for (int dt = 0; dt < NJ; dt++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const uint2 w = make_uint2(f32x2_to_bf16_bits(acc[dt][i] * inv, acc[dt][i + 1] * inv), f32x2_to_bf16_bits(acc[dt][i + 2] * inv, acc[dt][i + 3] * inv));
+        *reinterpret_cast<uint2*>(orow + dt * 32 + 8 * (i >> 2) + 4 * h) = w;
+      }
+  }
+}
+
+int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache, hipStream_t stream) {
+  // every sequence's last workgroup may be short: at most this many, those past the last one end at once
+  auto blocks = [&](int rows) { return ((int64_t)p.T + (int64_t)p.B * (rows - 1)) / rows * p.Nq; };
+  const bool wide = blocks(128) >= 400;
+  const int64_t wgs = wide ? blocks(128) : blocks(64);
+  TPPX_REQUIRE(wgs < ((int64_t)1 << 31), TPPX_ESHAPE, "%s: problem too large", who);
+  hipError_t e = hipSuccess;
+  mx4_for_head(H, [&](auto nj) {
+    constexpr int NJ = decltype(nj)::value;
+    auto go = [&](auto w, auto c) {
+      constexpr int W = decltype(w)::value;
+      auto kern = mx4_prompt_kernel<NJ, W, decltype(c)::value>;
+      const size_t lds = 2 * 2 * 64 * (size_t)(64 * NJ + 16);
+      e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
+      if (e == hipSuccess)
+        kern<<<dim3((unsigned)wgs), dim3(W * 64), lds, stream>>>(p);
+    };
+    auto with_source = [&](auto w) {
+      if (cache)
+        go(w, std::true_type{});
+      else
+        go(w, std::false_type{});
+    };
+    if (wide)
+      with_source(std::integral_constant<int, 4>{});
+    else
+      with_source(std::integral_constant<int, 2>{});
+  });
+  if (e != hipSuccess)
+    return check_hip(e, who);
+  return check_hip(hipGetLastError(), who);
+}
+
+} // namespace tppx

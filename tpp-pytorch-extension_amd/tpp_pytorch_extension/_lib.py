@@ -120,6 +120,10 @@ SIGNATURES = {
     "tppx_attn_decode_append_counted": [_vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64,
                                         _i64, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp],
     "tppx_attn_prefill": [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _vp],
+    "tppx_qk_norm_rotary": [_vp, _vp, _vp, _vp, _i32, _f32, _vp, _i32, _vp, _vp, _vp] + [_i64] * 8 + [_vp],
+    "tppx_append_mx4": [_vp] * 5 + [_i32, _f32, _vp, _i32] + [_vp] * 10 + [_i64] * 11 + [_vp],
+    "tppx_attn_mx4": [_vp] * 8 + [_i64, _vp] + [_i64] * 7 + [_vp, _i64, _vp, _i64, _vp],
+    "tppx_attn_packed": [_vp] * 5 + [_i64, _vp] + [_i64] * 8 + [_vp],
     "tppx_plan_linear_mxfp4": [_i64, _i64, _i64, _i32, _i64, ctypes.c_char_p, _i64],
     "tppx_plan_linear_qint8": [_i64, _i64, _i64, _i64, _i32, _i32, _i64, ctypes.c_char_p, _i64],
     "tppx_plan_multi_linear_mxfp4": [ctypes.POINTER(_i64), _i32, _i64, _i64, _i32, _i32, _i64, ctypes.c_char_p, _i64],

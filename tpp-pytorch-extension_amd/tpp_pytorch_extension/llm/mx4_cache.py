@@ -1,0 +1,218 @@
+"""Keys and values held in MXFP4, for sequences of different lengths, and attention of packed prompts.
+
+The reference keeps its cache in bf16 or fp32 and one length for the whole batch (`TppCache` / `LayerCache`,
+src/csrc/llm/attn.h:164-404); the operators here stand beside its `attn` (src/csrc/llm/attn.cpp:957-1043) and its rotary
+embeddings (src/csrc/llm/fused_llm_infer.cpp:150-253).
+
+Packed tokens are rows `[T][heads][H]`: sequence b owns rows `cu_seqlens[b] .. cu_seqlens[b + 1] - 1` (int32 `[B + 1]` on the
+device), or one row each where `cu_seqlens` is None.  `past[b]` (int32 `[B]`, device) is the number of keys that a sequence
+held before these tokens.  Rows of a batch behind the last sequence are neither read nor written: the results hold whatever
+`torch.empty` gave there.
+
+A layer of the cache is `Mx4Layer(k_codes, k_scales, v_codes, v_scales)`, uint8 `[B][Nkv][capacity][H/2]` (two E2M1 codes a
+byte, the even channel in the low half) and `[B][Nkv][capacity][H/32]` (E8M0).  Head sizes 64, 96, 128, 192 and 256.
+"""
+from collections import namedtuple
+
+import torch
+
+from .. import _lib
+from .._lib import TppxError
+
+Mx4Layer = namedtuple("Mx4Layer", "k_codes k_scales v_codes v_scales")
+
+HEAD_SIZES = (64, 96, 128, 192, 256)
+
+
+def _rows(t, name, like=None):
+    """Packed rows of heads: bf16 [T][heads][H] on the GPU (`like`: on that tensor's), heads of a row side by side; other
+    strides are copied."""
+    if t.dim() != 3 or not t.is_cuda or t.dtype != torch.bfloat16:
+        raise TppxError(_lib.EINVAL, f"{name} must be a bfloat16 tensor [tokens][heads][head size] on the GPU, got "
+                                     f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    if like is not None and t.get_device() != like.get_device():
+        raise TppxError(_lib.EINVAL, f"{name} is on {t.device}, not on {like.device}")
+    s = t.stride()
+    if s[2] != 1 or (s[1] != t.shape[2] and t.shape[1] != 1) or s[0] % 8 or s[0] < t.shape[1] * t.shape[2] or t.data_ptr() & 15:
+        return t.contiguous() if not t.is_contiguous() else t.clone()
+    return t
+
+
+def _index(t, name, n, like, dtype=torch.int32):
+    if t.dtype != dtype or t.shape != (n,) or t.get_device() != like.get_device() or not t.is_contiguous():
+        raise TppxError(_lib.EINVAL, f"{name} must be a contiguous {dtype} tensor [{n}] on {like.device}, got "
+                                     f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _norm_weights(q_weight, k_weight, H, like):
+    """(address, address, dtype number) of the per-head norms' weights; None: no norm."""
+    code = None
+    at = []
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is None:
+            at.append(None)
+            continue
+        if w.shape != (H,) or w.get_device() != like.get_device() or not w.is_contiguous() or w.data_ptr() & 15:
+            raise TppxError(_lib.EINVAL, f"{name} must be a contiguous, 16-byte aligned tensor [{H}] on {like.device}, got "
+                                         f"{tuple(w.shape)} on {w.device}")
+        kind = _lib.DT_F32 if w.dtype == torch.float32 else _lib.DT_BF16 if w.dtype == torch.bfloat16 else None
+        if kind is None or code not in (None, kind):
+            raise TppxError(_lib.EINVAL, f"{name}: norm weights are both float32 or both bfloat16, got {w.dtype}")
+        code = kind
+        at.append(w.data_ptr())
+    return at[0], at[1], _lib.DT_F32 if code is None else code
+
+
+def _rotation(emb_pos, style, H, like):
+    """(address, gptj, positions, width) of a rotary table: float32 [2][MP][HR] cos / sin ("llama") or [MP][HR] sin | cos ("gptj")."""
+    if style not in ("llama", "gptj", None):
+        raise TppxError(_lib.EINVAL, f"rotation style {style!r} (\"llama\", \"gptj\" or None)")
+    if emb_pos is None or style is None:
+        return None, 0, 0, 0
+    if (emb_pos.dtype != torch.float32 or emb_pos.get_device() != like.get_device() or not emb_pos.is_contiguous()
+            or emb_pos.dim() != (3 if style == "llama" else 2) or (style == "llama" and emb_pos.shape[0] != 2) or emb_pos.data_ptr() & 15):
+        raise TppxError(_lib.EINVAL, f"emb_pos must be a contiguous float32 table {'[2][positions][width]' if style == 'llama' else '[positions][width]'} "
+                                     f"on {like.device}, got {tuple(emb_pos.shape)} {emb_pos.dtype} on {emb_pos.device}")
+    MP, HR = emb_pos.shape[-2:]
+    if HR > H or HR % 16 or HR == 0 or MP == 0:
+        raise TppxError(_lib.ESHAPE, f"rotary width {HR} must be a multiple of 16 and at most the head size {H}")
+    return emb_pos.data_ptr(), int(style == "gptj"), MP, HR
+
+
+
+
+def qk_norm_rotary(q, k, q_weight=None, k_weight=None, eps=1e-6, emb_pos=None, pos=None, style="llama"):
+    """RMSNorm of every head of q [T][Nq][H] and k [T][Nkv][H] with weights [H] (None: no norm), then the rotation by
+    `emb_pos` at the positions `pos` (int64 [T]), in one pass; fp32 inside, rounded once.  Returns new (q, k).  The rotation alone, in
+    place, is `apply_rotary_pos_emb_llama` / `_gptj`."""
+    q = _rows(q, "q")
+    k = _rows(k, "k", q)
+    T, Nq, H = q.shape
+    if k.shape[0] != T or k.shape[2] != H:
+        raise TppxError(_lib.ESHAPE, f"qk_norm_rotary: q {tuple(q.shape)} and k {tuple(k.shape)}")
+    gq, gk, gdt = _norm_weights(q_weight, k_weight, H, q)
+    table, gptj, MP, HR = _rotation(emb_pos, style, H, q)
+    if table is not None and pos is None:
+        raise TppxError(_lib.EINVAL, "qk_norm_rotary: a rotation needs the positions")
+    at = _index(pos, "pos", T, q, torch.int64) if pos is not None else None
+    qo = torch.empty((T, Nq, H), dtype=q.dtype, device=q.device)
+    ko = torch.empty((T, k.shape[1], H), dtype=q.dtype, device=q.device)
+    if T == 0:
+        return qo, ko
+    with torch.cuda.device_of(q):
+        _lib.check(_lib.lib().tppx_qk_norm_rotary(q.data_ptr(), k.data_ptr(), gq, gk, gdt, eps, table, gptj, at, qo.data_ptr(), ko.data_ptr(),
+                                                  T, Nq, k.shape[1], H, q.stride(0), k.stride(0), MP, HR, _lib.stream_of(q)))
+    return qo, ko
+
+
+def _layer(layer, B, Nkv, H, like):
+    """Addresses and capacity of a cache layer, checked."""
+    kc, ks, vc, vs = layer
+    cap = kc.shape[2] if kc.dim() == 4 else 0
+    for name, t, w in (("key codes", kc, H // 2), ("key scales", ks, H // 32), ("value codes", vc, H // 2), ("value scales", vs, H // 32)):
+        if t.shape != (B, Nkv, cap, w) or t.dtype != torch.uint8 or not t.is_contiguous() or t.get_device() != like.get_device() or cap == 0:
+            raise TppxError(_lib.ESHAPE, f"cache layer: {name} must be a contiguous uint8 tensor [{B}][{Nkv}][capacity][{w}] on "
+                                         f"{like.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), cap
+
+
+def _sequences(T, past, cu_seqlens, like):
+    """(B, address of past, address of cu_seqlens)"""
+    B = past.shape[0] if past.dim() == 1 else 0
+    if B == 0:
+        raise TppxError(_lib.ESHAPE, f"past must be int32 [sequences], got {tuple(past.shape)}")
+    at = _index(past, "past", B, like)
+    if cu_seqlens is None:
+        if T != B:
+            raise TppxError(_lib.ESHAPE, f"{T} tokens of {B} sequences need cu_seqlens")
+        return B, at, None
+    return B, at, _index(cu_seqlens, "cu_seqlens", B + 1, like)
+
+
+def append_mx4(q, k, v, layer, past, cu_seqlens=None, q_weight=None, k_weight=None, eps=1e-6, emb_pos=None, pos=None, style="llama",
+               values=False):
+    """`qk_norm_rotary` of packed tokens with the append: the keys and the values v [T][Nkv][H] go to `layer` in MXFP4, at slots
+    past[b], past[b] + 1, ... of their sequence (what does not fit its capacity is dropped); `past` itself stays.  pos None:
+    the slots are the positions.  q may be None.  Returns (q, k, v): the queries, and with `values` the keys and values as the
+    cache holds them, in bf16 (None otherwise): attention over those (`attn_packed`) is attention over the cache."""
+    k = _rows(k, "k")
+    v = _rows(v, "v", k)
+    T, Nkv, H = k.shape
+    if v.shape != k.shape:
+        raise TppxError(_lib.ESHAPE, f"append_mx4: k {tuple(k.shape)} and v {tuple(v.shape)}")
+    Nq = 0
+    qo = None
+    if q is not None:
+        q = _rows(q, "q", k)
+        Nq = q.shape[1]
+        if q.shape[0] != T or q.shape[2] != H:
+            raise TppxError(_lib.ESHAPE, f"append_mx4: q {tuple(q.shape)} and k {tuple(k.shape)}")
+        qo = torch.empty((T, Nq, H), dtype=k.dtype, device=k.device)
+    B, past_at, cu_at = _sequences(T, past, cu_seqlens, k)
+    kc, ks, vc, vs, cap = _layer(layer, B, Nkv, H, k)
+    gq, gk, gdt = _norm_weights(q_weight, k_weight, H, k)
+    table, gptj, MP, HR = _rotation(emb_pos, style, H, k)
+    at = _index(pos, "pos", T, k, torch.int64) if pos is not None else None
+    ko = torch.empty((T, Nkv, H), dtype=k.dtype, device=k.device) if values else None
+    vo = torch.empty((T, Nkv, H), dtype=k.dtype, device=k.device) if values else None
+    if T == 0:
+        return qo, ko, vo
+    with torch.cuda.device_of(k):
+        _lib.check(_lib.lib().tppx_append_mx4(
+            None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), gq, gk, gdt, eps, table, gptj, at, kc, ks, vc, vs, past_at, cu_at,
+            _lib.ptr(qo), _lib.ptr(ko), _lib.ptr(vo), T, B, Nq, Nkv, H, cap, 0 if q is None else q.stride(0), k.stride(0), v.stride(0),
+            MP, HR, _lib.stream_of(k)))
+    return qo, ko, vo
+
+
+def _mask(mask, B, like):
+    if mask is None or mask.numel() == 0:
+        return None, 0
+    if mask.dim() != 2 or mask.shape[0] != B or mask.dtype != torch.bfloat16 or not mask.is_contiguous() or mask.get_device() != like.get_device():
+        raise TppxError(_lib.EINVAL, f"mask must be a contiguous bfloat16 tensor [{B}][keys] on {like.device}, got "
+                                     f"{tuple(mask.shape)} {mask.dtype} on {mask.device}")
+    return mask.data_ptr(), mask.shape[1]
+
+
+def attn_mx4(q, layer, past, cu_seqlens=None, mask=None):
+    """Attention of packed tokens q [T][Nq][H] over a layer of the MXFP4 cache, after their own keys were appended: token i of
+    sequence b sees the keys 0 .. past[b] + i.  mask: additive, bf16 [B][keys] (0 past its end; keys under -inf are not looked
+    at).  A token that sees nothing gets zeros.  Returns [T][Nq][H]."""
+    q = _rows(q, "q")
+    T, Nq, H = q.shape
+    B, past_at, cu_at = _sequences(T, past, cu_seqlens, q)
+    Nkv = layer[0].shape[1] if layer[0].dim() == 4 else 0
+    kc, ks, vc, vs, cap = _layer(layer, B, Nkv, H, q)
+    m_at, m_ld = _mask(mask, B, q)
+    out = torch.empty((T, Nq, H), dtype=q.dtype, device=q.device)
+    if T == 0:
+        return out
+    with torch.cuda.device_of(q):
+        st = _lib.stream_of(q)
+        _lib.check(_lib.lib().tppx_attn_mx4(q.data_ptr(), kc, ks, vc, vs, past_at, cu_at, m_at, m_ld, out.data_ptr(), T, B, Nq, Nkv, H, cap,
+                                            q.stride(0), *_lib.with_counters(_lib.workspace(q, st)), st))
+    return out
+
+
+def attn_packed(q, k, v, cu_seqlens, mask=None):
+    """Causal attention of packed prompts q [T][Nq][H] over their own k, v [T][Nkv][H] (bf16, query heads in groups of
+    Nq / Nkv): token i of a sequence sees its tokens 0 .. i.  mask: additive, bf16 [B][tokens of a sequence].  Returns [T][Nq][H]."""
+    q = _rows(q, "q")
+    k = _rows(k, "k", q)
+    v = _rows(v, "v", q)
+    T, Nq, H = q.shape
+    if k.shape != v.shape or k.shape[0] != T or k.shape[2] != H or k.shape[1] == 0 or Nq % k.shape[1]:
+        raise TppxError(_lib.ESHAPE, f"attn_packed: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    B = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else 0
+    if B < 1:
+        raise TppxError(_lib.ESHAPE, f"cu_seqlens must be int32 [sequences + 1], got {tuple(cu_seqlens.shape)}")
+    cu_at = _index(cu_seqlens, "cu_seqlens", B + 1, q)
+    m_at, m_ld = _mask(mask, B, q)
+    out = torch.empty((T, Nq, H), dtype=q.dtype, device=q.device)
+    if T == 0:
+        return out
+    with torch.cuda.device_of(q):
+        _lib.check(_lib.lib().tppx_attn_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_at, m_at, m_ld, out.data_ptr(), T, B, Nq,
+                                               k.shape[1], H, q.stride(0), k.stride(0), v.stride(0), _lib.stream_of(q)))
+    return out
