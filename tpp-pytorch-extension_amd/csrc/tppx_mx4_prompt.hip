@@ -10,8 +10,9 @@ namespace tppx {
 // those, rounded to bf16, are the second operand of the V product as they lie; V's operand is read by the transposing LDS read.
 // 32 queries per wave: an operand read from LDS feeds 32 columns, with 16 the LDS (128 bytes per cycle) would take twice the
 // MFMAs' time.  Scores in fp32, running maximum and sum per query, rescaled only in tiles where some maximum moves.
-// A key that a query does not see (a later token, a mask of -inf) adds nothing whatever it holds: its score is replaced, and
-// values that are infinite or NaN in tiles where some query misses a key go a way of their own, element by element.
+// A key that a query does not see (a later token, a mask of -inf) adds nothing whatever it holds: its score is replaced, and in
+// tiles where some query misses a key values that are infinite or NaN become zeros on the way to LDS; a workgroup that met
+// such values adds them, one by one, to the outputs of the queries that see them once those are written.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ bool mx4_non_finite(uint32_t pair) {
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
@@ -26,10 +27,9 @@ __global__ void __launch_bounds__(W * 64, NJ <= 4 ? 2 : 1)
 mx4_prompt_kernel(const Mx4AttnParams p) {
   constexpr int H = 32 * NJ, PITCH = 2 * H + 16, STAGE = 2 * 64 * PITCH; // K rows, then V rows
   constexpr int QB = 32 * W, TH = 64 * W;
-  constexpr int CH = 64 * 4 * NJ;              // 16-byte chunks of a tile of K or of V
-  constexpr int NC = CACHE ? (128 * NJ + TH - 1) / TH : 2 * CH / TH; // items of K and V a thread brings per tile
+  constexpr int PER = CACHE ? NJ : 4 * NJ, ITEMS = 64 * PER, NC = (ITEMS + TH - 1) / TH; // items of a row, of a tile, of a thread
   extern __shared__ __align__(16) uint8_t lds[]; // 2 stages
-  __shared__ int flags[2];
+  __shared__ int odd_values;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h = lane >> 5;
@@ -64,64 +64,66 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   const int keys = min(past + min(qblk * QB + QB, o.n), total), tiles = (keys + 63) / 64;
   const int first_limit = min(past + qblk * QB + 1, total); // keys that all of them see
 
-  // item i of thread tid: 16 bytes of a row, K items before V's; rows past the keys: zeros
+  // Item i of thread tid: 16 bytes of a row of K (V false) or of V; rows past the keys: zeros.  One of the two at a time is on its
+  // way through registers: the next tile's K under this tile's scores, its V under this tile's output.
   i32x4 item[NC];
   uint32_t byte[CACHE ? NC : 1];
-  auto request = [&](int kb) {
+  auto request = [&](auto V_, int kb) {
+    constexpr bool V = decltype(V_)::value;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
-      const int at = i * TH + tid;
+      const int at = i * TH + tid, row = at / PER, ch = at % PER, key = kb * 64 + row;
+      item[i] = i32x4{0, 0, 0, 0};
       if constexpr (CACHE) {
-        const bool is_v = at >= 64 * NJ;
-        const int row = (at - (is_v ? 64 * NJ : 0)) / NJ, bl = (at - (is_v ? 64 * NJ : 0)) % NJ;
-        const int key = kb * 64 + row;
-        item[i] = i32x4{0, 0, 0, 0};
         byte[i] = 0;
-        if (at < 128 * NJ && key < keys) {
-          item[i] = *reinterpret_cast<const i32x4*>((is_v ? vq : kq) + (int64_t)key * (16 * NJ) + bl * 16);
-          byte[i] = (is_v ? vs : ks)[(int64_t)key * NJ + bl];
+        if (at < ITEMS && key < keys) {
+          item[i] = *reinterpret_cast<const i32x4*>((V ? vq : kq) + (int64_t)key * (16 * NJ) + ch * 16);
+          byte[i] = (V ? vs : ks)[(int64_t)key * NJ + ch];
         }
-      } else {
-        const bool is_v = at >= CH;
-        const int row = (at - (is_v ? CH : 0)) / (4 * NJ), ch = (at - (is_v ? CH : 0)) % (4 * NJ);
-        const int key = kb * 64 + row;
-        item[i] = key < keys ? *reinterpret_cast<const i32x4*>((is_v ? vr + (int64_t)key * p.v_ld : kr + (int64_t)key * p.k_ld) + ch * 8) : i32x4{0, 0, 0, 0};
+      } else if (key < keys) {
+        item[i] = *reinterpret_cast<const i32x4*>((V ? vr + (int64_t)key * p.v_ld : kr + (int64_t)key * p.k_ld) + ch * 8);
       }
     }
   };
-  auto deliver = [&](int kb, int stage) {
-    uint8_t* const st = lds + stage * STAGE;
-    const bool partial = mrow || kb * 64 + 64 > first_limit; // (uniform)
+  auto deliver = [&](auto V_, int kb, int stage) {
+    constexpr bool V = decltype(V_)::value;
+    uint8_t* const st = lds + stage * STAGE + (V ? 64 * PITCH : 0);
+    const bool partial = V && (mrow || kb * 64 + 64 > first_limit); // (uniform)
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
-      const int at = i * TH + tid;
+      const int at = i * TH + tid, row = at / PER, ch = at % PER;
       if constexpr (CACHE) {
-        const bool is_v = at >= 64 * NJ;
-        const int row = (at - (is_v ? 64 * NJ : 0)) / NJ, bl = (at - (is_v ? 64 * NJ : 0)) % NJ;
-        uint8_t* const dst = st + (is_v ? 64 * PITCH : 0) + row * PITCH + bl * 64;
-        const float s = byte[i] == 255u ? NAN : e8m0_to_f32(byte[i]);
-        if ((128 * NJ) % TH == 0 || at < 128 * NJ) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const bf16x8 w = mx4_to_bf16((uint32_t)item[i][j], s);
-            *reinterpret_cast<bf16x8*>(dst + j * 16) = byte[i] == 255u ? __builtin_bit_cast(bf16x8, i32x4{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0}) : w;
-          }
-          odd |= is_v && byte[i] == 255u;
-        }
-      } else {
-        const bool is_v = at >= CH;
-        const int row = (at - (is_v ? CH : 0)) / (4 * NJ), ch = (at - (is_v ? CH : 0)) % (4 * NJ);
-        *reinterpret_cast<i32x4*>(st + (is_v ? 64 * PITCH : 0) + row * PITCH + ch * 16) = item[i];
-        if (partial && is_v)
+        uint8_t* const dst = st + row * PITCH + ch * 64;
+        if (ITEMS % TH == 0 || at < ITEMS) {
+          const bool nan = byte[i] == 255u, drop = nan && partial;
+          odd |= drop;
+          const float s = e8m0_to_f32(drop ? 0u : byte[i]);
 #pragma unroll
           for (int j = 0; j < 4; j++)
-            odd |= mx4_non_finite((uint32_t)item[i][j]);
+            *reinterpret_cast<bf16x8*>(dst + j * 16) = mx4_to_bf16(nan ? 0u : (uint32_t)item[i][j], s); // (zero times infinity)
+        }
+      } else {
+        if (partial) {
+          bool some = false;
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            some |= mx4_non_finite((uint32_t)item[i][j]);
+          if (some) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              item[i][j] = (int)mx4_finite((uint32_t)item[i][j]);
+          }
+          odd |= some;
+        }
+        *reinterpret_cast<i32x4*>(st + row * PITCH + ch * 16) = item[i];
       }
     }
-    if (partial && __builtin_amdgcn_ballot_w64(odd) != 0)
-      flags[stage] = kb; // (every wave that writes writes the same)
+    if (odd)
+      odd_values = 1;
   };
+  constexpr std::false_type K_{};
+  constexpr std::true_type V_{};
 
   float m = LOWEST, l = 0.f;
   f32x16 acc[NJ];
@@ -134,18 +136,22 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   const int wave_limit = min(past + min(q0 + 32, o.n), total); // keys that some query of this wave sees
   const bool idle = q0 >= o.n;
 
-  if (tid < 2)
-    flags[tid] = -1;
-  request(0);
+  if (tid == 0)
+    odd_values = 0;
+  request(K_, 0);
   __syncthreads();
-  deliver(0, 0);
+  deliver(K_, 0, 0);
+  request(V_, 0);
+  deliver(V_, 0, 0);
   for (int kb = 0; kb < tiles; kb++) {
     const int stage = kb & 1;
     __syncthreads(); // this tile has been written, the other stage has been read
-    if (kb + 1 < tiles)
-      request(kb + 1);
-    if (!idle && kb * 64 < wave_limit) {
-      const uint8_t* const st = lds + stage * STAGE;
+    const bool more = kb + 1 < tiles, busy = !idle && kb * 64 < wave_limit; // (uniform in a wave)
+    const uint8_t* const st = lds + stage * STAGE;
+    if (more)
+      request(K_, kb + 1);
+    bf16x8 pb[4];
+    if (busy) {
       f32x16 sc[2];
 #pragma unroll
       for (int t = 0; t < 2; t++) {
@@ -194,7 +200,6 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
         m = mx;
       }
       l *= alpha;
-      bf16x8 pb[4];
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -203,63 +208,30 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
           l += pr;
           pb[t * 2 + (i >> 3)][i & 7] = (__bf16)pr;
         }
+    }
+    if (more) {
+      deliver(K_, kb + 1, stage ^ 1);
+      request(V_, kb + 1);
+    }
+    if (busy) {
       // V operand of 16 keys (step u) and 32 channels: two transposing reads of 4 keys each for this lane's half
       const uint8_t* const vt = st + 64 * PITCH + (4 * h + ((lane & 15) >> 2)) * PITCH + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
       auto operand = [&](int dt, int u, int e) {
         return __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
             (__attribute__((address_space(3))) bf16x4*)(vt + (u * 16 + e * 8) * PITCH + dt * 64)));
       };
-      if (__builtin_expect(flags[stage] == kb, 0)) { // values that are not finite where some query misses a key
 #pragma unroll
-        for (int u = 0; u < 4; u++)
+      for (int u = 0; u < 4; u++)
 #pragma unroll
-          for (int dt = 0; dt < NJ; dt++) {
-            const i32x2 a = operand(dt, u, 0), b = operand(dt, u, 1);
-            const i32x4 w = {(int)mx4_finite((uint32_t)a[0]), (int)mx4_finite((uint32_t)a[1]), (int)mx4_finite((uint32_t)b[0]), (int)mx4_finite((uint32_t)b[1])};
-            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[dt], 0, 0, 0);
-          }
-        // the probabilities through the stage that nobody reads now, 32 keys at a time; -1: not seen
-        uint16_t* const mine = reinterpret_cast<uint16_t*>(lds + (stage ^ 1) * STAGE) + wave * 1024;
-#pragma unroll 1
-        for (int t = 0; t < 2; t++) {
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float x = t ? sc[1][i] : sc[0][i];
-            mine[((i & 3) + 8 * (i >> 2) + 4 * h) * 32 + c] = (uint16_t)f32_to_bf16_bits(x == -INFINITY ? -1.f : __builtin_amdgcn_exp2f((x - m) * unit));
-          }
-#pragma unroll 1
-          for (int key = 0; key < 32; key++) {
-            const float pv = bf16_bits_to_f32(mine[key * 32 + c]);
-            const uint16_t* vrow = reinterpret_cast<const uint16_t*>(st + 64 * PITCH + (t * 32 + key) * PITCH);
-#pragma unroll
-            for (int dt = 0; dt < NJ; dt++)
-#pragma unroll
-              for (int k = 0; k < 16; k++) {
-                const uint32_t w = vrow[dt * 32 + (k & 3) + 8 * (k >> 2) + 4 * h];
-                if ((w & 0x7f80u) == 0x7f80u && !(pv < 0.f))
-                  acc[dt][k] += pv * bf16_bits_to_f32(w);
-              }
-          }
+        for (int dt = 0; dt < NJ; dt++) {
+          const i32x2 a = operand(dt, u, 0), b = operand(dt, u, 1);
+          const i32x4 w = {a[0], a[1], b[0], b[1]};
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[dt], 0, 0, 0);
         }
-      } else {
-#pragma unroll
-        for (int u = 0; u < 4; u++)
-#pragma unroll
-          for (int dt = 0; dt < NJ; dt++) {
-            const i32x2 a = operand(dt, u, 0), b = operand(dt, u, 1);
-            const i32x4 w = {a[0], a[1], b[0], b[1]};
-            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[dt], 0, 0, 0);
-          }
-      }
     }
-    if (kb + 1 < tiles) {
-      if (__builtin_expect(flags[stage] == kb, 0))
-        __syncthreads(); // (the other stage was used)
-      deliver(kb + 1, stage ^ 1);
-    }
+    if (more)
+      deliver(V_, kb + 1, stage ^ 1);
   }
-  if (idle)
-    return;
   l += __shfl_xor(l, 32);
   if (q0 + c < o.n) {
     uint16_t* orow = p.out + ((int64_t)(o.start + q0 + c) * p.Nq + hq) * H;
@@ -271,6 +243,32 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
         const uint2 w = make_uint2(f32x2_to_bf16_bits(acc[dt][i] * inv, acc[dt][i + 1] * inv), f32x2_to_bf16_bits(acc[dt][i + 2] * inv, acc[dt][i + 3] * inv));
         *reinterpret_cast<uint2*>(orow + dt * 32 + 8 * (i >> 2) + 4 * h) = w;
       }
+    if (__builtin_expect(odd_values != 0, 0)) { // (a lane reads what it wrote itself)
+      const int from = mrow ? 0 : first_limit / 64 * 64;
+#pragma unroll 1
+      for (int d = 0; d < H; d += 8) {
+        uint16_t* const o4 = orow + d + 4 * h;
+        float f[4];
+        for (int e = 0; e < 4; e++)
+          f[e] = bf16_bits_to_f32(o4[e]);
+#pragma unroll 1
+        for (int key = from; key < limit; key++) {
+          if (mrow && key < p.mask_ld && bf16_bits_to_f32(mrow[key]) == -INFINITY)
+            continue;
+          for (int e = 0; e < 4; e++) {
+            uint32_t w;
+            if constexpr (CACHE)
+              w = vs[(int64_t)key * NJ + (d >> 5)] == 255 ? 0x7fc0u : 0u;
+            else
+              w = vr[(int64_t)key * p.v_ld + d + 4 * h + e];
+            if ((w & 0x7f80u) == 0x7f80u)
+              f[e] += bf16_bits_to_f32(w);
+          }
+        }
+        for (int e = 0; e < 4; e++)
+          o4[e] = (uint16_t)f32_to_bf16_bits(f[e]);
+      }
+    }
   }
 }
 
