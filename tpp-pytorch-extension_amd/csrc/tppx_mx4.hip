@@ -760,8 +760,8 @@ extern "C" int tppx_attn_packed(const void* q, const void* k, const void* v, con
   TPPX_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), TPPX_EINVAL, "%s: pointer not 16-byte aligned", who);
   if (int rc = attn_checks(who, T, B, Nq, Nkv, H, q_ld, mask, mask_ld))
     return rc;
-  TPPX_REQUIRE(k_ld >= Nkv * H && v_ld >= Nkv * H && (k_ld | v_ld) % 8 == 0, TPPX_ESHAPE,
-               "%s: row strides must be multiples of 8 elements and hold a row", who);
+  TPPX_REQUIRE(k_ld >= Nkv * H && v_ld >= Nkv * H && (k_ld | v_ld) % 8 == 0 && k_ld < (1 << 24) && v_ld < (1 << 24), TPPX_ESHAPE,
+               "%s: row strides must be multiples of 8 elements below 2^24 and hold a row", who);
   if (T == 0)
     return TPPX_OK;
   Mx4AttnParams p;

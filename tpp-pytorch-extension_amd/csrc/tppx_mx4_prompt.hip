@@ -4,12 +4,13 @@
 namespace tppx {
 
 // ---------------------------------------------------------------------------
-// Prompts: W waves of 32 queries of one head share K and V tiles of 64 keys, bf16 in LDS in two stages, from packed rows or
+// Prompts: QG groups of 32 queries of one head, each a wave, or with KT = 2 two that take half of every tile's keys (and are
+// merged at the end: launches of few workgroups), share K and V tiles of 64 keys, bf16 in LDS in two stages, from packed rows or
 // from the cache (its codes expanded once per workgroup on the way to LDS).  Both products run transposed on the 32 x 32 x 16
 // MFMA: scores^T[key][query] = K Q^T, out^T[channel][query] += V^T P^T; a lane holds 16 keys of one query in the score tile, and
 // those, rounded to bf16, are the second operand of the V product as they lie; V's operand is read by the transposing LDS read.
 // 32 queries per wave: an operand read from LDS feeds 32 columns, with 16 the LDS (128 bytes per cycle) would take twice the
-// MFMAs' time.  Scores in fp32, running maximum and sum per query, rescaled only in tiles where some maximum moves.
+// MFMAs' time.  Scores in fp32, running maximum and sum per query.
 // A key that a query does not see (a later token, a mask of -inf) adds nothing whatever it holds: its score is replaced, and in
 // tiles where some query misses a key values that are infinite or NaN become zeros on the way to LDS; a workgroup that met
 // such values adds them, one by one, to the outputs of the queries that see them once those are written.
@@ -22,16 +23,21 @@ __device__ __forceinline__ uint32_t mx4_finite(uint32_t pair) {
   return ((pair & 0x7f80u) == 0x7f80u ? 0u : pair & 0xffffu) | ((pair & 0x7f800000u) == 0x7f800000u ? 0u : pair & 0xffff0000u);
 }
 
-template <int NJ, int W, bool CACHE>
-__global__ void __launch_bounds__(W * 64, NJ <= 4 ? 2 : 1)
+// Pitch of a row in LDS.  K is read 16 bytes per lane, 16 rows at a time: rows 4 banks apart.  V is read 8 bytes per lane, 4 rows of
+// 64 bytes by 32 lanes: rows 16 banks apart (or 48); at K's pitch half of the cycles of LDS were bank conflicts.
+constexpr int mx4_k_pitch(int NJ) { return 64 * NJ + 16; }
+constexpr int mx4_v_pitch(int NJ) { return NJ % 4 == 3 ? 64 * NJ : 64 * NJ + 64; }
+
+template <int NJ, int QG, int KT, bool CACHE>
+__global__ void __launch_bounds__(QG * KT * 64, NJ <= 4 ? 2 : 1)
 mx4_prompt_kernel(const Mx4AttnParams p) {
-  constexpr int H = 32 * NJ, PITCH = 2 * H + 16, STAGE = 2 * 64 * PITCH; // K rows, then V rows
-  constexpr int QB = 32 * W, TH = 64 * W;
+  constexpr int H = 32 * NJ, KP = mx4_k_pitch(NJ), VP = mx4_v_pitch(NJ), STAGE = 64 * (KP + VP); // K rows, then V rows
+  constexpr int QB = 32 * QG, TH = 64 * QG * KT, NT = 2 / KT; // runs of 32 keys of a tile that a wave takes
   constexpr int PER = CACHE ? NJ : 4 * NJ, ITEMS = 64 * PER, NC = (ITEMS + TH - 1) / TH; // items of a row, of a tile, of a thread
   extern __shared__ __align__(16) uint8_t lds[]; // 2 stages
   __shared__ int odd_values;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % QG, team = __builtin_amdgcn_readfirstlane(tid >> 6) / QG;
   const int c = lane & 31, h = lane >> 5;
   // heads go round the XCDs, those of one K/V head to the same one
   const int hr = (int)blockIdx.x % p.Nq, hk = hr % p.Nkv, hq = hk * p.R + hr / p.Nkv;
@@ -64,30 +70,48 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   const int keys = min(past + min(qblk * QB + QB, o.n), total), tiles = (keys + 63) / 64;
   const int first_limit = min(past + qblk * QB + 1, total); // keys that all of them see
 
-  // Item i of thread tid: 16 bytes of a row of K (V false) or of V; rows past the keys: zeros.  One of the two at a time is on its
-  // way through registers: the next tile's K under this tile's scores, its V under this tile's output.
-  i32x4 item[NC];
-  uint32_t byte[CACHE ? NC : 1];
+  // Item i of thread tid: 16 bytes of a row of K (V false) or of V; rows past the keys: zeros.  They pass through registers, asked
+  // for a whole tile before they go to LDS.
+  i32x4 k_item[NC], v_item[NC];
+  uint32_t k_byte[CACHE ? NC : 1], v_byte[CACHE ? NC : 1];
+  // (buffers of a tile's rows: what lies past them reads as zero, with no branch and no access)
   auto request = [&](auto V_, int kb) {
     constexpr bool V = decltype(V_)::value;
+    auto& item = V ? v_item : k_item;
+    auto& byte = V ? v_byte : k_byte;
+    const int rows = min(max(keys - kb * 64, 0), 64);
+    auto rsrc = [](const void* at, uint32_t bytes) {
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, (int)bytes, 0x00020000);
+    };
+    if constexpr (CACHE) {
+      const auto codes = rsrc((V ? vq : kq) + (int64_t)kb * (64 * 16 * NJ), rows * (16 * NJ));
+      const auto scales = rsrc((V ? vs : ks) + (int64_t)kb * (64 * NJ), rows * NJ);
 #pragma unroll
-    for (int i = 0; i < NC; i++) {
-      const int at = i * TH + tid, row = at / PER, ch = at % PER, key = kb * 64 + row;
-      item[i] = i32x4{0, 0, 0, 0};
-      if constexpr (CACHE) {
-        byte[i] = 0;
-        if (at < ITEMS && key < keys) {
-          item[i] = *reinterpret_cast<const i32x4*>((V ? vq : kq) + (int64_t)key * (16 * NJ) + ch * 16);
-          byte[i] = (V ? vs : ks)[(int64_t)key * NJ + ch];
-        }
-      } else if (key < keys) {
-        item[i] = *reinterpret_cast<const i32x4*>((V ? vr + (int64_t)key * p.v_ld : kr + (int64_t)key * p.k_ld) + ch * 8);
+      for (int i = 0; i < NC; i++) {
+        const int at = i * TH + tid;
+        item[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(codes, at * 16, 0, 0));
+        byte[i] = __builtin_amdgcn_raw_buffer_load_b8(scales, at, 0, 0);
+      }
+    } else {
+      const int64_t ld = V ? p.v_ld : p.k_ld;
+      const auto src = rsrc((V ? vr : kr) + (int64_t)kb * 64 * ld, rows ? (uint32_t)(((rows - 1) * (uint32_t)ld + H) * 2) : 0u);
+#pragma unroll
+      for (int i = 0; i < NC; i++) {
+        const int at = i * TH + tid;
+        item[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(src, (at / PER) * ((uint32_t)ld * 2) + (at % PER) * 16, 0, 0));
       }
     }
   };
+  auto chunk_of = [](const i32x4& w, int j) { // (no indexed registers)
+    const int lo = j & 1 ? w[1] : w[0], hi = j & 1 ? w[3] : w[2];
+    return j & 2 ? hi : lo;
+  };
   auto deliver = [&](auto V_, int kb, int stage) {
     constexpr bool V = decltype(V_)::value;
-    uint8_t* const st = lds + stage * STAGE + (V ? 64 * PITCH : 0);
+    auto& item = V ? v_item : k_item;
+    auto& byte = V ? v_byte : k_byte;
+    uint8_t* const st = lds + stage * STAGE + (V ? 64 * KP : 0);
+    constexpr int PITCH = V ? VP : KP;
     const bool partial = V && (mrow || kb * 64 + 64 > first_limit); // (uniform)
     bool odd = false;
 #pragma unroll
@@ -100,8 +124,9 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
           odd |= drop;
           const float s = e8m0_to_f32(drop ? 0u : byte[i]);
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            *reinterpret_cast<bf16x8*>(dst + j * 16) = mx4_to_bf16(nan ? 0u : (uint32_t)item[i][j], s); // (zero times infinity)
+          for (int j = 0; j < 4; j++) // (V's rows are 16 banks apart, as a block's chunks are: another order of them in each row)
+            *reinterpret_cast<bf16x8*>(dst + (V ? (j ^ (row & 3)) * 16 : j * 16)) =
+                mx4_to_bf16(nan ? 0u : (uint32_t)(V ? chunk_of(item[i], j ^ (row & 3)) : item[i][j]), s); // (zero times infinity)
         }
       } else {
         if (partial) {
@@ -139,34 +164,34 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   if (tid == 0)
     odd_values = 0;
   request(K_, 0);
+  request(V_, 0);
   __syncthreads();
   deliver(K_, 0, 0);
-  request(V_, 0);
+  request(K_, 1);
   deliver(V_, 0, 0);
+  request(V_, 1);
   for (int kb = 0; kb < tiles; kb++) {
     const int stage = kb & 1;
     __syncthreads(); // this tile has been written, the other stage has been read
     const bool more = kb + 1 < tiles, busy = !idle && kb * 64 < wave_limit; // (uniform in a wave)
     const uint8_t* const st = lds + stage * STAGE;
-    if (more)
-      request(K_, kb + 1);
-    bf16x8 pb[4];
+    bf16x8 pb[2 * NT];
     if (busy) {
-      f32x16 sc[2];
+      f32x16 sc[NT];
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
+      for (int t = 0; t < NT; t++) {
 #pragma unroll
         for (int i = 0; i < 16; i++)
           sc[t][i] = 0.f;
 #pragma unroll
         for (int j = 0; j < 2 * NJ; j++)
-          sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(st + (t * 32 + c) * PITCH + j * 32 + h * 16), q[j], sc[t], 0, 0, 0);
+          sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(st + ((team + t) * 32 + c) * KP + j * 32 + h * 16), q[j], sc[t], 0, 0, 0);
       }
       // key of score i of run t
-      auto key_of = [&](int t, int i) { return kb * 64 + t * 32 + (i & 3) + 8 * (i >> 2) + 4 * h; };
+      auto key_of = [&](int t, int i) { return kb * 64 + (team + t) * 32 + (i & 3) + 8 * (i >> 2) + 4 * h; };
       if (mrow) {
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             const int key = key_of(t, i);
@@ -177,20 +202,22 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
       const bool partial = kb * 64 + 64 > min(past + q0 + 1, total); // (wave-uniform)
       if (partial) {
 #pragma unroll
-        for (int t = 0; t < 2; t++)
+        for (int t = 0; t < NT; t++)
 #pragma unroll
           for (int i = 0; i < 16; i++)
             sc[t][i] = key_of(t, i) < limit ? sc[t][i] : -INFINITY;
       }
       float mx = m;
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+      for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++)
           mx = fmaxf(mx, sc[t][i]);
       const float unit = mrow ? LOG2E : scale2;
       float alpha = 1.f;
-      if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
+      // The sums are relative to a maximum that follows the true one once that is 2^8 above it (the probabilities are then at most
+      // 2^8: their rounding is relative, and fp32 sums have the room); followed at once, nearly every tile would rescale.
+      if (__builtin_amdgcn_ballot_w64((mx - m) * unit > 8.f) != 0) {
         auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
         mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
         alpha = __builtin_amdgcn_exp2f((m - mx) * unit);
@@ -200,28 +227,35 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
         m = mx;
       }
       l *= alpha;
+      float off = -m * unit;
+      if (mrow) { // (the difference first: a mask's lowest value times log2 e is no number)
+        off = 0.f;
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+        for (int t = 0; t < NT; t++)
+          sc[t] -= m;
+      }
+#pragma unroll
+      for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const float pr = __builtin_amdgcn_exp2f((sc[t][i] - m) * unit);
+          const float pr = __builtin_amdgcn_exp2f(fmaf(sc[t][i], unit, off));
           l += pr;
           pb[t * 2 + (i >> 3)][i & 7] = (__bf16)pr;
         }
     }
     if (more) {
       deliver(K_, kb + 1, stage ^ 1);
-      request(V_, kb + 1);
+      request(K_, kb + 2);
     }
     if (busy) {
       // V operand of 16 keys (step u) and 32 channels: two transposing reads of 4 keys each for this lane's half
-      const uint8_t* const vt = st + 64 * PITCH + (4 * h + ((lane & 15) >> 2)) * PITCH + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+      const uint8_t* const vt = st + 64 * KP + (team * 32 + 4 * h + ((lane & 15) >> 2)) * VP + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
       auto operand = [&](int dt, int u, int e) {
         return __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-            (__attribute__((address_space(3))) bf16x4*)(vt + (u * 16 + e * 8) * PITCH + dt * 64)));
+            (__attribute__((address_space(3))) bf16x4*)(vt + (u * 16 + e * 8) * VP + dt * 64)));
       };
 #pragma unroll
-      for (int u = 0; u < 4; u++)
+      for (int u = 0; u < 2 * NT; u++)
 #pragma unroll
         for (int dt = 0; dt < NJ; dt++) {
           const i32x2 a = operand(dt, u, 0), b = operand(dt, u, 1);
@@ -229,10 +263,38 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
           acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[dt], 0, 0, 0);
         }
     }
-    if (more)
+    if (more) {
       deliver(V_, kb + 1, stage ^ 1);
+      request(V_, kb + 2);
+    }
   }
   l += __shfl_xor(l, 32);
+  if constexpr (KT > 1) { // the second team's state through LDS
+    float* const at = reinterpret_cast<float*>(lds) + (wave * 64 + lane) * 4;
+    constexpr int STEP = QG * 64 * 4;
+    const float unit = mrow ? LOG2E : scale2;
+    __syncthreads(); // the stages have been read
+    if (team) {
+#pragma unroll
+      for (int k = 0; k < 4 * NJ; k++)
+        *reinterpret_cast<f32x4*>(at + k * STEP) = f32x4{acc[k >> 2][(k & 3) * 4], acc[k >> 2][(k & 3) * 4 + 1], acc[k >> 2][(k & 3) * 4 + 2], acc[k >> 2][(k & 3) * 4 + 3]};
+      at[4 * NJ * STEP] = m;
+      at[4 * NJ * STEP + 1] = l;
+    }
+    __syncthreads();
+    if (team)
+      return;
+    const float m1 = at[4 * NJ * STEP], mm = fmaxf(m, m1);
+    const float a = __builtin_amdgcn_exp2f((m - mm) * unit), b = __builtin_amdgcn_exp2f((m1 - mm) * unit);
+    l = l * a + at[4 * NJ * STEP + 1] * b;
+#pragma unroll
+    for (int k = 0; k < 4 * NJ; k++) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(at + k * STEP);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        acc[k >> 2][(k & 3) * 4 + e] = acc[k >> 2][(k & 3) * 4 + e] * a + v[e] * b;
+    }
+  }
   if (q0 + c < o.n) {
     uint16_t* orow = p.out + ((int64_t)(o.start + q0 + c) * p.Nq + hq) * H;
     const float inv = l != 0.f ? 1.0f / l : 0.f; // (nothing seen: zeros)
@@ -281,19 +343,19 @@ int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache
   hipError_t e = hipSuccess;
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
-    auto go = [&](auto w, auto c) {
-      constexpr int W = decltype(w)::value;
-      auto kern = mx4_prompt_kernel<NJ, W, decltype(c)::value>;
-      const size_t lds = 2 * 2 * 64 * (size_t)(64 * NJ + 16);
+    auto go = [&](auto qg, auto c) {
+      constexpr int QG = decltype(qg)::value;
+      auto kern = mx4_prompt_kernel<NJ, QG, 4 / QG, decltype(c)::value>;
+      const size_t lds = 2 * 64 * (size_t)(mx4_k_pitch(NJ) + mx4_v_pitch(NJ));
       e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
       if (e == hipSuccess)
-        kern<<<dim3((unsigned)wgs), dim3(W * 64), lds, stream>>>(p);
+        kern<<<dim3((unsigned)wgs), dim3(256), lds, stream>>>(p);
     };
-    auto with_source = [&](auto w) {
+    auto with_source = [&](auto qg) {
       if (cache)
-        go(w, std::true_type{});
+        go(qg, std::true_type{});
       else
-        go(w, std::false_type{});
+        go(qg, std::false_type{});
     };
     if (wide)
       with_source(std::integral_constant<int, 4>{});
