@@ -178,6 +178,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
     bf16x8 pb[2 * NT];
     if (busy) {
       f32x16 sc[NT];
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < NT; t++) {
 #pragma unroll
@@ -187,6 +188,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
         for (int j = 0; j < 2 * NJ; j++)
           sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(st + ((team + t) * 32 + c) * KP + j * 32 + h * 16), q[j], sc[t], 0, 0, 0);
       }
+      __builtin_amdgcn_s_setprio(0);
       // key of score i of run t
       auto key_of = [&](int t, int i) { return kb * 64 + (team + t) * 32 + (i & 3) + 8 * (i >> 2) + 4 * h; };
       if (mrow) {
@@ -254,6 +256,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
         return __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
             (__attribute__((address_space(3))) bf16x4*)(vt + (u * 16 + e * 8) * VP + dt * 64)));
       };
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int u = 0; u < 2 * NT; u++)
 #pragma unroll
@@ -263,6 +266,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
           acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[dt], 0, 0, 0);
         }
     }
+    __builtin_amdgcn_s_setprio(0);
     if (more) {
       deliver(V_, kb + 1, stage ^ 1);
       request(V_, kb + 2);
