@@ -89,6 +89,8 @@ struct Mx4AttnParams {
 constexpr int MX4_COUNTER_STRIDE = 64; // arrival counters are 256 bytes apart
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x3 __attribute__((ext_vector_type(3)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef short i16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 

@@ -262,16 +262,17 @@ constexpr int mx4_scale_bytes() { // scale bytes of a lane's channels of a key: 
   return NJ % 4 == 0 ? NJ / 4 : NJ <= 2 ? 1 : NJ;
 }
 
-template <int NJ, int W, bool MASK>
+template <int NJ, int W, bool MASK, bool STREAM>
 __global__ void __launch_bounds__(W * 64)
 mx4_split_kernel(const Mx4AttnParams p) {
   constexpr int H = 32 * NJ, RB = 16 * NJ;          // bytes of a row's codes
   constexpr int PITCH = RB + 16;                     // of a row in LDS: 16 rows of a group on different banks
-  constexpr int SD = NJ > 4 ? 2 : 1;                 // dwords of a row's scales in LDS
-  constexpr int WAVE_LDS = 64 * PITCH + 64 * SD * 4; // per wave
+  constexpr int SD = NJ > 4 ? 2 : 1;                 // dwords of a row's scales in registers
+  constexpr int WAVE_LDS = 64 * PITCH + 128 * NJ;    // per wave: codes of the rows, exponents [block][row]
   constexpr int OP = H + 4;                          // pitch of a merged output row in floats
   constexpr int MERGE = (W * 16 * OP + W * 32) * 4, LDS = W * WAVE_LDS > MERGE ? W * WAVE_LDS : MERGE;
   constexpr int NS = mx4_scale_bytes<NJ>();
+  constexpr int AUX = STREAM ? 2 : 0; // codes with the non-temporal hint
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ float merged[16][33]; // weights of the splits, then the sum
   __shared__ int arrived_last;
@@ -282,12 +283,14 @@ mx4_split_kernel(const Mx4AttnParams p) {
   Block o;
   if (!locate(p.cu, p.B, p.T, p.R, 16, (int)blockIdx.x / p.Nkv, o))
     return;
-  const int S = p.splits;
   const int ncol = min(16, o.n * p.R - o.at * 16); // of this workgroup
   const int col = o.at * 16 + min(c, ncol - 1), tok = col / p.R, r0 = col - tok * p.R;
   const int past = p.past[o.b];
   const int limit = min(max(past + tok + 1, 0), p.Smax); // keys this lane's column sees
   const int L = min(max(past + (o.at * 16 + ncol - 1) / p.R + 1, 0), p.Smax);
+  const int S = max(min(p.splits, (L + W * 64 - 1) / (W * 64)), 1); // splits that have keys; the others take no part
+  if ((int)blockIdx.y >= S)
+    return;
 
   const int64_t head = ((int64_t)o.b * p.Nkv + hk) * p.Smax;
   const uint8_t* const kq = p.kq + head * RB;
@@ -306,42 +309,61 @@ mx4_split_kernel(const Mx4AttnParams p) {
   uint32_t kc[4][NJ], kb[4][NS]; // keys of the tile: codes and scale bytes
   i32x4 vc[NJ];                  // values: 16-byte chunks i * 64 + lane of the tile's rows
   uint32_t vb[SD];               // scales of the value of key `lane`
-  const int64_t vend = (int64_t)p.Smax * RB - 16;
-  auto request_k = [&](int base) { // rows past the cache's end repeat its last one
+  // (buffers of the tile's rows: what lies past the cache's end reads as zero, with no branch and no access)
+  auto rsrc = [](const uint8_t* at, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(at), 0, bytes, 0x00020000);
+  };
+  auto request_k = [&](int base) {
+    const int rows = min(max(p.Smax - base, 0), 64);
+    const auto codes = rsrc(kq + (int64_t)base * RB, rows * RB);
+    const auto scales = rsrc(ks + (int64_t)base * NJ, rows * NJ);
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      const int key = min(base + t * 16 + c, p.Smax - 1);
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(kq + (int64_t)key * RB + g * (4 * NJ));
+      const int at = (t * 16 + c) * RB + g * (4 * NJ);
+      if constexpr (NJ == 2 || NJ == 6) {
+        const i32x2 w = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(codes, at, 0, AUX));
+        kc[t][0] = (uint32_t)w[0];
+        kc[t][1] = (uint32_t)w[1];
+      } else if constexpr (NJ == 3) {
+        const i32x3 w = __builtin_bit_cast(i32x3, __builtin_amdgcn_raw_buffer_load_b96(codes, at, 0, AUX));
+        kc[t][0] = (uint32_t)w[0];
+        kc[t][1] = (uint32_t)w[1];
+        kc[t][2] = (uint32_t)w[2];
+      }
 #pragma unroll
-      for (int j = 0; j < NJ; j++)
-        kc[t][j] = src[j];
-      const uint8_t* sb = ks + (int64_t)key * NJ;
+      for (int j = NJ % 4 == 3 ? NJ : NJ % 4; j + 4 <= NJ; j += 4) {
+        const i32x4 w = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(codes, at + j * 4, 0, AUX));
+#pragma unroll
+        for (int d = 0; d < 4; d++)
+          kc[t][j + d] = (uint32_t)w[d];
+      }
 #pragma unroll
       for (int j = 0; j < NS; j++)
-        kb[t][j] = sb[NJ % 4 == 0 ? g * NS + j : (g * NJ + j) >> 2];
+        kb[t][j] = __builtin_amdgcn_raw_buffer_load_b8(scales, (t * 16 + c) * NJ + (NJ % 4 == 0 ? g * NS + j : (g * NJ + j) >> 2), 0, 0);
     }
   };
   auto request_v = [&](int base) {
-    const int64_t at = (int64_t)base * RB + lane * 16;
+    const int rows = min(max(p.Smax - base, 0), 64);
+    const auto codes = rsrc(vq + (int64_t)base * RB, rows * RB);
+    const auto scales = rsrc(vs + (int64_t)base * NJ, rows * NJ);
 #pragma unroll
     for (int i = 0; i < NJ; i++)
-      vc[i] = *reinterpret_cast<const i32x4*>(vq + min(at + i * 1024, vend));
-    const uint8_t* sb = vs + (int64_t)min(base + lane, p.Smax - 1) * NJ;
+      vc[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(codes, (i * 64 + lane) * 16, 0, AUX));
     if constexpr (NJ == 4) {
-      vb[0] = *reinterpret_cast<const uint32_t*>(sb);
+      vb[0] = __builtin_amdgcn_raw_buffer_load_b32(scales, lane * 4, 0, 0);
     } else if constexpr (NJ == 8) {
-      const i32x2 w = *reinterpret_cast<const i32x2*>(sb);
-      vb[0] = w[0];
-      vb[1] = w[1];
+      const i32x2 w = __builtin_bit_cast(i32x2, __builtin_amdgcn_raw_buffer_load_b64(scales, lane * 8, 0, 0));
+      vb[0] = (uint32_t)w[0];
+      vb[1] = (uint32_t)w[1];
     } else if constexpr (NJ == 2) {
-      vb[0] = *reinterpret_cast<const uint16_t*>(sb);
+      vb[0] = __builtin_amdgcn_raw_buffer_load_b16(scales, lane * 2, 0, 0);
     } else {
 #pragma unroll
       for (int j = 0; j < SD; j++)
         vb[j] = 0;
 #pragma unroll
       for (int j = 0; j < NJ; j++)
-        vb[j >> 2] |= (uint32_t)sb[j] << (8 * (j & 3));
+        vb[j >> 2] |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(scales, lane * NJ + j, 0, 0) << (8 * (j & 3));
     }
   };
 
@@ -354,7 +376,7 @@ mx4_split_kernel(const Mx4AttnParams p) {
   for (int dt = 0; dt < 2 * NJ; dt++)
     acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   const bf16x8 ones = {(__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f, (__bf16)1.f};
-  const float scale2 = p.scale * LOG2E;
+  const float to2 = MASK ? LOG2E : p.scale * LOG2E; // of a score in powers of two
 
   const int step = S * W * 64;
   int base = ((int)blockIdx.y * W + wave) * 64;
@@ -379,7 +401,7 @@ mx4_split_kernel(const Mx4AttnParams p) {
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; i++)
-      x[i] = sc[i >> 2][i & 3] * (MASK ? p.scale : scale2);
+      x[i] = MASK ? sc[i >> 2][i & 3] * p.scale : sc[i >> 2][i & 3];
     if (MASK) {
 #pragma unroll
       for (int i = 0; i < 16; i++) {
@@ -397,22 +419,25 @@ mx4_split_kernel(const Mx4AttnParams p) {
 #pragma unroll
     for (int i = 0; i < 16; i++)
       mx = fmaxf(mx, x[i]);
-    if (__builtin_amdgcn_ballot_w64(mx > m) != 0) { // some column's maximum moves
+    // The sums are relative to a maximum that follows the true one once that is 2^8 above it: the probabilities are then at most
+    // 2^8, their rounding is relative, and the fp32 sums have the room.
+    if (__builtin_amdgcn_ballot_w64((mx - m) * to2 > 8.f) != 0) {
       mx = max_of_groups(mx);
-      const float alpha = __builtin_amdgcn_exp2f(MASK ? (m - mx) * LOG2E : m - mx);
+      const float alpha = __builtin_amdgcn_exp2f((m - mx) * to2);
 #pragma unroll
       for (int dt = 0; dt < 2 * NJ; dt++)
         acc[dt] *= alpha;
       sum *= alpha;
       m = mx;
     }
+    const float off = -m * to2;
     uint32_t pr[8]; // bf16 pairs, slots 2 e, 2 e + 1
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
+    for (int e = 0; e < 8; e++) { // (with a mask the difference first: its lowest value times log2 e is no number)
       float f[2];
 #pragma unroll
       for (int h = 0; h < 2; h++)
-        f[h] = __builtin_amdgcn_exp2f(MASK ? (x[2 * e + h] - m) * LOG2E : x[2 * e + h] - m);
+        f[h] = __builtin_amdgcn_exp2f(MASK ? (x[2 * e + h] - m) * to2 : fmaf(x[2 * e + h], to2, off));
       pr[e] = f32x2_to_bf16_bits(f[0], f[1]);
     }
 #pragma unroll
@@ -433,49 +458,50 @@ mx4_split_kernel(const Mx4AttnParams p) {
       const int ch = i * 64 + lane;
       *reinterpret_cast<i32x4*>(mine + place(ch / NJ) * PITCH + (ch % NJ) * 16) = vc[i];
     }
+    {
+      // a scale as what it adds to the bits of a bf16; rows past the keys may hold anything: what makes every sum negative
+      uint16_t* const dst = reinterpret_cast<uint16_t*>(mine + 64 * PITCH) + place(lane);
+      const bool live = base + lane < L;
 #pragma unroll
-    for (int j = 0; j < SD; j++) // (rows past the keys may hold anything)
-      reinterpret_cast<uint32_t*>(mine + 64 * PITCH)[place(lane) * SD + j] = base + lane < L ? vb[j] : 0u;
+      for (int bl = 0; bl < NJ; bl++)
+        dst[bl * 64] = (uint16_t)(live ? ((vb[bl >> 2] >> (8 * (bl & 3))) & 0xffu) * 128u - 127u * 128u : 0x8000u);
+    }
     if (more)
       request_v(base + step);
-    uint32_t sd[16][SD];
-    {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(mine + 64 * PITCH) + g * 16 * SD;
-#pragma unroll
-      for (int i = 0; i < 16; i++)
-#pragma unroll
-        for (int j = 0; j < SD; j++)
-          sd[i][j] = src[i * SD + j];
-    }
+    const i32x4* const exps = reinterpret_cast<const i32x4*>(mine + 64 * PITCH) + g * 2; // [block][8]: of this group's 16 rows
     if (__builtin_amdgcn_ballot_w64(odd) != 0) { // a block of NaN: into the columns that see its key
 #pragma unroll
       for (int bl = 0; bl < NJ; bl++) {
         int bad = 0;
 #pragma unroll
         for (int i = 0; i < 16; i++)
-          bad |= ((sd[i][bl >> 2] >> (8 * (bl & 3))) & 0xffu) == 255u && x[i] != -INFINITY;
+          bad |= reinterpret_cast<const uint16_t*>(exps + bl * 8)[i] == 128 * 128 && x[i] != -INFINITY;
         bad |= __shfl_xor(bad, 16);
         bad |= __shfl_xor(bad, 32);
         if (bad)
           acc[2 * bl] = acc[2 * bl + 1] = f32x4{NAN, NAN, NAN, NAN};
       }
     }
-    i16x2 pe[8], nz[8];
+    // A probability of zero as the lowest integer, so that no scale lifts it; the sums saturate, negative ones are zero.
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      pe[e] = __builtin_bit_cast(i16x2, pr[e]) - (short)(127 * 128);
-      nz[e] = __builtin_bit_cast(i16x2, pr[e]) != i16x2{0, 0};
+      uint32_t some; // 1 where it is not zero (the compiler makes conditions of it)
+      asm("v_pk_min_u16 %0, %1, %2" : "=v"(some) : "v"(pr[e]), "s"(0x00010001u));
+      asm("v_pk_mad_u16 %0, %1, %2, %3" : "=v"(pr[e]) : "v"(some), "s"(0x80008000u), "v"(pr[e] ^ 0x80008000u));
     }
     const uint8_t* const vrow = mine + (g * 16 + c) * PITCH;
 #pragma unroll
     for (int bl = 0; bl < NJ; bl++) {
       i32x4 w[2];
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        constexpr uint32_t SEL = 0x0c040c00u;
-        const uint32_t s = __builtin_amdgcn_perm(sd[2 * e + 1][bl >> 2], sd[2 * e][bl >> 2], SEL + 0x00010001u * (bl & 3));
-        const i16x2 t = __builtin_elementwise_max(__builtin_bit_cast(i16x2, s) * (short)128 + pe[e], i16x2{0, 0});
-        w[e >> 2][e & 3] = __builtin_bit_cast(int, t & nz[e]);
+      for (int h = 0; h < 2; h++) {
+        const i32x4 ex = exps[bl * 8 + h];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t t;
+          asm("v_pk_add_i16 %0, %1, %2 clamp" : "=v"(t) : "v"(ex[e]), "v"(pr[h * 4 + e]));
+          w[h][e] = __builtin_bit_cast(int, __builtin_elementwise_max(__builtin_bit_cast(i16x2, t), i16x2{0, 0}));
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; h++) {
@@ -486,8 +512,7 @@ mx4_split_kernel(const Mx4AttnParams p) {
       }
     }
   }
-  if (!MASK)
-    m *= 1.0f / LOG2E; // natural units, as with a mask
+  m = m == LOWEST ? LOWEST : MASK ? m : m * p.scale; // natural units
 
   // the waves' states through LDS
   __syncthreads();
@@ -495,14 +520,15 @@ mx4_split_kernel(const Mx4AttnParams p) {
   float* const sm = mo + W * 16 * OP;              // [wave][col] maximum, then sum
 #pragma unroll
   for (int dt = 0; dt < 2 * NJ; dt++)
-    *reinterpret_cast<f32x4*>(mo + (wave * 16 + c) * OP + dt * 16 + g * 4) = acc[dt];
+    if (c < ncol)
+      *reinterpret_cast<f32x4*>(mo + (wave * 16 + c) * OP + dt * 16 + g * 4) = acc[dt];
   if (g == 0) {
     sm[wave * 16 + c] = m;
     sm[W * 16 + wave * 16 + c] = sum[0];
   }
   __syncthreads();
   float* const part_o = p.part;
-  float* const part_ml = p.part + (int64_t)gridDim.x * S * p.cols * H;
+  float* const part_ml = p.part + (int64_t)gridDim.x * p.splits * p.cols * H;
   const int64_t unit = blockIdx.x;
   auto store4 = [&](int cc, int d4, f32x4 v, float Ls) {
     const int cl = o.at * 16 + cc, tk = cl / p.R, rr = cl - tk * p.R;
@@ -534,7 +560,7 @@ mx4_split_kernel(const Mx4AttnParams p) {
       continue;
     }
     // device-scope stores: written through to the level that all XCDs share
-    const int64_t at = (unit * S + blockIdx.y) * p.cols + cc;
+    const int64_t at = (unit * p.splits + blockIdx.y) * p.cols + cc;
     uint64_t* const dst = reinterpret_cast<uint64_t*>(part_o + at * H + d4 * 4);
     __hip_atomic_store(dst, __builtin_bit_cast(uint64_t, make_float2(v[0], v[1])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(dst + 1, __builtin_bit_cast(uint64_t, make_float2(v[2], v[3])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -559,7 +585,7 @@ mx4_split_kernel(const Mx4AttnParams p) {
     const int cc = i >> 5, s = i & 31;
     float2 ml = {LOWEST, 0.f};
     if (s < S)
-      ml = load2(part_ml + ((unit * S + s) * p.cols + cc) * 2);
+      ml = load2(part_ml + ((unit * p.splits + s) * p.cols + cc) * 2);
     float M = ml.x;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2)
@@ -576,7 +602,7 @@ mx4_split_kernel(const Mx4AttnParams p) {
   __syncthreads();
   for (int i = tid; i < ncol * (H / 4); i += W * 64) {
     const int cc = i / (H / 4), d4 = i % (H / 4);
-    const float* src = part_o + (unit * S * p.cols + cc) * H + d4 * 4;
+    const float* src = part_o + (unit * p.splits * p.cols + cc) * H + d4 * 4;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < S; s0 += 8) { // eight splits' loads in flight
       float2 a[8][2];
@@ -644,19 +670,38 @@ static int split_launch(const char* who, Mx4AttnParams& p, int H, void* ws, int6
   TPPX_REQUIRE(units < ((int64_t)1 << 31), TPPX_ESHAPE, "%s: problem too large", who);
   p.cols = p.cu ? 16 : std::min(16, p.R);
   const int64_t trips = ((int64_t)p.Smax + W * 64 - 1) / (W * 64);
-  int64_t S = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(trips, 32), 768 / units));
+  // 512 workgroups, two per CU: 32 x 16000 keys of 8 K/V heads (256 units) 88.5 us with two splits, 93 with three, 105 with four;
+  // 8 x 3000 of 16, 256 wide (128) 23.4 with two, 24.0 with four, 26.9 with twelve; 1 x 2048 of 32 (32) 12.6 with one, 7.8 with four,
+  // 6.9 with eight; 1 x 16000 of 8 (8) 73 with one, 11.0 with 32; 16 x 2048 of 32 (512) 25.2 with one, 28.9 with two.  Splits beyond
+  // a sequence's keys end at once.
+  int64_t S = env_int("TPPX_MX4_SPLITS", 0);
+  if (S <= 0)
+    S = 512 / units;
+  S = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(trips, 32), S));
   if (!ws || units * S * p.cols * (H + 2) * (int64_t)sizeof(float) > ws_bytes || units * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) > counter_bytes)
     S = 1;
   p.splits = (int)S;
   p.part = (float*)ws;
   p.counters = (unsigned int*)counters;
   const dim3 grid((unsigned)units, (unsigned)S);
+  // A layer past the 256 MiB of the last-level cache cannot be there from a launch before: its codes go by without being kept (558 MB
+  // 102 -> 88.5 us, 6.3 TB/s); smaller ones may be (40 MB 12.3 us, with the hint 13.4; 143 MB 25.2 and 24.8).
+  const bool stream_codes = (int64_t)p.B * p.Nkv * p.Smax * H >= ((int64_t)256 << 20);
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
+    auto go = [&](auto m, auto st) {
+      mx4_split_kernel<NJ, W, decltype(m)::value, decltype(st)::value><<<grid, dim3(W * 64), 0, stream>>>(p);
+    };
+    auto with_mask = [&](auto m) {
+      if (stream_codes)
+        go(m, std::true_type{});
+      else
+        go(m, std::false_type{});
+    };
     if (p.mask)
-      mx4_split_kernel<NJ, W, true><<<grid, dim3(W * 64), 0, stream>>>(p);
+      with_mask(std::true_type{});
     else
-      mx4_split_kernel<NJ, W, false><<<grid, dim3(W * 64), 0, stream>>>(p);
+      with_mask(std::false_type{});
   });
   return check_hip(hipGetLastError(), who);
 }

@@ -24,6 +24,16 @@ Mx4Layer = namedtuple("Mx4Layer", "k_codes k_scales v_codes v_scales")
 HEAD_SIZES = (64, 96, 128, 192, 256)
 
 
+def _run(t, fn, *args):
+    """A call of the library on t's device and its current stream (the last argument)."""
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev)))
+
+
 def _rows(t, name, like=None):
     """Packed rows of heads: bf16 [T][heads][H] on the GPU (`like`: on that tensor's), heads of a row side by side; other
     strides are copied."""
@@ -32,8 +42,9 @@ def _rows(t, name, like=None):
                                      f"{tuple(t.shape)} {t.dtype} on {t.device}")
     if like is not None and t.get_device() != like.get_device():
         raise TppxError(_lib.EINVAL, f"{name} is on {t.device}, not on {like.device}")
-    s = t.stride()
-    if s[2] != 1 or (s[1] != t.shape[2] and t.shape[1] != 1) or s[0] % 8 or s[0] < t.shape[1] * t.shape[2] or t.data_ptr() & 15:
+    _, n, h = t.shape
+    a, b, c = t.stride()
+    if c != 1 or (b != h and n != 1) or a % 8 or a < n * h or t.data_ptr() & 15:
         return t.contiguous() if not t.is_contiguous() else t.clone()
     return t
 
@@ -96,13 +107,12 @@ def qk_norm_rotary(q, k, q_weight=None, k_weight=None, eps=1e-6, emb_pos=None, p
     if table is not None and pos is None:
         raise TppxError(_lib.EINVAL, "qk_norm_rotary: a rotation needs the positions")
     at = _index(pos, "pos", T, q, torch.int64) if pos is not None else None
-    qo = torch.empty((T, Nq, H), dtype=q.dtype, device=q.device)
-    ko = torch.empty((T, k.shape[1], H), dtype=q.dtype, device=q.device)
+    qo = q.new_empty((T, Nq, H))
+    ko = q.new_empty((T, k.shape[1], H))
     if T == 0:
         return qo, ko
-    with torch.cuda.device_of(q):
-        _lib.check(_lib.lib().tppx_qk_norm_rotary(q.data_ptr(), k.data_ptr(), gq, gk, gdt, eps, table, gptj, at, qo.data_ptr(), ko.data_ptr(),
-                                                  T, Nq, k.shape[1], H, q.stride(0), k.stride(0), MP, HR, _lib.stream_of(q)))
+    _run(q, _lib.lib().tppx_qk_norm_rotary, q.data_ptr(), k.data_ptr(), gq, gk, gdt, eps, table, gptj, at, qo.data_ptr(), ko.data_ptr(),
+         T, Nq, k.shape[1], H, q.stride(0), k.stride(0), MP, HR)
     return qo, ko
 
 
@@ -110,10 +120,13 @@ def _layer(layer, B, Nkv, H, like):
     """Addresses and capacity of a cache layer, checked."""
     kc, ks, vc, vs = layer
     cap = kc.shape[2] if kc.dim() == 4 else 0
-    for name, t, w in (("key codes", kc, H // 2), ("key scales", ks, H // 32), ("value codes", vc, H // 2), ("value scales", vs, H // 32)):
-        if t.shape != (B, Nkv, cap, w) or t.dtype != torch.uint8 or not t.is_contiguous() or t.get_device() != like.get_device() or cap == 0:
-            raise TppxError(_lib.ESHAPE, f"cache layer: {name} must be a contiguous uint8 tensor [{B}][{Nkv}][capacity][{w}] on "
-                                         f"{like.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    codes, scales, dev, u8 = (B, Nkv, cap, H // 2), (B, Nkv, cap, H // 32), like.get_device(), torch.uint8
+    if (cap == 0 or kc.shape != codes or vc.shape != codes or ks.shape != scales or vs.shape != scales
+            or kc.dtype != u8 or vc.dtype != u8 or ks.dtype != u8 or vs.dtype != u8
+            or not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous())
+            or kc.get_device() != dev or vc.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev):
+        raise TppxError(_lib.ESHAPE, f"cache layer: contiguous uint8 tensors [{B}][{Nkv}][capacity][{H // 2}] (codes) and [{H // 32}] (scales) of "
+                                     f"keys and values on {like.device} are wanted, got {[(tuple(t.shape), t.dtype, t.device) for t in layer]}")
     return kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), cap
 
 
@@ -141,28 +154,25 @@ def append_mx4(q, k, v, layer, past, cu_seqlens=None, q_weight=None, k_weight=No
     T, Nkv, H = k.shape
     if v.shape != k.shape:
         raise TppxError(_lib.ESHAPE, f"append_mx4: k {tuple(k.shape)} and v {tuple(v.shape)}")
-    Nq = 0
-    qo = None
+    Nq = q_ld = 0
+    q_at = qo = None
     if q is not None:
         q = _rows(q, "q", k)
         Nq = q.shape[1]
         if q.shape[0] != T or q.shape[2] != H:
             raise TppxError(_lib.ESHAPE, f"append_mx4: q {tuple(q.shape)} and k {tuple(k.shape)}")
-        qo = torch.empty((T, Nq, H), dtype=k.dtype, device=k.device)
+        q_at, q_ld, qo = q.data_ptr(), q.stride(0), k.new_empty((T, Nq, H))
     B, past_at, cu_at = _sequences(T, past, cu_seqlens, k)
     kc, ks, vc, vs, cap = _layer(layer, B, Nkv, H, k)
     gq, gk, gdt = _norm_weights(q_weight, k_weight, H, k)
     table, gptj, MP, HR = _rotation(emb_pos, style, H, k)
     at = _index(pos, "pos", T, k, torch.int64) if pos is not None else None
-    ko = torch.empty((T, Nkv, H), dtype=k.dtype, device=k.device) if values else None
-    vo = torch.empty((T, Nkv, H), dtype=k.dtype, device=k.device) if values else None
+    ko = k.new_empty((T, Nkv, H)) if values else None
+    vo = k.new_empty((T, Nkv, H)) if values else None
     if T == 0:
         return qo, ko, vo
-    with torch.cuda.device_of(k):
-        _lib.check(_lib.lib().tppx_append_mx4(
-            None if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), gq, gk, gdt, eps, table, gptj, at, kc, ks, vc, vs, past_at, cu_at,
-            _lib.ptr(qo), _lib.ptr(ko), _lib.ptr(vo), T, B, Nq, Nkv, H, cap, 0 if q is None else q.stride(0), k.stride(0), v.stride(0),
-            MP, HR, _lib.stream_of(k)))
+    _run(k, _lib.lib().tppx_append_mx4, q_at, k.data_ptr(), v.data_ptr(), gq, gk, gdt, eps, table, gptj, at, kc, ks, vc, vs, past_at, cu_at,
+         _lib.ptr(qo), _lib.ptr(ko), _lib.ptr(vo), T, B, Nq, Nkv, H, cap, q_ld, k.stride(0), v.stride(0), MP, HR)
     return qo, ko, vo
 
 
@@ -185,13 +195,12 @@ def attn_mx4(q, layer, past, cu_seqlens=None, mask=None):
     Nkv = layer[0].shape[1] if layer[0].dim() == 4 else 0
     kc, ks, vc, vs, cap = _layer(layer, B, Nkv, H, q)
     m_at, m_ld = _mask(mask, B, q)
-    out = torch.empty((T, Nq, H), dtype=q.dtype, device=q.device)
+    out = q.new_empty((T, Nq, H))
     if T == 0:
         return out
-    with torch.cuda.device_of(q):
-        st = _lib.stream_of(q)
-        _lib.check(_lib.lib().tppx_attn_mx4(q.data_ptr(), kc, ks, vc, vs, past_at, cu_at, m_at, m_ld, out.data_ptr(), T, B, Nq, Nkv, H, cap,
-                                            q.stride(0), *_lib.with_counters(_lib.workspace(q, st)), st))
+    ws, ws_bytes, counters, counter_bytes = _lib.with_counters(_lib.workspace(q))
+    _run(q, _lib.lib().tppx_attn_mx4, q.data_ptr(), kc, ks, vc, vs, past_at, cu_at, m_at, m_ld, out.data_ptr(), T, B, Nq, Nkv, H, cap, q.stride(0),
+         ws, ws_bytes, counters, counter_bytes)
     return out
 
 
@@ -209,10 +218,9 @@ def attn_packed(q, k, v, cu_seqlens, mask=None):
         raise TppxError(_lib.ESHAPE, f"cu_seqlens must be int32 [sequences + 1], got {tuple(cu_seqlens.shape)}")
     cu_at = _index(cu_seqlens, "cu_seqlens", B + 1, q)
     m_at, m_ld = _mask(mask, B, q)
-    out = torch.empty((T, Nq, H), dtype=q.dtype, device=q.device)
+    out = q.new_empty((T, Nq, H))
     if T == 0:
         return out
-    with torch.cuda.device_of(q):
-        _lib.check(_lib.lib().tppx_attn_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_at, m_at, m_ld, out.data_ptr(), T, B, Nq,
-                                               k.shape[1], H, q.stride(0), k.stride(0), v.stride(0), _lib.stream_of(q)))
+    _run(q, _lib.lib().tppx_attn_packed, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_at, m_at, m_ld, out.data_ptr(), T, B, Nq, k.shape[1], H,
+         q.stride(0), k.stride(0), v.stride(0))
     return out
