@@ -21,6 +21,7 @@ import torch
 
 from .. import _lib, _ops
 from .._lib import TppxError
+from . import mx4_cache
 
 
 # ---------------------------------------------------------------------------
@@ -93,6 +94,7 @@ class TppCache:
     `[S1][B][N][32][H]` layouts are internal to its CPU kernels; nothing outside the class sees them).
     The sequence length lives in a device int32 so that a decode step can be replayed as a graph."""
 
+    kv_dtype = "bfloat16"
     block_size = 32  # LayerCache::block_size, used by align_and_invert_mask
     SLAB_BYTES = 64 << 20  # layers are allocated together while a group stays under this
 
@@ -149,6 +151,15 @@ class TppCache:
         mask_pad = t_mask.new_full((B, S_pad), pad_value)
         mask_pad[:, :S].masked_fill_(t_mask == 1, 0.0)
         return mask_pad
+
+    # -- decode loops ---------------------------------------------------------------
+    def room_for(self, S):
+        """Whether S more keys per sequence fit."""
+        return self.get_seq_length() + S <= self.capacity
+
+    def positions(self, B, device):
+        """Position of the next token of every sequence, int64 [B][1]."""
+        return torch.full((B, 1), self.get_seq_length(), dtype=torch.int64, device=device)
 
     # -- storage ------------------------------------------------------------------
     def _ensure(self, layer_idx, B, Nkv, H, device):
@@ -235,13 +246,220 @@ class TppCache:
         self.capacity = new_capacity
 
 
-def rotate_append_attend(q, k, v, t_am, t_pid, cache, layer_idx, B, S, Nq, Nkv, H, t_EP, style):
+class Mx4Cache(TppCache):
+    """A TppCache whose keys and values are held in MXFP4 (`mx4_cache`), 17/64 of the bytes of bf16, and whose sequences have
+    lengths of their own (`seq_len_dev` is int32 [B]).  Attention always sees what the cache holds, a prompt's own keys
+    included.  The decoder blocks take it wherever they take a TppCache; `prompts()` makes their next pass one over packed prompts
+    of different lengths.  Head sizes as in `mx4_cache.HEAD_SIZES`."""
+
+    kv_dtype = "mxfp4"
+
+    def __init__(self, capacity=0):
+        super().__init__(capacity)
+        self._packed = None   # (bounds int32 [B + 1], lengths) of a pass over packed prompts
+        self._bounds = {}     # (B, S) -> bounds of B times S tokens
+        self._short = None    # by how much every sequence is shorter than the longest, or None: not at all
+
+    def _sequences(self, B, device):
+        if self.capacity <= 0:
+            raise TppxError(_lib.EINVAL, "Mx4Cache: give the cache a capacity (keys per sequence) before use")
+        if self.seq_len_dev is None:
+            self.seq_len_dev = torch.zeros(B, dtype=torch.int32, device=device)
+        if self.seq_len_dev.shape[0] != B:
+            raise TppxError(_lib.ESHAPE, f"Mx4Cache: {B} sequences in a cache of {self.seq_len_dev.shape[0]}")
+
+    def _ensure(self, layer_idx, B, Nkv, H, device):
+        self._sequences(B, device)
+        layer = self.layers.get(layer_idx)
+        if layer is None:
+            if H not in mx4_cache.HEAD_SIZES:
+                raise TppxError(_lib.EUNSUPPORTED, f"Mx4Cache: head size {H} ({', '.join(map(str, mx4_cache.HEAD_SIZES))} are built)")
+            layer = mx4_cache.Mx4Layer(*(torch.zeros((B, Nkv, self.capacity, w), dtype=torch.uint8, device=device)
+                                         for w in (H // 2, H // 32, H // 2, H // 32)))
+            self.layers[layer_idx] = layer
+        elif layer.k_codes.shape != (B, Nkv, self.capacity, H // 2):
+            raise TppxError(_lib.ESHAPE, f"Mx4Cache: {B} sequences, {Nkv} heads of {H} do not fit the layer {tuple(layer.k_codes.shape)}")
+        return layer
+
+    def _bounds_of(self, B, S, device):
+        at = self._bounds.get((B, S))
+        if at is None:
+            at = self._bounds[(B, S)] = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=device)
+        return at
+
+    def prompts(self, lengths, device="cuda"):
+        """The next pass of the blocks runs over packed prompts: hidden states [1][sum(lengths)][..], sequence b's tokens behind
+        sequence b - 1's, positions [1][sum(lengths)]; `advance()` without an argument ends it.  Returns the bounds int32 [B + 1]."""
+        lengths = [int(n) for n in lengths]
+        if not lengths or min(lengths) < 0:
+            raise TppxError(_lib.ESHAPE, f"Mx4Cache.prompts: lengths {lengths}")
+        self._sequences(len(lengths), device)
+        held = [self._host_len - s for s in self._short or [0] * len(lengths)]
+        if max(h + n for h, n in zip(held, lengths)) > self.capacity:
+            raise TppxError(_lib.ESHAPE, f"Mx4Cache.prompts: {held} cached + {lengths} new keys exceed the capacity {self.capacity}")
+        starts = [0]
+        for n in lengths:
+            starts.append(starts[-1] + n)
+        self._packed = (torch.tensor(starts, dtype=torch.int32, device=device), lengths)
+        return self._packed[0]
+
+    def room_for(self, S):
+        return self._packed is not None or super().room_for(S)
+
+    def positions(self, B, device):
+        return self.seq_len_dev.to(torch.int64).view(B, 1)
+
+    def advance(self, n=1):
+        """Every sequence holds n more keys; after a pass over packed prompts, each the keys of its prompt."""
+        if self._packed is None:
+            return super().advance(n)
+        lengths, self._packed = self._packed[1], None
+        self.seq_len_dev.add_(torch.tensor(lengths, dtype=torch.int32, device=self.seq_len_dev.device))
+        now = [self._host_len - s + k for s, k in zip(self._short or [0] * len(lengths), lengths)]
+        self._short = [max(now) - k for k in now]
+        self._advance_host(max(now) - self._host_len)
+
+    def crop(self, max_length):
+        if self.seq_len_dev is not None:
+            self.seq_len_dev.clamp_(max=int(max_length))
+        if self._short is not None:
+            now = [min(self._host_len - s, int(max_length)) for s in self._short]
+            self._short = [max(now) - k for k in now]
+        self._host_len = min(self._host_len, int(max_length))
+        self._sync_len = min(self._sync_len, int(max_length))
+        self._layer_len = {i: min(n, int(max_length)) for i, n in self._layer_len.items()}
+
+    def reorder_cache(self, beam_idx):
+        beam_idx = beam_idx.to(torch.int64)
+        n = self._host_len
+        for layer in self.layers.values():
+            if beam_idx.numel() != layer.k_codes.shape[0]:
+                raise TppxError(_lib.ESHAPE, f"Mx4Cache.reorder_cache: {beam_idx.numel()} indices for {layer.k_codes.shape[0]} sequences")
+            for t in layer:
+                t[:, :, :n].copy_(t[:, :, :n].index_select(0, beam_idx.to(t.device)))
+        if self.seq_len_dev is not None:
+            self.seq_len_dev.copy_(self.seq_len_dev.index_select(0, beam_idx.to(self.seq_len_dev.device)))
+        self._short = None  # (which is shorter now the device knows; the room that is left is judged by the longest)
+        self._sums_of = None
+
+    def get(self, layer_idx):
+        """[keys, values] as the cache holds them, bf16 [B][Nkv][longest length][H]; what lies behind a shorter sequence is whatever
+        is there."""
+        kc, ks, vc, vs = self.layers[layer_idx]
+        return [mx4_cache.read_mx4(c[:, :, :self._host_len], s[:, :, :self._host_len]) for c, s in ((kc, ks), (vc, vs))]
+
+    def _append(self, layer_idx, keys, values, past):
+        B, Nkv, S, H = keys.shape
+        if values.shape != keys.shape:
+            raise TppxError(_lib.ESHAPE, "Mx4Cache: keys and values differ in shape")
+        layer = self._ensure(layer_idx, B, Nkv, H, keys.device)
+        rows = [t.to(torch.bfloat16).transpose(1, 2).reshape(B * S, Nkv, H) for t in (keys, values)]
+        at = torch.full((B,), past, dtype=torch.int32, device=keys.device)
+        mx4_cache.append_mx4(None, *rows, layer, at, self._bounds_of(B, S, keys.device), style=None)
+
+    def fill_(self, layer_idx, keys, values):
+        S = keys.shape[2]
+        if S > self.capacity:
+            raise TppxError(_lib.ESHAPE, f"Mx4Cache.fill_: {S} keys exceed the capacity {self.capacity}")
+        self._append(layer_idx, keys, values, 0)
+        self._host_len = self._sync_len = S
+        self._layer_len, self._short = {}, None
+        self.seq_len_dev.fill_(S)
+        return self
+
+    def _append_states(self, keys, values, layer_idx):
+        """Appends to sequences of one length, at the layer's length, which is returned."""
+        if self._short is not None and any(self._short):
+            raise TppxError(_lib.EUNSUPPORTED, "Mx4Cache: states are appended to sequences of one length")
+        S = keys.shape[2]
+        base = self._layer_len.get(layer_idx, self._sync_len)
+        if self.capacity < base + S:
+            self._grow(base + S + int(os.environ.get("KV_CACHE_INC_SIZE", "128")))
+        self._append(layer_idx, keys, values, base)
+        self._layer_len[layer_idx] = base + S
+        if layer_idx == 0:
+            self._host_len = base + S
+            self.seq_len_dev.fill_(self._host_len)
+        self._sums_of = None
+        return base
+
+    def update(self, key_states, value_states, layer_idx):
+        """TppCache.update for rotated keys [B][Nkv][S][H] of sequences of one length; returns what the layer holds."""
+        S = key_states.shape[2]
+        base = self._append_states(key_states, value_states, layer_idx)
+        kc, ks, vc, vs = self.layers[layer_idx]
+        return [mx4_cache.read_mx4(c[:, :, :base + S], s[:, :, :base + S]) for c, s in ((kc, ks), (vc, vs))]
+
+    def _grow(self, new_capacity):
+        new_capacity = (new_capacity + self.block_size - 1) // self.block_size * self.block_size
+        for i, layer in list(self.layers.items()):
+            grown = []
+            for t in layer:
+                n = torch.zeros((t.shape[0], t.shape[1], new_capacity, t.shape[3]), dtype=torch.uint8, device=t.device)
+                n[:, :, :t.shape[2]].copy_(t)
+                grown.append(n)
+            self.layers[i] = mx4_cache.Mx4Layer(*grown)
+        self.capacity = new_capacity
+
+    def rotate_append_attend(self, q, k, v, t_am, t_pid, layer_idx, B, S, Nq, Nkv, H, t_EP, style, qk_norm=None):
+        """What the function of that name does for a bf16 cache, in two launches: norm, rotation and append, then attention.  The
+        prompts of an empty cache attend to their keys and values as the append rounded them, in bf16."""
+        T = B * S
+        if self._packed is not None:
+            bounds, lengths = self._packed
+            if T != sum(lengths):
+                raise TppxError(_lib.ESHAPE, f"Mx4Cache: a pass of {T} tokens over packed prompts of {sum(lengths)}")
+            if t_am is not None and t_am.numel():
+                raise TppxError(_lib.EUNSUPPORTED, "Mx4Cache: packed prompts take no padding mask")
+            B = len(lengths)
+        else:
+            bounds = None if S == 1 else self._bounds_of(B, S, q.device)
+        layer = self._ensure(layer_idx, B, Nkv, H, q.device)
+        wq, wk, eps = qk_norm or (None, None, 0.0)
+        pos = t_pid.reshape(-1) if t_pid.numel() == T else t_pid.expand(B, S).reshape(-1)
+        fresh = bounds is not None and self._host_len == 0
+        rows, kr, vr = mx4_cache.append_mx4(q.view(T, Nq, H), k.view(T, Nkv, H), v.view(T, Nkv, H), layer, self.seq_len_dev, bounds, wq, wk, eps,
+                                            t_EP, pos if style else None, style, values=fresh)
+        mask = t_am if t_am is not None and t_am.numel() else None
+        if fresh:
+            ctx = mx4_cache.attn_packed(rows, kr, vr, bounds, mask)
+        else:
+            ctx = mx4_cache.attn_mx4(rows, layer, self.seq_len_dev, bounds, mask)
+        return ctx.view(q.shape)
+
+    def attend(self, t_QL, t_KL, t_VL, t_AM, layer_idx):
+        """`attn` below over this cache."""
+        B, Nkv, Sq, R, H = t_QL.shape
+        past = self._append_states(t_KL, t_VL, layer_idx)
+        q = t_QL.permute(0, 2, 1, 3, 4).reshape(B * Sq, Nkv * R, H)
+        mask = t_AM.to(torch.bfloat16).contiguous() if t_AM is not None and t_AM.numel() else None
+        at = torch.full((B,), past, dtype=torch.int32, device=q.device)
+        out = mx4_cache.attn_mx4(q, self.layers[layer_idx], at, None if Sq == 1 else self._bounds_of(B, Sq, q.device), mask)
+        return out.view(B, Sq, Nkv, R, H).permute(0, 2, 1, 3, 4).contiguous()
+
+
+def kv_cache(capacity=0, kv_dtype="bfloat16"):
+    """A cache by the type that holds its keys and values: "bfloat16" (TppCache) or "mxfp4" (Mx4Cache)."""
+    if kv_dtype not in ("bfloat16", "mxfp4"):
+        raise TppxError(_lib.EUNSUPPORTED, f"kv_dtype {kv_dtype!r} (\"bfloat16\" or \"mxfp4\")")
+    return (Mx4Cache if kv_dtype == "mxfp4" else TppCache)(capacity)
+
+
+def rotate_append_attend(q, k, v, t_am, t_pid, cache, layer_idx, B, S, Nq, Nkv, H, t_EP, style, qk_norm=None):
     """What every decoder block of the reference does between its q/k/v GEMMs and its output projection
     (fused_llm_infer.cpp:784-789, 1025-1027, 1252-1257): rotary embedding on q and k in place (style "llama":
     rotate-half with a [2][MP][HR] cos / sin table; "gptj": adjacent pairs with a [MP][HR] sin | cos table; None:
     no rotation, OPT), append of the S new keys and values at the cache length (LayerCache::update, attn.h:198-222),
     attention over the cached and the new keys (attn<T>, attn.cpp:781-955).  Returns the context [B][S][Nq*H].  Decode
-    steps of heads that are not 128 wide do all three in one launch and leave q and k as they are."""
+    steps of heads that are not 128 wide do all three in one launch and leave q and k as they are.  qk_norm = (weight of the
+    queries' norm, of the keys', eps): RMSNorm of every head in front of the rotation."""
+    if cache.kv_dtype != "bfloat16":
+        return cache.rotate_append_attend(q, k, v, t_am, t_pid, layer_idx, B, S, Nq, Nkv, H, t_EP, style, qk_norm)
+    if qk_norm is not None:
+        rows = [t.view(B * S, -1, H) for t in (q, k)]
+        pos = t_pid.reshape(-1) if t_pid.numel() == B * S else t_pid.expand(B, S).reshape(-1)
+        rows = mx4_cache.qk_norm_rotary(*rows, qk_norm[0], qk_norm[1], qk_norm[2], t_EP, pos if style else None, style)
+        q, k, style = rows[0].view(q.shape), rows[1].view(k.shape), None
     L = _lib.lib()
     st = _lib.stream_of(q)
     kc, vc = cache._ensure(layer_idx, B, Nkv, H, q.device)
@@ -295,6 +513,8 @@ def attn(t_QL, t_KL, t_VL, t_AM, cache, layer_idx, isCausal=True):
     if tuple(t_KL.shape) != (B, Nkv, Sq, H) or tuple(t_VL.shape) != (B, Nkv, Sq, H):
         raise TppxError(_lib.ESHAPE, f"attn: keys / values must be [B][Nkv][Sq][H] = {(B, Nkv, Sq, H)}")
     core = cache.get_cpp() if hasattr(cache, "get_cpp") else cache
+    if core.kv_dtype != "bfloat16":
+        return core.attend(t_QL, _bf16_cuda(t_KL, "t_KL"), _bf16_cuda(t_VL, "t_VL"), t_AM, layer_idx)
     core.update(_bf16_cuda(t_KL, "t_KL"), _bf16_cuda(t_VL, "t_VL"), layer_idx)
     key_len = core.get_seq_length(layer_idx)
     kc, vc = core.layers[layer_idx]
@@ -317,7 +537,7 @@ def attn(t_QL, t_KL, t_VL, t_AM, cache, layer_idx, isCausal=True):
 def check_layer_inputs(who, t_HS, t_pid, cache):
     """Shape checks shared by the decoder blocks: room in the cache for the S new keys, int64 positions [B or 1][S]."""
     B, S, _ = t_HS.shape
-    if cache.get_seq_length() + S > cache.capacity:
+    if not cache.room_for(S):
         raise TppxError(_lib.ESHAPE, f"{who}: {cache.get_seq_length()} cached + {S} new keys exceed "
                                      f"the cache capacity {cache.capacity}")
     if t_pid.dim() != 2 or t_pid.shape[1] != S or t_pid.shape[0] not in (1, B) or t_pid.dtype != torch.int64:
@@ -375,8 +595,11 @@ class LlamaDecoderLayer(FormatSwitches):
          self.t_Wg, self.t_Wu, self.t_Wd, self.t_EP) = params
         self.t_Bq = self.t_Bk = self.t_Bv = None
 
-    def __init__(self, params, layer_idx, eps, H, max_positions, rotary_dim):
+    def __init__(self, params, layer_idx, eps, H, max_positions, rotary_dim, qk_norm=None):
+        """qk_norm (no counterpart in the reference): the weights [H] of an RMSNorm of every query and key head in front of the
+        rotation, (queries', keys'), with the layer's eps."""
         self._take_params(params)
+        self.qk_norm = None if qk_norm is None else (qk_norm[0], qk_norm[1], float(eps))
         self.layer_idx, self.eps, self.H = int(layer_idx), float(eps), int(H)
         self.max_positions, self.rotary_dim = int(max_positions), int(rotary_dim)
         # fused_llm_infer.cpp:1112-1162: quantized weights serve every pass; unquantized ones are quantized here
@@ -412,12 +635,12 @@ class LlamaDecoderLayer(FormatSwitches):
         # input RMSNorm + q/k/v GEMMs
         q, k, v = _ops.qkv_gemm(t_HS, [Wq, Wk, Wv], [self.t_Bq, self.t_Bk, self.t_Bv],
                                 norm=(self.t_Gi, self.eps, sums_in))
-        kc, vc = cache._ensure(self.layer_idx, B, self.Nkv, self.H, t_HS.device)
-        ws = _lib.workspace(t_HS, st)
-        mask_ptr = t_am.data_ptr() if t_am is not None and t_am.numel() else None
-        mask_ld = t_am.shape[-1] if mask_ptr else 0
-        if S == 1 and FUSE_ROTARY and self.H == 128 and self.t_EP.shape[2] == 128:
+        if S == 1 and FUSE_ROTARY and self.H == 128 and self.t_EP.shape[2] == 128 and cache.kv_dtype == "bfloat16" and self.qk_norm is None:
             # decode step: rotary, cache append and attention in one launch
+            kc, vc = cache._ensure(self.layer_idx, B, self.Nkv, self.H, t_HS.device)
+            ws = _lib.workspace(t_HS, st)
+            mask_ptr = t_am.data_ptr() if t_am is not None and t_am.numel() else None
+            mask_ld = t_am.shape[-1] if mask_ptr else 0
             ctx = torch.empty_like(q)
             _lib.check(L.tppx_attn_decode_rotary_counted(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), self.t_EP.data_ptr(), t_pid.data_ptr(), t_pid.shape[0],
@@ -426,7 +649,7 @@ class LlamaDecoderLayer(FormatSwitches):
                 *_lib.with_counters(ws), st))
             return self._after_attention(ctx, t_res, empty, cache, sums_attn, sums_out, Wp, Wg, Wu, Wd)
         ctx = rotate_append_attend(q, k, v, t_am, t_pid, cache, self.layer_idx, B, S, self.Nq, self.Nkv, self.H,
-                                   self.t_EP, "llama")
+                                   self.t_EP, "llama", self.qk_norm)
         return self._after_attention(ctx, t_res, empty, cache, sums_attn, sums_out, Wp, Wg, Wu, Wd)
 
     def _after_attention(self, ctx, t_res, empty, cache, sums_attn, sums_out, Wp, Wg, Wu, Wd):
@@ -454,10 +677,11 @@ class LlamaDecoder:
     and replayed per token."""
 
     def __init__(self, hidden=4096, inter=11008, n_layers=32, n_heads=32, n_kv_heads=32, vocab=32000,
-                 max_positions=4096, eps=1e-5, weight_dtype="mxfp4", seed=0, device="cuda"):
+                 max_positions=4096, eps=1e-5, weight_dtype="mxfp4", seed=0, device="cuda", kv_dtype="bfloat16", qk_norm=False):
         self.hidden, self.n_layers, self.vocab = hidden, n_layers, vocab
         self.H = hidden // n_heads
         self.eps, self.device = eps, torch.device(device)
+        self.kv_dtype = kv_dtype
         g = torch.Generator(device=self.device).manual_seed(seed)
         quant = _ops.remap_and_quantize_mxfp4 if weight_dtype == "mxfp4" else _ops.remap_and_quantize_qint8
 
@@ -474,7 +698,10 @@ class LlamaDecoder:
         for i in range(n_layers):
             params = [ones, lin(n_heads * self.H, hidden), lin(n_kv_heads * self.H, hidden), lin(n_kv_heads * self.H, hidden),
                       lin(hidden, n_heads * self.H), ones, lin(inter, hidden), lin(inter, hidden), lin(hidden, inter), self.EP]
-            self.layers.append(LlamaDecoderLayer(params, i, eps, self.H, max_positions, self.H))
+            per_head = None
+            if qk_norm:
+                per_head = tuple(1.0 + 0.1 * torch.randn(self.H, generator=g, device=self.device) for _ in range(2))
+            self.layers.append(LlamaDecoderLayer(params, i, eps, self.H, max_positions, self.H, per_head))
         self.norm_w = ones
         self.lm_head = lin(vocab, hidden)
         self.n_kv_heads = n_kv_heads
@@ -482,7 +709,7 @@ class LlamaDecoder:
 
     def new_cache(self, B, context, capacity, seed=1):
         """Cache pre-filled with `context` positions of N(0,1) keys / values in every layer."""
-        cache = TppCache(capacity)
+        cache = kv_cache(capacity, self.kv_dtype)
         g = torch.Generator(device=self.device).manual_seed(seed)
         for i in range(self.n_layers):
             shape = (B, self.n_kv_heads, context, self.H)
@@ -512,10 +739,13 @@ class LlamaDecoder:
         logits = _ops.fc_plain(x, self.lm_head, None)
         B = logits.shape[0]
         logits = logits.view(B, -1)
+        one = cache.seq_len_dev.numel() == 1  # (the launch moves a single counter)
         _lib.check(_lib.lib().tppx_greedy_next(
             logits.data_ptr(), B, logits.shape[1], self.embed.data_ptr(), self.hidden, cur.data_ptr(),
-            pos.data_ptr() if advance else None, cache.seq_len_dev.data_ptr() if advance else None,
+            pos.data_ptr() if advance else None, cache.seq_len_dev.data_ptr() if advance and one else None,
             h.data_ptr() if advance else None, _lib.stream_of(logits)))
+        if advance and not one:
+            cache.seq_len_dev.add_(1)
         return cur
 
     def _greedy_fusable(self, B):
@@ -536,11 +766,44 @@ class LlamaDecoder:
         logits = _ops.fc_plain(h, self.lm_head, None)
         return logits.view(B, -1).argmax(dim=-1)
 
+    def prefill_packed(self, prompts, cache):
+        """Prompts of different lengths (a list of i64 [n], n > 0) in one pass on top of whatever an Mx4Cache holds of each sequence,
+        laid one after the other without padding -> next tokens i64 [B]; advances the cache by every prompt's length."""
+        if cache.kv_dtype != "mxfp4":
+            raise TppxError(_lib.EINVAL, "prefill_packed: sequences of different lengths need an Mx4Cache (kv_dtype=\"mxfp4\")")
+        lengths = [int(p.numel()) for p in prompts]
+        if not lengths or min(lengths) < 1:
+            raise TppxError(_lib.ESHAPE, f"prefill_packed: prompts of {lengths} tokens")
+        bounds = cache.prompts(lengths, self.device)
+        try:
+            tokens = torch.cat([p.reshape(-1).to(self.device) for p in prompts])
+            each = torch.tensor(lengths, device=self.device)
+            first = cache.seq_len_dev.to(torch.int64) - bounds[:-1]  # position of a sequence's row 0, less that row
+            pos = (torch.arange(tokens.numel(), device=self.device) + torch.repeat_interleave(first, each, output_size=tokens.numel())).unsqueeze(0)
+            h = self.embed.index_select(0, tokens).unsqueeze(0)
+            for layer in self.layers:
+                h = layer.forward([h, None, pos], cache)[0]
+        except BaseException:
+            cache._packed = None
+            raise
+        cache.advance()
+        h = rms_norm(h[0].index_select(0, bounds[1:].to(torch.int64) - 1), self.norm_w, self.eps)
+        return _ops.fc_plain(h, self.lm_head, None).argmax(dim=-1)
+
+    def generate_packed(self, prompts, n_new, capacity=None, use_graph=True):
+        """`generate` for prompts of different lengths (a list of i64 [n]): one packed pass, then one token per sequence and step.
+        Returns i64 [B][n_new]."""
+        cache = Mx4Cache(capacity or max(int(p.numel()) for p in prompts) + n_new + 32)
+        first = self.prefill_packed(prompts, cache).view(-1, 1)
+        if n_new == 1:
+            return first
+        return torch.cat([first, self.greedy_decode(first.view(-1), cache, n_new - 1, use_graph=use_graph)], dim=1)
+
     def generate(self, prompt, n_new, capacity=None, use_graph=True):
         """Greedy generation as run_generation.py drives it: the prompt in one pass, then one token per step.
         Returns i64 [B][n_new]."""
         B, S = prompt.shape
-        cache = TppCache(capacity or S + n_new + 32)
+        cache = kv_cache(capacity or S + n_new + 32, self.kv_dtype)
         first = self.prefill(prompt, cache)
         if n_new == 1:
             return first.view(B, 1)
@@ -564,7 +827,7 @@ class LlamaDecoder:
         self._check_room(cache, n_new + 1)  # one untimed eager step precedes the replays
         B = tokens.shape[0]
         cur = tokens.clone()
-        pos = torch.full((B, 1), cache.get_seq_length(), dtype=torch.int64, device=self.device)
+        pos = cache.positions(B, self.device)
         fused = self._greedy_fusable(B)
         if fused:
             h = self.embed.index_select(0, cur).unsqueeze(1).contiguous()
@@ -596,7 +859,7 @@ class LlamaDecoder:
         self._check_room(cache, n_new)
         B = tokens.shape[0]
         cur = tokens.clone()
-        pos = torch.full((B, 1), cache.get_seq_length(), dtype=torch.int64, device=self.device)
+        pos = cache.positions(B, self.device)
         out = torch.empty((B, n_new), dtype=torch.int64, device=self.device)
         if use_graph:
             fused = self._greedy_fusable(B)

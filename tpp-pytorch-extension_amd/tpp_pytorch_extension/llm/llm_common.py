@@ -11,6 +11,7 @@ tracing wrapper of that file has no counterpart: decode steps are replayed
 as HIP graphs instead.
 """
 import inspect
+import os
 
 import torch
 
@@ -230,9 +231,10 @@ class TppCache:
     is_compileable = False
     is_sliding = False
 
-    def __init__(self, capacity=0, **kwargs):
-        from .fused_llama_infer import TppCache as _CoreCache
-        self.tpp_cache = _CoreCache(capacity)
+    def __init__(self, capacity=0, kv_dtype=None, **kwargs):
+        """kv_dtype: "bfloat16", "mxfp4" (keys and values in MXFP4), or None: what TPPX_KV_DTYPE says, bfloat16 without it."""
+        from .fused_llama_infer import kv_cache
+        self.tpp_cache = kv_cache(capacity, kv_dtype or os.environ.get("TPPX_KV_DTYPE") or "bfloat16")
         self.static_mask = None  # an additive mask over the whole capacity that replaces the aligned one (graph replay)
 
     def __len__(self):

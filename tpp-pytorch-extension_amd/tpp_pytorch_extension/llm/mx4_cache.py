@@ -224,3 +224,16 @@ def attn_packed(q, k, v, cu_seqlens, mask=None):
     _run(q, _lib.lib().tppx_attn_packed, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_at, m_at, m_ld, out.data_ptr(), T, B, Nq, k.shape[1], H,
          q.stride(0), k.stride(0), v.stride(0))
     return out
+
+
+def read_mx4(codes, scales):
+    """What codes [..][H/2] and their scales [..][H/32] of a cache layer stand for, bf16 [..][H]."""
+    _lib.require_gpu(codes, "cache codes")
+    shape = codes.shape[:-1] + (codes.shape[-1] * 2,)
+    codes, scales = codes.contiguous(), scales.to(codes.device).contiguous()
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or scales.shape != codes.shape[:-1] + (codes.shape[-1] // 16,):
+        raise TppxError(_lib.ESHAPE, f"read_mx4: codes {tuple(codes.shape)} {codes.dtype} with scales {tuple(scales.shape)} {scales.dtype}")
+    out = torch.empty(shape, dtype=torch.float32, device=codes.device)
+    if out.numel():
+        _run(codes, _lib.lib().tppx_dequantize_per_block, codes.data_ptr(), scales.data_ptr(), _lib.Q_MXFP4, scales.numel(), 16, 1, 2, out.data_ptr())
+    return out.to(torch.bfloat16)
