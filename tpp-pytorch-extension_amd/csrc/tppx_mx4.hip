@@ -16,14 +16,14 @@
 namespace tppx {
 
 // ---------------------------------------------------------------------------
-// Norm, rotation and append.  A workgroup works on one token; G lanes take a head's row, 8 channels each: the mean square is
-// a sum over the G lanes, the rotation's partner channels come from the lane that holds them, an MX block is four lanes.
+// Norm, rotation and append.  G lanes take a head's row, 16 channels each in two chunks of 8: chunk l and the one it is rotated with, so that no channel changes lanes; behind the rotated ones chunk l and one half of the
+// rest away.  The mean square is a sum over the G lanes.
 //   y = x * (1 / sqrt(mean(x^2) + eps)) * gamma;  y' = y cos -+ partner sin
 // A query is computed in fp32 and rounded once, to bf16.  A key that goes to the cache is computed in fp64: its code is a step
-// function of the value, and in fp32 one in some 10^6 falls on the other side of a border than the formula's (a few hundred
-// thousand fp64 operations on a card that does 10^13 a second).  Codes: scale 2^(floor(log2 max) - 2), nearest, ties to the
-// even code, 6 at most, as the MXFP4 weights; a block whose maximum is below 2^-124 is zero, one that holds an infinity or a NaN
-// has scale byte 255 and reads back as NaN.
+// function of the value, and in fp32 one in some 10^6 falls on the other side of a border than the formula's.  Codes: scale
+// 2^(floor(log2 max) - 2), nearest, ties to the even code, 6 at most, as the MXFP4 weights; a block whose maximum is below 2^-124 is
+// zero, one that holds an infinity or a NaN has scale byte 255 and reads back as NaN.  A block is four chunks: those of four
+// adjacent lanes (ALIGNED: rotated width and rest are multiples of 64), or found chunk by chunk.
 // ---------------------------------------------------------------------------
 struct Mx4RowsParams {
   const uint16_t *q, *k, *v; // [T][heads][H], rows q_ld, k_ld, v_ld elements apart; q or v may be null
@@ -39,106 +39,110 @@ struct Mx4RowsParams {
   float eps;
 };
 
-__device__ __forceinline__ double shfl_xor_t(double v, int d) { return __shfl_xor(v, d); }
-__device__ __forceinline__ float shfl_xor_t(float v, int d) { return __shfl_xor(v, d); }
-
-// channels u * 8 .. + 7 of a head's row, normalised and rotated; w holds them, all G lanes of the row take part
+template <int CTRL, typename A>
+__device__ __forceinline__ A dpp_t(A v) {
+  if constexpr (std::is_same_v<A, double>) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true);
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true), lo);
+  } else {
+    return dpp_mov<CTRL>(v);
+  }
+}
+// sum over G adjacent lanes, in all of them
 template <int G, typename A>
-__device__ __forceinline__ void mx4_turn(const Mx4RowsParams& p, const uint4& w, int u, const void* gamma, int64_t at, A (&y)[8]) {
-  float f[8];
-  unpack8(w, f);
+__device__ __forceinline__ A sum_of_lanes(A v) {
+  v += dpp_t<0xB1>(v); // quad_perm [1,0,3,2]
+  v += dpp_t<0x4E>(v); // quad_perm [2,3,0,1]
+  if constexpr (G >= 8)
+    v += dpp_t<0x141>(v); // row_half_mirror
+  if constexpr (G >= 16)
+    v += dpp_t<0x140>(v); // row_mirror
+  return v;
+}
+__device__ __forceinline__ float rsqrt_t(float v) { return 1.0f / sqrtf(v); }
+__device__ __forceinline__ double rsqrt_t(double v) { // the hardware's estimate and two steps of Newton's method
+  double r = __builtin_amdgcn_rsq(v);
+  r *= 1.5 - 0.5 * v * r * r;
+  return r * (1.5 - 0.5 * v * r * r);
+}
+
+// What the lanes of a row share out: chunks c[0], c[1] of 8 channels; their angles where they are rotated (adjacent pairs: four
+// of each chunk, otherwise eight that both share).
+struct Mx4Lane {
+  int c[2];
+  bool live, turn;
+  float cs[8], sn[8];
+};
+
+// a lane's 16 channels, normalised and rotated; all G lanes of the row take part
+template <int G, typename A>
+__device__ __forceinline__ void mx4_turn(const Mx4RowsParams& p, const uint4 (&w)[2], const Mx4Lane& t, const void* gamma, A (&y)[2][8]) {
 #pragma unroll
-  for (int e = 0; e < 8; e++)
-    y[e] = f[e];
-  A r = 1;
-  auto scale_of = [&](int c, A (&g)[8]) { // gamma of chunk c
-    if (p.gamma_f32) {
-      const f32x4* s = reinterpret_cast<const f32x4*>(gamma) + c * 2;
-      const f32x4 a = s[0], b = s[1];
+  for (int h = 0; h < 2; h++) {
+    float f[8];
+    unpack8(w[h], f);
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        g[e] = a[e];
-        g[4 + e] = b[e];
-      }
-    } else {
-      float h[8];
-      unpack8(reinterpret_cast<const uint4*>(gamma)[c], h);
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        g[e] = h[e];
-    }
-  };
-  const bool live = u * 8 < p.H;
+    for (int e = 0; e < 8; e++)
+      y[h][e] = f[e];
+  }
   if (gamma) {
     A ss = 0;
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      ss += y[e] * y[e];
-#pragma unroll
-    for (int d = 1; d < G; d *= 2)
-      ss += shfl_xor_t(ss, d);
-    r = (A)1 / sqrt(ss / (A)p.H + (A)p.eps);
-    A g[8];
-    scale_of(live ? u : 0, g);
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      y[e] = y[e] * r * g[e];
-  }
-  const bool rotate = p.emb && at >= 0 && at < p.MP; // positions outside the table are left unrotated
-  if (p.gptj) {
-    if (rotate && u * 8 < p.HR) {
-      const float* sn = p.emb + at * p.HR + u * 4;
-      const float* cs = sn + (p.HR >> 1);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const A a = y[2 * e], b = y[2 * e + 1], c = cs[e], s = sn[e];
-        if constexpr (std::is_same_v<A, float>) {
-          y[2 * e] = rotate_first(a, b, c, s);
-          y[2 * e + 1] = rotate_second(a, b, c, s);
-        } else {
-          y[2 * e] = a * c - b * s;
-          y[2 * e + 1] = b * c + a * s;
-        }
-      }
-    }
-    return;
-  }
-  const int half = p.HR >> 4; // chunks of the first half
-  const int mate = u < half ? u + half : u < 2 * half ? u - half : u;
-  const int lane = threadIdx.x & 63, src = (lane & ~(G - 1)) + mate;
-  const uint4 m = make_uint4(__shfl(w.x, src), __shfl(w.y, src), __shfl(w.z, src), __shfl(w.w, src));
-  if (rotate && u < 2 * half) {
-    unpack8(m, f);
-    A o[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      o[e] = f[e];
-    if (gamma) {
-      A g[8];
-      scale_of(mate, g);
+    for (int h = 0; h < 2; h++)
 #pragma unroll
       for (int e = 0; e < 8; e++)
-        o[e] = o[e] * r * g[e];
-    }
-    const f32x4* cp = reinterpret_cast<const f32x4*>(p.emb + at * p.HR + u * 8);
-    const f32x4* sp = reinterpret_cast<const f32x4*>(p.emb + ((int64_t)p.MP + at) * p.HR + u * 8);
-    const f32x4 c4[2] = {cp[0], cp[1]}, s4[2] = {sp[0], sp[1]};
+        ss = fma(y[h][e], y[h][e], ss);
+    ss = sum_of_lanes<G>(ss);
+    const A r = rsqrt_t(ss * ((A)1 / (A)p.H) + (A)p.eps);
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const A c = c4[e >> 2][e & 3], s = s4[e >> 2][e & 3];
-      if constexpr (std::is_same_v<A, float>)
-        y[e] = u < half ? rotate_first(y[e], o[e], c, s) : rotate_second(o[e], y[e], c, s);
-      else
-        y[e] = u < half ? y[e] * c - o[e] * s : y[e] * c + o[e] * s;
+    for (int h = 0; h < 2; h++) {
+      float g[8];
+      if (p.gamma_f32) {
+        const f32x4* s = reinterpret_cast<const f32x4*>(gamma) + t.c[h] * 2;
+        const f32x4 a = s[0], b = s[1];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          g[e] = a[e];
+          g[4 + e] = b[e];
+        }
+      } else {
+        unpack8(reinterpret_cast<const uint4*>(gamma)[t.c[h]], g);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        y[h][e] = y[h][e] * r * (A)g[e];
     }
+  }
+  if (!t.turn)
+    return;
+  auto rotate = [&](A& a, A& b, float c, float s) {
+    const A x = a, z = b;
+    if constexpr (std::is_same_v<A, float>) {
+      a = rotate_first(x, z, c, s);
+      b = rotate_second(x, z, c, s);
+    } else {
+      asm("" : "+v"(c), "+v"(s)); // (not as 32 registers of fp64 over the whole loop)
+      a = x * (A)c - z * (A)s;
+      b = z * (A)c + x * (A)s;
+    }
+  };
+  if (p.gptj) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        rotate(y[h][2 * e], y[h][2 * e + 1], t.cs[4 * h + e], t.sn[4 * h + e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      rotate(y[0][e], y[1][e], t.cs[e], t.sn[e]);
   }
 }
 
-// codes of a lane's 8 values (a dword) and the block's scale byte; a block is four adjacent lanes
+// biased fp32 exponent (up to 2047 from fp64, kept in that bias) of the largest magnitude of 8 values
 template <typename A>
-__device__ __forceinline__ uint32_t mx4_encode(const A (&y)[8], int& byte) {
-  constexpr int TOP = std::is_same_v<A, double> ? 0x7ff : 0xff, BIAS = std::is_same_v<A, double> ? 1023 : 127;
-  int top = 0; // biased exponent of the largest magnitude
+__device__ __forceinline__ int top_exponent(const A (&y)[8]) {
+  int top = 0;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     if constexpr (std::is_same_v<A, double>)
@@ -146,90 +150,187 @@ __device__ __forceinline__ uint32_t mx4_encode(const A (&y)[8], int& byte) {
     else
       top = max(top, (int)((__float_as_uint(y[e]) >> 23) & 0xffu));
   }
-  top = max(top, __builtin_amdgcn_update_dpp(0, top, 0xB1, 0xf, 0xf, true)); // quad_perm [1,0,3,2]
-  top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x4E, 0xf, 0xf, true)); // quad_perm [2,3,0,1]
-  byte = top == TOP ? 255 : min(max(top - BIAS + 125, 0), 254);
-  uint32_t codes = 0;
-  if (byte != 0 && byte != 255) {
-    A by;
-    if constexpr (std::is_same_v<A, double>)
-      by = __hiloint2double((1023 + 127 - byte) << 20, 0);
-    else
-      by = ldexpf(1.0f, 127 - byte);
+  return top;
+}
+// codes of 8 values of a block with that scale byte (a dword).  The conversion is the hardware's, nearest even and 6 at most; it
+// keeps the sign of a zero, which is dropped.  A fp64 value enters as fp32 by its upper dword, with the last bit set where the lower
+// one is not zero: every border between two codes has both zero, so that it stays on its side of all of them.  The division by the
+// scale is a difference of exponents there; what is below 2^-15 of it becomes 2^-15, whose code is zero too.
+template <typename A>
+__device__ __forceinline__ uint32_t mx4_encode(const A (&y)[8], int byte) {
+  if (byte == 0 || byte == 255)
+    return 0;
+  uint32_t q = 0;
+  if constexpr (std::is_same_v<A, double>) {
+    float f[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      const A a = fabs(y[e] * by);
-      uint32_t c = (a > (A)0.25) + (a >= (A)0.75) + (a > (A)1.25) + (a >= (A)1.75) + (a > (A)2.5) + (a >= (A)3.5) + (a > (A)5);
-      c |= c != 0 && y[e] < 0 ? 8u : 0u;
-      codes |= c << (4 * e);
+      const uint32_t hi = (uint32_t)__double2hiint(y[e]) | (__double2loint(y[e]) != 0 ? 1u : 0u);
+      const int t = max((int)(hi & 0x7fffffffu) + (127 - byte) * (1 << 20), 0x3f000000);
+      f[e] = __uint_as_float((((uint32_t)t << 3) - (896u << 23)) | (hi & 0x80000000u));
     }
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[0], f[1], 1.0f, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[2], f[3], 1.0f, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[4], f[5], 1.0f, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, f[6], f[7], 1.0f, 3);
+  } else {
+    const float s = e8m0_to_f32((uint32_t)byte);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[0], y[1], s, 0);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[2], y[3], s, 1);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[4], y[5], s, 2);
+    q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, y[6], y[7], s, 3);
   }
-  return codes;
+  const uint32_t nz = (q | (q >> 1) | (q >> 2)) & 0x11111111u;
+  return q & (0x77777777u | (nz << 3));
 }
 
-template <int G, bool CACHE>
-__global__ void __launch_bounds__(256)
+template <int G, bool CACHE, bool ALIGNED>
+__global__ void __launch_bounds__(256, ALIGNED ? CACHE ? 4 : 5 : 3)
 mx4_rows_kernel(const Mx4RowsParams p) {
-  const int tok = blockIdx.x;
+  // A thread's token stays, the heads go by: a wave works on one head (of q, k or v) of 64 / G tokens in a row, whose rows in
+  // the cache lie side by side, and a token's angles are read once.
+  constexpr int TB = 256 / G; // tokens of a workgroup
+  const int u = threadIdx.x % G, mine = (int)blockIdx.x * TB + (int)threadIdx.x / G, tok = min(mine, p.T - 1);
+  const int nq = p.q ? p.Nq : 0, nk = p.Nkv, total = nq + nk + (p.v ? p.Nkv : 0);
+  const int half = p.HR >> 4, rest = (p.H - p.HR) >> 4; // lanes of rotated chunks, of the others
+  Mx4Lane t;
+  t.live = u < half + rest;
+  t.c[0] = !t.live ? 0 : u < half ? u : u + half;
+  t.c[1] = !t.live ? 0 : u < half ? u + half : u + half + rest;
+  // rows of a token: queries, then keys, then values; the next one is under way while one is worked on
+  uint4 next[2];
+  auto load = [&](int i) {
+    if (i >= total)
+      return;
+    const uint16_t* const src = i < nq ? p.q + (int64_t)i * p.H : i < nq + nk ? p.k + (int64_t)(i - nq) * p.H : p.v + (int64_t)(i - nq - nk) * p.H;
+    const uint4* const at = reinterpret_cast<const uint4*>(src + (int64_t)tok * (i < nq ? p.q_ld : i < nq + nk ? p.k_ld : p.v_ld));
+    next[0] = at[t.c[0]];
+    next[1] = at[t.c[1]];
+  };
+  int row = (int)blockIdx.y;
+  load(row);
   int b = 0, slot = 0;
+  bool here = mine < p.T;
   if (CACHE) {
     int first = tok;
     b = tok;
     if (p.cu) {
-      b = sequence_of(p.cu, p.B, tok);
-      if (b >= p.B || tok < p.cu[0])
-        return; // rows behind the last sequence
+      b = sequence_of(p.cu, p.B, __builtin_amdgcn_readfirstlane(tok)); // of the wave's first token
+      while (b < p.B && p.cu[b + 1] <= tok)
+        b++;
+      here = here && b < p.B && tok >= p.cu[0]; // (not a row behind the last sequence)
+      b = min(b, p.B - 1);
       first = p.cu[b];
     }
     slot = p.past[b] + (tok - first);
   }
   const int64_t at = p.pos ? p.pos[tok] : (int64_t)slot;
   const bool room = slot >= 0 && slot < p.Smax;
-  const int nq = p.q ? p.Nq : 0, nk = p.Nkv, nv = p.v ? p.Nkv : 0;
-  int i = (int)blockIdx.y * (256 / G) + (int)threadIdx.x / G;
-  const int u = threadIdx.x % G;
-  if (i >= nq + nk + nv)
-    return; // (whole groups of G lanes)
-  const bool live = u * 8 < p.H;
-  const int kind = i < nq ? 0 : i < nq + nk ? 1 : 2;
-  i -= kind == 0 ? 0 : kind == 1 ? nq : nq + nk;
-  const uint16_t* src = kind == 0 ? p.q + (int64_t)tok * p.q_ld : kind == 1 ? p.k + (int64_t)tok * p.k_ld : p.v + (int64_t)tok * p.v_ld;
-  const uint4 w = live ? *reinterpret_cast<const uint4*>(src + (int64_t)i * p.H + u * 8) : make_uint4(0, 0, 0, 0);
-  if (kind == 0 || !CACHE) {
-    float y[8];
-    mx4_turn<G>(p, w, u, kind == 0 ? p.gq : p.gk, at, y);
-    if (live)
-      *reinterpret_cast<uint4*>((kind == 0 ? p.qo + ((int64_t)tok * p.Nq + i) * p.H : p.ko + ((int64_t)tok * p.Nkv + i) * p.H) + u * 8) = pack8(y);
-    return;
+  t.turn = p.emb && at >= 0 && at < p.MP && u < half; // positions outside the table are left unrotated
+  if (t.turn) {
+    const float* const c = p.emb + at * p.HR + (p.gptj ? p.HR >> 1 : 0);
+    const float* const s = p.emb + (p.gptj ? at : p.MP + at) * p.HR;
+    const int a0 = p.gptj ? t.c[0] * 4 : u * 8, a1 = p.gptj ? t.c[1] * 4 : u * 8 + 4;
+    const f32x4 c0 = *reinterpret_cast<const f32x4*>(c + a0), c1 = *reinterpret_cast<const f32x4*>(c + a1);
+    const f32x4 s0 = *reinterpret_cast<const f32x4*>(s + a0), s1 = *reinterpret_cast<const f32x4*>(s + a1);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      t.cs[e] = c0[e];
+      t.cs[4 + e] = c1[e];
+      t.sn[e] = s0[e];
+      t.sn[4 + e] = s1[e];
+    }
   }
-  uint32_t codes;
-  int byte;
-  if (kind == 1) {
-    double y[8];
-    mx4_turn<G>(p, w, u, p.gk, at, y);
-    codes = mx4_encode(y, byte);
-  } else {
-    float y[8];
-    unpack8(w, y);
-    codes = mx4_encode(y, byte);
+  uint4 w[2];
+  auto step = [&]() {
+    w[0] = next[0];
+    w[1] = next[1];
+    if (!t.live) // (heads of 96 and 192 leave lanes over)
+      w[0] = w[1] = make_uint4(0, 0, 0, 0);
+    load(row + (int)gridDim.y);
+  };
+  auto write = [&](uint16_t* to, int heads, int i, const float (&y)[2][8]) { // a row of [T][heads][H]
+    if (!t.live || !here)
+      return;
+    uint4* const dst = reinterpret_cast<uint4*>(to + ((int64_t)tok * heads + i) * p.H);
+    dst[t.c[0]] = pack8(y[0]);
+    dst[t.c[1]] = pack8(y[1]);
+  };
+  auto append = [&](auto& y, uint8_t* codes_at, uint8_t* scales_at, uint16_t* held, int i) {
+    using A = std::remove_reference_t<decltype(y[0][0])>;
+    constexpr int TOP = std::is_same_v<A, double> ? 0x7ff : 0xff, BIAS = std::is_same_v<A, double> ? 1023 : 127;
+    int top[2] = {top_exponent(y[0]), top_exponent(y[1])};
+    if constexpr (ALIGNED) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        top[h] = max(top[h], __builtin_amdgcn_update_dpp(0, top[h], 0xB1, 0xf, 0xf, true));
+        top[h] = max(top[h], __builtin_amdgcn_update_dpp(0, top[h], 0x4E, 0xf, 0xf, true));
+      }
+    } else {
+      const int lane0 = (threadIdx.x & 63) & ~(G - 1), own[2] = {top[0], top[1]};
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int ch = (t.c[h] & ~3) + j, r = ch - 2 * half; // lane and slot that hold chunk ch
+          const bool second = r < 0 ? ch >= half : r >= rest;
+          const int src = lane0 + (r < 0 ? ch - (second ? half : 0) : half + r - (second ? rest : 0));
+          const int a = __shfl(own[0], src), z = __shfl(own[1], src);
+          top[h] = max(top[h], second ? z : a);
+        }
+    }
+    const int64_t to = ((int64_t)b * p.Nkv + i) * p.Smax + slot;
+    float f[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int byte = top[h] == TOP ? 255 : min(max(top[h] - BIAS + 125, 0), 254);
+      const uint32_t codes = mx4_encode(y[h], byte);
+      if (t.live && here && room) {
+        *reinterpret_cast<uint32_t*>(codes_at + to * (p.H >> 1) + t.c[h] * 4) = codes;
+        if ((t.c[h] & 3) == 0)
+          scales_at[to * (p.H >> 5) + (t.c[h] >> 2)] = (uint8_t)byte;
+      }
+      if (held) {
+        typedef __attribute__((ext_vector_type(2))) float f32x2;
+        const float s = e8m0_to_f32((uint32_t)byte);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const f32x2 v = e == 0 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0) : e == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1)
+                        : e == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3);
+          f[h][2 * e] = v[0] * s;
+          f[h][2 * e + 1] = v[1] * s;
+        }
+      }
+    }
+    if (held)
+      write(held, p.Nkv, i, f);
+  };
+  for (; row < nq; row += (int)gridDim.y) {
+    step();
+    float y[2][8];
+    mx4_turn<G>(p, w, t, p.gq, y);
+    write(p.qo, p.Nq, row, y);
   }
-  if (!live)
-    return;
-  const int64_t row = ((int64_t)b * p.Nkv + i) * p.Smax + slot;
-  if (room) {
-    *reinterpret_cast<uint32_t*>((kind == 1 ? p.kq : p.vq) + row * (p.H >> 1) + u * 4) = codes;
-    if ((u & 3) == 0)
-      (kind == 1 ? p.ks : p.vs)[row * (p.H >> 5) + (u >> 2)] = (uint8_t)byte;
+  for (; row < nq + nk; row += (int)gridDim.y) {
+    step();
+    if constexpr (CACHE) {
+      double y[2][8];
+      mx4_turn<G>(p, w, t, p.gk, y);
+      append(y, p.kq, p.ks, p.ko, row - nq);
+    } else {
+      float y[2][8];
+      mx4_turn<G>(p, w, t, p.gk, y);
+      write(p.ko, p.Nkv, row - nq, y);
+    }
   }
-  uint16_t* held = kind == 1 ? p.ko : p.vo;
-  if (held) {
-    typedef __attribute__((ext_vector_type(2))) float f32x2;
-    const float s = e8m0_to_f32((uint32_t)byte);
-    const f32x2 v0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0), v1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1);
-    const f32x2 v2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2), v3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3);
-    const float y[8] = {v0[0] * s, v0[1] * s, v1[0] * s, v1[1] * s, v2[0] * s, v2[1] * s, v3[0] * s, v3[1] * s};
-    *reinterpret_cast<uint4*>(held + ((int64_t)tok * p.Nkv + i) * p.H + u * 8) = pack8(y);
-  }
+  if constexpr (CACHE)
+    for (; row < total; row += (int)gridDim.y) {
+      step();
+      float y[2][8];
+      unpack8(w[0], y[0]);
+      unpack8(w[1], y[1]);
+      append(y, p.vq, p.vs, p.vo, row - nq - nk);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -642,23 +743,30 @@ static int rows_launch(const char* who, Mx4RowsParams& p, bool cache, hipStream_
     return TPPX_OK;
   if (!p.emb)
     p.HR = 0;
-  const int G = p.H <= 64 ? 8 : p.H <= 128 ? 16 : 32;
-  const int64_t heads = (p.q ? p.Nq : 0) + p.Nkv + (p.v ? p.Nkv : 0), wgs = (heads * G + 255) / 256;
-  TPPX_REQUIRE(wgs <= 65535, TPPX_ESHAPE, "%s: too many heads", who);
-  const dim3 grid((unsigned)p.T, (unsigned)wgs);
+  const int G = p.H <= 64 ? 4 : p.H <= 128 ? 8 : 16;
+  const int64_t rows = (int64_t)(p.q ? p.Nq : 0) + p.Nkv + (p.v ? p.Nkv : 0), blocks = ((int64_t)p.T * G + 255) / 256;
+  // Some 1024 workgroups, what the registers let run at once: 2027 tokens of 32 + 2 x 32 heads 21.1 us (5.2 TB/s), 23.6 with 512, 25.3
+  // with 4096; 2048 of 64 + 2 x 8 behind the norm 17.3, 19.4, 20.1; without the cache 14.3, 16.3, 15.3.  (A workgroup per token, its
+  // heads side by side: 30.6, 27.1 and 18.8, of which the fp64 of the keys was 2.5: rows of the cache were written in pieces by
+  // workgroups far apart.)
+  const int64_t per_block = std::max<int64_t>(1, std::min<int64_t>({rows, 65535, env_int("TPPX_MX4_ROWS_WGS", 1024) / blocks}));
+  const dim3 grid((unsigned)blocks, (unsigned)per_block);
+  const bool aligned = p.HR % 64 == 0 && (p.H - p.HR) % 64 == 0;
   auto go = [&](auto g) {
     constexpr int GG = decltype(g)::value;
-    if (cache)
-      mx4_rows_kernel<GG, true><<<grid, dim3(256), 0, stream>>>(p);
+    if (!cache)
+      mx4_rows_kernel<GG, false, true><<<grid, dim3(256), 0, stream>>>(p);
+    else if (aligned)
+      mx4_rows_kernel<GG, true, true><<<grid, dim3(256), 0, stream>>>(p);
     else
-      mx4_rows_kernel<GG, false><<<grid, dim3(256), 0, stream>>>(p);
+      mx4_rows_kernel<GG, true, false><<<grid, dim3(256), 0, stream>>>(p);
   };
-  if (G == 8)
+  if (G == 4)
+    go(std::integral_constant<int, 4>{});
+  else if (G == 8)
     go(std::integral_constant<int, 8>{});
-  else if (G == 16)
-    go(std::integral_constant<int, 16>{});
   else
-    go(std::integral_constant<int, 32>{});
+    go(std::integral_constant<int, 16>{});
   return check_hip(hipGetLastError(), who);
 }
 
