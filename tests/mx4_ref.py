@@ -105,3 +105,21 @@ def attend(q, k, v, past, mask=None):
             rel = 2.0 * 2.0 ** -8 + 2 * es + 2.0 ** -12 + keys * 2.0 ** -23
             tol[i, h] = 2.0 ** -8 * out[i, h].abs() + rel * (p @ vv.abs()) * 1.01
     return out, tol + 2.0 ** -126
+
+
+def attend_rows(q, k, v, past):
+    """`attend` without a mask, one head at a time instead of one token and head."""
+    n, nq, H = q.shape
+    nkv, keys = k.shape[:2]
+    out, tol = torch.zeros((n, nq, H), dtype=F64), torch.zeros((n, nq, H), dtype=F64)
+    hidden = torch.ones((n, keys), dtype=torch.bool).triu(past + 1)
+    for h in range(nq):
+        qq, kk, vv = q[:, h].to(F64), k[h * nkv // nq], v[h * nkv // nq]
+        s = (qq @ kk.t() / math.sqrt(H)).masked_fill(hidden, -math.inf)
+        p = torch.softmax(s, 1)
+        out[:, h] = p @ vv
+        es = (H + 4) * 2.0 ** -24 * (qq.abs() @ kk.abs().t()).amax(1, keepdim=True) / math.sqrt(H)
+        es = es + 2.0 ** -23 * s.masked_fill(hidden, 0.0).abs().amax(1, keepdim=True)
+        rel = 2.0 * 2.0 ** -8 + 2 * es + 2.0 ** -12 + keys * 2.0 ** -23
+        tol[:, h] = 2.0 ** -8 * out[:, h].abs() + rel * (p @ vv.abs()) * 1.01
+    return out, tol + 2.0 ** -126

@@ -394,3 +394,90 @@ def test_bounds_on_the_device_that_do_not_fit_stay_inside():
     assert torch.equal(layer.k_codes[0, :, 0].cpu(), c)
     at.attn_mx4(q, layer, _i32([-3, 1 << 30]), _i32([0, 4, 99]))
     torch.cuda.synchronize()
+
+
+# -- the forms that larger calls take ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("H", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("queries", ["128", "64"])
+def test_prompt_forms(H, queries, monkeypatch):
+    """Both forms of a prompt's workgroup at sizes that the rule would give the other one: packed rows and the cache, tiles that end
+    in a sequence, blocks that end in a tile, a mask."""
+    monkeypatch.setenv("TPPX_MX4_PROMPT_QUERIES", queries)
+    at = _at()
+    Nq, Nkv, new, past = 4, 2, [150, 1, 129, 200], [0, 70, 33, 1]
+    cu = _starts(new)
+    layer, k, v = _filled(4, Nkv, 210, H, H)
+    _junk_behind(layer, [p + n for p, n in zip(past, new)])
+    q, kp, vp = R.randn((cu[-1], Nq, H), 1.3, 1), R.randn((cu[-1], Nkv, H), 1.0, 2), R.randn((cu[-1], Nkv, H), 1.0, 3)
+    got = at.attn_mx4(q.cuda(), layer, _i32(past), _i32(cu))
+    packed = at.attn_packed(q.cuda(), kp.cuda(), vp.cuda(), _i32(cu))
+    for b in range(4):
+        rows, n = slice(cu[b], cu[b + 1]), past[b] + new[b]
+        _within(got[rows], *R.attend_rows(q[rows], k[b, :, :n], v[b, :, :n], past[b]))
+        _within(packed[rows], *R.attend_rows(q[rows], kp[rows].transpose(0, 1).double(), vp[rows].transpose(0, 1).double(), 0))
+    zeros = torch.zeros((4, 210), dtype=torch.bfloat16, device="cuda")
+    assert torch.equal(at.attn_mx4(q.cuda(), layer, _i32(past), _i32(cu), zeros)[cu[1]:cu[2]].isnan(), torch.zeros((1, Nq, H), dtype=torch.bool, device="cuda"))
+    for b, rows in ((0, slice(0, 150)), (3, slice(cu[3], cu[4]))):
+        _within(at.attn_packed(q.cuda(), kp.cuda(), vp.cuda(), _i32(cu), zeros)[rows],
+                *R.attend_rows(q[rows], kp[rows].transpose(0, 1).double(), vp[rows].transpose(0, 1).double(), 0))
+    kp[cu[3] + 130], vp[cu[3] + 131] = math.nan, math.inf  # seen by later tokens alone
+    hit = at.attn_packed(q.cuda(), kp.cuda(), vp.cuda(), _i32(cu))
+    assert torch.equal(hit[:cu[3] + 130], packed[:cu[3] + 130]) and bool(hit[cu[3] + 130:].isnan().all())
+
+
+@pytest.mark.parametrize("H", [64, 96, 128])
+def test_prompts_of_many_heads(H):
+    """400 workgroups of 128 queries: the form of large launches, by its own rule."""
+    at = _at()
+    Nq, new, past = 104, [131, 130], [0, 40]
+    cu = _starts(new)
+    layer, k, v = _filled(2, Nq, 172, H, H)
+    q, kp, vp = (R.randn((cu[-1], Nq, H), 1.2, i) for i in range(3))
+    got = at.attn_mx4(q.cuda(), layer, _i32(past), _i32(cu))
+    packed = at.attn_packed(q.cuda(), kp.cuda(), vp.cuda(), _i32(cu))
+    for b in range(2):
+        rows, n = slice(cu[b], cu[b + 1]), past[b] + new[b]
+        _within(got[rows], *R.attend_rows(q[rows], k[b, :, :n], v[b, :, :n], past[b]))
+        _within(packed[rows], *R.attend_rows(q[rows], kp[rows].transpose(0, 1).double(), vp[rows].transpose(0, 1).double(), 0))
+
+
+@pytest.mark.parametrize("H", [64, 128, 192])
+@pytest.mark.parametrize("splits", ["1", "3", "32"])
+def test_splits(H, splits, monkeypatch):
+    """Every number of splits, also where sequences are too short for theirs."""
+    monkeypatch.setenv("TPPX_MX4_SPLITS", splits)
+    at = _at()
+    Nq, Nkv, past = 6, 2, [1500, 0, 255, 256, 700]
+    layer, k, v = _filled(5, Nkv, 1600, H, H)
+    _junk_behind(layer, [p + 1 for p in past])
+    q = R.randn((5, Nq, H), 1.2, 1)
+    for _ in range(2):
+        got = at.attn_mx4(q.cuda(), layer, _i32(past))
+        for b in range(5):
+            _within(got[b:b + 1], *R.attend_rows(q[b:b + 1], k[b, :, :past[b] + 1], v[b, :, :past[b] + 1], past[b]))
+
+
+@pytest.mark.parametrize("H,style,width", [(128, "llama", 128), (96, "llama", 96), (192, "gptj", 64)])
+@pytest.mark.parametrize("wgs", ["1", "100000"])
+def test_append_by_few_and_by_many_workgroups(H, style, width, wgs, monkeypatch):
+    """Some hundred tokens of sequences that begin and end inside a workgroup's tokens, one head or all of them to a workgroup."""
+    monkeypatch.setenv("TPPX_MX4_ROWS_WGS", wgs)
+    at = _at()
+    new, past, Nq, Nkv = [100, 0, 3, 1, 70], [5, 1, 0, 9, 31], 3, 2
+    cu = _starts(new)
+    q, k, v = (R.randn((cu[-1], n, H), 1.5, i) for i, n in enumerate((Nq, Nkv, Nkv)))
+    w = R.randn(H, 0.2, 9).float() + 1
+    table = _table(style, 128, H, width)
+    layer = _empty_layer(5, Nkv, 120, H)
+    qo, ko, vo = at.append_mx4(q.cuda(), k.cuda(), v.cuda(), layer, _i32(past), _i32(cu), w.cuda(), w.cuda(), 1e-6, table.cuda(), None, style, values=True)
+    pos = [p + i for n, p in zip(new, past) for i in range(n)]
+    want, size = R.turn(q, w, 1e-6, table, pos, style)
+    _within(qo, want, 2.0 ** -8 * want.abs() + 2.0 ** -20 * size + 2.0 ** -133)
+    kw, _ = R.turn(k, w, 1e-6, table, pos, style)
+    for i, x, held in ((0, kw, ko), (2, v.double(), vo)):
+        codes, scales = R.encode(x)
+        assert torch.equal(held.cpu().double(), R.decode(codes, scales).to(torch.bfloat16).double())
+        for b in range(5):
+            at_slots = slice(past[b], past[b] + new[b])
+            assert torch.equal(layer[i][b, :, at_slots].cpu(), codes[cu[b]:cu[b + 1]].transpose(0, 1))
+            assert torch.equal(layer[i + 1][b, :, at_slots].cpu(), scales[cu[b]:cu[b + 1]].transpose(0, 1))

@@ -22,10 +22,12 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int B, int tok) {
 
 // Workgroup `blk` of a launch whose sequences take ceil(tokens * per / rows) workgroups each: its sequence, that one's first
 // row and tokens, and the workgroup's number inside it.  False past the last one.  All lanes of a wave take part.
+// order(blk, all): the place of workgroup blk of `all`, applied for up to 64 sequences.
 struct Block {
   int b, start, n, at;
 };
-__device__ __forceinline__ bool locate(const int32_t* cu, int B, int T, int per, int rows, int blk, Block& o) {
+template <typename F>
+__device__ __forceinline__ bool locate(const int32_t* cu, int B, int T, int per, int rows, int blk, Block& o, F&& order) {
   if (!cu) { // one token per sequence
     const int each = (per + rows - 1) / rows;
     o.b = blk / each;
@@ -48,6 +50,8 @@ __device__ __forceinline__ bool locate(const int32_t* cu, int B, int T, int per,
       sum += lane >= d ? t : 0;
     }
     const int total = __builtin_amdgcn_readlane(sum, 63);
+    if (B <= 64)
+      blk = order(blk, total);
     if (blk < before + total) {
       const int j = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + sum > blk));
       o.b = i0 + j;
@@ -64,6 +68,10 @@ __device__ __forceinline__ bool locate(const int32_t* cu, int B, int T, int per,
 __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
   return make_uint4(f32x2_to_bf16_bits(f[0], f[1]), f32x2_to_bf16_bits(f[2], f[3]), f32x2_to_bf16_bits(f[4], f[5]),
                     f32x2_to_bf16_bits(f[6], f[7]));
+}
+
+__device__ __forceinline__ bool locate(const int32_t* cu, int B, int T, int per, int rows, int blk, Block& o) {
+  return locate(cu, B, T, per, rows, blk, o, [](int b, int) { return b; });
 }
 
 // eight E2M1 codes of a dword times the scale, exact in bf16
@@ -93,6 +101,14 @@ typedef int i32x3 __attribute__((ext_vector_type(3)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef short i16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+// maximum over the four 16-lane groups
+__device__ __forceinline__ float max_of_groups(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float LOWEST = -3.4028234e38f; // below every finite score, the bf16 lowest of a mask among them

@@ -350,14 +350,6 @@ mx4_rows_kernel(const Mx4RowsParams p) {
 // by their bytes and put into the result.
 // Scores, maximum and sums in fp32; the probabilities' sum is that of the bf16 ones, taken by an MFMA with ones.
 // ---------------------------------------------------------------------------
-// maximum over the four 16-lane groups
-__device__ __forceinline__ float max_of_groups(float v) {
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
 template <int NJ>
 constexpr int mx4_scale_bytes() { // scale bytes of a lane's channels of a key: whole blocks, or one that they lie in
   return NJ % 4 == 0 ? NJ / 4 : NJ <= 2 ? 1 : NJ;

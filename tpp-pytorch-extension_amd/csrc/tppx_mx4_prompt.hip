@@ -1,16 +1,23 @@
 // Attention of prompts, causal, over packed bf16 rows or over the MXFP4 cache.
+#include <algorithm>
+
 #include "tppx_mx4.h"
 
 namespace tppx {
 
 // ---------------------------------------------------------------------------
-// Prompts: QG groups of 32 queries of one head, each a wave, or with KT = 2 two that take half of every tile's keys (and are
+// Prompts: QG groups of QW queries of one head, each a wave, or with KT = 2 two that take half of every tile's keys (and are
 // merged at the end: launches of few workgroups), share K and V tiles of 64 keys, bf16 in LDS in two stages, from packed rows or
-// from the cache (its codes expanded once per workgroup on the way to LDS).  Both products run transposed on the 32 x 32 x 16
-// MFMA: scores^T[key][query] = K Q^T, out^T[channel][query] += V^T P^T; a lane holds 16 keys of one query in the score tile, and
-// those, rounded to bf16, are the second operand of the V product as they lie; V's operand is read by the transposing LDS read.
-// 32 queries per wave: an operand read from LDS feeds 32 columns, with 16 the LDS (128 bytes per cycle) would take twice the
-// MFMAs' time.  Scores in fp32, running maximum and sum per query.
+// from the cache (its codes expanded once per workgroup on the way to LDS).  Both products run transposed on the QW x QW MFMA:
+// scores^T[key][query] = K Q^T, out^T[channel][query] += V^T P^T; a lane holds the scores of one query, and those, rounded to bf16,
+// are the second operand of the V product as they lie; V's operand is read by the transposing LDS read.
+// 32 queries per wave: an operand read from LDS feeds 32 columns, with 16 the LDS (128 bytes per cycle) takes twice the MFMAs' time;
+// heads of 192 and 256 run on 16, for the registers.  Scores in fp32, running maximum and sum per query.
+// What bounds it: matrix instructions take a third of the time (4 prompts of up to 4100 tokens x 32 heads 183 us, 800 TFLOP/s, where a
+// large library product reaches 1138), the vector instructions of the softmax as much, LDS a quarter; two waves per SIMD overlap them
+// in part.  With neither exponentials nor sums it ran 10 % faster, without loads 14 %, without the way into LDS 6 % (over the cache,
+// where that expands the codes, 35 %).  Tried and slower: this tile's output and the next one's scores as one sequence of independent
+// matrix instructions (219), 256 queries in eight waves (195).
 // A key that a query does not see (a later token, a mask of -inf) adds nothing whatever it holds: its score is replaced, and in
 // tiles where some query misses a key values that are infinite or NaN become zeros on the way to LDS; a workgroup that met
 // such values adds them, one by one, to the outputs of the queries that see them once those are written.
@@ -25,29 +32,40 @@ __device__ __forceinline__ uint32_t mx4_finite(uint32_t pair) {
 
 // Pitch of a row in LDS.  K is read 16 bytes per lane, 16 rows at a time: rows 4 banks apart.  V is read 8 bytes per lane, 4 rows of
 // 64 bytes by 32 lanes: rows 16 banks apart (or 48); at K's pitch half of the cycles of LDS were bank conflicts.
+// (With 16 queries a wave: 8 rows of 32 bytes by 32 lanes, rows 8 banks apart or an odd multiple of that.)
 constexpr int mx4_k_pitch(int NJ) { return 64 * NJ + 16; }
-constexpr int mx4_v_pitch(int NJ) { return NJ % 4 == 3 ? 64 * NJ : 64 * NJ + 64; }
+constexpr int mx4_v_pitch(int NJ, int QW) { return QW == 16 ? 64 * NJ + 32 : NJ % 4 == 3 ? 64 * NJ : 64 * NJ + 64; }
 
-template <int NJ, int QG, int KT, bool CACHE>
-__global__ void __launch_bounds__(QG * KT * 64, NJ <= 4 ? 2 : 1)
+template <int NJ, int QW, int QG, int KT, bool CACHE>
+__global__ void __launch_bounds__(QG * KT * 64, QW == 16 ? (NJ <= 4 && QG == 8 ? 4 : 2) : NJ > 4 ? 1 : 2)
 mx4_prompt_kernel(const Mx4AttnParams p) {
-  constexpr int H = 32 * NJ, KP = mx4_k_pitch(NJ), VP = mx4_v_pitch(NJ), STAGE = 64 * (KP + VP); // K rows, then V rows
-  constexpr int QB = 32 * QG, TH = 64 * QG * KT, NT = 2 / KT; // runs of 32 keys of a tile that a wave takes
+  constexpr int H = 32 * NJ, KP = mx4_k_pitch(NJ), VP = mx4_v_pitch(NJ, QW), D = CACHE ? 2 : 1, STAGE = 64 * (KP + VP); // K rows, then V rows
+  // Scores of a lane: NT runs of QW keys of the tile, NV of each, for one query; its output: NA pieces of QW channels.
+  constexpr int QB = QW * QG, TH = 64 * QG * KT, NT = 64 / QW / KT, NV = QW / 2 * QW / 32, NA = H / QW, HALF = 64 / QW;
+  using Vec = std::conditional_t<QW == 32, f32x16, f32x4>;
   constexpr int PER = CACHE ? NJ : 4 * NJ, ITEMS = 64 * PER, NC = (ITEMS + TH - 1) / TH; // items of a row, of a tile, of a thread
   extern __shared__ __align__(16) uint8_t lds[]; // 2 stages
   __shared__ int odd_values;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % QG, team = __builtin_amdgcn_readfirstlane(tid >> 6) / QG;
-  const int c = lane & 31, h = lane >> 5;
+  const int c = lane % QW, h = lane / QW; // query, and group of lanes that share its keys
   // heads go round the XCDs, those of one K/V head to the same one
   const int hr = (int)blockIdx.x % p.Nq, hk = hr % p.Nkv, hq = hk * p.R + hr / p.Nkv;
+  // Two workgroups share a CU, and the dispatcher puts workgroup i + 256 beside workgroup i: every other run of whole query blocks
+  // within 256 workgroups is walked the other way round, so that a long block meets a short one (2048 tokens x 32 heads, 512
+  // workgroups: 69 us without).
   Block o;
-  if (!locate(p.cu, p.B, p.T, 1, QB, (int)blockIdx.x / p.Nq, o))
+  const int run = max(256 / p.Nq, 1);
+  const auto paired = [&](int k, int all) {
+    const int r = k / run;
+    return (r & 1) && (r + 1) * run <= all ? r * run + run - 1 - k % run : k;
+  };
+  if (!locate(p.cu, p.B, p.T, 1, QB, (int)blockIdx.x / p.Nq, o, paired))
     return;
   const int qblk = (o.n + QB - 1) / QB - 1 - o.at; // the last queries see the most keys: first
   const int past = CACHE ? max(p.past[o.b], 0) : 0;
   const int total = CACHE ? min(past + o.n, p.Smax) : o.n; // keys of the sequence
-  const int q0 = qblk * QB + wave * 32;
+  const int q0 = qblk * QB + wave * QW;
   const int qi = min(q0 + c, o.n - 1);
   const int limit = min(past + qi + 1, total); // keys this lane's query sees
   const int64_t head = ((int64_t)o.b * p.Nkv + hk) * p.Smax;
@@ -59,26 +77,29 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   const uint16_t* const vr = CACHE ? nullptr : p.v + (int64_t)o.start * p.v_ld + hk * H;
   const uint16_t* const mrow = p.mask ? p.mask + (int64_t)o.b * p.mask_ld : nullptr;
 
-  bf16x8 q[2 * NJ];
+  constexpr int NK = H / (8 * HALF); // steps of the score's sum
+  bf16x8 q[NK];
   {
     const uint16_t* qrow = p.q + (int64_t)(o.start + qi) * p.q_ld + (int64_t)hq * H + h * 8;
 #pragma unroll
-    for (int j = 0; j < 2 * NJ; j++)
-      q[j] = *reinterpret_cast<const bf16x8*>(qrow + j * 16);
+    for (int j = 0; j < NK; j++)
+      q[j] = *reinterpret_cast<const bf16x8*>(qrow + j * (8 * HALF));
   }
   // keys that some query of this workgroup sees
   const int keys = min(past + min(qblk * QB + QB, o.n), total), tiles = (keys + 63) / 64;
   const int first_limit = min(past + qblk * QB + 1, total); // keys that all of them see
 
   // Item i of thread tid: 16 bytes of a row of K (V false) or of V; rows past the keys: zeros.  They pass through registers, asked
-  // for a whole tile before they go to LDS.
-  i32x4 k_item[NC], v_item[NC];
-  uint32_t k_byte[CACHE ? NC : 1], v_byte[CACHE ? NC : 1];
+  // for D tiles before they go to LDS: two over the cache (2048 tokens behind 2048 132 -> 124 us), one for bf16 rows, whose second
+  // tile would take 32 registers (1000 tokens 28.0 -> 28.9).
+  i32x4 k_item[D][NC], v_item[D][NC];
+  uint32_t k_byte[D][CACHE ? NC : 1], v_byte[D][CACHE ? NC : 1];
   // (buffers of a tile's rows: what lies past them reads as zero, with no branch and no access)
-  auto request = [&](auto V_, int kb) {
+  auto request = [&](auto V_, auto S_, int kb) {
     constexpr bool V = decltype(V_)::value;
-    auto& item = V ? v_item : k_item;
-    auto& byte = V ? v_byte : k_byte;
+    constexpr int slot = decltype(S_)::value % D;
+    auto& item = V ? v_item[slot] : k_item[slot];
+    auto& byte = V ? v_byte[slot] : k_byte[slot];
     const int rows = min(max(keys - kb * 64, 0), 64);
     auto rsrc = [](const void* at, uint32_t bytes) {
       return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, (int)bytes, 0x00020000);
@@ -106,10 +127,12 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
     const int lo = j & 1 ? w[1] : w[0], hi = j & 1 ? w[3] : w[2];
     return j & 2 ? hi : lo;
   };
-  auto deliver = [&](auto V_, int kb, int stage) {
+  auto turn_of = [](int row) { return QW == 16 ? (row >> 1) & 3 : row & 3; };
+  auto deliver = [&](auto V_, auto S_, int kb) {
     constexpr bool V = decltype(V_)::value;
-    auto& item = V ? v_item : k_item;
-    auto& byte = V ? v_byte : k_byte;
+    constexpr int stage = decltype(S_)::value, slot = stage % D;
+    auto& item = V ? v_item[slot] : k_item[slot];
+    auto& byte = V ? v_byte[slot] : k_byte[slot];
     uint8_t* const st = lds + stage * STAGE + (V ? 64 * KP : 0);
     constexpr int PITCH = V ? VP : KP;
     const bool partial = V && (mrow || kb * 64 + 64 > first_limit); // (uniform)
@@ -125,8 +148,8 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
           const float s = e8m0_to_f32(drop ? 0u : byte[i]);
 #pragma unroll
           for (int j = 0; j < 4; j++) // (V's rows are 16 banks apart, as a block's chunks are: another order of them in each row)
-            *reinterpret_cast<bf16x8*>(dst + (V ? (j ^ (row & 3)) * 16 : j * 16)) =
-                mx4_to_bf16(nan ? 0u : (uint32_t)(V ? chunk_of(item[i], j ^ (row & 3)) : item[i][j]), s); // (zero times infinity)
+            *reinterpret_cast<bf16x8*>(dst + (V ? (j ^ turn_of(row)) * 16 : j * 16)) =
+                mx4_to_bf16(nan ? 0u : (uint32_t)(V ? chunk_of(item[i], j ^ turn_of(row)) : item[i][j]), s); // (zero times infinity)
         }
       } else {
         if (partial) {
@@ -141,7 +164,8 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
           }
           odd |= some;
         }
-        *reinterpret_cast<i32x4*>(st + row * PITCH + ch * 16) = item[i];
+        if (ITEMS % TH == 0 || at < ITEMS)
+          *reinterpret_cast<i32x4*>(st + row * PITCH + ch * 16) = item[i];
       }
     }
     if (odd)
@@ -151,51 +175,69 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   constexpr std::true_type V_{};
 
   float m = LOWEST, l = 0.f;
-  f32x16 acc[NJ];
+  Vec acc[NA];
 #pragma unroll
-  for (int dt = 0; dt < NJ; dt++)
+  for (int dt = 0; dt < NA; dt++)
 #pragma unroll
-    for (int i = 0; i < 16; i++)
+    for (int i = 0; i < NV; i++)
       acc[dt][i] = 0.f;
   const float scale2 = p.scale * LOG2E;
-  const int wave_limit = min(past + min(q0 + 32, o.n), total); // keys that some query of this wave sees
+  const int wave_limit = min(past + min(q0 + QW, o.n), total); // keys that some query of this wave sees
   const bool idle = q0 >= o.n;
 
   if (tid == 0)
     odd_values = 0;
-  request(K_, 0);
-  request(V_, 0);
+  constexpr std::integral_constant<int, 0> EVEN{};
+  constexpr std::integral_constant<int, 1> ODD{};
+  request(K_, EVEN, 0);
+  request(V_, EVEN, 0);
+  if constexpr (D == 2) {
+    request(K_, ODD, 1);
+    request(V_, ODD, 1);
+  }
   __syncthreads();
-  deliver(K_, 0, 0);
-  request(K_, 1);
-  deliver(V_, 0, 0);
-  request(V_, 1);
-  for (int kb = 0; kb < tiles; kb++) {
-    const int stage = kb & 1;
+  deliver(K_, EVEN, 0);
+  request(K_, EVEN, D);
+  deliver(V_, EVEN, 0);
+  request(V_, EVEN, D);
+  auto turn = [&](auto S_, int kb) { // tile kb, in stage kb & 1
+    constexpr int stage = decltype(S_)::value;
+    constexpr std::integral_constant<int, stage ^ 1> NEXT{};
     __syncthreads(); // this tile has been written, the other stage has been read
     const bool more = kb + 1 < tiles, busy = !idle && kb * 64 < wave_limit; // (uniform in a wave)
     const uint8_t* const st = lds + stage * STAGE;
-    bf16x8 pb[2 * NT];
+    bf16x8 pb[NT * NV / 8];
+    Vec sc[NT];
     if (busy) {
-      f32x16 sc[NT];
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int t = 0; t < NT; t++) {
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < NV; i++)
           sc[t][i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2 * NJ; j++)
-          sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(st + ((team + t) * 32 + c) * KP + j * 32 + h * 16), q[j], sc[t], 0, 0, 0);
+        for (int j = 0; j < NK; j++) {
+          const bf16x8 w = *reinterpret_cast<const bf16x8*>(st + (team * 32 + t * QW + c) * KP + (j * HALF + h) * 16);
+          if constexpr (QW == 32)
+            sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, q[j], sc[t], 0, 0, 0);
+          else
+            sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, q[j], sc[t], 0, 0, 0);
+        }
       }
       __builtin_amdgcn_s_setprio(0);
+    }
+    if (KT == 1 && more) { // under the matrix instructions (with half of them it comes better behind the softmax)
+      deliver(K_, NEXT, kb + 1);
+      request(K_, NEXT, kb + 1 + D);
+    }
+    if (busy) {
       // key of score i of run t
-      auto key_of = [&](int t, int i) { return kb * 64 + (team + t) * 32 + (i & 3) + 8 * (i >> 2) + 4 * h; };
+      auto key_of = [&](int t, int i) { return kb * 64 + team * 32 + t * QW + (QW == 32 ? (i & 3) + 8 * (i >> 2) : i) + 4 * h; };
       if (mrow) {
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
+          for (int i = 0; i < NV; i++) {
             const int key = key_of(t, i);
             const float mv = key < p.mask_ld ? bf16_bits_to_f32(mrow[min(key, p.mask_ld - 1)]) : 0.f;
             sc[t][i] = mv == -INFINITY ? -INFINITY : fmaf(sc[t][i], p.scale, mv);
@@ -206,25 +248,29 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-          for (int i = 0; i < 16; i++)
+          for (int i = 0; i < NV; i++)
             sc[t][i] = key_of(t, i) < limit ? sc[t][i] : -INFINITY;
       }
       float mx = m;
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < NV; i++)
           mx = fmaxf(mx, sc[t][i]);
       const float unit = mrow ? LOG2E : scale2;
       float alpha = 1.f;
       // The sums are relative to a maximum that follows the true one once that is 2^8 above it (the probabilities are then at most
       // 2^8: their rounding is relative, and fp32 sums have the room); followed at once, nearly every tile would rescale.
       if (__builtin_amdgcn_ballot_w64((mx - m) * unit > 8.f) != 0) {
-        auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        if constexpr (QW == 16) {
+          mx = max_of_groups(mx);
+        } else {
+          auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        }
         alpha = __builtin_amdgcn_exp2f((m - mx) * unit);
 #pragma unroll
-        for (int dt = 0; dt < NJ; dt++)
+        for (int dt = 0; dt < NA; dt++)
           acc[dt] *= alpha;
         m = mx;
       }
@@ -239,39 +285,51 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < NV; i++) {
           const float pr = __builtin_amdgcn_exp2f(fmaf(sc[t][i], unit, off));
           l += pr;
-          pb[t * 2 + (i >> 3)][i & 7] = (__bf16)pr;
+          pb[(t * NV + i) >> 3][(t * NV + i) & 7] = (__bf16)pr;
         }
     }
-    if (more) {
-      deliver(K_, kb + 1, stage ^ 1);
-      request(K_, kb + 2);
+    if (KT != 1 && more) {
+      deliver(K_, NEXT, kb + 1);
+      request(K_, NEXT, kb + 1 + D);
     }
     if (busy) {
-      // V operand of 16 keys (step u) and 32 channels: two transposing reads of 4 keys each for this lane's half
-      const uint8_t* const vt = st + 64 * KP + (team * 32 + 4 * h + ((lane & 15) >> 2)) * VP + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+      // V operand of the keys of a P operand and QW channels: two transposing reads of 4 keys each for this lane's group (32 queries a
+      // wave: 16 keys, 8 apart; 16: 32 keys, 16 apart)
+      constexpr int KEYS = QW == 32 ? 16 : 32;
+      const uint8_t* const vt = st + 64 * KP + (team * 32 + 4 * h + ((lane & 15) >> 2)) * VP + (QW == 32 ? ((lane >> 4) & 1) * 32 : 0) + (lane & 3) * 8;
       auto operand = [&](int dt, int u, int e) {
         return __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-            (__attribute__((address_space(3))) bf16x4*)(vt + (u * 16 + e * 8) * VP + dt * 64)));
+            (__attribute__((address_space(3))) bf16x4*)(vt + (u * KEYS + e * (KEYS / 2)) * VP + dt * (2 * QW))));
       };
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-      for (int u = 0; u < 2 * NT; u++)
+      for (int u = 0; u < NT * NV / 8; u++)
 #pragma unroll
-        for (int dt = 0; dt < NJ; dt++) {
+        for (int dt = 0; dt < NA; dt++) {
           const i32x2 a = operand(dt, u, 0), b = operand(dt, u, 1);
-          const i32x4 w = {a[0], a[1], b[0], b[1]};
-          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[dt], 0, 0, 0);
+          const bf16x8 w = __builtin_bit_cast(bf16x8, i32x4{a[0], a[1], b[0], b[1]});
+          if constexpr (QW == 32)
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, pb[u], acc[dt], 0, 0, 0);
+          else
+            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, pb[u], acc[dt], 0, 0, 0);
         }
     }
     __builtin_amdgcn_s_setprio(0);
     if (more) {
-      deliver(V_, kb + 1, stage ^ 1);
-      request(V_, kb + 2);
+      deliver(V_, NEXT, kb + 1);
+      request(V_, NEXT, kb + 1 + D);
     }
+  };
+  for (int kb = 0; kb < tiles; kb += 2) {
+    turn(EVEN, kb);
+    if (kb + 1 < tiles)
+      turn(ODD, kb + 1);
   }
+  if constexpr (QW == 16)
+    l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
   if constexpr (KT > 1) { // the second team's state through LDS
     float* const at = reinterpret_cast<float*>(lds) + (wave * 64 + lane) * 4;
@@ -303,16 +361,16 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
     uint16_t* orow = p.out + ((int64_t)(o.start + q0 + c) * p.Nq + hq) * H;
     const float inv = l != 0.f ? 1.0f / l : 0.f; // (nothing seen: zeros)
 #pragma unroll
-    for (int dt = 0; dt < NJ; dt++)
+    for (int dt = 0; dt < NA; dt++)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
+      for (int i = 0; i < NV; i += 4) {
         const uint2 w = make_uint2(f32x2_to_bf16_bits(acc[dt][i] * inv, acc[dt][i + 1] * inv), f32x2_to_bf16_bits(acc[dt][i + 2] * inv, acc[dt][i + 3] * inv));
-        *reinterpret_cast<uint2*>(orow + dt * 32 + 8 * (i >> 2) + 4 * h) = w;
+        *reinterpret_cast<uint2*>(orow + dt * QW + 8 * (i >> 2) + 4 * h) = w;
       }
     if (__builtin_expect(odd_values != 0, 0)) { // (a lane reads what it wrote itself)
       const int from = mrow ? 0 : first_limit / 64 * 64;
 #pragma unroll 1
-      for (int d = 0; d < H; d += 8) {
+      for (int d = 0; d < H; d += 4 * HALF) {
         uint16_t* const o4 = orow + d + 4 * h;
         float f[4];
         for (int e = 0; e < 4; e++)
@@ -341,34 +399,63 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache, hipStream_t stream) {
   // every sequence's last workgroup may be short: at most this many, those past the last one end at once
   auto blocks = [&](int rows) { return ((int64_t)p.T + (int64_t)p.B * (rows - 1)) / rows * p.Nq; };
-  const bool wide = blocks(128) >= 400;
-  const int64_t wgs = wide ? blocks(128) : blocks(64);
-  TPPX_REQUIRE(wgs < ((int64_t)1 << 31), TPPX_ESHAPE, "%s: problem too large", who);
+  const int queries = env_int("TPPX_MX4_PROMPT_QUERIES", blocks(128) >= (cache || H > 128 ? 200 : 400) ? 128 : 64);
   hipError_t e = hipSuccess;
+  int rc = TPPX_OK;
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
-    auto go = [&](auto qg, auto c) {
-      constexpr int QG = decltype(qg)::value;
-      auto kern = mx4_prompt_kernel<NJ, QG, 4 / QG, decltype(c)::value>;
-      const size_t lds = 2 * 64 * (size_t)(mx4_k_pitch(NJ) + mx4_v_pitch(NJ));
+    auto go = [&](auto qw, auto qg, auto kt, auto c) {
+      constexpr int QW = decltype(qw)::value, QG = decltype(qg)::value, KT = decltype(kt)::value;
+      auto kern = mx4_prompt_kernel<NJ, QW, QG, KT, decltype(c)::value>;
+      const int64_t wgs = blocks(QW * QG);
+      const size_t stages = 2 * 64 * (size_t)(mx4_k_pitch(NJ) + mx4_v_pitch(NJ, QW)), teams = KT > 1 ? QG * 64 * 16 * (size_t)(4 * NJ + 1) : 0;
+      const size_t lds = std::max(stages, teams); // (the state of a second team)
+      if (wgs >= ((int64_t)1 << 31)) {
+        rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
+        return;
+      }
       e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
       if (e == hipSuccess)
-        kern<<<dim3((unsigned)wgs), dim3(256), lds, stream>>>(p);
+        kern<<<dim3((unsigned)wgs), dim3(QG * KT * 64), lds, stream>>>(p);
     };
-    auto with_source = [&](auto qg) {
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, 2> two{};
+    constexpr std::integral_constant<int, 4> four{};
+    constexpr std::integral_constant<int, 8> eight{};
+    constexpr std::integral_constant<int, 16> q16{};
+    constexpr std::integral_constant<int, 32> q32{};
+    auto with_source = [&](auto qw, auto qg, auto kt) {
       if (cache)
-        go(qg, std::true_type{});
+        go(qw, qg, kt, std::true_type{});
       else
-        go(qg, std::false_type{});
+        go(qw, qg, kt, std::false_type{});
     };
-    if (wide)
-      with_source(std::integral_constant<int, 4>{});
-    else
-      with_source(std::integral_constant<int, 2>{});
+    if constexpr (NJ > 4) {
+      // 192 and 256 wide: one workgroup's tiles fill the LDS of a CU, and 32 queries a wave its registers at one wave per SIMD; with 16
+      // queries two fit (2048 tokens x 16 heads of 256: 94.7 us, four waves of 32 queries 118; four waves of 16 112).  Few: 500 tokens
+      // behind 700, 64 workgroups of 128 queries: 58.9, of 64: 51.7.
+      if (queries >= 128)
+        with_source(q16, eight, one);
+      else
+        with_source(q16, four, one);
+    } else {
+      // 128 queries in four waves, two workgroups on a CU, from 400 of them on (2048 tokens x 32 heads, 512: 63.7 us, the others 70.7 and
+      // 68.1; 4 prompts of up to 4100 186, 220 and 241; 32-wide waves in eight 128-register ones of 16 queries 59.7 and 210).  Below that
+      // two teams halve the way through a tile: over the cache four groups of queries share an expanded tile from 200 on (512 tokens x
+      // 64 heads behind 6000 keys, 256: 134, 153 with two groups and 167 with one team; 64 tokens behind 4000, 64: 82 and 85), otherwise two
+      // groups (1000 tokens x 32 heads, 256: 28.0, four 28.3, one team 32.8; 333 tokens 12.7, 14.5 and 15.4).
+      if (queries >= 128 && (!cache || blocks(128) >= 400))
+        with_source(q32, four, one);
+      else if (queries >= 128)
+        go(q32, four, two, std::true_type{});
+      else
+        with_source(q32, two, two);
+    }
   });
+  if (rc)
+    return rc;
   if (e != hipSuccess)
     return check_hip(e, who);
   return check_hip(hipGetLastError(), who);
 }
-
 } // namespace tppx
