@@ -512,9 +512,9 @@ mx4_split_kernel(const Mx4AttnParams p) {
 #pragma unroll
     for (int i = 0; i < 16; i++)
       mx = fmaxf(mx, x[i]);
-    // The sums are relative to a maximum that follows the true one once that is 2^8 above it: the probabilities are then at most
-    // 2^8, their rounding is relative, and the fp32 sums have the room.
-    if (__builtin_amdgcn_ballot_w64((mx - m) * to2 > 8.f) != 0) {
+    // The maximum is followed at once: the largest probability is then exactly 1, and the relative error against 64 bits 1.8e-3 for
+    // 16000 keys (2.3e-3 where it follows in steps of 2^8, which saves less than 1 % here).
+    if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
       mx = max_of_groups(mx);
       const float alpha = __builtin_amdgcn_exp2f((m - mx) * to2);
 #pragma unroll

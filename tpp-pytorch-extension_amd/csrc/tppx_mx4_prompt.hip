@@ -260,7 +260,9 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
       const float unit = mrow ? LOG2E : scale2;
       float alpha = 1.f;
       // The sums are relative to a maximum that follows the true one once that is 2^8 above it (the probabilities are then at most
-      // 2^8: their rounding is relative, and fp32 sums have the room); followed at once, nearly every tile would rescale.
+      // 2^8: their rounding is relative, and fp32 sums have the room).  Followed at once, nearly every tile rescales: 4 prompts of up to
+      // 4100 206 us instead of 190.  What it costs is that the largest probability is no longer exactly 1: relative error against 64
+      // bits 2.0e-3 there, 1.8e-3 followed at once, 1.65e-3 the rounding of the output alone.
       if (__builtin_amdgcn_ballot_w64((mx - m) * unit > 8.f) != 0) {
         if constexpr (QW == 16) {
           mx = max_of_groups(mx);
@@ -285,10 +287,11 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-          const float pr = __builtin_amdgcn_exp2f(fmaf(sc[t][i], unit, off));
-          l += pr;
-          pb[(t * NV + i) >> 3][(t * NV + i) & 7] = (__bf16)pr;
+        for (int i = 0; i < NV; i += 2) { // (the sum is that of the rounded ones: where a key outweighs the others its rounding cancels)
+          const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(sc[t][i], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(sc[t][i + 1], unit, off))};
+          l = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l, false);
+          pb[(t * NV + i) >> 3][(t * NV + i) & 7] = pr[0];
+          pb[(t * NV + i) >> 3][((t * NV + i) & 7) + 1] = pr[1];
         }
     }
     if (KT != 1 && more) {
