@@ -90,3 +90,25 @@ def test_plain_forms():
     v = torch.randn((1, 5, 64), dtype=torch.float64)
     out, _ = R.attend(x, torch.zeros((1, 5, 64), dtype=torch.float64), v, 3)
     assert torch.allclose(out[:, 0], torch.stack((v[0, :4].mean(0), v[0].mean(0))))
+
+
+def test_lengths_of_sequences_follow_a_reorder():
+    """Host and device agree on every sequence's length after packed prompts, a beam reorder and a crop; appends of one length are
+    refused while the lengths differ and taken once they do not."""
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    cache = F.Mx4Cache(40)
+    cache.prompts([9, 3, 5], "cpu")
+    cache.advance()
+    cache.reorder_cache(torch.tensor([1, 1, 2]))
+    assert cache.seq_len_dev.tolist() == [3, 3, 5] and cache.get_seq_length() == 5
+    with pytest.raises(F.TppxError):
+        cache.update(torch.zeros(3, 1, 1, 64), torch.zeros(3, 1, 1, 64), 0)
+    with pytest.raises(F.TppxError):
+        cache.prompts([1, 1, 36], "cpu")
+    cache.prompts([37, 0, 1], "cpu")
+    cache.advance()
+    assert cache.seq_len_dev.tolist() == [40, 3, 6] and cache.get_seq_length() == 40
+    cache.crop(4)
+    assert cache.seq_len_dev.tolist() == [4, 3, 4] and cache.get_seq_length() == 4
+    cache.reorder_cache(torch.tensor([1, 1, 1]))
+    assert cache.seq_len_dev.tolist() == [3, 3, 3] and cache.get_seq_length() == 3 and not any(cache._short)

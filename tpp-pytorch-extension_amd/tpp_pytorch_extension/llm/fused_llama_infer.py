@@ -339,7 +339,10 @@ class Mx4Cache(TppCache):
                 t[:, :, :n].copy_(t[:, :, :n].index_select(0, beam_idx.to(t.device)))
         if self.seq_len_dev is not None:
             self.seq_len_dev.copy_(self.seq_len_dev.index_select(0, beam_idx.to(self.seq_len_dev.device)))
-        self._short = None  # (which is shorter now the device knows; the room that is left is judged by the longest)
+        if self._short is not None and any(self._short):  # (the host keeps the lengths too: a ragged cache's order is copied to it)
+            now = [self._host_len - self._short[i] for i in beam_idx.tolist()]
+            self._short = [max(now) - k for k in now]
+            self._advance_host(max(now) - self._host_len)
         self._sums_of = None
 
     def get(self, layer_idx):
