@@ -165,6 +165,14 @@ def test_attention_entry_point_and_cache_methods():
     assert cache.get_seq_length() == 7 and cache.seq_len_dev.tolist() == [7, 7]
     nk, _ = cache.update(R.randn((B, Nkv, 2, H), 1.0, 90).cuda(), R.randn((B, Nkv, 2, H), 1.0, 91).cuda(), 0)
     assert nk.shape[2] == 9 and torch.equal(nk[:, :, :7], k[1:].expand(2, -1, -1, -1)[:, :, :7])
+    mask = torch.zeros((B, 9), dtype=torch.bfloat16)
+    mask[1, 2:5] = float("-inf")
+    q, k, v = R.randn((B, Nkv, 1, Rr, H), 1.0, 92), R.randn((B, Nkv, 1, H), 1.0, 93), R.randn((B, Nkv, 1, H), 1.0, 94)
+    outs = []
+    for m in (mask, mask.view(B, 1, 1, 9)):  # the same mask in two shapes
+        outs.append(at.attn(q.cuda(), k.cuda(), v.cuda(), m.cuda(), cache, 0))
+        cache.crop(9)
+    assert torch.equal(outs[0], outs[1])
     with pytest.raises(F.TppxError):
         at.attn(R.randn((B, Nkv, 1, 1, 80), 1.0, 1).cuda(), R.randn((B, Nkv, 1, 80), 1.0, 1).cuda(), R.randn((B, Nkv, 1, 80), 1.0, 1).cuda(), None,
                 at.kv_cache(8, "mxfp4"), 0)
