@@ -682,8 +682,8 @@ int tppx_attn_prefill(const void* q, const void* kcache, const void* vcache,
  * 128, 192, 256 (others TPPX_EUNSUPPORTED).
  * Packed tokens: rows of q, k, v, out; sequence b owns rows cu[b] .. cu[b + 1] - 1 (cu: device i32 [B + 1], ascending;
  * NULL: one token per sequence, T == B); it held past[b] (device i32 [B]) keys before them.  Row strides *_ld in elements
- * (multiples of 8), heads of a row contiguous.  Rows of T behind cu[B] are neither read nor written.  Values in cu and
- * past that do not fit are clamped on the device.
+ * (multiples of 8), heads of a row contiguous.  Rows of T behind cu[B] take no part: out and the cache are left as they were
+ * there.  Values in cu and past that do not fit are clamped on the device.
  * A cache layer: codes u8 [B][Nkv][Smax][H/2] (E2M1, channel 2i in the low half of byte i; 16-byte aligned) and scales u8
  * [B][Nkv][Smax][H/32] (E8M0) of the keys and of the values.  A block of 32 channels has the scale byte
  * floor(log2 max) + 125; nearest, ties to the even code, 6 at most.  A block whose maximum is below 2^-124 is zero (byte 0), one
@@ -691,7 +691,8 @@ int tppx_attn_prefill(const void* q, const void* kcache, const void* vcache,
 
 /* Per-head RMSNorm of q [T][Nq][H] and k [T][Nkv][H] (bf16; gamma_q / gamma_k f32 or bf16 [H], each may be NULL: no norm)
  * followed by the rotation at pos (i64 [T]; positions outside the table are left unrotated): emb_pos f32 [2][MP][HR] cos / sin
- * on pairs (i, HR/2 + i), or with gptj [MP][HR] sin | cos on adjacent pairs, or NULL.  fp32 inside, one rounding;
+ * on pairs (i, HR/2 + i), the first HR/2 entries of a row being those of both, or with gptj [MP][HR] sin | cos on adjacent pairs, or
+ * NULL.  fp32 inside, one rounding;
  * q_out [T][Nq][H], k_out [T][Nkv][H] contiguous (may be q and k where those are). */
 int tppx_qk_norm_rotary(const void* q, const void* k, const void* gamma_q,
                         const void* gamma_k, int gamma_dtype, float eps,

@@ -6,8 +6,8 @@ embeddings (src/csrc/llm/fused_llm_infer.cpp:150-253).
 
 Packed tokens are rows `[T][heads][H]`: sequence b owns rows `cu_seqlens[b] .. cu_seqlens[b + 1] - 1` (int32 `[B + 1]` on the
 device), or one row each where `cu_seqlens` is None.  `past[b]` (int32 `[B]`, device) is the number of keys that a sequence
-held before these tokens.  Rows of a batch behind the last sequence are neither read nor written: the results hold whatever
-`torch.empty` gave there.
+held before these tokens.  Rows of a batch behind the last sequence take no part: the cache is left as it was, and the results hold
+whatever `torch.empty` gave there.
 
 A layer of the cache is `Mx4Layer(k_codes, k_scales, v_codes, v_scales)`, uint8 `[B][Nkv][capacity][H/2]` (two E2M1 codes a
 byte, the even channel in the low half) and `[B][Nkv][capacity][H/32]` (E8M0).  Head sizes 64, 96, 128, 192 and 256.
@@ -76,7 +76,8 @@ def _norm_weights(q_weight, k_weight, H, like):
 
 
 def _rotation(emb_pos, style, H, like):
-    """(address, gptj, positions, width) of a rotary table: float32 [2][MP][HR] cos / sin ("llama") or [MP][HR] sin | cos ("gptj")."""
+    """(address, gptj, positions, width) of a rotary table: float32 [2][MP][HR] cos / sin ("llama"; a row's first HR/2 entries serve
+    both halves) or [MP][HR] sin | cos ("gptj")."""
     if style not in ("llama", "gptj", None):
         raise TppxError(_lib.EINVAL, f"rotation style {style!r} (\"llama\", \"gptj\" or None)")
     if emb_pos is None or style is None:
@@ -89,8 +90,6 @@ def _rotation(emb_pos, style, H, like):
     if HR > H or HR % 16 or HR == 0 or MP == 0:
         raise TppxError(_lib.ESHAPE, f"rotary width {HR} must be a multiple of 16 and at most the head size {H}")
     return emb_pos.data_ptr(), int(style == "gptj"), MP, HR
-
-
 
 
 def qk_norm_rotary(q, k, q_weight=None, k_weight=None, eps=1e-6, emb_pos=None, pos=None, style="llama"):
