@@ -425,6 +425,26 @@ def test_prompt_forms(H, queries, monkeypatch):
     assert torch.equal(hit[:cu[3] + 130], packed[:cu[3] + 130]) and bool(hit[cu[3] + 130:].isnan().all())
 
 
+@pytest.mark.parametrize("H", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("queries", ["128", "64"])
+def test_prompt_forms_with_values_that_are_not_finite(H, queries, monkeypatch):
+    """Infinite and NaN keys and values behind a mask of -inf, of a neighbouring sequence and of later tokens, in both forms."""
+    monkeypatch.setenv("TPPX_MX4_PROMPT_QUERIES", queries)
+    at = _at()
+    Nq, Nkv, new = 2, 1, [133, 70]
+    cu = _starts(new)
+    q, k, v = (R.randn((cu[-1] + 3, n, H), 1.0, 60 + i) for i, n in enumerate((Nq, Nkv, Nkv)))
+    mask = torch.zeros((2, 133), dtype=torch.bfloat16)
+    mask[0, 3:7] = mask[0, 66] = -math.inf
+    k[3:7], v[5:7], v[66] = math.nan, math.inf, math.nan
+    v[132], k[cu[1] + 69], v[cu[2]:] = -math.inf, math.nan, math.nan  # seen by the last token alone, by the last of the other one, by none
+    got = at.attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu), mask.cuda()).cpu()
+    assert bool((got[132] == -math.inf).all()) and bool(got[cu[2] - 1].isnan().all())
+    for b in range(2):
+        rows = slice(cu[b], cu[b + 1] - 1)
+        _within(got[rows], *R.attend(q[rows], k[rows].transpose(0, 1).double(), v[rows].transpose(0, 1).double(), 0, mask[b]))
+
+
 @pytest.mark.parametrize("H", [64, 96, 128])
 def test_prompts_of_many_heads(H):
     """400 workgroups of 128 queries: the form of large launches, by its own rule."""

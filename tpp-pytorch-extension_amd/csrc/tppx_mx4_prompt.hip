@@ -6,21 +6,18 @@
 namespace tppx {
 
 // ---------------------------------------------------------------------------
-// Prompts: QG groups of QW queries of one head, each a wave, or with KT = 2 two that take half of every tile's keys (and are
-// merged at the end: launches of few workgroups), share K and V tiles of 64 keys, bf16 in LDS in two stages, from packed rows or
-// from the cache (its codes expanded once per workgroup on the way to LDS).  Both products run transposed on the QW x QW MFMA:
-// scores^T[key][query] = K Q^T, out^T[channel][query] += V^T P^T; a lane holds the scores of one query, and those, rounded to bf16,
-// are the second operand of the V product as they lie; V's operand is read by the transposing LDS read.
-// 32 queries per wave: an operand read from LDS feeds 32 columns, with 16 the LDS (128 bytes per cycle) takes twice the MFMAs' time;
-// heads of 192 and 256 run on 16, for the registers.  Scores in fp32, running maximum and sum per query.
-// What bounds it: matrix instructions take a third of the time (4 prompts of up to 4100 tokens x 32 heads 183 us, 800 TFLOP/s, where a
-// large library product reaches 1138), the vector instructions of the softmax as much, LDS a quarter; two waves per SIMD overlap them
-// in part.  With neither exponentials nor sums it ran 10 % faster, without loads 14 %, without the way into LDS 6 % (over the cache,
-// where that expands the codes, 35 %).  Tried and slower: this tile's output and the next one's scores as one sequence of independent
-// matrix instructions (219), 256 queries in eight waves (195).
+// In both kernels a workgroup takes the queries of one head in groups, a wave each, which share K and V tiles of 64 keys, bf16 in LDS in
+// two stages.  Both products run transposed: scores^T[key][query] = K Q^T, out^T[channel][query] += V^T P^T; a lane holds the
+// scores of one query, and those, rounded to bf16, are the second operand of the V product as they lie; V's operand is read by the
+// transposing LDS read.  Scores in fp32, running maximum and sum per query.
+// The sums are relative to a maximum that follows the true one once that is 2^8 above it (the probabilities are then at most 2^8: their
+// rounding is relative, and fp32 sums have the room).  Followed at once, nearly every tile rescales: 4 prompts of up to 4100 206 us
+// instead of 190 when that was measured.  What it costs is that the largest probability is no longer exactly 1: relative error against
+// 64 bits 2.0e-3 there, 1.8e-3 followed at once, 1.65e-3 the rounding of the output alone.  The probabilities' sum is that of the rounded
+// ones: where a key outweighs the others its rounding cancels.
 // A key that a query does not see (a later token, a mask of -inf) adds nothing whatever it holds: its score is replaced, and in
-// tiles where some query misses a key values that are infinite or NaN become zeros on the way to LDS; a workgroup that met
-// such values adds them, one by one, to the outputs of the queries that see them once those are written.
+// tiles where some query misses a key values that are infinite or NaN become zeros in LDS; a workgroup that met such values adds them,
+// one by one, to the outputs of the queries that see them once those are written.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ bool mx4_non_finite(uint32_t pair) {
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
@@ -30,20 +27,50 @@ __device__ __forceinline__ uint32_t mx4_finite(uint32_t pair) {
   return ((pair & 0x7f80u) == 0x7f80u ? 0u : pair & 0xffffu) | ((pair & 0x7f800000u) == 0x7f800000u ? 0u : pair & 0xffff0000u);
 }
 
+// Values that are not finite, added one by one to what a lane wrote itself: channels d + 4 lane .. + 3 of a row of H, keys from .. limit - 1.
+template <int H, int LANES, typename F>
+__device__ __forceinline__ void mx4_add_non_finite(uint16_t* orow, int lane, int from, int limit, const uint16_t* mrow, int mask_ld, F&& value) {
+#pragma unroll 1
+  for (int d = 4 * lane; d < H; d += 4 * LANES) {
+    float f[4];
+    for (int e = 0; e < 4; e++)
+      f[e] = bf16_bits_to_f32(orow[d + e]);
+#pragma unroll 1
+    for (int key = from; key < limit; key++) {
+      if (mrow && key < mask_ld && bf16_bits_to_f32(mrow[key]) == -INFINITY)
+        continue;
+      for (int e = 0; e < 4; e++) {
+        const uint32_t w = value(key, d + e);
+        if ((w & 0x7f80u) == 0x7f80u)
+          f[e] += bf16_bits_to_f32(w);
+      }
+    }
+    for (int e = 0; e < 4; e++)
+      orow[d + e] = (uint16_t)f32_to_bf16_bits(f[e]);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Over the MXFP4 cache: QG groups of QW queries, or with KT = 2 two waves for each that take half of every tile's keys (and are
+// merged at the end: launches of few workgroups).  Codes are expanded once per workgroup on the way to LDS.  32 queries per wave: an
+// operand read from LDS feeds 32 columns; heads of 192 and 256 run on 16, for the registers.
+// What bounds it: the way of the codes into LDS (without it 35 % less) and, as in the packed kernel, the chain scores, softmax, output
+// of a wave.  512 tokens x 64 heads behind 6000 keys 134 .. 147 us (boxes differ), 720 .. 780 TFLOP/s.
+// ---------------------------------------------------------------------------
 // Pitch of a row in LDS.  K is read 16 bytes per lane, 16 rows at a time: rows 4 banks apart.  V is read 8 bytes per lane, 4 rows of
 // 64 bytes by 32 lanes: rows 16 banks apart (or 48); at K's pitch half of the cycles of LDS were bank conflicts.
 // (With 16 queries a wave: 8 rows of 32 bytes by 32 lanes, rows 8 banks apart or an odd multiple of that.)
 constexpr int mx4_k_pitch(int NJ) { return 64 * NJ + 16; }
 constexpr int mx4_v_pitch(int NJ, int QW) { return QW == 16 ? 64 * NJ + 32 : NJ % 4 == 3 ? 64 * NJ : 64 * NJ + 64; }
 
-template <int NJ, int QW, int QG, int KT, bool CACHE>
+template <int NJ, int QW, int QG, int KT>
 __global__ void __launch_bounds__(QG * KT * 64, QW == 16 ? (NJ <= 4 && QG == 8 ? 4 : 2) : NJ > 4 ? 1 : 2)
 mx4_prompt_kernel(const Mx4AttnParams p) {
-  constexpr int H = 32 * NJ, KP = mx4_k_pitch(NJ), VP = mx4_v_pitch(NJ, QW), D = CACHE ? 2 : 1, STAGE = 64 * (KP + VP); // K rows, then V rows
+  constexpr int H = 32 * NJ, KP = mx4_k_pitch(NJ), VP = mx4_v_pitch(NJ, QW), D = 2, STAGE = 64 * (KP + VP); // K rows, then V rows
   // Scores of a lane: NT runs of QW keys of the tile, NV of each, for one query; its output: NA pieces of QW channels.
   constexpr int QB = QW * QG, TH = 64 * QG * KT, NT = 64 / QW / KT, NV = QW / 2 * QW / 32, NA = H / QW, HALF = 64 / QW;
   using Vec = std::conditional_t<QW == 32, f32x16, f32x4>;
-  constexpr int PER = CACHE ? NJ : 4 * NJ, ITEMS = 64 * PER, NC = (ITEMS + TH - 1) / TH; // items of a row, of a tile, of a thread
+  constexpr int PER = NJ, ITEMS = 64 * PER, NC = (ITEMS + TH - 1) / TH; // items of a row, of a tile, of a thread
   extern __shared__ __align__(16) uint8_t lds[]; // 2 stages
   __shared__ int odd_values;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -63,18 +90,16 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   if (!locate(p.cu, p.B, p.T, 1, QB, (int)blockIdx.x / p.Nq, o, paired))
     return;
   const int qblk = (o.n + QB - 1) / QB - 1 - o.at; // the last queries see the most keys: first
-  const int past = CACHE ? max(p.past[o.b], 0) : 0;
-  const int total = CACHE ? min(past + o.n, p.Smax) : o.n; // keys of the sequence
+  const int past = max(p.past[o.b], 0);
+  const int total = min(past + o.n, p.Smax); // keys of the sequence
   const int q0 = qblk * QB + wave * QW;
   const int qi = min(q0 + c, o.n - 1);
   const int limit = min(past + qi + 1, total); // keys this lane's query sees
   const int64_t head = ((int64_t)o.b * p.Nkv + hk) * p.Smax;
-  const uint8_t* const kq = CACHE ? p.kq + head * (16 * NJ) : nullptr;
-  const uint8_t* const vq = CACHE ? p.vq + head * (16 * NJ) : nullptr;
-  const uint8_t* const ks = CACHE ? p.ks + head * NJ : nullptr;
-  const uint8_t* const vs = CACHE ? p.vs + head * NJ : nullptr;
-  const uint16_t* const kr = CACHE ? nullptr : p.k + (int64_t)o.start * p.k_ld + hk * H;
-  const uint16_t* const vr = CACHE ? nullptr : p.v + (int64_t)o.start * p.v_ld + hk * H;
+  const uint8_t* const kq = p.kq + head * (16 * NJ);
+  const uint8_t* const vq = p.vq + head * (16 * NJ);
+  const uint8_t* const ks = p.ks + head * NJ;
+  const uint8_t* const vs = p.vs + head * NJ;
   const uint16_t* const mrow = p.mask ? p.mask + (int64_t)o.b * p.mask_ld : nullptr;
 
   constexpr int NK = H / (8 * HALF); // steps of the score's sum
@@ -89,11 +114,10 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   const int keys = min(past + min(qblk * QB + QB, o.n), total), tiles = (keys + 63) / 64;
   const int first_limit = min(past + qblk * QB + 1, total); // keys that all of them see
 
-  // Item i of thread tid: 16 bytes of a row of K (V false) or of V; rows past the keys: zeros.  They pass through registers, asked
-  // for D tiles before they go to LDS: two over the cache (2048 tokens behind 2048 132 -> 124 us), one for bf16 rows, whose second
-  // tile would take 32 registers (1000 tokens 28.0 -> 28.9).
+  // Item i of thread tid: a block of a row of K (V false) or of V; rows past the keys: zeros.  They pass through registers, asked for two
+  // tiles before they are expanded on the way to LDS (2048 tokens behind 2048 124 us, one tile before 132).
   i32x4 k_item[D][NC], v_item[D][NC];
-  uint32_t k_byte[D][CACHE ? NC : 1], v_byte[D][CACHE ? NC : 1];
+  uint32_t k_byte[D][NC], v_byte[D][NC];
   // (buffers of a tile's rows: what lies past them reads as zero, with no branch and no access)
   auto request = [&](auto V_, auto S_, int kb) {
     constexpr bool V = decltype(V_)::value;
@@ -104,23 +128,13 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
     auto rsrc = [](const void* at, uint32_t bytes) {
       return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, (int)bytes, 0x00020000);
     };
-    if constexpr (CACHE) {
-      const auto codes = rsrc((V ? vq : kq) + (int64_t)kb * (64 * 16 * NJ), rows * (16 * NJ));
-      const auto scales = rsrc((V ? vs : ks) + (int64_t)kb * (64 * NJ), rows * NJ);
+    const auto codes = rsrc((V ? vq : kq) + (int64_t)kb * (64 * 16 * NJ), rows * (16 * NJ));
+    const auto scales = rsrc((V ? vs : ks) + (int64_t)kb * (64 * NJ), rows * NJ);
 #pragma unroll
-      for (int i = 0; i < NC; i++) {
-        const int at = i * TH + tid;
-        item[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(codes, at * 16, 0, 0));
-        byte[i] = __builtin_amdgcn_raw_buffer_load_b8(scales, at, 0, 0);
-      }
-    } else {
-      const int64_t ld = V ? p.v_ld : p.k_ld;
-      const auto src = rsrc((V ? vr : kr) + (int64_t)kb * 64 * ld, rows ? (uint32_t)(((rows - 1) * (uint32_t)ld + H) * 2) : 0u);
-#pragma unroll
-      for (int i = 0; i < NC; i++) {
-        const int at = i * TH + tid;
-        item[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(src, (at / PER) * ((uint32_t)ld * 2) + (at % PER) * 16, 0, 0));
-      }
+    for (int i = 0; i < NC; i++) {
+      const int at = i * TH + tid;
+      item[i] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(codes, at * 16, 0, 0));
+      byte[i] = __builtin_amdgcn_raw_buffer_load_b8(scales, at, 0, 0);
     }
   };
   auto chunk_of = [](const i32x4& w, int j) { // (no indexed registers)
@@ -140,32 +154,15 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 #pragma unroll
     for (int i = 0; i < NC; i++) {
       const int at = i * TH + tid, row = at / PER, ch = at % PER;
-      if constexpr (CACHE) {
-        uint8_t* const dst = st + row * PITCH + ch * 64;
-        if (ITEMS % TH == 0 || at < ITEMS) {
-          const bool nan = byte[i] == 255u, drop = nan && partial;
-          odd |= drop;
-          const float s = e8m0_to_f32(drop ? 0u : byte[i]);
+      uint8_t* const dst = st + row * PITCH + ch * 64;
+      if (ITEMS % TH == 0 || at < ITEMS) {
+        const bool nan = byte[i] == 255u, drop = nan && partial;
+        odd |= drop;
+        const float s = e8m0_to_f32(drop ? 0u : byte[i]);
 #pragma unroll
-          for (int j = 0; j < 4; j++) // (V's rows are 16 banks apart, as a block's chunks are: another order of them in each row)
-            *reinterpret_cast<bf16x8*>(dst + (V ? (j ^ turn_of(row)) * 16 : j * 16)) =
-                mx4_to_bf16(nan ? 0u : (uint32_t)(V ? chunk_of(item[i], j ^ turn_of(row)) : item[i][j]), s); // (zero times infinity)
-        }
-      } else {
-        if (partial) {
-          bool some = false;
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-            some |= mx4_non_finite((uint32_t)item[i][j]);
-          if (some) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              item[i][j] = (int)mx4_finite((uint32_t)item[i][j]);
-          }
-          odd |= some;
-        }
-        if (ITEMS % TH == 0 || at < ITEMS)
-          *reinterpret_cast<i32x4*>(st + row * PITCH + ch * 16) = item[i];
+        for (int j = 0; j < 4; j++) // (V's rows are 16 banks apart, as a block's chunks are: another order of them in each row)
+          *reinterpret_cast<bf16x8*>(dst + (V ? (j ^ turn_of(row)) * 16 : j * 16)) =
+              mx4_to_bf16(nan ? 0u : (uint32_t)(V ? chunk_of(item[i], j ^ turn_of(row)) : item[i][j]), s); // (zero times infinity)
       }
     }
     if (odd)
@@ -191,10 +188,8 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   constexpr std::integral_constant<int, 1> ODD{};
   request(K_, EVEN, 0);
   request(V_, EVEN, 0);
-  if constexpr (D == 2) {
-    request(K_, ODD, 1);
-    request(V_, ODD, 1);
-  }
+  request(K_, ODD, 1);
+  request(V_, ODD, 1);
   __syncthreads();
   deliver(K_, EVEN, 0);
   request(K_, EVEN, D);
@@ -259,10 +254,6 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
           mx = fmaxf(mx, sc[t][i]);
       const float unit = mrow ? LOG2E : scale2;
       float alpha = 1.f;
-      // The sums are relative to a maximum that follows the true one once that is 2^8 above it (the probabilities are then at most
-      // 2^8: their rounding is relative, and fp32 sums have the room).  Followed at once, nearly every tile rescales: 4 prompts of up to
-      // 4100 206 us instead of 190.  What it costs is that the largest probability is no longer exactly 1: relative error against 64
-      // bits 2.0e-3 there, 1.8e-3 followed at once, 1.65e-3 the rounding of the output alone.
       if (__builtin_amdgcn_ballot_w64((mx - m) * unit > 8.f) != 0) {
         if constexpr (QW == 16) {
           mx = max_of_groups(mx);
@@ -287,7 +278,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int i = 0; i < NV; i += 2) { // (the sum is that of the rounded ones: where a key outweighs the others its rounding cancels)
+        for (int i = 0; i < NV; i += 2) {
           const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(sc[t][i], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(sc[t][i + 1], unit, off))};
           l = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l, false);
           pb[(t * NV + i) >> 3][(t * NV + i) & 7] = pr[0];
@@ -370,56 +361,321 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
         const uint2 w = make_uint2(f32x2_to_bf16_bits(acc[dt][i] * inv, acc[dt][i + 1] * inv), f32x2_to_bf16_bits(acc[dt][i + 2] * inv, acc[dt][i + 3] * inv));
         *reinterpret_cast<uint2*>(orow + dt * QW + 8 * (i >> 2) + 4 * h) = w;
       }
-    if (__builtin_expect(odd_values != 0, 0)) { // (a lane reads what it wrote itself)
-      const int from = mrow ? 0 : first_limit / 64 * 64;
-#pragma unroll 1
-      for (int d = 0; d < H; d += 4 * HALF) {
-        uint16_t* const o4 = orow + d + 4 * h;
-        float f[4];
-        for (int e = 0; e < 4; e++)
-          f[e] = bf16_bits_to_f32(o4[e]);
-#pragma unroll 1
-        for (int key = from; key < limit; key++) {
-          if (mrow && key < p.mask_ld && bf16_bits_to_f32(mrow[key]) == -INFINITY)
-            continue;
-          for (int e = 0; e < 4; e++) {
-            uint32_t w;
-            if constexpr (CACHE)
-              w = vs[(int64_t)key * NJ + (d >> 5)] == 255 ? 0x7fc0u : 0u;
-            else
-              w = vr[(int64_t)key * p.v_ld + d + 4 * h + e];
-            if ((w & 0x7f80u) == 0x7f80u)
-              f[e] += bf16_bits_to_f32(w);
-          }
-        }
-        for (int e = 0; e < 4; e++)
-          o4[e] = (uint16_t)f32_to_bf16_bits(f[e]);
+    if (__builtin_expect(odd_values != 0, 0))
+      mx4_add_non_finite<H, HALF>(orow, h, mrow ? 0 : first_limit / 64 * 64, limit, mrow, p.mask_ld,
+                                  [&](int key, int ch) { return vs[(int64_t)key * NJ + (ch >> 5)] == 255 ? 0x7fc0u : 0u; });
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Packed bf16 prompts: W waves of 16 queries, tiles brought by loads straight into LDS, one ahead.  The chunks of 16 bytes of a row lie
+// permuted (those loads write 1024 bytes in a row), so that neither the rows of a K operand nor the pieces that the transposing read
+// of V takes meet in a bank.
+// What bounds it: the chain scores, softmax, output of a wave (matrix instructions take 0.35 of the time); so four waves per SIMD in 128
+// registers count for more than operands that feed 32 queries.  Measured against 32 queries a wave, two per SIMD, the tiles through
+// registers: 4 prompts of up to 4100 tokens x 32 heads 187 -> 171 us (860 TFLOP/s, where a large library product reaches 1138), 2048 x
+// 32 heads 64 -> 52, 2048 x 64 on 8 95 -> 85, 2048 x 16 of 256 93 -> 77, 333 x 32 12.7 -> 10.6, 4 x 1000 x 12 of 64 28 -> 24.
+// Tried in that other form and slower: this tile's output and the next one's scores as one sequence of independent matrix
+// instructions (219 where it took 190), 256 queries in eight waves (195).
+// ---------------------------------------------------------------------------
+constexpr int packed_k_turn(int NJ, int row) { return NJ % 4 == 0 ? row & 15 : NJ % 2 == 0 ? (row >> 1) & 7 : (row >> 2) & 3; }
+constexpr int packed_v_turn(int NJ, int row) { return 2 * (NJ % 4 == 0 ? row & 7 : NJ % 2 == 0 ? (row >> 1) & 3 : (row >> 2) & 1); }
+
+// The transposing reads of V for 32 keys and N pieces of 16 channels, issued and waited for in one block (around the builtin the
+// compiler waits for every load into LDS under way): piece d at a[d % X] + d / X * STEP, keys 16 .. 31 at + ROWS.
+template <int OFF, int ROWS>
+__device__ __forceinline__ void packed_v_operands(i32x2 (&v)[8][2], const uint32_t (&a)[8]) {
+  asm volatile("ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %1, %16 offset:%25\n\t"
+               "ds_read_b64_tr_b16 %2, %17 offset:%24\n\tds_read_b64_tr_b16 %3, %17 offset:%25\n\t"
+               "ds_read_b64_tr_b16 %4, %18 offset:%24\n\tds_read_b64_tr_b16 %5, %18 offset:%25\n\t"
+               "ds_read_b64_tr_b16 %6, %19 offset:%24\n\tds_read_b64_tr_b16 %7, %19 offset:%25\n\t"
+               "ds_read_b64_tr_b16 %8, %20 offset:%24\n\tds_read_b64_tr_b16 %9, %20 offset:%25\n\t"
+               "ds_read_b64_tr_b16 %10, %21 offset:%24\n\tds_read_b64_tr_b16 %11, %21 offset:%25\n\t"
+               "ds_read_b64_tr_b16 %12, %22 offset:%24\n\tds_read_b64_tr_b16 %13, %22 offset:%25\n\t"
+               "ds_read_b64_tr_b16 %14, %23 offset:%24\n\tds_read_b64_tr_b16 %15, %23 offset:%25\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]),
+                 "=&v"(v[3][1]), "=&v"(v[4][0]), "=&v"(v[4][1]), "=&v"(v[5][0]), "=&v"(v[5][1]), "=&v"(v[6][0]), "=&v"(v[6][1]),
+                 "=&v"(v[7][0]), "=&v"(v[7][1])
+               : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "n"(OFF), "n"(OFF + ROWS)
+               : "memory");
+}
+template <int OFF, int ROWS>
+__device__ __forceinline__ void packed_v_operands(i32x2 (&v)[4][2], const uint32_t (&a)[4]) {
+  asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]),
+                 "=&v"(v[3][1])
+               : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF), "n"(OFF + ROWS)
+               : "memory");
+}
+template <int OFF, int ROWS> // (96 wide: six pieces at two addresses)
+__device__ __forceinline__ void packed_v_operands(i32x2 (&v)[6][2], const uint32_t (&a)[2]) {
+  asm volatile("ds_read_b64_tr_b16 %0, %12 offset:%14\n\tds_read_b64_tr_b16 %1, %12 offset:%15\n\t"
+               "ds_read_b64_tr_b16 %2, %13 offset:%14\n\tds_read_b64_tr_b16 %3, %13 offset:%15\n\t"
+               "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %12 offset:%17\n\t"
+               "ds_read_b64_tr_b16 %6, %13 offset:%16\n\tds_read_b64_tr_b16 %7, %13 offset:%17\n\t"
+               "ds_read_b64_tr_b16 %8, %12 offset:%18\n\tds_read_b64_tr_b16 %9, %12 offset:%19\n\t"
+               "ds_read_b64_tr_b16 %10, %13 offset:%18\n\tds_read_b64_tr_b16 %11, %13 offset:%19\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]),
+                 "=&v"(v[3][1]), "=&v"(v[4][0]), "=&v"(v[4][1]), "=&v"(v[5][0]), "=&v"(v[5][1])
+               : "v"(a[0]), "v"(a[1]), "n"(OFF), "n"(OFF + ROWS), "n"(OFF + 64), "n"(OFF + 64 + ROWS), "n"(OFF + 128), "n"(OFF + 128 + ROWS)
+               : "memory");
+}
+
+// 16 bytes per lane straight into LDS, 1024 in a row from `to` on
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t src, uint8_t* to, uint32_t offset) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 16, offset, 0, 0, 0);
+}
+
+template <int NJ, int W>
+__global__ void __launch_bounds__(W * 64, W == 8 && NJ <= 4 ? 4 : 2)
+mx4_packed_kernel(const Mx4AttnParams p) {
+  constexpr int H = 32 * NJ, ROW = 64 * NJ, PER = 4 * NJ, SIDE = 64 * ROW, QB = 16 * W, TH = 64 * W, NA = H / 16;
+  // Addresses of operands that differ in the turn of their chunks (the others lie at fixed distances), pieces of V per read.
+  constexpr int XK = NJ % 4 == 0 ? 4 : NJ % 2 == 0 ? 2 : 1, XV = NJ % 4 == 0 ? 8 : NJ % 2 == 0 ? 4 : 2, NR = NJ == 3 ? 6 : XV;
+  extern __shared__ __align__(16) uint8_t lds[]; // V of two stages, then K
+  __shared__ int odd_values;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  const int hr = (int)blockIdx.x % p.Nq, hk = hr % p.Nkv, hq = hk * p.R + hr / p.Nkv;
+  Block o;
+  const int run = max(256 / p.Nq, 1);
+  const auto paired = [&](int k, int all) {
+    const int r = k / run;
+    return (r & 1) && (r + 1) * run <= all ? r * run + run - 1 - k % run : k;
+  };
+  if (!locate(p.cu, p.B, p.T, 1, QB, (int)blockIdx.x / p.Nq, o, paired))
+    return;
+  const int qblk = (o.n + QB - 1) / QB - 1 - o.at; // the last queries see the most keys: first
+  const int q0 = qblk * QB + wave * 16;
+  const int qi = min(q0 + c, o.n - 1); // this lane's query: sees the keys 0 .. qi
+  const uint16_t* const kr = p.k + (int64_t)o.start * p.k_ld + hk * H;
+  const uint16_t* const vr = p.v + (int64_t)o.start * p.v_ld + hk * H;
+  const uint16_t* const mrow = p.mask ? p.mask + (int64_t)o.b * p.mask_ld : nullptr;
+  bf16x8 q[NJ];
+  {
+    const uint16_t* qrow = p.q + (int64_t)(o.start + qi) * p.q_ld + (int64_t)hq * H + g * 8;
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+      q[j] = *reinterpret_cast<const bf16x8*>(qrow + j * 32);
+  }
+  const int keys = min(qblk * QB + QB, o.n), tiles = (keys + 63) / 64; // keys that some query of this workgroup sees
+  const int first_limit = qblk * QB + 1;                              // keys that all of them see
+
+  // Pieces of 1024 bytes: with eight waves four bring K and four V, NJ pieces each; with four each brings NJ of both.
+  constexpr int SIDES = W == 8 ? 1 : 2;
+  uint32_t from[SIDES][NJ]; // offset of this lane's chunk in the tile's rows
+  auto side_of = [&](int s) { return W == 8 ? wave >> 2 : s; }; // 1: V
+  auto offset = [&](int s, int i, int rows) {
+    const int item = ((W == 8 ? wave & 3 : wave) * NJ + i) * 64 + lane, row = item / PER, ch = item % PER;
+    const int turn = side_of(s) ? packed_v_turn(NJ, row) : packed_k_turn(NJ, row);
+    return ((uint32_t)min(row, rows - 1) * (uint32_t)(side_of(s) ? p.v_ld : p.k_ld) + (uint32_t)(ch ^ turn) * 8u) * 2u;
+  };
+#pragma unroll
+  for (int s = 0; s < SIDES; s++)
+#pragma unroll
+    for (int i = 0; i < NJ; i++)
+      from[s][i] = offset(s, i, 64);
+  auto request = [&](int kb, int stage) {
+    const int rows = min(keys - kb * 64, 64);
+#pragma unroll
+    for (int s = 0; s < SIDES; s++) {
+      const int64_t ld = side_of(s) ? p.v_ld : p.k_ld;
+      const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>((side_of(s) ? vr : kr) + (int64_t)kb * 64 * ld), 0,
+                                                         (int)(((uint32_t)(rows - 1) * (uint32_t)ld + H) * 2u), 0x00020000);
+      uint8_t* const dst = lds + (side_of(s) ? 0 : 2 * SIDE) + stage * SIDE + (W == 8 ? wave & 3 : wave) * (NJ * 1024);
+#pragma unroll
+      for (int i = 0; i < NJ; i++) { // (rows past the keys repeat the last one)
+        const uint32_t at = rows < 64 ? offset(s, i, rows) : from[s][i];
+        load_to_lds(src, dst + i * 1024, at);
       }
     }
+  };
+  uint32_t kaddr[XK], vaddr[XV];
+#pragma unroll
+  for (int j = 0; j < XK; j++)
+    kaddr[j] = (uint32_t)(2 * SIDE + c * ROW + ((j * 4 + g) ^ packed_k_turn(NJ, c)) * 16);
+  {
+    const int r = g * 4 + (c >> 2);
+#pragma unroll
+    for (int d = 0; d < XV; d++)
+      vaddr[d] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds + (uint32_t)(r * ROW + ((d * 2 + ((c >> 1) & 1)) ^ packed_v_turn(NJ, r)) * 16 + (c & 1) * 8);
+  }
+
+  float m, l;
+  f32x4 acc[NA];
+  // Values that are not finite leave V (in LDS) where some query may not see them.  Four waves look for them only once a sum came out
+  // infinite or NaN, in a second run over the tiles (333 tokens x 32 heads 11.0 -> 10.4 us, 2 masked prompts of 700 41 -> 36); eight look in
+  // the first (the second run's registers are more than 128: 52 -> 56 us for 2048).
+  bool careful = W == 8;
+  const float unit = mrow ? LOG2E : p.scale * LOG2E;
+  if (tid == 0)
+    odd_values = 0;
+  auto tile = [&](auto S_, int kb) {
+    constexpr int stage = decltype(S_)::value;
+    // this tile has landed and the other stage has been read, for this wave and then for every wave
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    if (careful && (mrow || kb * 64 + 64 > first_limit)) { // (uniform) some query may not see some key
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < (256 * NJ + TH - 1) / TH; i++) {
+        const int at = i * TH + tid;
+        if (256 * NJ % TH == 0 || at < 256 * NJ) {
+          i32x4* const it = reinterpret_cast<i32x4*>(lds + stage * SIDE) + at;
+          const i32x4 w = *it;
+          bool some = false;
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            some |= mx4_non_finite((uint32_t)w[j]);
+          if (some)
+            *it = i32x4{(int)mx4_finite((uint32_t)w[0]), (int)mx4_finite((uint32_t)w[1]), (int)mx4_finite((uint32_t)w[2]), (int)mx4_finite((uint32_t)w[3])};
+          odd |= some;
+        }
+      }
+      if (odd)
+        odd_values = 1;
+      __syncthreads();
+    }
+    if (kb + 1 < tiles)
+      request(kb + 1, stage ^ 1); // in flight during the arithmetic below
+    if (kb * 64 > min(q0 + 15, o.n - 1) || q0 >= o.n)
+      return; // past what this wave's queries see
+    const uint8_t* const st = lds + stage * SIDE;
+    f32x4 sc[4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+      sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(st + kaddr[j % XK] + t * (16 * ROW) + j / XK * (XK * 64)), q[j], sc[t], 0, 0, 0);
+    }
+    if (mrow) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int key = kb * 64 + (i >> 2) * 16 + g * 4 + (i & 3);
+        const float mv = key < p.mask_ld ? bf16_bits_to_f32(mrow[min(key, p.mask_ld - 1)]) : 0.f;
+        sc[i >> 2][i & 3] = mv == -INFINITY ? -INFINITY : fmaf(sc[i >> 2][i & 3], p.scale, mv);
+      }
+    }
+    if (kb * 64 + 63 > q0) { // (wave-uniform)
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        sc[i >> 2][i & 3] = kb * 64 + (i >> 2) * 16 + g * 4 + (i & 3) <= qi ? sc[i >> 2][i & 3] : -INFINITY;
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      mx = fmaxf(mx, sc[i >> 2][i & 3]);
+    if (__builtin_amdgcn_ballot_w64((mx - m) * unit > 8.f) != 0) {
+      mx = max_of_groups(mx);
+      const float alpha = __builtin_amdgcn_exp2f((m - mx) * unit);
+#pragma unroll
+      for (int dt = 0; dt < NA; dt++)
+        acc[dt] *= alpha;
+      l *= alpha;
+      m = mx;
+    }
+    float off = -m * unit;
+    if (mrow) { // (the difference first: a mask's lowest value times log2 e is no number)
+      off = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; t++)
+        sc[t] -= m;
+    }
+    bf16x8 pb[2];
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(sc[i >> 2][(i & 3) + 1], unit, off))};
+      l = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l, false);
+      pb[i >> 3][i & 7] = pr[0];
+      pb[i >> 3][(i & 7) + 1] = pr[1];
+    }
+    static_for<0, 2 * (NA / NR)>([&](auto I) { // 32 keys, NR pieces of channels
+      constexpr int u = decltype(I)::value / (NA / NR), d0 = decltype(I)::value % (NA / NR) * NR;
+      i32x2 vv[NR][2];
+      packed_v_operands<stage * SIDE + u * 32 * ROW + d0 * 32, 16 * ROW>(vv, vaddr);
+#pragma unroll
+      for (int d = 0; d < NR; d++) {
+        const i32x4 w = {vv[d][0][0], vv[d][0][1], vv[d][1][0], vv[d][1][1]};
+        acc[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[d0 + d], 0, 0, 0);
+      }
+    });
+  };
+  for (;;) {
+    m = LOWEST;
+    l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NA; dt++)
+      acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    request(0, 0);
+    for (int kb = 0; kb < tiles; kb += 2) {
+      tile(std::integral_constant<int, 0>{}, kb);
+      if (kb + 1 < tiles)
+        tile(std::integral_constant<int, 1>{}, kb + 1);
+    }
+    if (careful)
+      break;
+    f32x4 none = {0.f, 0.f, 0.f, 0.f}; // NaN where a sum is infinite or NaN
+#pragma unroll
+    for (int dt = 0; dt < NA; dt++)
+      none += acc[dt] * 0.f;
+    if (!__syncthreads_or(!(none[0] + none[1] + none[2] + none[3] == 0.f)))
+      break;
+    careful = true; // once more: an unseen value may be among them
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  if (q0 + c < o.n) {
+    uint16_t* orow = p.out + ((int64_t)(o.start + q0 + c) * p.Nq + hq) * H;
+    const float inv = l != 0.f ? 1.0f / l : 0.f; // (nothing seen: zeros)
+#pragma unroll
+    for (int dt = 0; dt < NA; dt++)
+      *reinterpret_cast<uint2*>(orow + dt * 16 + g * 4) =
+          make_uint2(f32x2_to_bf16_bits(acc[dt][0] * inv, acc[dt][1] * inv), f32x2_to_bf16_bits(acc[dt][2] * inv, acc[dt][3] * inv));
+    if (__builtin_expect(odd_values != 0, 0))
+      mx4_add_non_finite<H, 4>(orow, g, mrow ? 0 : first_limit / 64 * 64, qi + 1, mrow, p.mask_ld, [&](int key, int ch) { return (uint32_t)vr[(int64_t)key * p.v_ld + ch]; });
   }
 }
 
 int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache, hipStream_t stream) {
   // every sequence's last workgroup may be short: at most this many, those past the last one end at once
   auto blocks = [&](int rows) { return ((int64_t)p.T + (int64_t)p.B * (rows - 1)) / rows * p.Nq; };
-  const int queries = env_int("TPPX_MX4_PROMPT_QUERIES", blocks(128) >= (cache || H > 128 ? 200 : 400) ? 128 : 64);
+  const bool many = env_int("TPPX_MX4_PROMPT_QUERIES", blocks(128) >= (cache || H > 128 ? 200 : 400) ? 128 : 64) >= 128;
   hipError_t e = hipSuccess;
   int rc = TPPX_OK;
+  auto go = [&](auto kern, int queries, int threads, size_t lds) {
+    const int64_t wgs = blocks(queries);
+    if (wgs >= ((int64_t)1 << 31)) {
+      rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
+      return;
+    }
+    e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
+    if (e == hipSuccess)
+      kern<<<dim3((unsigned)wgs), dim3(threads), lds, stream>>>(p);
+  };
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
-    auto go = [&](auto qw, auto qg, auto kt, auto c) {
+    if (!cache) {
+      // 128 queries in eight waves from some 400 workgroups of them on, else 64 in four (2048 tokens x 32 heads, 512: 52.0 us, of 64 59.9; 4
+      // prompts of up to 4100 171 and 209; 2048 x 16 heads of 256, 256: 77 and 91; 1000 x 32 heads, 256: 25.3 and 24.1; 4 x 1000 x 12 of 64,
+      // 384: 23.5 and 22.0; 333 x 32 11.7 and 11.4).
+      constexpr size_t lds = 4 * 64 * 64 * (size_t)NJ;
+      if (many)
+        go(mx4_packed_kernel<NJ, 8>, 128, 512, lds);
+      else
+        go(mx4_packed_kernel<NJ, 4>, 64, 256, lds);
+      return;
+    }
+    auto over = [&](auto qw, auto qg, auto kt) {
       constexpr int QW = decltype(qw)::value, QG = decltype(qg)::value, KT = decltype(kt)::value;
-      auto kern = mx4_prompt_kernel<NJ, QW, QG, KT, decltype(c)::value>;
-      const int64_t wgs = blocks(QW * QG);
       const size_t stages = 2 * 64 * (size_t)(mx4_k_pitch(NJ) + mx4_v_pitch(NJ, QW)), teams = KT > 1 ? QG * 64 * 16 * (size_t)(4 * NJ + 1) : 0;
-      const size_t lds = std::max(stages, teams); // (the state of a second team)
-      if (wgs >= ((int64_t)1 << 31)) {
-        rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
-        return;
-      }
-      e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
-      if (e == hipSuccess)
-        kern<<<dim3((unsigned)wgs), dim3(QG * KT * 64), lds, stream>>>(p);
+      go(mx4_prompt_kernel<NJ, QW, QG, KT>, QW * QG, QG * KT * 64, std::max(stages, teams)); // (the state of a second team)
     };
     constexpr std::integral_constant<int, 1> one{};
     constexpr std::integral_constant<int, 2> two{};
@@ -427,38 +683,28 @@ int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache
     constexpr std::integral_constant<int, 8> eight{};
     constexpr std::integral_constant<int, 16> q16{};
     constexpr std::integral_constant<int, 32> q32{};
-    auto with_source = [&](auto qw, auto qg, auto kt) {
-      if (cache)
-        go(qw, qg, kt, std::true_type{});
-      else
-        go(qw, qg, kt, std::false_type{});
-    };
     if constexpr (NJ > 4) {
       // 192 and 256 wide: one workgroup's tiles fill the LDS of a CU, and 32 queries a wave its registers at one wave per SIMD; with 16
-      // queries two fit (2048 tokens x 16 heads of 256: 94.7 us, four waves of 32 queries 118; four waves of 16 112).  Few: 500 tokens
-      // behind 700, 64 workgroups of 128 queries: 58.9, of 64: 51.7.
-      if (queries >= 128)
-        with_source(q16, eight, one);
+      // queries two fit.  Few: 500 tokens behind 700, 64 workgroups of 128 queries: 58.9, of 64: 51.7.
+      if (many)
+        over(q16, eight, one);
       else
-        with_source(q16, four, one);
+        over(q16, four, one);
     } else {
-      // 128 queries in four waves, two workgroups on a CU, from 400 of them on (2048 tokens x 32 heads, 512: 63.7 us, the others 70.7 and
-      // 68.1; 4 prompts of up to 4100 186, 220 and 241; 32-wide waves in eight 128-register ones of 16 queries 59.7 and 210).  Below that
-      // two teams halve the way through a tile: over the cache four groups of queries share an expanded tile from 200 on (512 tokens x
-      // 64 heads behind 6000 keys, 256: 134, 153 with two groups and 167 with one team; 64 tokens behind 4000, 64: 82 and 85), otherwise two
-      // groups (1000 tokens x 32 heads, 256: 28.0, four 28.3, one team 32.8; 333 tokens 12.7, 14.5 and 15.4).
-      if (queries >= 128 && (!cache || blocks(128) >= 400))
-        with_source(q32, four, one);
-      else if (queries >= 128)
-        go(q32, four, two, std::true_type{});
+      // 128 queries in four waves, two workgroups on a CU, from 400 of them on.  Below that two teams halve the way through a tile: four
+      // groups of queries share an expanded tile from 200 on (512 tokens x 64 heads behind 6000 keys, 256: 134, 153 with two groups and 167
+      // with one team; 64 tokens behind 4000, 64: 82 and 85), otherwise two groups.  Eight waves of 16 queries that expand into the layout
+      // of the packed kernel: 168 and 81 there, 2048 tokens x 32 heads behind 2048 127, as here.
+      if (many && blocks(128) >= 400)
+        over(q32, four, one);
+      else if (many)
+        over(q32, four, two);
       else
-        with_source(q32, two, two);
+        over(q32, two, two);
     }
   });
   if (rc)
     return rc;
-  if (e != hipSuccess)
-    return check_hip(e, who);
-  return check_hip(hipGetLastError(), who);
+  return check_hip(e != hipSuccess ? e : hipGetLastError(), who);
 }
 } // namespace tppx
