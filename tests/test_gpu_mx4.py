@@ -34,6 +34,12 @@ def _within(got, want, tol):
                                  f"{float(((got.double().cpu() - want).abs() / tol).max()):.3g} times it, first {bad.nonzero()[:3].tolist()}")
 
 
+def _prompt_form(queries, monkeypatch):
+    """Empty: the form that the sizes give; "64", "128": the prompt kernels with so many queries per workgroup, whatever they are."""
+    if queries:
+        monkeypatch.setenv("TPPX_MX4_PROMPT_QUERIES", queries)
+
+
 # -- norm and rotation ----------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("H,width,style", [(64, 64, "llama"), (96, 96, "llama"), (128, 128, "llama"), (128, 64, "llama"), (192, 48, "llama"),
                                            (256, 256, "llama"), (256, 64, "gptj"), (96, 96, "gptj"), (128, 128, None)])
@@ -157,8 +163,10 @@ def test_single_tokens(H, Nq, Nkv, past, cap):
 @pytest.mark.parametrize("H", [64, 96, 128, 256])
 @pytest.mark.parametrize("Nq,Nkv,new,past", [(4, 4, [2, 1, 0, 3], [0, 70, 5, 1]), (14, 2, [9, 5], [120, 64]), (8, 1, [3], [700]), (2, 2, [70, 33], [0, 90]),
                                              (4, 2, [130, 1, 65], [0, 3, 64])])
-def test_several_tokens(H, Nq, Nkv, new, past):
+@pytest.mark.parametrize("queries", ["", "64"])
+def test_several_tokens(H, Nq, Nkv, new, past, queries, monkeypatch):
     at = _at()
+    _prompt_form(queries, monkeypatch)
     B, cu = len(new), _starts(new)
     cap = max(p + n for p, n in zip(past, new)) + 3
     layer, k, v = _filled(B, Nkv, cap, H, H + cap)
@@ -194,8 +202,10 @@ def _masks(kind, B, keys):
 @pytest.mark.parametrize("kind", ["padding", "lowest everywhere", "nothing", "some", "short"])
 @pytest.mark.parametrize("H,Nq,Nkv,new,past", [(128, 8, 2, None, [100, 3]), (64, 4, 4, None, [64, 300]), (128, 6, 3, [4, 2], [90, 0]),
                                                (128, 2, 1, [140, 70], [10, 0]), (256, 2, 2, [130], [5])])
-def test_masks(kind, H, Nq, Nkv, new, past):
+@pytest.mark.parametrize("queries", ["", "128", "64"])
+def test_masks(kind, H, Nq, Nkv, new, past, queries, monkeypatch):
     at = _at()
+    _prompt_form(queries, monkeypatch)
     B = len(past)
     lens = new or [1] * B
     cu = _starts(lens)
@@ -216,8 +226,10 @@ def test_masks(kind, H, Nq, Nkv, new, past):
 
 
 @pytest.mark.parametrize("new,past", [([1], [80]), ([3], [80]), ([140], [0])])
-def test_a_block_of_nan_reaches_the_tokens_that_see_it_alone(new, past):
+@pytest.mark.parametrize("queries", ["", "128", "64"])
+def test_a_block_of_nan_reaches_the_tokens_that_see_it_alone(new, past, queries, monkeypatch):
     at = _at()
+    _prompt_form(queries, monkeypatch)
     H, Nq, Nkv = 128, 4, 2
     n = past[0] + new[0]
     layer, k, v = _filled(1, Nkv, n, H, 9)
@@ -447,7 +459,7 @@ def test_prompt_forms_with_values_that_are_not_finite(H, queries, monkeypatch):
 
 @pytest.mark.parametrize("H", [64, 96, 128])
 def test_prompts_of_many_heads(H):
-    """400 workgroups of 128 queries: the form of large launches, by its own rule."""
+    """More than 400 workgroups of 128 queries: the form of large launches, by its own rule."""
     at = _at()
     Nq, new, past = 104, [131, 130], [0, 40]
     cu = _starts(new)

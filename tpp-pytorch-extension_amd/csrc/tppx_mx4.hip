@@ -780,12 +780,19 @@ static int split_launch(const char* who, Mx4AttnParams& p, int H, void* ws, int6
   p.cols = p.cu ? 16 : std::min(16, p.R);
   const int64_t trips = ((int64_t)p.Smax + W * 64 - 1) / (W * 64);
   // 512 workgroups, two per CU: 32 x 16000 keys of 8 K/V heads (256 units) 88.5 us with two splits, 93 with three, 105 with four;
-  // 8 x 3000 of 16, 256 wide (128) 23.4 with two, 24.0 with four, 26.9 with twelve; 1 x 2048 of 32 (32) 12.6 with one, 7.8 with four,
-  // 6.9 with eight; 1 x 16000 of 8 (8) 73 with one, 11.0 with 32; 16 x 2048 of 32 (512) 25.2 with one, 28.9 with two.  Splits beyond
-  // a sequence's keys end at once.
+  // 8 x 3000 of 16, 256 wide (128) 34 with one, 24.3 with two, 24.7 with four, 27 with twelve; 1 x 2048 of 32 (32) 12.6 with one, 7.8
+  // with four, 6.9 with eight; 1 x 16000 of 8 (8) 73 with one, 11.0 with 32; 16 x 2048 of 32 (512) 25.2 with one, 28.9 with two.  Splits
+  // beyond a sequence's keys end at once.
+  // The merge costs 2 to 4 us, most with 16 columns and many units; a trip over W * 64 keys is about one: split where that saves five
+  // trips (24 x 2000 of 8 (192): 15.4 with one split, 16.4 with two; 32 x 500 (256) 7.0 and 8.8; 6 x 12 tokens of 28 heads on 4 behind 1500
+  // (148) 12.0, with three 14.6; 64 of 32 heads behind 2000 (128) 16.2, with four 14.4), with single tokens and up to 128 units two
+  // (4 x 700 of 16, 256 wide (64) 12.4, with three 8.6; 4 x 1000 of 32 (128) 8.5, with four 8.0).
   int64_t S = env_int("TPPX_MX4_SPLITS", 0);
-  if (S <= 0)
-    S = 512 / units;
+  if (S <= 0) {
+    S = std::min<int64_t>(std::max<int64_t>(512 / units, 1), trips);
+    if (trips - (trips + S - 1) / S < (p.cu || units > 128 ? 5 : 2))
+      S = 1;
+  }
   S = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(trips, 32), S));
   if (!ws || units * S * p.cols * (H + 2) * (int64_t)sizeof(float) > ws_bytes || units * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) > counter_bytes)
     S = 1;
@@ -901,7 +908,13 @@ extern "C" int tppx_attn_mx4(const void* q, const void* k_codes, const void* k_s
   p.past = (const int32_t*)past; p.cu = (const int32_t*)cu; p.mask = (const uint16_t*)mask; p.mask_ld = (int)mask_ld; p.out = (uint16_t*)out;
   p.T = (int)T; p.B = (int)B; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.R = (int)(Nq / Nkv); p.Smax = (int)Smax;
   p.scale = 1.0f / sqrtf((float)H);
-  if (!cu || T * p.R <= 128 * B)
+  // The prompt kernel expands a tile of the cache for 64 or 128 queries of one head, this one reads it for 16 (token, head) pairs: from
+  // enough queries on to fill the chip (T * Nq) the former does less for each, below that its few workgroups walk all keys.  Split
+  // kernel and prompt kernel, us: 64 tokens x 64 heads on 8 behind 6000 keys 36 and 120, 256 tokens 94 and 124, 384 133 and 149;
+  // 512 x 32 heads behind 2000 46 and 56, 768 66 and 64; 4 x 500 x 12 of 64 19.7 and 22.4; 1200 x 16 of 256 75 and 82.
+  // Many sequences of few tokens leave its blocks of queries empty: 32 x 32 tokens x 32 heads 37 and 57, x 48 53 and 68, x 64 67 and 69.
+  const int64_t blocks = (T + B * 127) / 128 * Nq;
+  if (!cu || (env_int("TPPX_MX4_PROMPT_QUERIES", 0) == 0 && T * Nq * 640 <= 24576 * std::max<int64_t>(640, blocks)))
     return split_launch(who, p, (int)H, ws, ws_bytes, counters, counter_bytes, (hipStream_t)stream);
   return mx4_prompt_launch(who, p, (int)H, true, (hipStream_t)stream);
 }

@@ -371,7 +371,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 // Packed bf16 prompts: W waves of 16 queries, tiles brought by loads straight into LDS, one ahead.  The chunks of 16 bytes of a row lie
 // permuted (those loads write 1024 bytes in a row), so that neither the rows of a K operand nor the pieces that the transposing read
 // of V takes meet in a bank.
-// What bounds it: the chain scores, softmax, output of a wave (matrix instructions take 0.35 of the time); so four waves per SIMD in 128
+// What bounds it: the chain scores, softmax, output of a wave (matrix instructions take 0.39 of the time); so four waves per SIMD in 128
 // registers count for more than operands that feed 32 queries.  Measured against 32 queries a wave, two per SIMD, the tiles through
 // registers: 4 prompts of up to 4100 tokens x 32 heads 187 -> 171 us (860 TFLOP/s, where a large library product reaches 1138), 2048 x
 // 32 heads 64 -> 52, 2048 x 64 on 8 95 -> 85, 2048 x 16 of 256 93 -> 77, 333 x 32 12.7 -> 10.6, 4 x 1000 x 12 of 64 28 -> 24.
