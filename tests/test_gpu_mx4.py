@@ -408,6 +408,53 @@ def test_bounds_on_the_device_that_do_not_fit_stay_inside():
     torch.cuda.synchronize()
 
 
+def test_offsets_beyond_32_bits(monkeypatch):
+    """Slots whose codes lie more than 4 GiB into a layer: the append, single tokens, several, and the prompt kernel over the cache."""
+    at = _at()
+    H, far = 256, 1 << 25  # 128 bytes of codes a slot
+    layer = _empty_layer(1, 1, far + 300, H)
+    layer.v_codes.fill_(0x22)  # 1.0
+    layer.v_scales.fill_(127)
+    k = torch.ones((130, 1, H), dtype=torch.bfloat16, device="cuda")
+    cu = _i32([0, 130])
+    at.append_mx4(None, k, 2 * k, layer, _i32([far]), cu, style=None)
+    assert bool((layer.v_codes[0, 0, far:far + 130] == layer.v_codes[0, 0, far, 0]).all()) and bool((layer.k_scales[0, 0, far:far + 130] == 125).all())
+    assert not bool(layer.k_scales[0, 0, :far].any()) and bool((layer.v_codes[0, 0, far + 130:] == 0x22).all())
+    # scores: 0 before slot `far`, sqrt(H) = 16 from it on
+    q = torch.ones((130, 1, H), dtype=torch.bfloat16, device="cuda")
+
+    def want(n):
+        return (far + 2 * n * math.exp(16)) / (far + n * math.exp(16))
+
+    one = at.attn_mx4(q[:1], layer, _i32([far + 129]))
+    some = at.attn_mx4(q, layer, _i32([far]), cu)
+    _prompt_form("64", monkeypatch)
+    many = at.attn_mx4(q, layer, _i32([far]), cu)
+    # (the sums of 2^25 equal terms are exact in fp32, 32 or more at a time; what rounds is the output, the probabilities and exp)
+    for n, got in ((130, one[0]), (1, some[0]), (130, some[129]), (1, many[0]), (130, many[129])):
+        assert bool(((got.double() - want(n)).abs() <= (2.0 ** -8 + 2.0 ** -8 + 2.0 ** -12) * want(n)).all()), (n, got[0, 0].item(), want(n))
+
+
+def test_two_streams_at_once():
+    """Split attention on two streams at the same time: each has its own partial results and counters."""
+    at = _at()
+    H, Nq, Nkv, cap = 128, 8, 2, 4000
+    layer, _, _ = _filled(2, Nkv, cap, H, 41)
+    qs = [R.randn((2, Nq, H), 1.0, 42 + i).cuda() for i in range(2)]
+    past = [_i32([3990, 2700]), _i32([900, 3999])]
+    alone = [at.attn_mx4(q, layer, p) for q, p in zip(qs, past)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i].append(at.attn_mx4(qs[i], layer, past[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in outs[i])
+
+
 # -- the forms that larger calls take ------------------------------------------------------------------------------------
 @pytest.mark.parametrize("H", [64, 96, 128, 192, 256])
 @pytest.mark.parametrize("queries", ["128", "64"])

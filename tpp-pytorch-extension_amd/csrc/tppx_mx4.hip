@@ -913,6 +913,8 @@ extern "C" int tppx_attn_mx4(const void* q, const void* k_codes, const void* k_s
   // kernel and prompt kernel, us: 64 tokens x 64 heads on 8 behind 6000 keys 36 and 120, 256 tokens 94 and 124, 384 133 and 149;
   // 512 x 32 heads behind 2000 46 and 56, 768 66 and 64; 4 x 500 x 12 of 64 19.7 and 22.4; 1200 x 16 of 256 75 and 82.
   // Many sequences of few tokens leave its blocks of queries empty: 32 x 32 tokens x 32 heads 37 and 57, x 48 53 and 68, x 64 67 and 69.
+  // (32 columns for a wave of the split kernel, whose expanded operands then serve twice: 512 x 32 heads 45 -> 39, 384 x 64 129 -> 119, below
+  // 900 units and from 512 x 64 on slower than what runs there: left out.)
   const int64_t blocks = (T + B * 127) / 128 * Nq;
   if (!cu || (env_int("TPPX_MX4_PROMPT_QUERIES", 0) == 0 && T * Nq * 640 <= 24576 * std::max<int64_t>(640, blocks)))
     return split_launch(who, p, (int)H, ws, ws_bytes, counters, counter_bytes, (hipStream_t)stream);
