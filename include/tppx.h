@@ -716,10 +716,10 @@ int tppx_append_mx4(const void* q, const void* k, const void* v,
 
 /* Attention over the cache, after the tokens' own keys went to it: token i of sequence b sees the keys 0 .. past[b] + i.
  * softmax(q K^T / sqrt(H) + mask) V; mask bf16 [B][mask_ld] over key positions or NULL (0 past mask_ld); a key under -inf is not
- * looked at; rows that see nothing are zeros.  Few tokens per sequence: keys split over workgroups where ws
- * (256-byte aligned scratch, no state) holds the partial results and counters (u32 words 256 bytes apart, zero before the
- * first launch, left zero) has one per 16 (token, query head) pairs of a K/V head; otherwise unsplit.  Launches that share
- * either must be ordered. */
+ * looked at; rows that see nothing are zeros.  Sums are divided at the end, in fp32, which holds those of values below 2^95 at
+ * any length.  Few tokens: keys split over workgroups where ws (256-byte aligned scratch, no state) holds the partial results and
+ * counters (u32 words 256 bytes apart, zero before the first launch, left zero) has one per 16 (token, query head) pairs of a
+ * K/V head; otherwise unsplit.  Launches that share either must be ordered. */
 int tppx_attn_mx4(const void* q, const void* k_codes, const void* k_scales,
                   const void* v_codes, const void* v_scales, const void* past,
                   const void* cu, const void* mask, int64_t mask_ld, void* out,

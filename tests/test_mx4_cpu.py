@@ -112,3 +112,9 @@ def test_lengths_of_sequences_follow_a_reorder():
     assert cache.seq_len_dev.tolist() == [4, 3, 4] and cache.get_seq_length() == 4
     cache.reorder_cache(torch.tensor([1, 1, 1]))
     assert cache.seq_len_dev.tolist() == [3, 3, 3] and cache.get_seq_length() == 3 and not any(cache._short)
+
+
+def test_generate_packed_refuses_no_prompts():
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    with pytest.raises(F.TppxError):
+        F.LlamaDecoder.generate_packed(None, [], 3)

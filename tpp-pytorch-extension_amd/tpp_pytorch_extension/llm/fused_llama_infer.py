@@ -796,6 +796,8 @@ class LlamaDecoder:
     def generate_packed(self, prompts, n_new, capacity=None, use_graph=True):
         """`generate` for prompts of different lengths (a list of i64 [n]): one packed pass, then one token per sequence and step.
         Returns i64 [B][n_new]."""
+        if not prompts:
+            raise TppxError(_lib.ESHAPE, "generate_packed: no prompts")
         cache = Mx4Cache(capacity or max(int(p.numel()) for p in prompts) + n_new + 32)
         first = self.prefill_packed(prompts, cache).view(-1, 1)
         if n_new == 1:
