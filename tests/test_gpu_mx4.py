@@ -520,6 +520,35 @@ def test_prompts_of_many_heads(H):
         _within(packed[rows], *R.attend_rows(q[rows], kp[rows].transpose(0, 1).double(), vp[rows].transpose(0, 1).double(), 0))
 
 
+@pytest.mark.parametrize("H,Nq,Nkv", [(128, 72, 8), (192, 26, 13), (256, 26, 26)])
+def test_many_short_prompts(H, Nq, Nkv):
+    """The form of large launches of short prompts, by its own rule: a mask, keys and values that are not finite where they are not
+    seen, prompts of one token and of none."""
+    at = _at()
+    new = [70, 1, 33, 0, 32, 97, 64, 65]
+    cu = _starts(new)
+    q, k, v = (R.randn((cu[-1], n, H), 1.1, 90 + i) for i, n in enumerate((Nq, Nkv, Nkv)))
+    got = at.attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu))
+    for b in range(len(new)):
+        rows = slice(cu[b], cu[b + 1])
+        if new[b]:
+            _within(got[rows], *R.attend_rows(q[rows], k[rows].transpose(0, 1).double(), v[rows].transpose(0, 1).double(), 0))
+    v[cu[5] + 40, 0], k[cu[5] + 96, Nkv - 1] = math.inf, math.nan  # seen from there on, by the last token alone
+    hit = at.attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu))
+    first = Nq // Nkv
+    assert torch.equal(hit[cu[5]:cu[5] + 40], got[cu[5]:cu[5] + 40]) and bool((hit[cu[5] + 40:cu[5] + 96, :first] == math.inf).all())
+    assert torch.equal(hit[cu[5] + 40:cu[5] + 96, first:], got[cu[5] + 40:cu[5] + 96, first:]) and bool(hit[cu[5] + 96, -first:].isnan().all())
+    assert torch.equal(hit[:cu[5]], got[:cu[5]]) and torch.equal(hit[cu[6]:], got[cu[6]:])
+    mask = _masks("some", 8, 97)
+    k[cu[5] + 96] = 0.0
+    v[cu[5] + 40] = 0.0
+    k[cu[5] + 3], v[cu[5] + 6] = math.nan, math.nan  # behind -inf
+    got = at.attn_packed(q.cuda(), k.cuda(), v.cuda(), _i32(cu), mask.cuda())
+    rows = slice(cu[5], cu[6])
+    _within(got[rows, ::13], *R.attend(q[rows, ::13], k[rows].transpose(0, 1).double()[torch.arange(0, Nq, 13) * Nkv // Nq],
+                                       v[rows].transpose(0, 1).double()[torch.arange(0, Nq, 13) * Nkv // Nq], 0, mask[5]))
+
+
 @pytest.mark.parametrize("H", [64, 128, 192])
 @pytest.mark.parametrize("splits", ["1", "3", "32"])
 def test_splits(H, splits, monkeypatch):

@@ -368,7 +368,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Packed bf16 prompts: W waves of 16 queries, tiles brought by loads straight into LDS, one ahead.  The chunks of 16 bytes of a row lie
+// Packed bf16 prompts: W waves of 16 queries, tiles of KEYS keys brought by loads straight into LDS, one ahead.  The chunks of 16 bytes of a row lie
 // permuted (those loads write 1024 bytes in a row), so that neither the rows of a K operand nor the pieces that the transposing read
 // of V takes meet in a bank.
 // What bounds it: the chain scores, softmax, output of a wave (matrix instructions take 0.39 of the time); so four waves per SIMD in 128
@@ -432,10 +432,10 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t src, uint8_t*
   __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 16, offset, 0, 0, 0);
 }
 
-template <int NJ, int W>
-__global__ void __launch_bounds__(W * 64, W == 8 && NJ <= 4 ? 4 : 2)
+template <int NJ, int W, int KEYS>
+__global__ void __launch_bounds__(W * 64, NJ == 4 && (W == 8 || KEYS == 32) ? 4 : 2)
 mx4_packed_kernel(const Mx4AttnParams p) {
-  constexpr int H = 32 * NJ, ROW = 64 * NJ, PER = 4 * NJ, SIDE = 64 * ROW, QB = 16 * W, TH = 64 * W, NA = H / 16;
+  constexpr int H = 32 * NJ, ROW = 64 * NJ, PER = 4 * NJ, SIDE = KEYS * ROW, QB = 16 * W, TH = 64 * W, NA = H / 16;
   // Addresses of operands that differ in the turn of their chunks (the others lie at fixed distances), pieces of V per read.
   constexpr int XK = NJ % 4 == 0 ? 4 : NJ % 2 == 0 ? 2 : 1, XV = NJ % 4 == 0 ? 8 : NJ % 2 == 0 ? 4 : 2, NR = NJ == 3 ? 6 : XV;
   extern __shared__ __align__(16) uint8_t lds[]; // V of two stages, then K
@@ -465,15 +465,15 @@ mx4_packed_kernel(const Mx4AttnParams p) {
     for (int j = 0; j < NJ; j++)
       q[j] = *reinterpret_cast<const bf16x8*>(qrow + j * 32);
   }
-  const int keys = min(qblk * QB + QB, o.n), tiles = (keys + 63) / 64; // keys that some query of this workgroup sees
+  const int keys = min(qblk * QB + QB, o.n), tiles = (keys + KEYS - 1) / KEYS; // keys that some query of this workgroup sees
   const int first_limit = qblk * QB + 1;                              // keys that all of them see
 
-  // Pieces of 1024 bytes: with eight waves four bring K and four V, NJ pieces each; with four each brings NJ of both.
-  constexpr int SIDES = W == 8 ? 1 : 2;
+  // Pieces of 1024 bytes: KEYS / 16 waves bring K, NJ pieces each, and as many V, others or the same.
+  constexpr int SW = KEYS / 16, SIDES = W == SW ? 2 : 1;
   uint32_t from[SIDES][NJ]; // offset of this lane's chunk in the tile's rows
-  auto side_of = [&](int s) { return W == 8 ? wave >> 2 : s; }; // 1: V
+  auto side_of = [&](int s) { return SIDES == 1 ? wave / SW : s; }; // 1: V
   auto offset = [&](int s, int i, int rows) {
-    const int item = ((W == 8 ? wave & 3 : wave) * NJ + i) * 64 + lane, row = item / PER, ch = item % PER;
+    const int item = (wave % SW * NJ + i) * 64 + lane, row = item / PER, ch = item % PER;
     const int turn = side_of(s) ? packed_v_turn(NJ, row) : packed_k_turn(NJ, row);
     return ((uint32_t)min(row, rows - 1) * (uint32_t)(side_of(s) ? p.v_ld : p.k_ld) + (uint32_t)(ch ^ turn) * 8u) * 2u;
   };
@@ -481,18 +481,18 @@ mx4_packed_kernel(const Mx4AttnParams p) {
   for (int s = 0; s < SIDES; s++)
 #pragma unroll
     for (int i = 0; i < NJ; i++)
-      from[s][i] = offset(s, i, 64);
+      from[s][i] = offset(s, i, KEYS);
   auto request = [&](int kb, int stage) {
-    const int rows = min(keys - kb * 64, 64);
+    const int rows = min(keys - kb * KEYS, KEYS);
 #pragma unroll
     for (int s = 0; s < SIDES; s++) {
       const int64_t ld = side_of(s) ? p.v_ld : p.k_ld;
-      const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>((side_of(s) ? vr : kr) + (int64_t)kb * 64 * ld), 0,
+      const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>((side_of(s) ? vr : kr) + (int64_t)kb * KEYS * ld), 0,
                                                          (int)(((uint32_t)(rows - 1) * (uint32_t)ld + H) * 2u), 0x00020000);
-      uint8_t* const dst = lds + (side_of(s) ? 0 : 2 * SIDE) + stage * SIDE + (W == 8 ? wave & 3 : wave) * (NJ * 1024);
+      uint8_t* const dst = lds + (side_of(s) ? 0 : 2 * SIDE) + stage * SIDE + wave % SW * (NJ * 1024);
 #pragma unroll
       for (int i = 0; i < NJ; i++) { // (rows past the keys repeat the last one)
-        const uint32_t at = rows < 64 ? offset(s, i, rows) : from[s][i];
+        const uint32_t at = rows < KEYS ? offset(s, i, rows) : from[s][i];
         load_to_lds(src, dst + i * 1024, at);
       }
     }
@@ -510,10 +510,10 @@ mx4_packed_kernel(const Mx4AttnParams p) {
 
   float m, l;
   f32x4 acc[NA];
-  // Values that are not finite leave V (in LDS) where some query may not see them.  Four waves look for them only once a sum came out
-  // infinite or NaN, in a second run over the tiles (333 tokens x 32 heads 11.0 -> 10.4 us, 2 masked prompts of 700 41 -> 36); eight look in
-  // the first (the second run's registers are more than 128: 52 -> 56 us for 2048).
-  bool careful = W == 8;
+  // Values that are not finite leave V (in LDS) where some query may not see them.  Four waves on tiles of 64 keys look for them only once
+  // a sum came out infinite or NaN, in a second run over the tiles (333 tokens x 32 heads 11.0 -> 10.4 us, 2 masked prompts of 700 41 -> 36);
+  // the other forms look in the first (the second run's registers are more than 128: 52 -> 56 us for 2048).
+  bool careful = NJ >= 4 && (W == 8 || KEYS == 32);
   const float unit = mrow ? LOG2E : p.scale * LOG2E;
   if (tid == 0)
     odd_values = 0;
@@ -521,12 +521,12 @@ mx4_packed_kernel(const Mx4AttnParams p) {
     constexpr int stage = decltype(S_)::value;
     // this tile has landed and the other stage has been read, for this wave and then for every wave
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    if (careful && (mrow || kb * 64 + 64 > first_limit)) { // (uniform) some query may not see some key
+    if (careful && (mrow || kb * KEYS + KEYS > first_limit)) { // (uniform) some query may not see some key
       bool odd = false;
 #pragma unroll
-      for (int i = 0; i < (256 * NJ + TH - 1) / TH; i++) {
+      for (int i = 0; i < (KEYS * PER + TH - 1) / TH; i++) {
         const int at = i * TH + tid;
-        if (256 * NJ % TH == 0 || at < 256 * NJ) {
+        if (KEYS * PER % TH == 0 || at < KEYS * PER) {
           i32x4* const it = reinterpret_cast<i32x4*>(lds + stage * SIDE) + at;
           const i32x4 w = *it;
           bool some = false;
@@ -544,12 +544,13 @@ mx4_packed_kernel(const Mx4AttnParams p) {
     }
     if (kb + 1 < tiles)
       request(kb + 1, stage ^ 1); // in flight during the arithmetic below
-    if (kb * 64 > min(q0 + 15, o.n - 1) || q0 >= o.n)
+    if (kb * KEYS > min(q0 + 15, o.n - 1) || q0 >= o.n)
       return; // past what this wave's queries see
     const uint8_t* const st = lds + stage * SIDE;
-    f32x4 sc[4];
+    constexpr int NT = KEYS / 16; // runs of 16 keys
+    f32x4 sc[NT];
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
+    for (int t = 0; t < NT; t++) {
       sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NJ; j++)
@@ -557,20 +558,20 @@ mx4_packed_kernel(const Mx4AttnParams p) {
     }
     if (mrow) {
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int key = kb * 64 + (i >> 2) * 16 + g * 4 + (i & 3);
+      for (int i = 0; i < 4 * NT; i++) {
+        const int key = kb * KEYS + (i >> 2) * 16 + g * 4 + (i & 3);
         const float mv = key < p.mask_ld ? bf16_bits_to_f32(mrow[min(key, p.mask_ld - 1)]) : 0.f;
         sc[i >> 2][i & 3] = mv == -INFINITY ? -INFINITY : fmaf(sc[i >> 2][i & 3], p.scale, mv);
       }
     }
-    if (kb * 64 + 63 > q0) { // (wave-uniform)
+    if (kb * KEYS + KEYS - 1 > q0) { // (wave-uniform)
 #pragma unroll
-      for (int i = 0; i < 16; i++)
-        sc[i >> 2][i & 3] = kb * 64 + (i >> 2) * 16 + g * 4 + (i & 3) <= qi ? sc[i >> 2][i & 3] : -INFINITY;
+      for (int i = 0; i < 4 * NT; i++)
+        sc[i >> 2][i & 3] = kb * KEYS + (i >> 2) * 16 + g * 4 + (i & 3) <= qi ? sc[i >> 2][i & 3] : -INFINITY;
     }
     float mx = m;
 #pragma unroll
-    for (int i = 0; i < 16; i++)
+    for (int i = 0; i < 4 * NT; i++)
       mx = fmaxf(mx, sc[i >> 2][i & 3]);
     if (__builtin_amdgcn_ballot_w64((mx - m) * unit > 8.f) != 0) {
       mx = max_of_groups(mx);
@@ -585,18 +586,18 @@ mx4_packed_kernel(const Mx4AttnParams p) {
     if (mrow) { // (the difference first: a mask's lowest value times log2 e is no number)
       off = 0.f;
 #pragma unroll
-      for (int t = 0; t < 4; t++)
+      for (int t = 0; t < NT; t++)
         sc[t] -= m;
     }
-    bf16x8 pb[2];
+    bf16x8 pb[KEYS / 32];
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
+    for (int i = 0; i < 4 * NT; i += 2) {
       const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(sc[i >> 2][(i & 3) + 1], unit, off))};
       l = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l, false);
       pb[i >> 3][i & 7] = pr[0];
       pb[i >> 3][(i & 7) + 1] = pr[1];
     }
-    static_for<0, 2 * (NA / NR)>([&](auto I) { // 32 keys, NR pieces of channels
+    static_for<0, KEYS / 32 * (NA / NR)>([&](auto I) { // 32 keys, NR pieces of channels
       constexpr int u = decltype(I)::value / (NA / NR), d0 = decltype(I)::value % (NA / NR) * NR;
       i32x2 vv[NR][2];
       packed_v_operands<stage * SIDE + u * 32 * ROW + d0 * 32, 16 * ROW>(vv, vaddr);
@@ -639,14 +640,15 @@ mx4_packed_kernel(const Mx4AttnParams p) {
       *reinterpret_cast<uint2*>(orow + dt * 16 + g * 4) =
           make_uint2(f32x2_to_bf16_bits(acc[dt][0] * inv, acc[dt][1] * inv), f32x2_to_bf16_bits(acc[dt][2] * inv, acc[dt][3] * inv));
     if (__builtin_expect(odd_values != 0, 0))
-      mx4_add_non_finite<H, 4>(orow, g, mrow ? 0 : first_limit / 64 * 64, qi + 1, mrow, p.mask_ld, [&](int key, int ch) { return (uint32_t)vr[(int64_t)key * p.v_ld + ch]; });
+      mx4_add_non_finite<H, 4>(orow, g, mrow ? 0 : first_limit / KEYS * KEYS, qi + 1, mrow, p.mask_ld, [&](int key, int ch) { return (uint32_t)vr[(int64_t)key * p.v_ld + ch]; });
   }
 }
 
 int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache, hipStream_t stream) {
   // every sequence's last workgroup may be short: at most this many, those past the last one end at once
   auto blocks = [&](int rows) { return ((int64_t)p.T + (int64_t)p.B * (rows - 1)) / rows * p.Nq; };
-  const bool many = env_int("TPPX_MX4_PROMPT_QUERIES", blocks(128) >= (cache || H > 128 ? 200 : 400) ? 128 : 64) >= 128;
+  const int queries = env_int("TPPX_MX4_PROMPT_QUERIES", 0);
+  const bool many = queries ? queries >= 128 : blocks(128) >= (cache || H > 128 ? 200 : 400);
   hipError_t e = hipSuccess;
   int rc = TPPX_OK;
   auto go = [&](auto kern, int queries, int threads, size_t lds) {
@@ -662,14 +664,24 @@ int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
     if (!cache) {
-      // 128 queries in eight waves from some 400 workgroups of them on, else 64 in four (2048 tokens x 32 heads, 512: 52.0 us, of 64 59.9; 4
-      // prompts of up to 4100 171 and 209; 2048 x 16 heads of 256, 256: 77 and 91; 1000 x 32 heads, 256: 25.3 and 24.1; 4 x 1000 x 12 of 64,
-      // 384: 23.5 and 22.0; 333 x 32 11.7 and 11.4).
+      // Heads of 64 and 96: 64 queries in four waves (24 x 50..500 tokens x 12 heads of 64 12.0 us, of 128 in eight 14.5; 4000 x 12 48 and 54; 4 x
+      // 4000 x 10 of 96 171 and 175).  Wider ones in launches of some 400 (200 beyond 128 wide) workgroups of 128 queries and more: those
+      // (2048 tokens x 32 heads, 512: 51, of 64 57; 2048 x 16 heads of 256, 256: 77 and 91; 1000 x 32 heads, 256: 25.3 and 23.1; 333 x 32 11.5
+      // and 10.6), and where the prompts are short on average 64 queries on tiles of 32 keys, whose LDS lets four workgroups run on a CU
+      // (16 x 17..200 x 28 heads 13.3 -> 11.8, 8 x 50..500 x 64 on 8 31.3 -> 28.7, 16 x 300 x 32 41 -> 38, 16 x 300 x 16 of 256 33.0 -> 30.7; 4 x 1000 x 64 on
+      // 8 95 and 101, 6 x 60..1500 x 32 43.5 and 45.9).
       constexpr size_t lds = 4 * 64 * 64 * (size_t)NJ;
-      if (many)
-        go(mx4_packed_kernel<NJ, 8>, 128, 512, lds);
-      else
-        go(mx4_packed_kernel<NJ, 4>, 64, 256, lds);
+      if constexpr (NJ >= 4) {
+        if (many && !queries && p.T < (int64_t)512 * p.B) {
+          go(mx4_packed_kernel<NJ, 4, 32>, 64, 256, lds / 2);
+          return;
+        }
+        if (many) {
+          go(mx4_packed_kernel<NJ, 8, 64>, 128, 512, lds);
+          return;
+        }
+      }
+      go(mx4_packed_kernel<NJ, 4, 64>, 64, 256, lds);
       return;
     }
     auto over = [&](auto qw, auto qg, auto kt) {
