@@ -35,7 +35,7 @@ def _within(got, want, tol):
 
 
 def _prompt_form(queries, monkeypatch):
-    """Empty: the form that the sizes give; "64", "128": the prompt kernels with so many queries per workgroup, whatever they are."""
+    """Empty: the form that the sizes give; "64", "128": the prompt kernels in the form of small or of large launches."""
     if queries:
         monkeypatch.setenv("TPPX_MX4_PROMPT_QUERIES", queries)
 

@@ -6,8 +6,8 @@
 namespace tppx {
 
 // ---------------------------------------------------------------------------
-// In both kernels a workgroup takes the queries of one head in groups, a wave each, which share K and V tiles of 64 keys, bf16 in LDS in
-// two stages.  Both products run transposed: scores^T[key][query] = K Q^T, out^T[channel][query] += V^T P^T; a lane holds the
+// In both kernels a workgroup takes the queries of one head in groups, a wave each, which share K and V tiles of 64 (or 32) keys, bf16 in
+// LDS in two stages.  Both products run transposed: scores^T[key][query] = K Q^T, out^T[channel][query] += V^T P^T; a lane holds the
 // scores of one query, and those, rounded to bf16, are the second operand of the V product as they lie; V's operand is read by the
 // transposing LDS read.  Scores in fp32, running maximum and sum per query.
 // The sums are relative to a maximum that follows the true one once that is 2^8 above it (the probabilities are then at most 2^8: their
@@ -51,8 +51,8 @@ __device__ __forceinline__ void mx4_add_non_finite(uint16_t* orow, int lane, int
 }
 
 // ---------------------------------------------------------------------------
-// Over the MXFP4 cache: QG groups of QW queries, or with KT = 2 two waves for each that take half of every tile's keys (and are
-// merged at the end: launches of few workgroups).  Codes are expanded once per workgroup on the way to LDS.  32 queries per wave: an
+// Over the MXFP4 cache: 128 queries in groups of QW, or with KT = 2 two waves for each group that take half of every tile's keys (and
+// are merged at the end: launches of few workgroups).  Codes are expanded once per workgroup on the way to LDS.  32 queries per wave: an
 // operand read from LDS feeds 32 columns; heads of 192 and 256 run on 16, for the registers.
 // What bounds it: the way of the codes into LDS (without it 35 % less) and, as in the packed kernel, the chain scores, softmax, output
 // of a wave.  512 tokens x 64 heads behind 6000 keys 134 .. 147 us (boxes differ), 720 .. 780 TFLOP/s.
@@ -63,9 +63,10 @@ __device__ __forceinline__ void mx4_add_non_finite(uint16_t* orow, int lane, int
 constexpr int mx4_k_pitch(int NJ) { return 64 * NJ + 16; }
 constexpr int mx4_v_pitch(int NJ, int QW) { return QW == 16 ? 64 * NJ + 32 : NJ % 4 == 3 ? 64 * NJ : 64 * NJ + 64; }
 
-template <int NJ, int QW, int QG, int KT>
-__global__ void __launch_bounds__(QG * KT * 64, QW == 16 ? (NJ <= 4 && QG == 8 ? 4 : 2) : NJ > 4 ? 1 : 2)
+template <int NJ, int QW, int KT>
+__global__ void __launch_bounds__(128 / QW * KT * 64, 2)
 mx4_prompt_kernel(const Mx4AttnParams p) {
+  constexpr int QG = 128 / QW; // groups of queries
   constexpr int H = 32 * NJ, KP = mx4_k_pitch(NJ), VP = mx4_v_pitch(NJ, QW), D = 2, STAGE = 64 * (KP + VP); // K rows, then V rows
   // Scores of a lane: NT runs of QW keys of the tile, NV of each, for one query; its output: NA pieces of QW channels.
   constexpr int QB = QW * QG, TH = 64 * QG * KT, NT = 64 / QW / KT, NV = QW / 2 * QW / 32, NA = H / QW, HALF = 64 / QW;
@@ -368,9 +369,9 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Packed bf16 prompts: W waves of 16 queries, tiles of KEYS keys brought by loads straight into LDS, one ahead.  The chunks of 16 bytes of a row lie
-// permuted (those loads write 1024 bytes in a row), so that neither the rows of a K operand nor the pieces that the transposing read
-// of V takes meet in a bank.
+// Packed bf16 prompts: W waves of 16 queries, tiles of KEYS keys brought by loads straight into LDS, one ahead.  The chunks of 16 bytes
+// of a row lie permuted (those loads write 1024 bytes in a row), so that neither the rows of a K operand nor the pieces that the
+// transposing read of V takes meet in a bank.
 // What bounds it: the chain scores, softmax, output of a wave (matrix instructions take 0.39 of the time); so four waves per SIMD in 128
 // registers count for more than operands that feed 32 queries.  Measured against 32 queries a wave, two per SIMD, the tiles through
 // registers: 4 prompts of up to 4100 tokens x 32 heads 187 -> 171 us (860 TFLOP/s, where a large library product reaches 1138), 2048 x
@@ -647,12 +648,12 @@ mx4_packed_kernel(const Mx4AttnParams p) {
 int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache, hipStream_t stream) {
   // every sequence's last workgroup may be short: at most this many, those past the last one end at once
   auto blocks = [&](int rows) { return ((int64_t)p.T + (int64_t)p.B * (rows - 1)) / rows * p.Nq; };
-  const int queries = env_int("TPPX_MX4_PROMPT_QUERIES", 0);
-  const bool many = queries ? queries >= 128 : blocks(128) >= (cache || H > 128 ? 200 : 400);
+  const int form = env_int("TPPX_MX4_PROMPT_QUERIES", 0);
+  const bool many = form ? form >= 128 : blocks(128) >= (H > 128 ? 200 : 400);
   hipError_t e = hipSuccess;
   int rc = TPPX_OK;
-  auto go = [&](auto kern, int queries, int threads, size_t lds) {
-    const int64_t wgs = blocks(queries);
+  auto go = [&](auto kern, int rows, int threads, size_t lds) {
+    const int64_t wgs = blocks(rows);
     if (wgs >= ((int64_t)1 << 31)) {
       rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
       return;
@@ -672,7 +673,7 @@ int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache
       // 8 95 and 101, 6 x 60..1500 x 32 43.5 and 45.9).
       constexpr size_t lds = 4 * 64 * 64 * (size_t)NJ;
       if constexpr (NJ >= 4) {
-        if (many && !queries && p.T < (int64_t)512 * p.B) {
+        if (many && !form && p.T < (int64_t)512 * p.B) {
           go(mx4_packed_kernel<NJ, 4, 32>, 64, 256, lds / 2);
           return;
         }
@@ -684,36 +685,23 @@ int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache
       go(mx4_packed_kernel<NJ, 4, 64>, 64, 256, lds);
       return;
     }
-    auto over = [&](auto qw, auto qg, auto kt) {
-      constexpr int QW = decltype(qw)::value, QG = decltype(qg)::value, KT = decltype(kt)::value;
+    auto over = [&](auto qw, auto kt) {
+      constexpr int QW = decltype(qw)::value, KT = decltype(kt)::value, QG = 128 / QW;
       const size_t stages = 2 * 64 * (size_t)(mx4_k_pitch(NJ) + mx4_v_pitch(NJ, QW)), teams = KT > 1 ? QG * 64 * 16 * (size_t)(4 * NJ + 1) : 0;
-      go(mx4_prompt_kernel<NJ, QW, QG, KT>, QW * QG, QG * KT * 64, std::max(stages, teams)); // (the state of a second team)
+      go(mx4_prompt_kernel<NJ, QW, KT>, 128, QG * KT * 64, std::max(stages, teams)); // (the state of a second team)
     };
     constexpr std::integral_constant<int, 1> one{};
     constexpr std::integral_constant<int, 2> two{};
-    constexpr std::integral_constant<int, 4> four{};
-    constexpr std::integral_constant<int, 8> eight{};
-    constexpr std::integral_constant<int, 16> q16{};
-    constexpr std::integral_constant<int, 32> q32{};
-    if constexpr (NJ > 4) {
-      // 192 and 256 wide: one workgroup's tiles fill the LDS of a CU, and 32 queries a wave its registers at one wave per SIMD; with 16
-      // queries two fit.  Few: 500 tokens behind 700, 64 workgroups of 128 queries: 58.9, of 64: 51.7.
-      if (many)
-        over(q16, eight, one);
-      else
-        over(q16, four, one);
-    } else {
-      // 128 queries in four waves, two workgroups on a CU, from 400 of them on.  Below that two teams halve the way through a tile: four
-      // groups of queries share an expanded tile from 200 on (512 tokens x 64 heads behind 6000 keys, 256: 134, 153 with two groups and 167
-      // with one team; 64 tokens behind 4000, 64: 82 and 85), otherwise two groups.  Eight waves of 16 queries that expand into the layout
-      // of the packed kernel: 168 and 81 there, 2048 tokens x 32 heads behind 2048 127, as here.
-      if (many && blocks(128) >= 400)
-        over(q32, four, one);
-      else if (many)
-        over(q32, four, two);
-      else
-        over(q32, two, two);
-    }
+    // 192 and 256 wide: one workgroup's tiles fill the LDS of a CU, and 32 queries a wave its registers at one wave per SIMD; with 16
+    // queries two fit.  Others: 128 queries in four waves, two workgroups on a CU, from 400 of them on, below that two teams that halve the
+    // way through a tile (512 tokens x 64 heads behind 6000 keys, 256: 134 us, 167 with one team).  Eight waves of 16 queries that expand
+    // into the layout of the packed kernel, with one team or two, were no faster (158 and 134 there; 1024 tokens 246 and 277, here 235).
+    if constexpr (NJ > 4)
+      over(std::integral_constant<int, 16>{}, one);
+    else if (many)
+      over(std::integral_constant<int, 32>{}, one);
+    else
+      over(std::integral_constant<int, 32>{}, two);
   });
   if (rc)
     return rc;
