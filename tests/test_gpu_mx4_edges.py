@@ -1,0 +1,75 @@
+"""The MXFP4 cache and its operators at the edges of what their documentation allows: lengths at the ends of their type, sequences of
+different lengths in a second turn, positions and masks in every shape that the blocks take, refused calls that change nothing."""
+import math
+
+import pytest
+import torch
+
+import mx4_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def _at():
+    import tpp_pytorch_extension  # noqa: F401
+    from tpp_pytorch_extension._C import _tpp_attn
+    return _tpp_attn
+
+
+def _llm():
+    import tpp_pytorch_extension  # noqa: F401
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    return F
+
+
+def _i32(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _starts(lengths):
+    return [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+
+
+def _within(got, want, tol):
+    bad = ~((got.double().cpu() - want).abs() <= tol)
+    assert not bool(bad.any()), (int(bad.sum()), bad.numel(), float(((got.double().cpu() - want).abs() / tol).max()))
+
+
+def _filled(B, Nkv, cap, H, seed):
+    """A layer of normal keys and values, and the layer's values in 64 bits."""
+    kc, ks = R.encode(R.randn((B, Nkv, cap, H), 1.0, seed))
+    vc, vs = R.encode(R.randn((B, Nkv, cap, H), 1.0, seed + 1))
+    return _at().Mx4Layer(kc.cuda(), ks.cuda(), vc.cuda(), vs.cuda()), R.decode(kc, ks), R.decode(vc, vs)
+
+
+def _prompt_form(queries, monkeypatch):
+    """Empty: the form that the sizes give (here the split kernel); "64": the prompt kernel."""
+    if queries:
+        monkeypatch.setenv("TPPX_MX4_PROMPT_QUERIES", queries)
+
+
+def _decoder(**kw):
+    F = _llm()
+    return F, F.LlamaDecoder(hidden=512, inter=1024, n_layers=2, n_heads=4, n_kv_heads=2, vocab=512, max_positions=256, seed=3, **kw)
+
+
+@pytest.mark.parametrize("H", [64, 128, 256])
+@pytest.mark.parametrize("queries", ["", "64"])
+def test_past_at_the_end_of_its_type(H, queries, monkeypatch):
+    """past at the end of int32: an append finds no slot, attention sees the whole cache, in both kernels."""
+    at = _at()
+    _prompt_form(queries, monkeypatch)
+    Nq, Nkv, new, cap = 4, 2, [70, 130, 2], 40
+    past = [2 ** 31 - 1, 2 ** 31 - 100, 2 ** 31 - 2]
+    cu = _starts(new)
+    layer, k, v = _filled(3, Nkv, cap, H, H)
+    before = [t.clone() for t in layer]
+    q, kn, vn = (R.randn((cu[-1], n, H), 1.2, i) for i, n in enumerate((Nq, Nkv, Nkv)))
+    qo, _, _ = at.append_mx4(q.cuda(), kn.cuda(), vn.cuda(), layer, _i32(past), _i32(cu), emb_pos=R.llama_table(64, H).cuda())
+    assert all(torch.equal(a, b) for a, b in zip(layer, before)) and torch.equal(qo.cpu(), q)  # (positions outside the table)
+    got = at.attn_mx4(q.cuda(), layer, _i32(past), _i32(cu))
+    one = at.attn_mx4(q[:3].cuda(), layer, _i32(past))
+    for b in range(3):
+        rows = slice(cu[b], cu[b + 1])
+        _within(got[rows], *R.attend_rows(q[rows], k[b], v[b], cap))
+        _within(one[b:b + 1], *R.attend_rows(q[b:b + 1], k[b], v[b], cap))

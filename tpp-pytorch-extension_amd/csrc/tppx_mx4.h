@@ -96,6 +96,10 @@ struct Mx4AttnParams {
 };
 constexpr int MX4_COUNTER_STRIDE = 64; // arrival counters are 256 bytes apart
 
+// The number of keys before a sequence's tokens, so that its sums with numbers of tokens and of keys (both below 2^30) stay in 32
+// bits: more than the cache holds is all of it, and what lies 2^30 before the first slot sees none of it.
+__device__ __forceinline__ int mx4_past(int past, int Smax) { return min(max(past, -(1 << 30)), Smax); }
+
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x3 __attribute__((ext_vector_type(3)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));

@@ -213,7 +213,8 @@ mx4_rows_kernel(const Mx4RowsParams p) {
   };
   int row = (int)blockIdx.y;
   load(row);
-  int b = 0, slot = 0;
+  int b = 0;
+  int64_t slot = 0; // (past may hold anything: in 64 bits)
   bool here = mine < p.T;
   if (CACHE) {
     int first = tok;
@@ -226,9 +227,9 @@ mx4_rows_kernel(const Mx4RowsParams p) {
       b = min(b, p.B - 1);
       first = p.cu[b];
     }
-    slot = p.past[b] + (tok - first);
+    slot = (int64_t)p.past[b] + tok - first;
   }
-  const int64_t at = p.pos ? p.pos[tok] : (int64_t)slot;
+  const int64_t at = p.pos ? p.pos[tok] : slot;
   const bool room = slot >= 0 && slot < p.Smax;
   t.turn = p.emb && at >= 0 && at < p.MP && u < half; // positions outside the table are left unrotated
   if (t.turn) {
@@ -387,7 +388,7 @@ mx4_split_kernel(const Mx4AttnParams p) {
     return;
   const int ncol = min(16, o.n * p.R - o.at * 16); // of this workgroup
   const int col = o.at * 16 + min(c, ncol - 1), tok = col / p.R, r0 = col - tok * p.R;
-  const int past = p.past[o.b];
+  const int past = mx4_past(p.past[o.b], p.Smax);
   const int limit = min(max(past + tok + 1, 0), p.Smax); // keys this lane's column sees
   const int L = min(max(past + (o.at * 16 + ncol - 1) / p.R + 1, 0), p.Smax);
   const int S = max(min(p.splits, (L + W * 64 - 1) / (W * 64)), 1); // splits that have keys; the others take no part

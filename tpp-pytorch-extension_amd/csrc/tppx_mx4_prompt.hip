@@ -91,7 +91,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   if (!locate(p.cu, p.B, p.T, 1, QB, (int)blockIdx.x / p.Nq, o, paired))
     return;
   const int qblk = (o.n + QB - 1) / QB - 1 - o.at; // the last queries see the most keys: first
-  const int past = max(p.past[o.b], 0);
+  const int past = max(mx4_past(p.past[o.b], p.Smax), 0);
   const int total = min(past + o.n, p.Smax); // keys of the sequence
   const int q0 = qblk * QB + wave * QW;
   const int qi = min(q0 + c, o.n - 1);
