@@ -681,9 +681,10 @@ int tppx_attn_prefill(const void* q, const void* kcache, const void* vcache,
  * No counterpart in the reference, whose cache is bf16 / fp32 and whose batches share one length.  Head sizes H: 64, 96,
  * 128, 192, 256 (others TPPX_EUNSUPPORTED).
  * Packed tokens: rows of q, k, v, out; sequence b owns rows cu[b] .. cu[b + 1] - 1 (cu: device i32 [B + 1], ascending;
- * NULL: one token per sequence, T == B); it held past[b] (device i32 [B]) keys before them.  Row strides *_ld in elements
- * (multiples of 8), heads of a row contiguous.  Rows of T behind cu[B] take no part: out and the cache are left as they were
- * there.  Values in cu and past that do not fit are clamped on the device.
+ * NULL: one token per sequence, T == B); it held past[b] (device i32 [B]) keys before them (negative: its first -past[b]
+ * tokens have no slot and see nothing).  Row strides *_ld in elements (multiples of 8), heads of a row contiguous.  Rows of
+ * T behind cu[B] take no part: out and the cache are left as they were there.  Rows past T in cu and more keys than Smax in
+ * past are clamped on the device: no value in them leads out of a buffer.
  * A cache layer: codes u8 [B][Nkv][Smax][H/2] (E2M1, channel 2i in the low half of byte i; 16-byte aligned) and scales u8
  * [B][Nkv][Smax][H/32] (E8M0) of the keys and of the values.  A block of 32 channels has the scale byte
  * floor(log2 max) + 125; nearest, ties to the even code, 6 at most.  A block whose maximum is below 2^-124 is zero (byte 0), one

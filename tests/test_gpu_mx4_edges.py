@@ -73,3 +73,32 @@ def test_past_at_the_end_of_its_type(H, queries, monkeypatch):
         rows = slice(cu[b], cu[b + 1])
         _within(got[rows], *R.attend_rows(q[rows], k[b], v[b], cap))
         _within(one[b:b + 1], *R.attend_rows(q[b:b + 1], k[b], v[b], cap))
+
+
+@pytest.mark.parametrize("H", [64, 128, 256])
+@pytest.mark.parametrize("queries", ["", "64"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_tokens_before_the_first_slot(H, queries, masked, monkeypatch):
+    """A negative past: token i sees the keys 0 .. past + i, those before the first slot none, in both kernels and appended alike; a block of
+    NaN in a seen key reaches the tokens that see it."""
+    at = _at()
+    _prompt_form(queries, monkeypatch)
+    Nq, Nkv, new, past, cap = 4, 2, [70, 230, 9, 5], [-3, -200, -9, -2 ** 31], 68
+    cu = _starts(new)
+    layer, k, v = _filled(4, Nkv, cap, H, H + 5)
+    q = R.randn((cu[-1], Nq, H), 1.2, 3)
+    mask = torch.zeros((4, 70), dtype=torch.bfloat16)
+    if masked:
+        mask[:, 1] = -math.inf
+    args = (q.cuda(), layer, _i32(past), _i32(cu), mask.cuda() if masked else None)
+    got = at.attn_mx4(*args)
+    for b in range(4):
+        rows = slice(cu[b], cu[b + 1])
+        n = max(past[b] + new[b], 0)
+        _within(got[rows], *R.attend(q[rows], k[b, :, :n], v[b, :, :n], past[b], mask[b] if masked else None))
+        assert not bool(got[cu[b]:cu[b] - past[b]].any())
+    layer.v_scales[1, 0, 10, 0] = 255
+    hit = at.attn_mx4(*args)
+    bad = torch.zeros(got.shape, dtype=torch.bool)
+    bad[cu[1] + 210:cu[2], :Nq // Nkv, :32] = True
+    assert torch.equal(hit.isnan().cpu(), bad) and torch.equal(hit.cpu()[~bad], got.cpu()[~bad])

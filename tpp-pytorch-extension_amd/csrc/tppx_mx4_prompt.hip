@@ -91,7 +91,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
   if (!locate(p.cu, p.B, p.T, 1, QB, (int)blockIdx.x / p.Nq, o, paired))
     return;
   const int qblk = (o.n + QB - 1) / QB - 1 - o.at; // the last queries see the most keys: first
-  const int past = max(mx4_past(p.past[o.b], p.Smax), 0);
+  const int past = mx4_past(p.past[o.b], p.Smax);
   const int total = min(past + o.n, p.Smax); // keys of the sequence
   const int q0 = qblk * QB + wave * QW;
   const int qi = min(q0 + c, o.n - 1);
@@ -363,7 +363,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
         *reinterpret_cast<uint2*>(orow + dt * QW + 8 * (i >> 2) + 4 * h) = w;
       }
     if (__builtin_expect(odd_values != 0, 0))
-      mx4_add_non_finite<H, HALF>(orow, h, mrow ? 0 : first_limit / 64 * 64, limit, mrow, p.mask_ld,
+      mx4_add_non_finite<H, HALF>(orow, h, mrow ? 0 : max(first_limit, 0) / 64 * 64, limit, mrow, p.mask_ld,
                                   [&](int key, int ch) { return vs[(int64_t)key * NJ + (ch >> 5)] == 255 ? 0x7fc0u : 0u; });
   }
 }

@@ -6,8 +6,8 @@ embeddings (src/csrc/llm/fused_llm_infer.cpp:150-253).
 
 Packed tokens are rows `[T][heads][H]`: sequence b owns rows `cu_seqlens[b] .. cu_seqlens[b + 1] - 1` (int32 `[B + 1]` on the
 device), or one row each where `cu_seqlens` is None.  `past[b]` (int32 `[B]`, device) is the number of keys that a sequence
-held before these tokens.  Rows of a batch behind the last sequence take no part: the cache is left as it was, and the results hold
-whatever `torch.empty` gave there.
+held before these tokens (negative: the first of them have no slot and see nothing).  Rows of a batch behind the last sequence
+take no part: the cache is left as it was, and the results hold whatever `torch.empty` gave there.
 
 A layer of the cache is `Mx4Layer(k_codes, k_scales, v_codes, v_scales)`, uint8 `[B][Nkv][capacity][H/2]` (two E2M1 codes a
 byte, the even channel in the low half) and `[B][Nkv][capacity][H/32]` (E8M0).  Head sizes 64, 96, 128, 192 and 256.
