@@ -102,3 +102,33 @@ def test_tokens_before_the_first_slot(H, queries, masked, monkeypatch):
     bad = torch.zeros(got.shape, dtype=torch.bool)
     bad[cu[1] + 210:cu[2], :Nq // Nkv, :32] = True
     assert torch.equal(hit.isnan().cpu(), bad) and torch.equal(hit.cpu()[~bad], got.cpu()[~bad])
+
+
+def test_a_second_turn_behind_sequences_of_different_lengths():
+    """prefill on a cache whose sequences differ: each sequence's tokens are rotated at its own positions."""
+    F, dec = _decoder(kv_dtype="mxfp4")
+    g = torch.Generator().manual_seed(11)
+    first = [torch.randint(0, 512, (n,), generator=g).cuda() for n in (40, 7)]
+    turn = torch.randint(0, 512, (2, 5), generator=g).cuda()
+    caches = [F.Mx4Cache(80) for _ in range(2)]
+    for c in caches:
+        dec.prefill_packed(first, c)
+    dec.prefill(turn, caches[0])
+    h = dec.embed.index_select(0, turn.reshape(-1)).view(2, 5, 512)
+    pos = torch.stack([torch.arange(n, n + 5) for n in (40, 7)]).cuda()
+    for layer in dec.layers:
+        h = layer.forward([h, None, pos], caches[1])[0]
+    caches[1].advance(5)
+    assert caches[0].seq_len_dev.tolist() == caches[1].seq_len_dev.tolist() == [45, 12]
+    for i in range(2):
+        for a, b in zip(caches[0].layers[i], caches[1].layers[i]):
+            assert torch.equal(a, b)
+    # and as the sequences alone: the first layer's keys differ by what a step of bf16 (2^-7) moves, one code in 2^-7 / (1/4) at most,
+    # each by half of its value at most: rel-L2 sqrt(2^-5 / 4) < 0.09
+    for b in range(2):
+        c = F.Mx4Cache(80)
+        dec.prefill(first[b].view(1, -1), c)
+        dec.prefill(turn[b:b + 1], c)
+        n = first[b].numel()
+        want, got = c.get(0)[0][0, :, n:n + 5].double(), caches[0].get(0)[0][b, :, n:n + 5].double()
+        assert float((got - want).norm() / want.norm()) < 0.09

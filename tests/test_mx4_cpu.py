@@ -118,3 +118,20 @@ def test_generate_packed_refuses_no_prompts():
     from tpp_pytorch_extension.llm import fused_llama_infer as F
     with pytest.raises(F.TppxError):
         F.LlamaDecoder.generate_packed(None, [], 3)
+
+
+def test_positions_of_the_next_tokens():
+    """One row for sequences of one length, a row each otherwise; a cache that was not used yet begins at 0."""
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    for cache in (F.TppCache(40), F.Mx4Cache(40)):
+        assert cache.positions(2, "cpu").tolist() == [[0], [0]]
+        assert cache.next_positions(3, "cpu").tolist() == [[0, 1, 2]]
+    cache = F.Mx4Cache(40)
+    cache.prompts([9, 3], "cpu")
+    cache.advance()
+    assert cache.positions(2, "cpu").tolist() == [[9], [3]]
+    assert cache.next_positions(3, "cpu").tolist() == [[9, 10, 11], [3, 4, 5]]
+    cache.crop(3)
+    assert cache.next_positions(2, "cpu").tolist() == [[3, 4]]
+    with pytest.raises(F.TppxError):
+        cache.positions(3, "cpu")

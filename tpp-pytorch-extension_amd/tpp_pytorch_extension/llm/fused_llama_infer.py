@@ -161,6 +161,11 @@ class TppCache:
         """Position of the next token of every sequence, int64 [B][1]."""
         return torch.full((B, 1), self.get_seq_length(), dtype=torch.int64, device=device)
 
+    def next_positions(self, S, device):
+        """Positions of the next S tokens, int64 [1][S] where they are the same for every sequence, else [B][S]."""
+        past = self.get_seq_length()
+        return torch.arange(past, past + S, dtype=torch.int64, device=device).unsqueeze(0)
+
     # -- storage ------------------------------------------------------------------
     def _ensure(self, layer_idx, B, Nkv, H, device):
         if self.capacity <= 0:
@@ -307,7 +312,13 @@ class Mx4Cache(TppCache):
         return self._packed is not None or super().room_for(S)
 
     def positions(self, B, device):
+        self._sequences(B, device)
         return self.seq_len_dev.to(torch.int64).view(B, 1)
+
+    def next_positions(self, S, device):
+        if self._short is None or not any(self._short):
+            return super().next_positions(S, device)
+        return self.positions(len(self._short), device) + torch.arange(S, dtype=torch.int64, device=device)
 
     def advance(self, n=1):
         """Every sequence holds n more keys; after a pass over packed prompts, each the keys of its prompt."""
@@ -759,8 +770,7 @@ class LlamaDecoder:
         """prompt i64 [B][S] (device) on top of whatever the cache holds -> next tokens i64 [B]; advances the cache
         by S.  mask: additive bf16 [B][keys] over cache positions (TppCache.align_and_invert_mask) or None."""
         B, S = prompt.shape
-        past = cache.get_seq_length()
-        pos = torch.arange(past, past + S, dtype=torch.int64, device=self.device).unsqueeze(0)
+        pos = cache.next_positions(S, self.device)
         h = self.embed.index_select(0, prompt.reshape(-1)).view(B, S, self.hidden)
         for layer in self.layers:
             h = layer.forward([h, mask, pos], cache)[0]
