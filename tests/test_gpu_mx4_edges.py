@@ -132,3 +132,56 @@ def test_a_second_turn_behind_sequences_of_different_lengths():
         n = first[b].numel()
         want, got = c.get(0)[0][0, :, n:n + 5].double(), caches[0].get(0)[0][b, :, n:n + 5].double()
         assert float((got - want).norm() / want.norm()) < 0.09
+
+
+def _tiny(family):
+    T = pytest.importorskip("transformers")
+    F = _llm()
+    torch.manual_seed(43)
+    if family in ("llama", "qwen2"):
+        cls, model = (T.LlamaConfig, T.LlamaForCausalLM) if family == "llama" else (T.Qwen2Config, T.Qwen2ForCausalLM)
+        kw = dict(head_dim=128) if family == "llama" else {}
+        cfg = cls(hidden_size=512, intermediate_size=1024, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2, vocab_size=1024,
+                  max_position_embeddings=256, attn_implementation="eager", **kw)
+        if family == "llama":
+            return F.OptimizeModelForLlama(model(cfg).eval(), torch.bfloat16, "cuda", "mxfp4").eval()
+        from tpp_pytorch_extension.llm import fused_qwen2_infer as Q
+        return Q.OptimizeModelForQwen2(model(cfg).eval(), torch.bfloat16, "cuda", "mxfp4").eval()
+    if family == "gptj":
+        from tpp_pytorch_extension.llm import fused_gptj_infer as G
+        return G.OptimizeModelForGPTJ(T.GPTJForCausalLM(T.GPTJConfig(n_embd=512, n_head=2, n_layer=2, n_positions=256, rotary_dim=64, vocab_size=1600,
+                                                                     bos_token_id=1, eos_token_id=2)).eval(), torch.bfloat16, "cuda", "mxfp4").eval()
+    from tpp_pytorch_extension.llm import fused_opt_infer as O
+    cfg = T.OPTConfig(hidden_size=512, ffn_dim=1024, num_hidden_layers=2, num_attention_heads=4, vocab_size=1600, max_position_embeddings=256,
+                      word_embed_proj_dim=512, attn_implementation="eager")
+    return O.OptimizeModelForOPT(T.OPTForCausalLM(cfg).eval(), torch.bfloat16, "cuda", "mxfp4").eval()
+
+
+@pytest.mark.parametrize("family", ["llama", "qwen2", "gptj", "opt"])
+def test_front_ends_count_the_positions_of_every_sequence(family):
+    """Packed prompts through a front-end's forward, then a turn of both sequences, without position_ids: what explicit ones give."""
+    from tpp_pytorch_extension.llm.llm_common import TppCache
+    opt = _tiny(family)
+    core = next(m for m in opt.modules() if getattr(m, "_tpp_core_model", False))
+    g = torch.Generator().manual_seed(12)
+    packed, turn = (torch.randint(3, 1000, s, generator=g).cuda() for s in ((1, 13), (2, 3)))
+    outs, keys = [], []
+    for explicit in (False, True):
+        cache = TppCache(capacity=64, kv_dtype="mxfp4")
+        where = [torch.cat([torch.arange(9), torch.arange(4)]).unsqueeze(0).cuda(), torch.stack([torch.arange(9, 12), torch.arange(4, 7)]).cuda()]
+        with torch.no_grad():
+            if family != "opt":  # (whose forward makes a padding mask, which packed prompts do not take)
+                cache.get_cpp().prompts([9, 4])
+                a = core(input_ids=packed, past_key_values=cache, position_ids=where[0] if explicit else None).last_hidden_state
+            else:
+                core(input_ids=turn.repeat(1, 3), past_key_values=cache)
+                cache.get_cpp()._short = [0, 5]
+                cache.get_cpp().seq_len_dev.sub_(_i32([0, 5]))
+                a = None
+            b = core(input_ids=turn, past_key_values=cache, position_ids=where[1] if explicit else None).last_hidden_state
+        outs.append((a, b))
+        keys.append([t.clone() for layer in cache.get_cpp().layers.values() for t in layer])
+        assert cache.get_cpp().seq_len_dev.tolist() == [12, 7]
+    for x, y in zip(outs[0], outs[1]):
+        assert x is y or torch.equal(x, y)
+    assert all(torch.equal(x, y) for x, y in zip(*keys))

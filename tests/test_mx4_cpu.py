@@ -135,3 +135,13 @@ def test_positions_of_the_next_tokens():
     assert cache.next_positions(2, "cpu").tolist() == [[3, 4]]
     with pytest.raises(F.TppxError):
         cache.positions(3, "cpu")
+
+
+def test_positions_of_packed_tokens():
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    cache = F.Mx4Cache(40)
+    cache.prompts([3, 0, 2], "cpu")
+    assert cache.next_positions(5, "cpu").tolist() == [[0, 1, 2, 0, 1]]
+    cache.advance()
+    cache.prompts([1, 2, 1], "cpu")
+    assert cache.next_positions(4, "cpu").tolist() == [[3, 0, 1, 2]]

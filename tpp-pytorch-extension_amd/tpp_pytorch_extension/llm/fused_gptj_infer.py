@@ -144,12 +144,9 @@ def GPTJModel_forward(self, input_ids=None, past_key_values=None, attention_mask
             past_key_values = HFTppCache(capacity=self._tpp_kv_capacity)
         else:
             raise ValueError("past_key_values must be of TppCache type")
-    past_seen = past_key_values.get_seq_length()
     S = inputs_embeds.shape[1]
-    if cache_position is None:
-        cache_position = torch.arange(past_seen, past_seen + S, device=inputs_embeds.device)
     if position_ids is None:
-        position_ids = cache_position.unsqueeze(0)
+        position_ids = past_key_values.get_cpp().next_positions(S, inputs_embeds.device) if cache_position is None else cache_position.unsqueeze(0)
     mask = None if attention_mask is None else past_key_values.align_and_invert_mask(attention_mask, inputs_embeds)
     hidden_states = inputs_embeds
     if token_type_ids is not None:

@@ -316,6 +316,12 @@ class Mx4Cache(TppCache):
         return self.seq_len_dev.to(torch.int64).view(B, 1)
 
     def next_positions(self, S, device):
+        if self._packed is not None:  # of the packed tokens, [1][S]
+            bounds, lengths = self._packed
+            first = self.seq_len_dev.to(torch.int64) - bounds[:-1]  # position of a sequence's row 0, less that row
+            each = torch.tensor(lengths, device=first.device)
+            rows = torch.arange(sum(lengths), device=first.device)
+            return (rows + torch.repeat_interleave(first, each, output_size=sum(lengths))).unsqueeze(0)
         if self._short is None or not any(self._short):
             return super().next_positions(S, device)
         return self.positions(len(self._short), device) + torch.arange(S, dtype=torch.int64, device=device)
@@ -790,9 +796,7 @@ class LlamaDecoder:
         bounds = cache.prompts(lengths, self.device)
         try:
             tokens = torch.cat([p.reshape(-1).to(self.device) for p in prompts])
-            each = torch.tensor(lengths, device=self.device)
-            first = cache.seq_len_dev.to(torch.int64) - bounds[:-1]  # position of a sequence's row 0, less that row
-            pos = (torch.arange(tokens.numel(), device=self.device) + torch.repeat_interleave(first, each, output_size=tokens.numel())).unsqueeze(0)
+            pos = cache.next_positions(tokens.numel(), self.device)
             h = self.embed.index_select(0, tokens).unsqueeze(0)
             for layer in self.layers:
                 h = layer.forward([h, None, pos], cache)[0]
@@ -971,12 +975,9 @@ def LlamaModel_forward(self, input_ids=None, attention_mask=None, position_ids=N
             past_key_values = HFTppCache(capacity=self._tpp_kv_capacity)
         else:
             raise ValueError("past_key_values must be of TppCache type")
-    past_seen = past_key_values.get_seq_length()
     S = inputs_embeds.shape[1]
-    if cache_position is None:
-        cache_position = torch.arange(past_seen, past_seen + S, device=inputs_embeds.device)
     if position_ids is None:
-        position_ids = cache_position.unsqueeze(0)
+        position_ids = past_key_values.get_cpp().next_positions(S, inputs_embeds.device) if cache_position is None else cache_position.unsqueeze(0)
     mask = None if attention_mask is None else past_key_values.align_and_invert_mask(attention_mask, inputs_embeds)
     hidden_states = inputs_embeds.to(torch.bfloat16)
     for layer in self.layers[: self.config.num_hidden_layers]:

@@ -143,7 +143,13 @@ def OPTDecoder_forward(self, input_ids=None, attention_mask=None, past_key_value
     if position_ids is None:
         position_ids = torch.cumsum(attention_mask, dim=1)
         position_ids = (position_ids * attention_mask - 1).long()
-        position_ids = position_ids[:, past_seen:]  # cut positions if there are cached keys
+        where = past_key_values.get_cpp().next_positions(S, inputs_embeds.device)
+        if where.shape[0] == 1:
+            position_ids = position_ids[:, past_seen:]  # cut positions if there are cached keys
+        else:  # sequences of different lengths: each one's new tokens stand behind its own keys
+            if attention_mask.shape[1] != past_seen + S:
+                raise ValueError(f"attention_mask must cover {past_seen} cached and {S} new keys, got {tuple(attention_mask.shape)}")
+            position_ids = position_ids.gather(1, where)
     pos_embeds = self.embed_positions(attention_mask, past_seen, position_ids=position_ids)
     if self.project_in is not None:
         inputs_embeds = self.project_in(inputs_embeds)
