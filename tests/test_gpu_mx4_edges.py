@@ -185,3 +185,32 @@ def test_front_ends_count_the_positions_of_every_sequence(family):
     for x, y in zip(outs[0], outs[1]):
         assert x is y or torch.equal(x, y)
     assert all(torch.equal(x, y) for x, y in zip(*keys))
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("kv", ["mxfp4", "bfloat16"])
+def test_one_position_for_all_sequences(norm, kv):
+    """Single tokens of several sequences with position_ids [1][1], as the blocks take them."""
+    F = _llm()
+    B, Nq, Nkv, H = 3, 4, 2, 128
+    table = R.llama_table(64, H).cuda()
+    w = (1 + 0.1 * R.randn(H, 1.0, 5).float()).cuda()
+    q, k, v = (R.randn((B, 1, n * H), 1.0, i).cuda() for i, n in enumerate((Nq, Nkv, Nkv)))
+    outs = []
+    for pos in (torch.tensor([[9]]).cuda(), torch.tensor([[9]] * B).cuda(), torch.tensor([[9]]).cuda().expand(B, 1)):
+        cache = F.kv_cache(32, kv)
+        outs.append(F.rotate_append_attend(q.clone(), k.clone(), v, None, pos.contiguous() if kv == "bfloat16" else pos, cache, 0, B, 1, Nq, Nkv, H, table,
+                                           "llama", (w, w, 1e-6) if norm else None))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[2], outs[1])
+
+
+@pytest.mark.parametrize("family", ["llama", "qwen2", "gptj", "opt"])
+def test_front_ends_without_a_mask(family, monkeypatch):
+    """Greedy loops of two sequences without an attention mask (one row of positions for both) on the MXFP4 cache, eager and replayed."""
+    monkeypatch.setenv("TPPX_KV_DTYPE", "mxfp4")
+    F = _llm()
+    opt = _tiny(family)
+    ids = torch.randint(3, 1000, (2, 21), generator=torch.Generator().manual_seed(8)).cuda()
+    out = F.generate_greedy(opt, ids, 8)
+    assert out.shape == (2, 29) and torch.equal(F.generate_greedy(opt, ids, 8, torch.ones_like(ids)), out)
+    assert torch.equal(F.generate_greedy_graph(opt, ids, 8), out)

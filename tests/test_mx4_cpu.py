@@ -145,3 +145,12 @@ def test_positions_of_packed_tokens():
     cache.advance()
     cache.prompts([1, 2, 1], "cpu")
     assert cache.next_positions(4, "cpu").tolist() == [[3, 0, 1, 2]]
+
+
+def test_positions_of_every_token():
+    from tpp_pytorch_extension.llm.fused_llama_infer import _token_positions
+    one, row = torch.tensor([[7]]), torch.tensor([[3, 4]])
+    for pos, T, S, want in ((one, 3, 1, [7, 7, 7]), (one.expand(3, 1), 3, 1, [7, 7, 7]), (row, 4, 2, [3, 4, 3, 4]), (row, 2, 2, [3, 4]),
+                            (torch.tensor([[1, 2], [5, 6]]), 4, 2, [1, 2, 5, 6])):
+        got = _token_positions(pos, T, S)
+        assert got.is_contiguous() and got.stride() == (1,) and got.tolist() == want

@@ -436,10 +436,10 @@ class Mx4Cache(TppCache):
             bounds = None if S == 1 else self._bounds_of(B, S, q.device)
         layer = self._ensure(layer_idx, B, Nkv, H, q.device)
         wq, wk, eps = qk_norm or (None, None, 0.0)
-        pos = t_pid.reshape(-1) if t_pid.numel() == T else t_pid.expand(B, S).reshape(-1)
+        pos = _token_positions(t_pid, T, S) if style else None
         fresh = bounds is not None and self._host_len == 0
         rows, kr, vr = mx4_cache.append_mx4(q.view(T, Nq, H), k.view(T, Nkv, H), v.view(T, Nkv, H), layer, self.seq_len_dev, bounds, wq, wk, eps,
-                                            t_EP, pos if style else None, style, values=fresh)
+                                            t_EP, pos, style, values=fresh)
         mask = t_am if t_am is not None and t_am.numel() else None
         if fresh:
             ctx = mx4_cache.attn_packed(rows, kr, vr, bounds, mask)
@@ -465,6 +465,14 @@ def kv_cache(capacity=0, kv_dtype="bfloat16"):
     return (Mx4Cache if kv_dtype == "mxfp4" else TppCache)(capacity)
 
 
+def _token_positions(t_pid, T, S):
+    """Positions [T / S or 1][S] as one of every token, contiguous [T] (a row for several sequences expands with a stride of 0, which a
+    reshape of single tokens keeps)."""
+    if t_pid.numel() != T:
+        t_pid = t_pid.expand(T // S, S)
+    return t_pid.reshape(-1).contiguous()
+
+
 def rotate_append_attend(q, k, v, t_am, t_pid, cache, layer_idx, B, S, Nq, Nkv, H, t_EP, style, qk_norm=None):
     """What every decoder block of the reference does between its q/k/v GEMMs and its output projection
     (fused_llm_infer.cpp:784-789, 1025-1027, 1252-1257): rotary embedding on q and k in place (style "llama":
@@ -477,8 +485,8 @@ def rotate_append_attend(q, k, v, t_am, t_pid, cache, layer_idx, B, S, Nq, Nkv, 
         return cache.rotate_append_attend(q, k, v, t_am, t_pid, layer_idx, B, S, Nq, Nkv, H, t_EP, style, qk_norm)
     if qk_norm is not None:
         rows = [t.view(B * S, -1, H) for t in (q, k)]
-        pos = t_pid.reshape(-1) if t_pid.numel() == B * S else t_pid.expand(B, S).reshape(-1)
-        rows = mx4_cache.qk_norm_rotary(*rows, qk_norm[0], qk_norm[1], qk_norm[2], t_EP, pos if style else None, style)
+        pos = _token_positions(t_pid, B * S, S) if style else None
+        rows = mx4_cache.qk_norm_rotary(*rows, qk_norm[0], qk_norm[1], qk_norm[2], t_EP, pos, style)
         q, k, style = rows[0].view(q.shape), rows[1].view(k.shape), None
     L = _lib.lib()
     st = _lib.stream_of(q)
