@@ -214,3 +214,23 @@ def test_front_ends_without_a_mask(family, monkeypatch):
     out = F.generate_greedy(opt, ids, 8)
     assert out.shape == (2, 29) and torch.equal(F.generate_greedy(opt, ids, 8, torch.ones_like(ids)), out)
     assert torch.equal(F.generate_greedy_graph(opt, ids, 8), out)
+
+
+def test_one_token_with_any_stride():
+    """The row stride of a single token is not looked at."""
+    at = _at()
+    H, Nq, Nkv = 128, 4, 2
+    x = [R.randn((1, n, H), 1.0, n).cuda() for n in (Nq, Nkv, Nkv + 1)]
+    x[2] = x[2][:, :Nkv].contiguous()
+    odd = []
+    for t, stride in zip(x, (7, 8, 0)):
+        o = torch.empty_strided(t.shape, (stride, H, 1), dtype=t.dtype, device="cuda")
+        odd.append(o.copy_(t))
+    a, b = at.qk_norm_rotary(*x[:2]), at.qk_norm_rotary(*odd[:2])
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+    outs = []
+    for q, k, v in (x, odd):
+        layer = at.Mx4Layer(*(torch.zeros((1, Nkv, 4, n), dtype=torch.uint8, device="cuda") for n in (64, 4, 64, 4)))
+        r, kr, vr = at.append_mx4(q, k, v, layer, _i32([0]), style=None, values=True)
+        outs.append([r, kr, vr, *layer, at.attn_mx4(q, layer, _i32([0])), at.attn_packed(q, k, v, _i32([0, 1]))])
+    assert all(torch.equal(s, t) for s, t in zip(*outs))

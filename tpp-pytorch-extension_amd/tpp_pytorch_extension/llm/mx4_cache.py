@@ -51,9 +51,11 @@ def _rows(t, name, dev=None):
     T, n, h = t.shape
     a, b, c = t.stride()
     ptr = t.data_ptr()
+    if T == 1:
+        a = n * h  # (of a single row the stride may be anything)
     if c != 1 or (b != h and n != 1) or a % 8 or a < n * h or ptr & 15:
-        t = t.contiguous() if not t.is_contiguous() else t.clone()
-        a, ptr = t.stride(0), t.data_ptr()
+        t = t.clone(memory_format=torch.contiguous_format)
+        a, ptr = n * h, t.data_ptr()
     return t, at, T, n, h, a, ptr
 
 
