@@ -234,3 +234,14 @@ def test_one_token_with_any_stride():
         r, kr, vr = at.append_mx4(q, k, v, layer, _i32([0]), style=None, values=True)
         outs.append([r, kr, vr, *layer, at.attn_mx4(q, layer, _i32([0])), at.attn_packed(q, k, v, _i32([0, 1]))])
     assert all(torch.equal(s, t) for s, t in zip(*outs))
+
+
+def test_a_context_of_no_tokens():
+    """new_cache with a context of no tokens, on both caches."""
+    for kv in ("bfloat16", "mxfp4"):
+        F, dec = _decoder(kv_dtype=kv)
+        cache = dec.new_cache(2, 0, 40)
+        assert cache.get_seq_length() == 0 and set(cache.seq_len_dev.tolist()) == {0}
+        out = dec.greedy_decode(torch.tensor([3, 5]).cuda(), cache, 4)
+        again = dec.greedy_decode(torch.tensor([3, 5]).cuda(), dec.new_cache(2, 0, 40), 4, use_graph=False)
+        assert torch.equal(out, again) and cache.get_seq_length() == 4

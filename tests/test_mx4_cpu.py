@@ -154,3 +154,11 @@ def test_positions_of_every_token():
                             (torch.tensor([[1, 2], [5, 6]]), 4, 2, [1, 2, 5, 6])):
         got = _token_positions(pos, T, S)
         assert got.is_contiguous() and got.stride() == (1,) and got.tolist() == want
+
+
+def test_bounds_of_sequences_of_one_length():
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    cache = F.Mx4Cache(8)
+    for B, S in ((3, 0), (1, 1), (2, 5)):
+        b = cache._bounds_of(B, S, "cpu")
+        assert b.dtype == torch.int32 and b.tolist() == [S * i for i in range(B + 1)]

@@ -289,7 +289,7 @@ class Mx4Cache(TppCache):
     def _bounds_of(self, B, S, device):
         at = self._bounds.get((B, S))
         if at is None:
-            at = self._bounds[(B, S)] = torch.arange(0, B * S + 1, S, dtype=torch.int32, device=device)
+            at = self._bounds[(B, S)] = torch.arange(B + 1, dtype=torch.int32, device=device) * S
         return at
 
     def prompts(self, lengths, device="cuda"):
