@@ -245,3 +245,38 @@ def test_a_context_of_no_tokens():
         out = dec.greedy_decode(torch.tensor([3, 5]).cuda(), cache, 4)
         again = dec.greedy_decode(torch.tensor([3, 5]).cuda(), dec.new_cache(2, 0, 40), 4, use_graph=False)
         assert torch.equal(out, again) and cache.get_seq_length() == 4
+
+
+def test_several_tokens_first_asked_for_inside_a_capture():
+    """A pass of several tokens that is captured first and run eagerly before the first replay, then replayed."""
+    F = _llm()
+    B, S, Nq, Nkv, H = 2, 3, 4, 2, 128
+    q, k, v = (R.randn((B, S, n * H), 1.0, i).cuda() for i, n in enumerate((Nq, Nkv, Nkv)))
+
+    def fresh():
+        c = F.Mx4Cache(32)
+        zeros = torch.zeros((B, Nkv, 5, H), dtype=torch.bfloat16, device="cuda")
+        return c.fill_(0, zeros, zeros + 1)
+
+    pos = torch.zeros((1, S), dtype=torch.int64, device="cuda")
+
+    def run(cache, q):
+        return F.rotate_append_attend(q, k, v, None, pos, cache, 0, B, S, Nq, Nkv, H, None, None)
+
+    want = run(fresh(), q)  # (and the workspace exists)
+    cache = fresh()
+    x = q.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(cache, x)
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        assert torch.equal(run(cache, q), want)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        junk = [torch.full((B + 1,), 77, dtype=torch.int32, device="cuda") for _ in range(20)]
+        del junk

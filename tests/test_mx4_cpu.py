@@ -162,3 +162,14 @@ def test_bounds_of_sequences_of_one_length():
     for B, S in ((3, 0), (1, 1), (2, 5)):
         b = cache._bounds_of(B, S, "cpu")
         assert b.dtype == torch.int32 and b.tolist() == [S * i for i in range(B + 1)]
+
+
+def test_few_bounds_are_kept():
+    """The last ones that were asked for: a prompt of every length leaves no tensor each."""
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    cache = F.Mx4Cache(8)
+    first = cache._bounds_of(2, 1, "cpu")
+    for S in range(2, 40):
+        cache._bounds_of(2, S, "cpu")
+        assert cache._bounds_of(2, 1, "cpu") is first
+    assert len(cache._bounds) <= cache.KEPT_BOUNDS and cache._bounds_of(2, 39, "cpu").tolist() == [0, 39, 78]

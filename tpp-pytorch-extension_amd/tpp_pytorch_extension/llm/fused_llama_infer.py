@@ -258,11 +258,12 @@ class Mx4Cache(TppCache):
     of different lengths.  Head sizes as in `mx4_cache.HEAD_SIZES`."""
 
     kv_dtype = "mxfp4"
+    KEPT_BOUNDS = 8
 
     def __init__(self, capacity=0):
         super().__init__(capacity)
         self._packed = None   # (bounds int32 [B + 1], lengths) of a pass over packed prompts
-        self._bounds = {}     # (B, S) -> bounds of B times S tokens
+        self._bounds = {}     # (B, S, device, stream) -> bounds of B times S tokens, the last few
         self._short = None    # by how much every sequence is shorter than the longest, or None: not at all
 
     def _sequences(self, B, device):
@@ -287,9 +288,23 @@ class Mx4Cache(TppCache):
         return layer
 
     def _bounds_of(self, B, S, device):
-        at = self._bounds.get((B, S))
+        """Bounds of B sequences of S tokens.  Kept for the stream that they were made on, which orders them; a capture makes its own,
+        which hold something in its replays alone."""
+        device = torch.device(device)
+        stream = None
+        if device.type == "cuda":
+            if torch.cuda.is_current_stream_capturing():
+                return torch.arange(B + 1, dtype=torch.int32, device=device) * S
+            if device.index is None:
+                device = torch.device("cuda", torch.cuda.current_device())
+            stream = torch._C._cuda_getCurrentRawStream(device.index)
+        key = (B, S, device, stream)
+        at = self._bounds.pop(key, None)
         if at is None:
-            at = self._bounds[(B, S)] = torch.arange(B + 1, dtype=torch.int32, device=device) * S
+            at = torch.arange(B + 1, dtype=torch.int32, device=device) * S
+            if len(self._bounds) >= self.KEPT_BOUNDS:
+                del self._bounds[next(iter(self._bounds))]
+        self._bounds[key] = at  # (last: the one used longest ago goes first)
         return at
 
     def prompts(self, lengths, device="cuda"):
