@@ -280,3 +280,18 @@ def test_several_tokens_first_asked_for_inside_a_capture():
         assert torch.equal(out, want)
         junk = [torch.full((B + 1,), 77, dtype=torch.int32, device="cuda") for _ in range(20)]
         del junk
+
+
+def test_a_refused_mask_leaves_the_cache_as_it_was():
+    F = _llm()
+    B, Nkv, Rr, H = 2, 2, 2, 64
+    cache = F.kv_cache(16, "mxfp4")
+    q, k, v = (R.randn((B, Nkv, 3, n, H), 1.0, n).cuda() for n in (Rr, 1, 3))
+    k, v = k[:, :, :, 0].contiguous(), v[:, :, :, 1].contiguous()
+    F.attn(q, k, v, None, cache, 0)
+    before = [t.clone() for t in cache.layers[0]]
+    for mask in (torch.zeros(1, 6), torch.zeros(B, 1, 3, 6), torch.zeros(B, 6).cuda().expand(3, B, 6)):
+        with pytest.raises(F.TppxError):
+            F.attn(q, k, v, mask.to(torch.bfloat16).cuda(), cache, 0)
+        assert cache.get_seq_length() == 3 and cache.seq_len_dev.tolist() == [3, 3] and cache.get_capacity() == 16
+        assert all(torch.equal(a, b) for a, b in zip(cache.layers[0], before))

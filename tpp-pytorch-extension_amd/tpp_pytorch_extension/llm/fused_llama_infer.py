@@ -465,9 +465,12 @@ class Mx4Cache(TppCache):
     def attend(self, t_QL, t_KL, t_VL, t_AM, layer_idx):
         """`attn` below over this cache."""
         B, Nkv, Sq, R, H = t_QL.shape
+        mask = None
+        if t_AM is not None and t_AM.numel():  # (refused before the cache changes)
+            mask = t_AM.to(torch.bfloat16).reshape(-1, t_AM.shape[-1]).contiguous()
+            mx4_cache.check_mask(mask, B, t_QL.get_device())
         past = self._append_states(t_KL, t_VL, layer_idx)
         q = t_QL.permute(0, 2, 1, 3, 4).reshape(B * Sq, Nkv * R, H)
-        mask = t_AM.to(torch.bfloat16).reshape(-1, t_AM.shape[-1]).contiguous() if t_AM is not None and t_AM.numel() else None
         at = torch.full((B,), past, dtype=torch.int32, device=q.device)
         out = mx4_cache.attn_mx4(q, self.layers[layer_idx], at, None if Sq == 1 else self._bounds_of(B, Sq, q.device), mask)
         return out.view(B, Sq, Nkv, R, H).permute(0, 2, 1, 3, 4).contiguous()

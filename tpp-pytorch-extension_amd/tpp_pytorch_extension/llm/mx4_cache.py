@@ -191,7 +191,8 @@ def append_mx4(q, k, v, layer, past, cu_seqlens=None, q_weight=None, k_weight=No
     return qo, ko, vo
 
 
-def _mask(mask, B, dev):
+def check_mask(mask, B, dev):
+    """(address, keys) of an additive mask, or (None, 0)."""
     if mask is None or mask.numel() == 0:
         return None, 0
     if mask.dim() != 2 or mask.shape[0] != B or mask.dtype is not BF16 or not mask.is_contiguous() or mask.get_device() != dev:
@@ -208,7 +209,7 @@ def attn_mx4(q, layer, past, cu_seqlens=None, mask=None):
     B, past_at, cu_at = _sequences(T, past, cu_seqlens, dev)
     Nkv = layer[0].shape[1] if layer[0].dim() == 4 else 0
     kc, ks, vc, vs, cap = _layer(layer, B, Nkv, H, dev)
-    m_at, m_ld = _mask(mask, B, dev)
+    m_at, m_ld = check_mask(mask, B, dev)
     out = q.new_empty(T, Nq, H)
     if T == 0:
         return out
@@ -229,7 +230,7 @@ def attn_packed(q, k, v, cu_seqlens, mask=None):
     if B < 1:
         raise TppxError(_lib.ESHAPE, f"cu_seqlens must be int32 [sequences + 1], got {tuple(cu_seqlens.shape)}")
     cu_at = _index(cu_seqlens, "cu_seqlens", B + 1, dev)
-    m_at, m_ld = _mask(mask, B, dev)
+    m_at, m_ld = check_mask(mask, B, dev)
     out = q.new_empty(T, Nq, H)
     if T == 0:
         return out
