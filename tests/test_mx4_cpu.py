@@ -173,3 +173,43 @@ def test_few_bounds_are_kept():
         cache._bounds_of(2, S, "cpu")
         assert cache._bounds_of(2, 1, "cpu") is first
     assert len(cache._bounds) <= cache.KEPT_BOUNDS and cache._bounds_of(2, 39, "cpu").tolist() == [0, 39, 78]
+
+
+def test_an_announced_pass_over_packed_prompts():
+    """Other passes, appends and reorders are refused until it ends or is dropped; a crop and new contents drop it."""
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    cache = F.Mx4Cache(40)
+    pos = torch.zeros((1, 3), dtype=torch.int64)
+
+    def announce(lengths):
+        cache.prompts(lengths, "cpu")
+
+    def refused(call):
+        with pytest.raises(F.TppxError):
+            call()
+        assert cache._packed is not None
+
+    announce([4, 2])
+    refused(lambda: F.check_layer_inputs("block", torch.zeros((2, 3, 8)), pos, cache))  # as many tokens, another shape
+    refused(lambda: F.check_layer_inputs("block", torch.zeros((2, 1, 8)), pos[:, :1], cache))
+    refused(lambda: cache.rotate_append_attend(None, None, None, None, None, 0, 2, 3, 2, 1, 64, None, None))
+    refused(lambda: cache.rotate_append_attend(None, None, None, None, None, 0, 2, 6, 2, 1, 64, None, None))
+    refused(lambda: cache.advance(1))
+    refused(lambda: cache.advance(100))
+    refused(lambda: cache.reorder_cache(torch.tensor([0, 0])))
+    refused(lambda: cache.update(torch.zeros(2, 1, 1, 64), torch.zeros(2, 1, 1, 64), 0))
+    assert cache.room_for(6) and cache.seq_len_dev.tolist() == [0, 0] and cache.get_seq_length() == 0
+    cache.advance(6)
+    assert cache.seq_len_dev.tolist() == [4, 2] and cache._packed is None
+    announce([1, 36])
+    cache.cancel_prompts()
+    assert cache.seq_len_dev.tolist() == [4, 2] and cache.room_for(36) and not cache.room_for(37)
+    cache.advance()
+    cache.advance(2)
+    assert cache.seq_len_dev.tolist() == [7, 5]
+    announce([1, 1])
+    cache.crop(6)
+    assert cache._packed is None and cache.seq_len_dev.tolist() == [6, 5]
+    cache.reorder_cache(torch.tensor([1, 1]))
+    cache.advance(1)
+    assert cache.seq_len_dev.tolist() == [6, 6]

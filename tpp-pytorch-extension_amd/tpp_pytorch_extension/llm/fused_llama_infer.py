@@ -309,7 +309,8 @@ class Mx4Cache(TppCache):
 
     def prompts(self, lengths, device="cuda"):
         """The next pass of the blocks runs over packed prompts: hidden states [1][sum(lengths)][..], sequence b's tokens behind
-        sequence b - 1's, positions [1][sum(lengths)]; `advance()` without an argument ends it.  Returns the bounds int32 [B + 1]."""
+        sequence b - 1's, positions [1][sum(lengths)] (`next_positions`); `advance()` ends it, `cancel_prompts()` where the pass failed.
+        Until then other passes and appends are refused.  Returns the bounds int32 [B + 1]."""
         lengths = [int(n) for n in lengths]
         if not lengths or min(lengths) < 0:
             raise TppxError(_lib.ESHAPE, f"Mx4Cache.prompts: lengths {lengths}")
@@ -323,8 +324,21 @@ class Mx4Cache(TppCache):
         self._packed = (torch.tensor(starts, dtype=torch.int32, device=device), lengths)
         return self._packed[0]
 
+    def cancel_prompts(self):
+        """The pass that `prompts()` announced does not take place: the sequences hold what they held before."""
+        self._packed = None
+
+    def _refuse_while_packed(self, what):
+        if self._packed is not None:
+            raise TppxError(_lib.EINVAL, f"Mx4Cache: {what} while a pass over packed prompts of {self._packed[1]} is announced (advance() ends it, "
+                                         "cancel_prompts() drops it)")
+
     def room_for(self, S):
-        return self._packed is not None or super().room_for(S)
+        if self._packed is None:
+            return super().room_for(S)
+        if S != sum(self._packed[1]):
+            self._refuse_while_packed(f"a pass of {S} tokens a row")
+        return True  # (prompts() has seen to it)
 
     def positions(self, B, device):
         self._sequences(B, device)
@@ -341,10 +355,13 @@ class Mx4Cache(TppCache):
             return super().next_positions(S, device)
         return self.positions(len(self._short), device) + torch.arange(S, dtype=torch.int64, device=device)
 
-    def advance(self, n=1):
-        """Every sequence holds n more keys; after a pass over packed prompts, each the keys of its prompt."""
+    def advance(self, n=None):
+        """Every sequence holds n more keys (default 1); after a pass over packed prompts, each the keys of its prompt (n, if it is
+        given, is the number of all their tokens)."""
         if self._packed is None:
-            return super().advance(n)
+            return super().advance(1 if n is None else n)
+        if n is not None and n != sum(self._packed[1]):
+            self._refuse_while_packed(f"advance({n})")
         lengths, self._packed = self._packed[1], None
         self.seq_len_dev.add_(torch.tensor(lengths, dtype=torch.int32, device=self.seq_len_dev.device))
         now = [self._host_len - s + k for s, k in zip(self._short or [0] * len(lengths), lengths)]
@@ -352,6 +369,7 @@ class Mx4Cache(TppCache):
         self._advance_host(max(now) - self._host_len)
 
     def crop(self, max_length):
+        self._packed = None
         if self.seq_len_dev is not None:
             self.seq_len_dev.clamp_(max=int(max_length))
         if self._short is not None:
@@ -362,6 +380,7 @@ class Mx4Cache(TppCache):
         self._layer_len = {i: min(n, int(max_length)) for i, n in self._layer_len.items()}
 
     def reorder_cache(self, beam_idx):
+        self._refuse_while_packed("a reorder")
         beam_idx = beam_idx.to(torch.int64)
         n = self._host_len
         for layer in self.layers.values():
@@ -396,6 +415,7 @@ class Mx4Cache(TppCache):
         S = keys.shape[2]
         if S > self.capacity:
             raise TppxError(_lib.ESHAPE, f"Mx4Cache.fill_: {S} keys exceed the capacity {self.capacity}")
+        self._packed = None
         self._append(layer_idx, keys, values, 0)
         self._host_len = self._sync_len = S
         self._layer_len, self._short = {}, None
@@ -404,6 +424,7 @@ class Mx4Cache(TppCache):
 
     def _append_states(self, keys, values, layer_idx):
         """Appends to sequences of one length, at the layer's length, which is returned."""
+        self._refuse_while_packed("an append of states")
         if self._short is not None and any(self._short):
             raise TppxError(_lib.EUNSUPPORTED, "Mx4Cache: states are appended to sequences of one length")
         S = keys.shape[2]
@@ -442,8 +463,8 @@ class Mx4Cache(TppCache):
         T = B * S
         if self._packed is not None:
             bounds, lengths = self._packed
-            if T != sum(lengths):
-                raise TppxError(_lib.ESHAPE, f"Mx4Cache: a pass of {T} tokens over packed prompts of {sum(lengths)}")
+            if B != 1 or S != sum(lengths):
+                raise TppxError(_lib.ESHAPE, f"Mx4Cache: a pass of [{B}][{S}] tokens over packed prompts of [1][{sum(lengths)}]")
             if t_am is not None and t_am.numel():
                 raise TppxError(_lib.EUNSUPPORTED, "Mx4Cache: packed prompts take no padding mask")
             B = len(lengths)
@@ -827,7 +848,7 @@ class LlamaDecoder:
             for layer in self.layers:
                 h = layer.forward([h, None, pos], cache)[0]
         except BaseException:
-            cache._packed = None
+            cache.cancel_prompts()
             raise
         cache.advance()
         h = rms_norm(h[0].index_select(0, bounds[1:].to(torch.int64) - 1), self.norm_w, self.eps)
