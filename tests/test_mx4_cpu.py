@@ -213,3 +213,11 @@ def test_an_announced_pass_over_packed_prompts():
     cache.reorder_cache(torch.tensor([1, 1]))
     cache.advance(1)
     assert cache.seq_len_dev.tolist() == [6, 6]
+
+
+def test_generate_packed_refuses_a_decoder_on_the_bf16_cache():
+    from types import SimpleNamespace
+    from tpp_pytorch_extension.llm import fused_llama_infer as F
+    with pytest.raises(F.TppxError) as e:
+        F.LlamaDecoder.generate_packed(SimpleNamespace(kv_dtype="bfloat16"), [torch.tensor([1, 2])], 3)
+    assert e.value.code == F._lib.EINVAL and "kv_dtype" in str(e.value)

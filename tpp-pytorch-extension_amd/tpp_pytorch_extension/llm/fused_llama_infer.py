@@ -855,10 +855,12 @@ class LlamaDecoder:
         return _ops.fc_plain(h, self.lm_head, None).argmax(dim=-1)
 
     def generate_packed(self, prompts, n_new, capacity=None, use_graph=True):
-        """`generate` for prompts of different lengths (a list of i64 [n]): one packed pass, then one token per sequence and step.
-        Returns i64 [B][n_new]."""
+        """`generate` for prompts of different lengths (a list of i64 [n]): one packed pass, then one token per sequence and step, on an
+        MXFP4 cache: for a decoder with kv_dtype="mxfp4".  Returns i64 [B][n_new]."""
         if not prompts:
             raise TppxError(_lib.ESHAPE, "generate_packed: no prompts")
+        if self.kv_dtype != "mxfp4":  # (not four bits in the place of sixteen unasked)
+            raise TppxError(_lib.EINVAL, f"generate_packed: sequences of different lengths need an MXFP4 cache, the decoder's kv_dtype is {self.kv_dtype!r}")
         cache = Mx4Cache(capacity or max(int(p.numel()) for p in prompts) + n_new + 32)
         first = self.prefill_packed(prompts, cache).view(-1, 1)
         if n_new == 1:
