@@ -295,3 +295,18 @@ def test_a_refused_mask_leaves_the_cache_as_it_was():
             F.attn(q, k, v, mask.to(torch.bfloat16).cuda(), cache, 0)
         assert cache.get_seq_length() == 3 and cache.seq_len_dev.tolist() == [3, 3] and cache.get_capacity() == 16
         assert all(torch.equal(a, b) for a, b in zip(cache.layers[0], before))
+
+
+@pytest.mark.parametrize("S", [1, 4])
+def test_masks_of_the_blocks_in_four_dimensions(S):
+    """The additive mask [B][1][1][keys] through a decoder block: what [B][keys] gives, on both caches."""
+    for kv in ("bfloat16", "mxfp4"):
+        F, dec = _decoder(kv_dtype=kv)
+        mask = torch.zeros((2, 32), dtype=torch.bfloat16, device="cuda")
+        mask[1, :6] = torch.finfo(torch.bfloat16).min
+        h = R.randn((2, S, 512), 1.0, 4).cuda()
+        outs = []
+        for m in (mask, mask.view(2, 1, 1, 32)):
+            cache = dec.new_cache(2, 20, 40)
+            outs.append(dec.layers[0].forward([h, m, cache.positions(2, "cuda") + torch.arange(S, device="cuda")], cache)[0])
+        assert torch.equal(outs[0], outs[1])

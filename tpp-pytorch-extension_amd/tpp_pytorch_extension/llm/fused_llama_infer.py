@@ -476,7 +476,7 @@ class Mx4Cache(TppCache):
         fresh = bounds is not None and self._host_len == 0
         rows, kr, vr = mx4_cache.append_mx4(q.view(T, Nq, H), k.view(T, Nkv, H), v.view(T, Nkv, H), layer, self.seq_len_dev, bounds, wq, wk, eps,
                                             t_EP, pos, style, values=fresh)
-        mask = t_am if t_am is not None and t_am.numel() else None
+        mask = t_am.reshape(-1, t_am.shape[-1]) if t_am is not None and t_am.numel() else None  # ([B][1][1][keys] too)
         if fresh:
             ctx = mx4_cache.attn_packed(rows, kr, vr, bounds, mask)
         else:
