@@ -310,3 +310,24 @@ def test_masks_of_the_blocks_in_four_dimensions(S):
             cache = dec.new_cache(2, 20, 40)
             outs.append(dec.layers[0].forward([h, m, cache.positions(2, "cuda") + torch.arange(S, device="cuda")], cache)[0])
         assert torch.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("H,style,width", [(128, "llama", 128), (96, "llama", 64), (256, "gptj", 64)])
+def test_norms_of_heads_that_hold_an_infinity(H, style, width):
+    """Their mean square is infinite: the finite channels become zeros and the infinite ones NaN, for queries and for the codes of keys."""
+    at = _at()
+    T, Nq, Nkv = 4, 2, 2
+    table = (R.llama_table if style == "llama" else R.gptj_table)(16, width)
+    w = R.randn(H, 0.2, 9).float() + 1
+    q, k, v = (R.randn((T, n, H), 1.0, i) for i, n in enumerate((Nq, Nkv, Nkv)))
+    q[0, 0, 5], k[0, 1, 3], k[1, 0, H - 1], k[2, 1, 7] = math.inf, math.inf, -math.inf, math.nan
+    layer = at.Mx4Layer(*(torch.zeros((1, Nkv, 8, n), dtype=torch.uint8, device="cuda") for n in (H // 2, H // 32, H // 2, H // 32)))
+    qo, ko, _ = at.append_mx4(q.cuda(), k.cuda(), v.cuda(), layer, _i32([1]), _i32([0, T]), w.cuda(), w.cuda(), 1e-6, table.cuda(), None, style, values=True)
+    pos = range(1, 1 + T)
+    want, size = R.turn(q, w, 1e-6, table, pos, style)
+    assert torch.equal(qo.isnan().cpu(), want.isnan())
+    _within(qo.nan_to_num(), want.nan_to_num(), (2.0 ** -8 * want.abs() + 2.0 ** -20 * size.abs()).nan_to_num() + 2.0 ** -133)
+    codes, scales = R.encode(R.turn(k, w, 1e-6, table, pos, style)[0])
+    assert torch.equal(layer.k_scales[0, :, 1:1 + T].cpu(), scales.transpose(0, 1))
+    held = R.decode(codes, scales)
+    assert torch.equal(ko.isnan().cpu(), held.isnan()) and torch.equal(ko.nan_to_num().cpu().double(), held.nan_to_num().to(torch.bfloat16).double())

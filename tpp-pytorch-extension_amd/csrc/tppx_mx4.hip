@@ -66,8 +66,8 @@ __device__ __forceinline__ A sum_of_lanes(A v) {
 __device__ __forceinline__ float rsqrt_t(float v) { return 1.0f / sqrtf(v); }
 __device__ __forceinline__ double rsqrt_t(double v) { // the hardware's estimate and two steps of Newton's method
   double r = __builtin_amdgcn_rsq(v);
-  r *= 1.5 - 0.5 * v * r * r;
-  return r * (1.5 - 0.5 * v * r * r);
+  const double a = r * (1.5 - 0.5 * v * r * r);
+  return v == (double)INFINITY ? r : a * (1.5 - 0.5 * v * a * a); // (of infinity zero, which Newton's step makes NaN)
 }
 
 // What the lanes of a row share out: chunks c[0], c[1] of 8 channels; their angles where they are rotated (adjacent pairs: four
