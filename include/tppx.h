@@ -729,7 +729,8 @@ int tppx_attn_mx4(const void* q, const void* k_codes, const void* k_scales,
                   void* counters, int64_t counter_bytes, tppx_stream_t stream);
 
 /* Causal attention of packed prompts over their own bf16 keys and values: token i of a sequence sees its tokens 0 .. i;
- * mask [B][mask_ld] over these, as above. */
+ * mask [B][mask_ld] over these, as above.  Values that are not finite reach the tokens that see them, and those alone; an
+ * infinite one under a probability below fp32's range gives an infinity or NaN. */
 int tppx_attn_packed(const void* q, const void* k, const void* v,
                      const void* cu, const void* mask, int64_t mask_ld,
                      void* out, int64_t T, int64_t B, int64_t Nq, int64_t Nkv,

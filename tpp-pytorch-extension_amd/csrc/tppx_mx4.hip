@@ -357,7 +357,7 @@ mx4_rows_kernel(const Mx4RowsParams p) {
 // What bounds it: large layers the cache's bytes (32 sequences x 16000 keys x 8 K/V heads of 128, 558 MB: 88 us, 6.3 TB/s; a large
 // copy moves 5.15, in and out); smaller ones a wave's way through a tile (about a microsecond: loads, two chains of matrix instructions, the
 // softmax between them), the number of tiles that it takes one after the other, and the merge behind them (1 x 2048 keys of 32 heads,
-// 8.9 MB: 7.0 us; 16 uneven sequences of 28 heads on 4, 20 MB: 14.0).  The bf16 cache's kernel takes 85 us for 16 x 2048 keys of 32 heads, this
+// 8.9 MB: 7.0 us; 16 uneven sequences of 64 heads on 8, 20 MB: 14.0 .. 14.6).  The bf16 cache's kernel takes 85 us for 16 x 2048 keys of 32 heads, this
 // one 25.
 // ---------------------------------------------------------------------------
 template <int NJ>
@@ -780,7 +780,7 @@ static int split_launch(const char* who, Mx4AttnParams& p, int H, void* ws, int6
   TPPX_REQUIRE(units < ((int64_t)1 << 31), TPPX_ESHAPE, "%s: problem too large", who);
   p.cols = p.cu ? 16 : std::min(16, p.R);
   const int64_t trips = ((int64_t)p.Smax + W * 64 - 1) / (W * 64);
-  // 512 workgroups, two per CU: 32 x 16000 keys of 8 K/V heads (256 units) 88.5 us with two splits, 93 with three, 105 with four;
+  // 512 workgroups, two per CU (behind a mask and 192 or 256 wide one: 258 registers): 32 x 16000 keys of 8 K/V heads (256 units) 88.5 us with two splits, 93 with three, 105 with four;
   // 8 x 3000 of 16, 256 wide (128) 34 with one, 24.3 with two, 24.7 with four, 27 with twelve; 1 x 2048 of 32 (32) 12.6 with one, 7.8
   // with four, 6.9 with eight; 1 x 16000 of 8 (8) 73 with one, 11.0 with 32; 16 x 2048 of 32 (512) 25.2 with one, 28.9 with two.  Splits
   // beyond a sequence's keys end at once.
@@ -788,6 +788,10 @@ static int split_launch(const char* who, Mx4AttnParams& p, int H, void* ws, int6
   // trips (24 x 2000 of 8 (192): 15.4 with one split, 16.4 with two; 32 x 500 (256) 7.0 and 8.8; 6 x 12 tokens of 28 heads on 4 behind 1500
   // (148) 12.0, with three 14.6; 64 of 32 heads behind 2000 (128) 16.2, with four 14.4), with single tokens and up to 128 units two
   // (4 x 700 of 16, 256 wide (64) 12.4, with three 8.6; 4 x 1000 of 32 (128) 8.5, with four 8.0).
+  // Those were measured in caches as long as their keys.  The lengths are on the device: the rule goes by the capacity, and in a longer
+  // cache some short sequences are split where they were better not: 32 x 500 of 8 in 4096 slots 8.5, unsplit 5.8; 16 x 300 of 28 heads on 4 in
+  // 4096 7.1 and 5.7; 24 x 2000 of 8 in 4096 15.9 and 14.8.  1 x 2048 of 32 in 16384 takes the 6.7 that it takes in 2112, unsplit 12.6.  A few new
+  // tokens gain nothing either: 6 x 7 of 28 heads on 4 behind 1500 12.5 with five splits, unsplit 11.4.
   int64_t S = env_int("TPPX_MX4_SPLITS", 0);
   if (S <= 0) {
     S = std::min<int64_t>(std::max<int64_t>(512 / units, 1), trips);
@@ -802,7 +806,8 @@ static int split_launch(const char* who, Mx4AttnParams& p, int H, void* ws, int6
   p.counters = (unsigned int*)counters;
   const dim3 grid((unsigned)units, (unsigned)S);
   // A layer past the 256 MiB of the last-level cache cannot be there from a launch before: its codes go by without being kept (558 MB
-  // 102 -> 88.5 us, 6.3 TB/s); smaller ones may be (40 MB 12.3 us, with the hint 13.4; 143 MB 25.2 and 24.8).
+  // 102 -> 88.5 us, 6.3 TB/s); smaller ones may be (40 MB 12.3 us, with the hint 13.4; 143 MB 25.2 and 24.8).  This too goes by the
+  // capacity: 70 MB of keys in a layer of 285 MB take 13.3 us with the hint, in one of 74 MB 15.1 without it.
   const bool stream_codes = (int64_t)p.B * p.Nkv * p.Smax * H >= ((int64_t)256 << 20);
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
@@ -909,7 +914,7 @@ extern "C" int tppx_attn_mx4(const void* q, const void* k_codes, const void* k_s
   p.past = (const int32_t*)past; p.cu = (const int32_t*)cu; p.mask = (const uint16_t*)mask; p.mask_ld = (int)mask_ld; p.out = (uint16_t*)out;
   p.T = (int)T; p.B = (int)B; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.R = (int)(Nq / Nkv); p.Smax = (int)Smax;
   p.scale = 1.0f / sqrtf((float)H);
-  // The prompt kernel expands a tile of the cache for 64 or 128 queries of one head, this one reads it for 16 (token, head) pairs: from
+  // The prompt kernel expands a tile of the cache for 128 queries of one head, the split kernel reads it for 16 (token, head) pairs: from
   // enough queries on to fill the chip (T * Nq) the former does less for each, below that its few workgroups walk all keys.  Split
   // kernel and prompt kernel, us: 64 tokens x 64 heads on 8 behind 6000 keys 36 and 120, 256 tokens 94 and 124, 384 133 and 149;
   // 512 x 32 heads behind 2000 46 and 56, 768 66 and 64; 4 x 500 x 12 of 64 19.7 and 22.4; 1200 x 16 of 256 75 and 82.

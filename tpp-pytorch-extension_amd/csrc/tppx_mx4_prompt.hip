@@ -55,7 +55,8 @@ __device__ __forceinline__ void mx4_add_non_finite(uint16_t* orow, int lane, int
 // are merged at the end: launches of few workgroups).  Codes are expanded once per workgroup on the way to LDS.  32 queries per wave: an
 // operand read from LDS feeds 32 columns; heads of 192 and 256 run on 16, for the registers.
 // What bounds it: the way of the codes into LDS (without it 35 % less) and, as in the packed kernel, the chain scores, softmax, output
-// of a wave.  512 tokens x 64 heads behind 6000 keys 134 .. 147 us (boxes differ), 720 .. 780 TFLOP/s.
+// of a wave (matrix instructions take 0.30 of the time).  512 tokens x 64 heads behind 6000 keys 131 .. 147 us (boxes differ), 715 .. 800
+// TFLOP/s.
 // ---------------------------------------------------------------------------
 // Pitch of a row in LDS.  K is read 16 bytes per lane, 16 rows at a time: rows 4 banks apart.  V is read 8 bytes per lane, 4 rows of
 // 64 bytes by 32 lanes: rows 16 banks apart (or 48); at K's pitch half of the cycles of LDS were bank conflicts.
@@ -372,9 +373,12 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 // Packed bf16 prompts: W waves of 16 queries, tiles of KEYS keys brought by loads straight into LDS, one ahead.  The chunks of 16 bytes
 // of a row lie permuted (those loads write 1024 bytes in a row), so that neither the rows of a K operand nor the pieces that the
 // transposing read of V takes meet in a bank.
+// A value that is infinite where a query sees it but its probability is below fp32's range gives NaN by the matrix instruction in
+// whole tiles (zero times infinity) and its infinity in those that end inside the sequence, where it is added by itself.
 // What bounds it: the chain scores, softmax, output of a wave (matrix instructions take 0.39 of the time); so four waves per SIMD in 128
 // registers count for more than operands that feed 32 queries.  Measured against 32 queries a wave, two per SIMD, the tiles through
-// registers: 4 prompts of up to 4100 tokens x 32 heads 187 -> 171 us (860 TFLOP/s, where a large library product reaches 1138), 2048 x
+// registers: 4 prompts of up to 4100 tokens x 32 heads 187 -> 171 us (on other boxes 161 .. 183, 800 .. 910 TFLOP/s, where a large library
+// product reaches 1138 .. 1417), 2048 x
 // 32 heads 64 -> 52, 2048 x 64 on 8 95 -> 85, 2048 x 16 of 256 93 -> 77, 333 x 32 12.7 -> 10.6, 4 x 1000 x 12 of 64 28 -> 24.
 // Tried in that other form and slower: this tile's output and the next one's scores as one sequence of independent matrix
 // instructions (219 where it took 190), 256 queries in eight waves (195).
@@ -668,7 +672,7 @@ int mx4_prompt_launch(const char* who, const Mx4AttnParams& p, int H, bool cache
       // Heads of 64 and 96: 64 queries in four waves (24 x 50..500 tokens x 12 heads of 64 12.0 us, of 128 in eight 14.5; 4000 x 12 48 and 54; 4 x
       // 4000 x 10 of 96 171 and 175).  Wider ones in launches of some 400 (200 beyond 128 wide) workgroups of 128 queries and more: those
       // (2048 tokens x 32 heads, 512: 51, of 64 57; 2048 x 16 heads of 256, 256: 77 and 91; 1000 x 32 heads, 256: 25.3 and 23.1; 333 x 32 11.5
-      // and 10.6), and where the prompts are short on average 64 queries on tiles of 32 keys, whose LDS lets four workgroups run on a CU
+      // and 10.6), and where the prompts are short on average 64 queries on tiles of 32 keys, of whose workgroups four (128 wide; 192 three, 256 two) run on a CU
       // (16 x 17..200 x 28 heads 13.3 -> 11.8, 8 x 50..500 x 64 on 8 31.3 -> 28.7, 16 x 300 x 32 41 -> 38, 16 x 300 x 16 of 256 33.0 -> 30.7; 4 x 1000 x 64 on
       // 8 95 and 101, 6 x 60..1500 x 32 43.5 and 45.9).
       constexpr size_t lds = 4 * 64 * 64 * (size_t)NJ;
