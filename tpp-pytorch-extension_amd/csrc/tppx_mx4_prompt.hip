@@ -55,7 +55,7 @@ __device__ __forceinline__ void mx4_add_non_finite(uint16_t* orow, int lane, int
 // are merged at the end: launches of few workgroups).  Codes are expanded once per workgroup on the way to LDS.  32 queries per wave: an
 // operand read from LDS feeds 32 columns; heads of 192 and 256 run on 16, for the registers.
 // What bounds it: the way of the codes into LDS (without it 35 % less) and, as in the packed kernel, the chain scores, softmax, output
-// of a wave (matrix instructions take 0.30 of the time).  512 tokens x 64 heads behind 6000 keys 131 .. 147 us (boxes differ), 715 .. 800
+// of a wave (matrix instructions take 0.30 of the time).  512 tokens x 64 heads behind 6000 keys 131 .. 147 us (cards differ), 715 .. 800
 // TFLOP/s.
 // ---------------------------------------------------------------------------
 // Pitch of a row in LDS.  K is read 16 bytes per lane, 16 rows at a time: rows 4 banks apart.  V is read 8 bytes per lane, 4 rows of
@@ -377,7 +377,7 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 // whole tiles (zero times infinity) and its infinity in those that end inside the sequence, where it is added by itself.
 // What bounds it: the chain scores, softmax, output of a wave (matrix instructions take 0.39 of the time); so four waves per SIMD in 128
 // registers count for more than operands that feed 32 queries.  Measured against 32 queries a wave, two per SIMD, the tiles through
-// registers: 4 prompts of up to 4100 tokens x 32 heads 187 -> 171 us (on other boxes 161 .. 183, 800 .. 910 TFLOP/s, where a large library
+// registers: 4 prompts of up to 4100 tokens x 32 heads 187 -> 171 us (on other cards 161 .. 183, 800 .. 910 TFLOP/s, where a large library
 // product reaches 1138 .. 1417), 2048 x
 // 32 heads 64 -> 52, 2048 x 64 on 8 95 -> 85, 2048 x 16 of 256 93 -> 77, 333 x 32 12.7 -> 10.6, 4 x 1000 x 12 of 64 28 -> 24.
 // Tried in that other form and slower: this tile's output and the next one's scores as one sequence of independent matrix
