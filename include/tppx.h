@@ -737,6 +737,71 @@ int tppx_attn_packed(const void* q, const void* k, const void* v,
                      int64_t H, int64_t q_ld, int64_t k_ld, int64_t v_ld,
                      tppx_stream_t stream);
 
+/* ---- key/value cache in pages, drafted tokens ----
+ * No counterpart in the reference, whose cache is one block per batch and which decodes one token per step.  Head sizes H: 64,
+ * 96, 128, 192, 256; pages of a power of two of slots from 16 to 65536 (others TPPX_EUNSUPPORTED).
+ * A cache layer: bf16 [2][pages][Nkv][page][H], keys then values, 16-byte aligned.  Slot s of sequence b lies in page table[b][s / page]
+ * (device i32 [B][table_ld]) at s % page; an entry outside of 0 .. pages - 1 is no page.  Nodes are the packed tokens of a step: rows
+ * cu[b] .. cu[b + 1] - 1 of sequence b (device i32 [B + 1], ascending; NULL: one each, T == B), which held past[b] (device i32 [B]) keys
+ * before them; a sequence whose past is negative takes no part.  Node i of a sequence has slot past[b] + i.  parents (device i32 [T], or
+ * NULL): the number within its sequence of the node that a node continues, smaller than its own; anything else: none.  NULL: the
+ * node before it, so that a sequence's nodes are a piece of its text.  Rows of T behind cu[B] take no part: results and the cache are
+ * left as they were there.  No value in these arrays leads out of a buffer. */
+
+/* tppx_qk_norm_rotary of nodes with their keys and values v [T][Nkv][H] written to their slots (a slot without a page: dropped).  pos
+ * (i64 [T]) or NULL: past[b] plus the number of nodes that a node continues.  fp32 inside, one rounding.  q may be NULL; q_out
+ * [T][Nq][H] contiguous. */
+int tppx_append_paged(const void* q, const void* k, const void* v,
+                      const void* gamma_q, const void* gamma_k, int gamma_dtype,
+                      float eps, const void* emb_pos, int gptj, const void* pos,
+                      void* layer, const void* table, const void* past,
+                      const void* cu, const void* parents, void* q_out,
+                      int64_t T, int64_t B, int64_t Nq, int64_t Nkv, int64_t H,
+                      int64_t pages, int64_t page, int64_t table_ld,
+                      int64_t q_ld, int64_t k_ld, int64_t v_ld, int64_t MP,
+                      int64_t HR, tppx_stream_t stream);
+
+/* Attention of nodes over the cache, after their own keys went to it: node i of sequence b sees the slots 0 .. past[b] - 1, its own and
+ * those of the nodes that it continues.  softmax(q K^T / sqrt(H)) V, q and out bf16 [T][Nq][H]; a node that sees nothing gets zeros.  A
+ * slot without a page within what a node sees makes that sequence's results arbitrary.  ws: 256-byte aligned scratch (no state) and
+ * counters (u32 words 256 bytes apart, zero before the first launch, left zero): with enough of both, keys split over workgroups
+ * where nodes are few; launches that share either must be ordered. */
+int tppx_attn_paged(const void* q, const void* layer, const void* table,
+                    const void* past, const void* cu, const void* parents,
+                    void* out, int64_t T, int64_t B, int64_t Nq, int64_t Nkv,
+                    int64_t H, int64_t pages, int64_t page, int64_t table_ld,
+                    int64_t q_ld, void* ws, int64_t ws_bytes, void* counters,
+                    int64_t counter_bytes, tppx_stream_t stream);
+
+/* Which drafted nodes stand against the target's probabilities, and the token behind them.  tokens i64 [T]; target and draft
+ * logits [T][V] of dtype (TPPX_DT_*), rows t_ld, d_ld elements apart: row i is what follows node i.  p = softmax(target / t), with t
+ * temperatures[b] (f32 [B]) or temperature; t = 0: one for the first maximal logit.  From node 0 on the children of a node are tried in
+ * order; child x stands where uniforms[x] * M < p(x), M = 1 - p of the siblings before it (a token tried twice stands only once), or
+ * with draft logits (chains, parents NULL; q = softmax(draft / t)) where uniforms[x] * q(x) < p(x).  Where none stands the next token is the
+ * first whose cumulative sum of what is left (p without the children; max(p - q, 0); p where there is no child or nothing left) exceeds
+ * sample[b] times all of it.  uniforms f32 [T] and sample f32 [B] in [0, 1); both may be NULL at temperature 0.  fp64 inside.  A NaN
+ * logit is -inf; infinite ones share the row; a token outside of 0 .. V - 1 never stands.  Results: path i32 [T] (the numbers of
+ * the nodes that stand, node 0 first, then -1), count i32 [B] (how many, node 0 with them), next i64 [B].  A sequence without
+ * nodes has count 0 and next 0.  ws: 256-byte aligned scratch of tppx_verify_drafts_bytes(T, B, V, draft != NULL) bytes, no state;
+ * launches that share it must be ordered. */
+int tppx_verify_drafts(const void* tokens, const void* target, const void* draft,
+                       int dtype, const void* cu, const void* parents,
+                       const void* uniforms, const void* sample,
+                       const void* temperatures, float temperature, void* path,
+                       void* count, void* next, int64_t T, int64_t B, int64_t V,
+                       int64_t t_ld, int64_t d_ld, void* ws, int64_t ws_bytes,
+                       tppx_stream_t stream);
+int64_t tppx_verify_drafts_bytes(int64_t T, int64_t B, int64_t V, int drafts);
+
+/* The keys and values of accepted paths to the slots from past[b] on, in all layers of cache [layers][2][pages][Nkv][page][H]: for i <
+ * count[b] those of slot past[b] + path[cu[b] + i] go to slot past[b] + i.  path ascends within a sequence, path[cu[b] + i] >= i (others
+ * are skipped), as tppx_verify_drafts leaves it. */
+int tppx_keep_paged(void* cache, const void* table, const void* past,
+                    const void* path, const void* count, const void* cu,
+                    int64_t layers, int64_t T, int64_t B, int64_t Nkv, int64_t H,
+                    int64_t pages, int64_t page, int64_t table_ld,
+                    tppx_stream_t stream);
+
 /* The element-type switch of fc_plain_wrap (src/csrc/llm/fused_llm_infer.cpp:
  * 1526-1545) for QINT8-family weights and float / half activations, or a
  * pre-quantized qint8 input whose compute type is float

@@ -74,6 +74,135 @@ __device__ __forceinline__ bool locate(const int32_t* cu, int B, int T, int per,
   return locate(cu, B, T, per, rows, blk, o, [](int b, int) { return b; });
 }
 
+// ---------------------------------------------------------------------------
+// per-head norm and rotation: G lanes take a head's row, 16 channels each in two chunks of 8
+// ---------------------------------------------------------------------------
+template <int CTRL, typename A>
+__device__ __forceinline__ A dpp_t(A v) {
+  if constexpr (std::is_same_v<A, double>) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true);
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true), lo);
+  } else {
+    return dpp_mov<CTRL>(v);
+  }
+}
+// sum over G adjacent lanes, in all of them
+template <int G, typename A>
+__device__ __forceinline__ A sum_of_lanes(A v) {
+  v += dpp_t<0xB1>(v); // quad_perm [1,0,3,2]
+  v += dpp_t<0x4E>(v); // quad_perm [2,3,0,1]
+  if constexpr (G >= 8)
+    v += dpp_t<0x141>(v); // row_half_mirror
+  if constexpr (G >= 16)
+    v += dpp_t<0x140>(v); // row_mirror
+  return v;
+}
+__device__ __forceinline__ float rsqrt_t(float v) { return 1.0f / sqrtf(v); }
+__device__ __forceinline__ double rsqrt_t(double v) { // the hardware's estimate and two steps of Newton's method
+  double r = __builtin_amdgcn_rsq(v);
+  const double a = r * (1.5 - 0.5 * v * r * r);
+  return v == (double)INFINITY ? r : a * (1.5 - 0.5 * v * a * a); // (of infinity zero, which Newton's step makes NaN)
+}
+
+// What the lanes of a row share out: chunks c[0], c[1] of 8 channels; their angles where they are rotated (adjacent pairs: four
+// of each chunk, otherwise eight that both share).
+struct Mx4Lane {
+  int c[2];
+  bool live, turn;
+  float cs[8], sn[8];
+};
+template <int G, typename P>
+__device__ __forceinline__ void mx4_share(const P& p, int u, Mx4Lane& t) {
+  const int half = p.HR >> 4, rest = (p.H - p.HR) >> 4; // lanes of rotated chunks, of the others
+  t.live = u < half + rest;
+  t.c[0] = !t.live ? 0 : u < half ? u : u + half;
+  t.c[1] = !t.live ? 0 : u < half ? u + half : u + half + rest;
+}
+// the angles of position `at` (outside the table: not rotated) for lane u
+template <typename P>
+__device__ __forceinline__ void mx4_angles(const P& p, int u, int64_t at, Mx4Lane& t) {
+  t.turn = p.emb && at >= 0 && at < p.MP && u < (p.HR >> 4);
+  if (t.turn) {
+    const float* const c = p.emb + at * p.HR + (p.gptj ? p.HR >> 1 : 0);
+    const float* const s = p.emb + (p.gptj ? at : p.MP + at) * p.HR;
+    const int a0 = p.gptj ? t.c[0] * 4 : u * 8, a1 = p.gptj ? t.c[1] * 4 : u * 8 + 4;
+    const f32x4 c0 = *reinterpret_cast<const f32x4*>(c + a0), c1 = *reinterpret_cast<const f32x4*>(c + a1);
+    const f32x4 s0 = *reinterpret_cast<const f32x4*>(s + a0), s1 = *reinterpret_cast<const f32x4*>(s + a1);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      t.cs[e] = c0[e];
+      t.cs[4 + e] = c1[e];
+      t.sn[e] = s0[e];
+      t.sn[4 + e] = s1[e];
+    }
+  }
+}
+
+// a lane's 16 channels, normalised and rotated; all G lanes of the row take part
+template <int G, typename A, typename P>
+__device__ __forceinline__ void mx4_turn(const P& p, const uint4 (&w)[2], const Mx4Lane& t, const void* gamma, A (&y)[2][8]) {
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    float f[8];
+    unpack8(w[h], f);
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      y[h][e] = f[e];
+  }
+  if (gamma) {
+    A ss = 0;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        ss = fma(y[h][e], y[h][e], ss);
+    ss = sum_of_lanes<G>(ss);
+    const A r = rsqrt_t(ss * ((A)1 / (A)p.H) + (A)p.eps);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      float g[8];
+      if (p.gamma_f32) {
+        const f32x4* s = reinterpret_cast<const f32x4*>(gamma) + t.c[h] * 2;
+        const f32x4 a = s[0], b = s[1];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          g[e] = a[e];
+          g[4 + e] = b[e];
+        }
+      } else {
+        unpack8(reinterpret_cast<const uint4*>(gamma)[t.c[h]], g);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        y[h][e] = y[h][e] * r * (A)g[e];
+    }
+  }
+  if (!t.turn)
+    return;
+  auto rotate = [&](A& a, A& b, float c, float s) {
+    const A x = a, z = b;
+    if constexpr (std::is_same_v<A, float>) {
+      a = rotate_first(x, z, c, s);
+      b = rotate_second(x, z, c, s);
+    } else {
+      asm("" : "+v"(c), "+v"(s)); // (not as 32 registers of fp64 over the whole loop)
+      a = x * (A)c - z * (A)s;
+      b = z * (A)c + x * (A)s;
+    }
+  };
+  if (p.gptj) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        rotate(y[h][2 * e], y[h][2 * e + 1], t.cs[4 * h + e], t.sn[4 * h + e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      rotate(y[0][e], y[1][e], t.cs[e], t.sn[e]);
+  }
+}
+
 // eight E2M1 codes of a dword times the scale, exact in bf16
 __device__ __forceinline__ bf16x8 mx4_to_bf16(uint32_t codes, float scale) {
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);

@@ -43,106 +43,6 @@ struct Mx4RowsParams {
   float eps;
 };
 
-template <int CTRL, typename A>
-__device__ __forceinline__ A dpp_t(A v) {
-  if constexpr (std::is_same_v<A, double>) {
-    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true);
-    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true), lo);
-  } else {
-    return dpp_mov<CTRL>(v);
-  }
-}
-// sum over G adjacent lanes, in all of them
-template <int G, typename A>
-__device__ __forceinline__ A sum_of_lanes(A v) {
-  v += dpp_t<0xB1>(v); // quad_perm [1,0,3,2]
-  v += dpp_t<0x4E>(v); // quad_perm [2,3,0,1]
-  if constexpr (G >= 8)
-    v += dpp_t<0x141>(v); // row_half_mirror
-  if constexpr (G >= 16)
-    v += dpp_t<0x140>(v); // row_mirror
-  return v;
-}
-__device__ __forceinline__ float rsqrt_t(float v) { return 1.0f / sqrtf(v); }
-__device__ __forceinline__ double rsqrt_t(double v) { // the hardware's estimate and two steps of Newton's method
-  double r = __builtin_amdgcn_rsq(v);
-  const double a = r * (1.5 - 0.5 * v * r * r);
-  return v == (double)INFINITY ? r : a * (1.5 - 0.5 * v * a * a); // (of infinity zero, which Newton's step makes NaN)
-}
-
-// What the lanes of a row share out: chunks c[0], c[1] of 8 channels; their angles where they are rotated (adjacent pairs: four
-// of each chunk, otherwise eight that both share).
-struct Mx4Lane {
-  int c[2];
-  bool live, turn;
-  float cs[8], sn[8];
-};
-
-// a lane's 16 channels, normalised and rotated; all G lanes of the row take part
-template <int G, typename A>
-__device__ __forceinline__ void mx4_turn(const Mx4RowsParams& p, const uint4 (&w)[2], const Mx4Lane& t, const void* gamma, A (&y)[2][8]) {
-#pragma unroll
-  for (int h = 0; h < 2; h++) {
-    float f[8];
-    unpack8(w[h], f);
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      y[h][e] = f[e];
-  }
-  if (gamma) {
-    A ss = 0;
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        ss = fma(y[h][e], y[h][e], ss);
-    ss = sum_of_lanes<G>(ss);
-    const A r = rsqrt_t(ss * ((A)1 / (A)p.H) + (A)p.eps);
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      float g[8];
-      if (p.gamma_f32) {
-        const f32x4* s = reinterpret_cast<const f32x4*>(gamma) + t.c[h] * 2;
-        const f32x4 a = s[0], b = s[1];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          g[e] = a[e];
-          g[4 + e] = b[e];
-        }
-      } else {
-        unpack8(reinterpret_cast<const uint4*>(gamma)[t.c[h]], g);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        y[h][e] = y[h][e] * r * (A)g[e];
-    }
-  }
-  if (!t.turn)
-    return;
-  auto rotate = [&](A& a, A& b, float c, float s) {
-    const A x = a, z = b;
-    if constexpr (std::is_same_v<A, float>) {
-      a = rotate_first(x, z, c, s);
-      b = rotate_second(x, z, c, s);
-    } else {
-      asm("" : "+v"(c), "+v"(s)); // (not as 32 registers of fp64 over the whole loop)
-      a = x * (A)c - z * (A)s;
-      b = z * (A)c + x * (A)s;
-    }
-  };
-  if (p.gptj) {
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        rotate(y[h][2 * e], y[h][2 * e + 1], t.cs[4 * h + e], t.sn[4 * h + e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      rotate(y[0][e], y[1][e], t.cs[e], t.sn[e]);
-  }
-}
-
 // biased fp32 exponent (up to 2047 from fp64, kept in that bias) of the largest magnitude of 8 values
 template <typename A>
 __device__ __forceinline__ int top_exponent(const A (&y)[8]) {
@@ -198,9 +98,7 @@ mx4_rows_kernel(const Mx4RowsParams p) {
   const int nq = p.q ? p.Nq : 0, nk = p.Nkv, total = nq + nk + (p.v ? p.Nkv : 0);
   const int half = p.HR >> 4, rest = (p.H - p.HR) >> 4; // lanes of rotated chunks, of the others
   Mx4Lane t;
-  t.live = u < half + rest;
-  t.c[0] = !t.live ? 0 : u < half ? u : u + half;
-  t.c[1] = !t.live ? 0 : u < half ? u + half : u + half + rest;
+  mx4_share<G>(p, u, t);
   // rows of a token: queries, then keys, then values; the next one is under way while one is worked on
   uint4 next[2];
   auto load = [&](int i) {
@@ -231,21 +129,7 @@ mx4_rows_kernel(const Mx4RowsParams p) {
   }
   const int64_t at = p.pos ? p.pos[tok] : slot;
   const bool room = slot >= 0 && slot < p.Smax;
-  t.turn = p.emb && at >= 0 && at < p.MP && u < half; // positions outside the table are left unrotated
-  if (t.turn) {
-    const float* const c = p.emb + at * p.HR + (p.gptj ? p.HR >> 1 : 0);
-    const float* const s = p.emb + (p.gptj ? at : p.MP + at) * p.HR;
-    const int a0 = p.gptj ? t.c[0] * 4 : u * 8, a1 = p.gptj ? t.c[1] * 4 : u * 8 + 4;
-    const f32x4 c0 = *reinterpret_cast<const f32x4*>(c + a0), c1 = *reinterpret_cast<const f32x4*>(c + a1);
-    const f32x4 s0 = *reinterpret_cast<const f32x4*>(s + a0), s1 = *reinterpret_cast<const f32x4*>(s + a1);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      t.cs[e] = c0[e];
-      t.cs[4 + e] = c1[e];
-      t.sn[e] = s0[e];
-      t.sn[4 + e] = s1[e];
-    }
-  }
+  mx4_angles(p, u, at, t);
   uint4 w[2];
   auto step = [&]() {
     w[0] = next[0];
