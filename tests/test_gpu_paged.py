@@ -133,14 +133,20 @@ def test_attention_of_single_tokens(H, Nq, Nkv, page):
 
 @pytest.mark.parametrize("H,Nq,Nkv", [(64, 12, 4), (96, 10, 2), (128, 8, 8), (128, 16, 2), (192, 3, 1), (256, 4, 2)])
 @pytest.mark.parametrize("page", [16, 32, 256])
-def test_attention_of_trees(H, Nq, Nkv, page):
+@pytest.mark.parametrize("form", ["", "1", "2", "3"])
+def test_attention_of_trees(H, Nq, Nkv, page, form, monkeypatch):
+    if form:  # (one of the kernel's forms instead of the one that the sizes give)
+        monkeypatch.setenv("TPPX_PAGED_FORM", form)
     new, past = [9, 1, 0, 30, 70, 17], [40, 0, 3, 129, 63, 300]
     _check_attention(new, past, page, Nq, Nkv, H, [R.tree(n, n + page) if n else [] for n in new], seed=H + page, spare_rows=3)
 
 
 @pytest.mark.parametrize("H,Nq,Nkv", [(64, 12, 4), (96, 10, 2), (128, 8, 8), (128, 16, 2), (192, 3, 1), (256, 4, 2)])
 @pytest.mark.parametrize("new,past", [([70, 1, 200], [0, 500, 33]), ([130], [1000]), ([3, 2, 2], [15, -1, 0])])
-def test_attention_of_pieces_of_prompts(H, Nq, Nkv, new, past):
+@pytest.mark.parametrize("chunk", ["", "64"])
+def test_attention_of_pieces_of_prompts(H, Nq, Nkv, new, past, chunk, monkeypatch):
+    if chunk:  # (splits of 64 keys)
+        monkeypatch.setenv("TPPX_PAGED_CHUNK", chunk)
     _check_attention(new, past, 32, Nq, Nkv, H, None, seed=H + len(new), spare_rows=2)
 
 
@@ -178,9 +184,11 @@ def test_attention_past_the_table():
 
 @pytest.mark.parametrize("H,Nq,Nkv", [(64, 4, 2), (96, 4, 2), (128, 16, 2), (256, 4, 2)])
 @pytest.mark.parametrize("new", [4, 40])
-def test_what_a_node_does_not_see_may_be_anything(H, Nq, Nkv, new):
+@pytest.mark.parametrize("form", ["1", "2", "3"])
+def test_what_a_node_does_not_see_may_be_anything(H, Nq, Nkv, new, form, monkeypatch):
     """Infinities and NaN in the keys and values of nodes that another does not continue, and behind the last one, stay there."""
     at = _at()
+    monkeypatch.setenv("TPPX_PAGED_FORM", form)
     page, past = 16, 37
     parents = [-1, 0, 0, 1] + [R.tree(new, 9)[i] for i in range(4, new)]
     parents = [p if p != 2 else 0 for p in parents]  # nobody continues node 2

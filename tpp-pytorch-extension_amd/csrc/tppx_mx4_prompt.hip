@@ -19,14 +19,6 @@ namespace tppx {
 // tiles where some query misses a key values that are infinite or NaN become zeros in LDS; a workgroup that met such values adds them,
 // one by one, to the outputs of the queries that see them once those are written.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ bool mx4_non_finite(uint32_t pair) {
-  return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
-}
-// the pair with what is not finite set to zero
-__device__ __forceinline__ uint32_t mx4_finite(uint32_t pair) {
-  return ((pair & 0x7f80u) == 0x7f80u ? 0u : pair & 0xffffu) | ((pair & 0x7f800000u) == 0x7f800000u ? 0u : pair & 0xffff0000u);
-}
-
 // Values that are not finite, added one by one to what a lane wrote itself: channels d + 4 lane .. + 3 of a row of H, keys from .. limit - 1.
 template <int H, int LANES, typename F>
 __device__ __forceinline__ void mx4_add_non_finite(uint16_t* orow, int lane, int from, int limit, const uint16_t* mrow, int mask_ld, F&& value) {
@@ -383,60 +375,6 @@ mx4_prompt_kernel(const Mx4AttnParams p) {
 // Tried in that other form and slower: this tile's output and the next one's scores as one sequence of independent matrix
 // instructions (219 where it took 190), 256 queries in eight waves (195).
 // ---------------------------------------------------------------------------
-constexpr int packed_k_turn(int NJ, int row) { return NJ % 4 == 0 ? row & 15 : NJ % 2 == 0 ? (row >> 1) & 7 : (row >> 2) & 3; }
-constexpr int packed_v_turn(int NJ, int row) { return 2 * (NJ % 4 == 0 ? row & 7 : NJ % 2 == 0 ? (row >> 1) & 3 : (row >> 2) & 1); }
-
-// The transposing reads of V for 32 keys and N pieces of 16 channels, issued and waited for in one block (around the builtin the
-// compiler waits for every load into LDS under way): piece d at a[d % X] + d / X * STEP, keys 16 .. 31 at + ROWS.
-template <int OFF, int ROWS>
-__device__ __forceinline__ void packed_v_operands(i32x2 (&v)[8][2], const uint32_t (&a)[8]) {
-  asm volatile("ds_read_b64_tr_b16 %0, %16 offset:%24\n\tds_read_b64_tr_b16 %1, %16 offset:%25\n\t"
-               "ds_read_b64_tr_b16 %2, %17 offset:%24\n\tds_read_b64_tr_b16 %3, %17 offset:%25\n\t"
-               "ds_read_b64_tr_b16 %4, %18 offset:%24\n\tds_read_b64_tr_b16 %5, %18 offset:%25\n\t"
-               "ds_read_b64_tr_b16 %6, %19 offset:%24\n\tds_read_b64_tr_b16 %7, %19 offset:%25\n\t"
-               "ds_read_b64_tr_b16 %8, %20 offset:%24\n\tds_read_b64_tr_b16 %9, %20 offset:%25\n\t"
-               "ds_read_b64_tr_b16 %10, %21 offset:%24\n\tds_read_b64_tr_b16 %11, %21 offset:%25\n\t"
-               "ds_read_b64_tr_b16 %12, %22 offset:%24\n\tds_read_b64_tr_b16 %13, %22 offset:%25\n\t"
-               "ds_read_b64_tr_b16 %14, %23 offset:%24\n\tds_read_b64_tr_b16 %15, %23 offset:%25\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]),
-                 "=&v"(v[3][1]), "=&v"(v[4][0]), "=&v"(v[4][1]), "=&v"(v[5][0]), "=&v"(v[5][1]), "=&v"(v[6][0]), "=&v"(v[6][1]),
-                 "=&v"(v[7][0]), "=&v"(v[7][1])
-               : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "n"(OFF), "n"(OFF + ROWS)
-               : "memory");
-}
-template <int OFF, int ROWS>
-__device__ __forceinline__ void packed_v_operands(i32x2 (&v)[4][2], const uint32_t (&a)[4]) {
-  asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
-               "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
-               "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
-               "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]),
-                 "=&v"(v[3][1])
-               : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF), "n"(OFF + ROWS)
-               : "memory");
-}
-template <int OFF, int ROWS> // (96 wide: six pieces at two addresses)
-__device__ __forceinline__ void packed_v_operands(i32x2 (&v)[6][2], const uint32_t (&a)[2]) {
-  asm volatile("ds_read_b64_tr_b16 %0, %12 offset:%14\n\tds_read_b64_tr_b16 %1, %12 offset:%15\n\t"
-               "ds_read_b64_tr_b16 %2, %13 offset:%14\n\tds_read_b64_tr_b16 %3, %13 offset:%15\n\t"
-               "ds_read_b64_tr_b16 %4, %12 offset:%16\n\tds_read_b64_tr_b16 %5, %12 offset:%17\n\t"
-               "ds_read_b64_tr_b16 %6, %13 offset:%16\n\tds_read_b64_tr_b16 %7, %13 offset:%17\n\t"
-               "ds_read_b64_tr_b16 %8, %12 offset:%18\n\tds_read_b64_tr_b16 %9, %12 offset:%19\n\t"
-               "ds_read_b64_tr_b16 %10, %13 offset:%18\n\tds_read_b64_tr_b16 %11, %13 offset:%19\n\t"
-               "s_waitcnt lgkmcnt(0)"
-               : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]),
-                 "=&v"(v[3][1]), "=&v"(v[4][0]), "=&v"(v[4][1]), "=&v"(v[5][0]), "=&v"(v[5][1])
-               : "v"(a[0]), "v"(a[1]), "n"(OFF), "n"(OFF + ROWS), "n"(OFF + 64), "n"(OFF + 64 + ROWS), "n"(OFF + 128), "n"(OFF + 128 + ROWS)
-               : "memory");
-}
-
-// 16 bytes per lane straight into LDS, 1024 in a row from `to` on
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t src, uint8_t* to, uint32_t offset) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (__attribute__((address_space(3))) void*)to, 16, offset, 0, 0, 0);
-}
-
 template <int NJ, int W, int KEYS>
 __global__ void __launch_bounds__(W * 64, NJ == 4 && (W == 8 || KEYS == 32) ? 4 : 2)
 mx4_packed_kernel(const Mx4AttnParams p) {

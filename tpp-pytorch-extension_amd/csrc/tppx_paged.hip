@@ -145,87 +145,400 @@ paged_rows_kernel(const PagedRowsParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// Attention: a workgroup for a node's query head, a wave takes 64 keys at a time.
+// Attention.  The columns of a sequence's K/V head are its (node, query head) pairs; a workgroup takes 16 CW of them, the columns of 16 x 16
+// x 32 MFMAs, for a part of the keys.  Both products run transposed, scores^T[key][col] = K Q^T and out^T[channel][col] += V^T P^T: the
+// scores of a lane are those of one column, and rounded to bf16 they are the second operand of the V product as they lie.  TW teams of
+// CW waves take tiles of KEYS keys in turn, from the last one down.  A tile's rows come by loads straight into LDS, one tile ahead,
+// a run of 16 rows at a time: a page holds whole runs, so its number is the same for all lanes.
+// A node sees the slots before the step's and of the step's those of the nodes that it continues: in the tiles that hold such slots a
+// lane follows its column's node up and sets a bit for each of the tile's keys that it meets; as tiles descend, it goes on where the
+// tile above ended.
+// A key that a column does not see adds nothing whatever it holds: its score is replaced, and in those tiles values that are infinite
+// or NaN are added one by one to the columns that see them and become zeros in LDS.
 // ---------------------------------------------------------------------------
 struct PagedAttnParams {
   const uint16_t *q, *layer;
   const int32_t *past, *cu, *parents;
   uint16_t* out; // [T][Nq][H]
+  float* part;   // [unit][split][cols][H], then [unit][split][cols][2]
+  unsigned int* counters;
   Pages g;
   int64_t q_ld;
-  int T, B, Nq, Nkv, H;
+  int T, B, Nq, Nkv, R, splits, chunk; // chunk: tiles of a split
   float scale;
 };
+typedef const __attribute__((address_space(4))) int32_t* ConstantInts; // (scalar loads)
 
-__global__ void __launch_bounds__(256)
+template <int NJ, int CW, int TW, int KEYS>
+__global__ void __launch_bounds__(64 * CW * TW, CW == 8 ? 4 : CW * TW == 4 && CW > 1 ? 2 : 1)
 paged_attn_kernel(const PagedAttnParams p) {
-  __shared__ float q[256], part[4][256], stat[4][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = (int)blockIdx.x, hq = (int)blockIdx.y, hk = hq / (p.Nq / p.Nkv);
-  int b, first, n;
-  if (!sequence_at(p.cu, p.B, p.T, row, b, first, n))
+  constexpr int H = 32 * NJ, ROW = 64 * NJ, PER = 4 * NJ, SIDE = KEYS * ROW, COLS = 16 * CW, TH = 64 * CW * TW, NA = H / 16, NT = KEYS / 16;
+  constexpr int XK = NJ % 4 == 0 ? 4 : NJ % 2 == 0 ? 2 : 1, XV = NJ % 4 == 0 ? 8 : NJ % 2 == 0 ? 4 : 2, NR = NJ == 3 ? 6 : XV;
+  constexpr int RUNS = 2 * NT, MINE = RUNS / CW; // runs of 16 rows of a tile, K then V; of a wave
+  static_assert(RUNS % CW == 0 && (KEYS == 32 || KEYS == 64));
+  extern __shared__ __align__(16) uint8_t lds[]; // V [team][stage], K [team][stage]
+  __shared__ int arrived_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % CW, team = __builtin_amdgcn_readfirstlane(tid >> 6) / CW;
+  const int g = lane >> 4, c = lane & 15;
+  const int hk = (int)blockIdx.x % p.Nkv;
+  Block o;
+  if (!locate(p.cu, p.B, p.T, p.R, COLS, (int)blockIdx.x / p.Nkv, o))
     return;
-  const int node = row - first, past = p.past[b];
-  const int capacity = (int)min(p.g.table_ld << p.g.shift, (int64_t)1 << 30);
-  const int keys = past < 0 ? 0 : (int)min((int64_t)past + node + 1, (int64_t)capacity);
-  const int32_t* const parents = p.parents ? p.parents + first : nullptr;
-  if (tid < p.H)
-    q[tid] = bf16_bits_to_f32(p.q[(int64_t)row * p.q_ld + (int64_t)hq * p.H + tid]) * p.scale;
-  __syncthreads();
-  const int64_t values = (((int64_t)p.g.pages * p.Nkv) << p.g.shift) * p.H;
-  float m = LOWEST, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k0 = wave * 64; k0 < keys; k0 += 256) {
-    const int key = k0 + lane;
-    bool seen = key < keys;
-    if (seen && key >= past && parents) {
-      int j = node;
-      while (j > key - past)
-        j = parent_of(parents, j);
-      seen = j == key - past;
+  const int ncol = min(COLS, o.n * p.R - o.at * COLS); // of this workgroup
+  const int col0 = o.at * COLS;
+  const int capacity = (int)(p.g.table_ld << p.g.shift);
+  const int past = min(p.past[o.b], capacity);
+  const int keys = past < 0 ? 0 : (int)min((int64_t)past + (col0 + ncol - 1) / p.R + 1, (int64_t)capacity); // that some column sees
+  const int tiles = (keys + KEYS - 1) / KEYS;
+  const int S = max((tiles + p.chunk - 1) / p.chunk, 1); // splits that have tiles; the others take no part
+  if ((int)blockIdx.y >= S)
+    return;
+  const bool idle = wave * 16 >= ncol;
+  const int col = col0 + min(wave * 16 + c, ncol - 1), node = col / p.R, r0 = col - node * p.R;
+  const int32_t* const parents = p.parents ? p.parents + o.start : nullptr;
+
+  bf16x8 q[NJ];
+  {
+    const uint16_t* qrow = p.q + (int64_t)(o.start + node) * p.q_ld + (hk * p.R + r0) * H + g * 8;
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+      q[j] = *reinterpret_cast<const bf16x8*>(qrow + j * 32);
+  }
+  // Tiles top, top - TW, .. of this team, down to the split's last one.
+  const int low = (S - 1 - (int)blockIdx.y) * tiles / S, top = (S - (int)blockIdx.y) * tiles / S - 1 - team, most = (top + team - low) / TW + 1;
+  const ConstantInts table = (ConstantInts)(uintptr_t)(p.g.table + (int64_t)o.b * p.g.table_ld);
+  const int64_t values = (((int64_t)p.g.pages * p.Nkv) << p.g.shift) * H;
+  int ids[MINE]; // pages of this wave's runs of the tile that is asked for next
+  auto look_up = [&](int t) {
+    if (t >= low) {
+#pragma unroll
+      for (int i = 0; i < MINE; i++) {
+        const int run = (i * CW + wave) % NT;
+        ids[i] = table[min(t * KEYS + run * 16, keys - 1) >> p.g.shift];
+      }
     }
-    const int id = seen ? page_of(p.g, b, key) : -1;
-    const int64_t at = id >= 0 ? slot_at(p.g, id, p.Nkv, hk, key, p.H) : -1;
-    float s = -INFINITY;
-    if (at >= 0) {
-      s = 0.f;
-      for (int d = 0; d < p.H; d++)
-        s = fmaf(q[d], bf16_bits_to_f32(p.layer[at + d]), s);
+  };
+  uint32_t from[2][NJ]; // offset of this lane's chunk in a run's rows: K, V
+#pragma unroll
+  for (int s = 0; s < 2; s++)
+#pragma unroll
+    for (int i = 0; i < NJ; i++) {
+      const int item = i * 64 + lane, row = item / PER, ch = item % PER;
+      from[s][i] = (uint32_t)(row * ROW + (ch ^ (s ? packed_v_turn(NJ, row) : packed_k_turn(NJ, row))) * 16);
     }
-    float mx = fmaxf(m, s);
-    for (int d = 1; d < 64; d *= 2)
-      mx = fmaxf(mx, __shfl_xor(mx, d));
-    const float alpha = expf(m - mx), e = at >= 0 ? expf(s - mx) : 0.f;
-    m = mx;
-    l = l * alpha + e;
-    for (int i = 0; i < 4; i++)
-      acc[i] *= alpha;
-    for (int j = 0; j < 64; j++) {
-      const int64_t from = __shfl(at, j);
-      const float pj = __shfl(e, j);
-      if (from >= 0)
-        for (int i = 0; i * 64 + lane < p.H; i++)
-          acc[i] = fmaf(pj, bf16_bits_to_f32(p.layer[values + from + i * 64 + lane]), acc[i]);
+  auto request = [&](int t, int stage) {
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+      const int run = (i * CW + wave) % NT, side = (i * CW + wave) / NT;
+      const int key = min(t * KEYS + run * 16, keys - 1), rows = min(keys - key, 16);
+      // (a page that does not exist: the first one)
+      const int id = (unsigned)ids[i] < (unsigned)p.g.pages ? ids[i] : 0;
+      const uint16_t* const at = p.layer + (side ? values : 0) + slot_at(p.g, id, p.Nkv, hk, key, H);
+      const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(at), 0, rows * ROW, 0x00020000);
+      uint8_t* const dst = lds + (((side ? 0 : TW) + team) * 2 + stage) * SIDE + run * (NJ * 1024);
+#pragma unroll
+      for (int j = 0; j < NJ; j++) { // (rows past the keys repeat the last one)
+        uint32_t off = side ? from[1][j] : from[0][j];
+        if (rows < 16) {
+          const int item = j * 64 + lane, row = item / PER;
+          off -= (uint32_t)(max(row - (rows - 1), 0) * ROW);
+        }
+        load_to_lds(src, dst + j * 1024, off);
+      }
+    }
+  };
+  uint32_t kaddr[XK], vaddr[XV];
+#pragma unroll
+  for (int j = 0; j < XK; j++)
+    kaddr[j] = (uint32_t)((TW + team) * 2 * SIDE + c * ROW + ((j * 4 + g) ^ packed_k_turn(NJ, c)) * 16);
+  {
+    const int r = g * 4 + (c >> 2);
+#pragma unroll
+    for (int d = 0; d < XV; d++)
+      vaddr[d] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)lds +
+                 (uint32_t)(team * 2 * SIDE + r * ROW + ((d * 2 + ((c >> 1) & 1)) ^ packed_v_turn(NJ, r)) * 16 + (c & 1) * 8);
+  }
+
+  float m = LOWEST, l = 0.f;
+  f32x4 acc[NA];
+#pragma unroll
+  for (int dt = 0; dt < NA; dt++)
+    acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float unit = p.scale * LOG2E;
+  int up = node; // where this column's way up has come to
+  auto tile = [&](auto S_, int t, int highest) { // highest: the tile of the first team, at the same time
+    constexpr int stage = decltype(S_)::value;
+    const int kb = t * KEYS;
+    // this tile has landed and the other stage has been read, for this wave and then for every wave that shares them
+    if constexpr (CW == 1)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    const bool mine = t >= low; // (uniform in a team)
+    bool odd = false;
+    if ((CW == 1 ? kb : highest * KEYS) + KEYS > past) { // some column may not see some key
+      if (mine) {
+#pragma unroll
+        for (int i = 0; i < (KEYS * PER + 64 * CW - 1) / (64 * CW); i++) {
+          const int at = i * 64 * CW + wave * 64 + lane;
+          if (KEYS * PER % (64 * CW) != 0 && at >= KEYS * PER)
+            continue;
+          const i32x4 w = *(reinterpret_cast<const i32x4*>(lds + (team * 2 + stage) * SIDE) + at);
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            odd |= mx4_non_finite((uint32_t)w[j]);
+        }
+      }
+      odd = CW == 1 ? __builtin_amdgcn_ballot_w64(odd) != 0 : __syncthreads_or(odd);
+    }
+    if (t - TW >= low) {
+      request(t - TW, stage ^ 1); // in flight during the arithmetic below
+      look_up(t - 2 * TW);
+    }
+    bf16x8 pb[NT / 2];
+    uint64_t seen = ~0ull;
+    const bool busy = mine && !idle;
+    if (busy) {
+      const uint8_t* const st = lds + stage * SIDE;
+      f32x4 sc[NT];
+#pragma unroll
+      for (int u = 0; u < NT; u++) {
+        sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+          sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(st + kaddr[j % XK] + u * (16 * ROW) + j / XK * (XK * 64)), q[j], sc[u], 0, 0, 0);
+      }
+      if (kb + KEYS > past) { // (uniform in a team)
+        const int lo = kb - past; // the node whose slot is the tile's first key
+        seen = lo < 0 ? (1ull << -lo) - 1 : 0ull; // (above -KEYS)
+        if (!parents) {
+          const int last = node - lo; // (the capacity ends the keys: what lies behind is not asked about)
+          seen = last >= 63 ? ~0ull : last < 0 ? 0ull : (2ull << last) - 1;
+        } else {
+          while (up >= max(lo + KEYS, 0))
+            up = parent_of(parents, up);
+          while (up >= max(lo, 0)) {
+            seen |= 1ull << (up - lo);
+            up = parent_of(parents, up);
+          }
+        }
+        const int behind = keys - kb;
+        if (behind < 64)
+          seen &= (1ull << behind) - 1;
+        const uint64_t bits = seen >> (g * 4);
+#pragma unroll
+        for (int i = 0; i < 4 * NT; i++)
+          sc[i >> 2][i & 3] = bits >> ((i >> 2) * 16 + (i & 3)) & 1 ? sc[i >> 2][i & 3] : -INFINITY;
+      }
+      float mx = m;
+#pragma unroll
+      for (int i = 0; i < 4 * NT; i++)
+        mx = fmaxf(mx, sc[i >> 2][i & 3]);
+      if (__builtin_amdgcn_ballot_w64((mx - m) * unit > 8.f) != 0) {
+        mx = max_of_groups(mx);
+        const float alpha = __builtin_amdgcn_exp2f((m - mx) * unit);
+#pragma unroll
+        for (int dt = 0; dt < NA; dt++)
+          acc[dt] *= alpha;
+        l *= alpha;
+        m = mx;
+      }
+      const float off = -m * unit;
+#pragma unroll
+      for (int i = 0; i < 4 * NT; i += 2) {
+        const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(sc[i >> 2][(i & 3) + 1], unit, off))};
+        l = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l, false);
+        pb[i >> 3][i & 7] = pr[0];
+        pb[i >> 3][(i & 7) + 1] = pr[1];
+      }
+    }
+    if (__builtin_expect(odd, 0)) { // values that are not finite: to the columns that see them, then zeros
+      uint8_t* const vt = lds + (team * 2 + stage) * SIDE;
+      if (busy) {
+#pragma unroll 1
+        for (int key = 0; key < KEYS; key++)
+          if (seen >> key & 1)
+#pragma unroll
+            for (int dt = 0; dt < NA; dt++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const int ch = dt * 16 + g * 4 + e;
+                const uint32_t w = *reinterpret_cast<const uint16_t*>(vt + key * ROW + ((ch >> 3) ^ packed_v_turn(NJ, key)) * 16 + (ch & 7) * 2);
+                if ((w & 0x7f80u) == 0x7f80u)
+                  acc[dt][e] += bf16_bits_to_f32(w);
+              }
+      }
+      if constexpr (CW > 1)
+        __syncthreads();
+      if (mine) {
+        for (int at = wave * 64 + lane; at < KEYS * PER; at += 64 * CW) {
+          i32x4* const it = reinterpret_cast<i32x4*>(vt) + at;
+          const i32x4 w = *it;
+          *it = i32x4{(int)mx4_finite((uint32_t)w[0]), (int)mx4_finite((uint32_t)w[1]), (int)mx4_finite((uint32_t)w[2]), (int)mx4_finite((uint32_t)w[3])};
+        }
+      }
+      if constexpr (CW > 1)
+        __syncthreads();
+      else
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    }
+    if (busy) {
+      static_for<0, KEYS / 32 * (NA / NR)>([&](auto I) { // 32 keys, NR pieces of channels
+        constexpr int u = decltype(I)::value / (NA / NR), d0 = decltype(I)::value % (NA / NR) * NR;
+        i32x2 vv[NR][2];
+        packed_v_operands<stage * SIDE + u * 32 * ROW + d0 * 32, 16 * ROW>(vv, vaddr);
+#pragma unroll
+        for (int d = 0; d < NR; d++) {
+          const i32x4 w = {vv[d][0][0], vv[d][0][1], vv[d][1][0], vv[d][1][1]};
+          acc[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[d0 + d], 0, 0, 0);
+        }
+      });
+    }
+  };
+  if (top >= low) {
+    look_up(top);
+    request(top, 0);
+    look_up(top - TW);
+  }
+  for (int k = 0; k < most; k += 2) {
+    tile(std::integral_constant<int, 0>{}, top - k * TW, top + team - k * TW);
+    if (k + 1 < most)
+      tile(std::integral_constant<int, 1>{}, top - (k + 1) * TW, top + team - (k + 1) * TW);
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  m = m == LOWEST ? LOWEST : m * unit; // in powers of two
+
+  float* const part_ml = p.part + (int64_t)gridDim.x * p.splits * COLS * H;
+  auto store4 = [&](int cc, int ch, f32x4 v, float sum) { // (nothing seen: zeros)
+    const int cl = col0 + cc, nd = cl / p.R, rr = cl - nd * p.R;
+    const float inv = sum != 0.f ? 1.0f / sum : 0.f;
+    *reinterpret_cast<uint2*>(p.out + ((int64_t)(o.start + nd) * p.Nq + hk * p.R + rr) * H + ch) =
+        make_uint2(f32x2_to_bf16_bits(v[0] * inv, v[1] * inv), f32x2_to_bf16_bits(v[2] * inv, v[3] * inv));
+  };
+  // a split's result for the merge: device-scope stores, written through to the level that all XCDs share
+  const int64_t part_at = ((int64_t)blockIdx.x * p.splits + blockIdx.y) * COLS;
+  auto leave4 = [&](int cc, int ch, f32x4 v) {
+    uint64_t* const dst = reinterpret_cast<uint64_t*>(p.part + (part_at + cc) * H + ch);
+    __hip_atomic_store(dst, __builtin_bit_cast(uint64_t, make_float2(v[0], v[1])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(dst + 1, __builtin_bit_cast(uint64_t, make_float2(v[2], v[3])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  auto leave_state = [&](int cc, float mm, float ll) {
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(part_ml + (part_at + cc) * 2), __builtin_bit_cast(uint64_t, make_float2(mm, ll)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  if constexpr (TW == 1) {
+    const int cc = wave * 16 + c;
+    if (cc < ncol) {
+#pragma unroll
+      for (int dt = 0; dt < NA; dt++) {
+        if (S == 1)
+          store4(cc, dt * 16 + g * 4, acc[dt], l);
+        else
+          leave4(cc, dt * 16 + g * 4, acc[dt]);
+      }
+      if (S > 1 && g == 0)
+        leave_state(cc, m, l);
+    }
+  } else { // the teams' states through LDS
+    constexpr int OP = H + 4;
+    float* const mo = reinterpret_cast<float*>(lds); // [team][col][OP]
+    float* const sm = mo + TW * COLS * OP;           // [team][col] maximum, then sum
+    __syncthreads();
+    const int cc = wave * 16 + c;
+#pragma unroll
+    for (int dt = 0; dt < NA; dt++)
+      if (cc < ncol)
+        *reinterpret_cast<f32x4*>(mo + (team * COLS + cc) * OP + dt * 16 + g * 4) = acc[dt];
+    if (g == 0) {
+      sm[team * COLS + cc] = m;
+      sm[TW * COLS + team * COLS + cc] = l;
+    }
+    __syncthreads();
+    for (int i = tid; i < ncol * (H / 4); i += TH) {
+      const int cl = i / (H / 4), d4 = i % (H / 4);
+      float M = sm[cl];
+#pragma unroll
+      for (int w = 1; w < TW; w++)
+        M = fmaxf(M, sm[w * COLS + cl]);
+      float Ls = 0.f;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < TW; w++) {
+        const float wt = __builtin_amdgcn_exp2f(sm[w * COLS + cl] - M);
+        Ls = fmaf(wt, sm[TW * COLS + w * COLS + cl], Ls);
+        const f32x4 ow = *reinterpret_cast<const f32x4*>(mo + (w * COLS + cl) * OP + d4 * 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          v[e] = fmaf(wt, ow[e], v[e]);
+      }
+      if (S == 1) {
+        store4(cl, d4 * 4, v, Ls);
+      } else {
+        leave4(cl, d4 * 4, v);
+        if (d4 == 0)
+          leave_state(cl, M, Ls);
+      }
     }
   }
-  for (int d = 1; d < 64; d *= 2)
-    l += __shfl_xor(l, d);
-  for (int i = 0; i < 4; i++)
-    part[wave][i * 64 + lane] = acc[i];
-  if (lane == 0) {
-    stat[wave][0] = m;
-    stat[wave][1] = l;
+  if (S == 1)
+    return;
+  // The split that arrives last merges all of them, in split order (the same sums whichever that is).  Every thread waits until
+  // its own stores are acknowledged, then the barrier, the arrival, and the device-scope loads; nobody waits for another workgroup.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0)
+    arrived_last = atomicInc(p.counters + (int64_t)blockIdx.x * MX4_COUNTER_STRIDE, (unsigned)S - 1) == (unsigned)S - 1;
+  __syncthreads();
+  if (!arrived_last)
+    return;
+  auto load2 = [](const float* src) {
+    return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(src), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  };
+  float* const merged = reinterpret_cast<float*>(lds); // [col][33]: weights of the splits, then the sum
+  const int64_t unit_at = (int64_t)blockIdx.x * p.splits * COLS;
+  for (int i = tid; i < ncol * 32; i += TH) { // 32 lanes per column, one split each
+    const int cc = i >> 5, s = i & 31;
+    float2 ml = {LOWEST, 0.f};
+    if (s < S)
+      ml = load2(part_ml + (unit_at + s * COLS + cc) * 2);
+    float M = ml.x;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2)
+      M = fmaxf(M, __shfl_xor(M, d));
+    const float wt = __builtin_amdgcn_exp2f(ml.x - M);
+    float Ls = wt * ml.y;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2)
+      Ls += __shfl_xor(Ls, d);
+    merged[cc * 33 + s] = wt;
+    if (s == 0)
+      merged[cc * 33 + 32] = Ls;
   }
   __syncthreads();
-  if (tid < p.H) {
-    float mx = LOWEST, sum = 0.f, v = 0.f;
-    for (int w = 0; w < 4; w++)
-      mx = fmaxf(mx, stat[w][0]);
-    for (int w = 0; w < 4; w++) {
-      const float a = expf(stat[w][0] - mx);
-      sum = fmaf(a, stat[w][1], sum);
-      v = fmaf(a, part[w][tid], v);
+  for (int i = tid; i < ncol * (H / 4); i += TH) {
+    const int cc = i / (H / 4), d4 = i % (H / 4);
+    const float* src = p.part + (unit_at + cc) * H + d4 * 4;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < S; s0 += 8) { // eight splits' loads in flight
+      float2 a[8][2];
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const float* at = src + (int64_t)min(s0 + u, S - 1) * COLS * H;
+        a[u][0] = load2(at);
+        a[u][1] = load2(at + 2);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        if (s0 + u < S) {
+          const float wt = merged[cc * 33 + s0 + u];
+          v[0] = fmaf(wt, a[u][0].x, v[0]);
+          v[1] = fmaf(wt, a[u][0].y, v[1]);
+          v[2] = fmaf(wt, a[u][1].x, v[2]);
+          v[3] = fmaf(wt, a[u][1].y, v[3]);
+        }
     }
-    p.out[((int64_t)row * p.Nq + hq) * p.H + tid] = (uint16_t)f32_to_bf16_bits(sum != 0.f ? v / sum : 0.f);
+    store4(cc, d4 * 4, v, merged[cc * 33 + 32]);
   }
 }
 
@@ -282,6 +595,69 @@ static int paged_checks(const char* who, const void* table, const void* past, co
   g.pages = (int)pages;
   g.shift = __builtin_ctzll((unsigned long long)page);
   return TPPX_OK;
+}
+
+static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_bytes, int64_t counter_bytes, hipStream_t stream) {
+  hipError_t e = hipSuccess;
+  int rc = TPPX_OK;
+  auto go = [&](auto nj, auto cw, auto tw, auto kt) {
+    constexpr int NJ = decltype(nj)::value, CW = decltype(cw)::value, TW = decltype(tw)::value, KEYS = decltype(kt)::value, COLS = 16 * CW;
+    const int64_t blocks = p.cu ? ((int64_t)p.T * p.R + (int64_t)p.B * (COLS - 1)) / COLS : (int64_t)p.B * ((p.R + COLS - 1) / COLS);
+    const int64_t units = blocks * p.Nkv;
+    if (units >= ((int64_t)1 << 31)) {
+      rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
+      return;
+    }
+    const int64_t tiles = ((p.g.table_ld << p.g.shift) + KEYS - 1) / KEYS;
+    int64_t chunk = env_int("TPPX_PAGED_CHUNK", 0) / KEYS;
+    if (chunk <= 0)
+      chunk = std::max<int64_t>(tiles * units / 1024, 256 / KEYS);
+    chunk = std::max<int64_t>(chunk, (tiles + 31) / 32);
+    int64_t S = (tiles + chunk - 1) / chunk;
+    if (units * S * COLS * (32 * NJ + 2) * (int64_t)sizeof(float) > ws_bytes || units * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) > counter_bytes) {
+      S = 1;
+      chunk = tiles;
+    }
+    p.splits = (int)S;
+    p.chunk = (int)chunk;
+    const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ, teams = TW > 1 ? TW * COLS * (32 * NJ + 6) * sizeof(float) : 0;
+    const size_t lds = std::max(stages, teams);
+    auto kern = paged_attn_kernel<NJ, CW, TW, KEYS>;
+    e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
+    if (e == hipSuccess)
+      kern<<<dim3((unsigned)units, (unsigned)S), dim3(64 * CW * TW), lds, stream>>>(p);
+  };
+  const int64_t cols = (p.cu ? (p.T + p.B - 1) / p.B : 1) * (int64_t)p.R; // of a sequence's K/V head, on average
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, 4> four{};
+  constexpr std::integral_constant<int, 8> eight{};
+  constexpr std::integral_constant<int, 32> k32{};
+  constexpr std::integral_constant<int, 64> k64{};
+  const int form = env_int("TPPX_PAGED_FORM", 0);
+  mx4_for_head(H, [&](auto nj) {
+    constexpr int NJ = decltype(nj)::value;
+    const int f = form ? form : cols <= 16 ? 1 : cols <= 64 ? 2 : 3;
+    if (f == 1) {
+      if constexpr (NJ > 4)
+        go(nj, one, two, k32);
+      else
+        go(nj, one, four, k32);
+    } else if (f == 2) {
+      if constexpr (NJ > 4)
+        go(nj, four, one, k32);
+      else
+        go(nj, four, one, k64);
+    } else {
+      if constexpr (NJ > 4)
+        go(nj, four, one, k32);
+      else
+        go(nj, eight, one, k64);
+    }
+  });
+  if (rc)
+    return rc;
+  return check_hip(e != hipSuccess ? e : hipGetLastError(), who);
 }
 
 } // namespace tppx
@@ -349,10 +725,11 @@ extern "C" int tppx_attn_paged(const void* q, const void* layer, const void* tab
     return TPPX_OK;
   p.q = (const uint16_t*)q; p.q_ld = q_ld; p.layer = (const uint16_t*)layer; p.out = (uint16_t*)out;
   p.past = (const int32_t*)past; p.cu = (const int32_t*)cu; p.parents = (const int32_t*)parents;
-  p.T = (int)T; p.B = (int)B; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.H = (int)H;
+  p.T = (int)T; p.B = (int)B; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.R = (int)(Nq / Nkv);
   p.scale = 1.0f / sqrtf((float)H);
-  paged_attn_kernel<<<dim3((unsigned)T, (unsigned)Nq), dim3(256), 0, (hipStream_t)stream>>>(p);
-  return check_hip(hipGetLastError(), who);
+  p.part = (float*)ws;
+  p.counters = (unsigned int*)counters;
+  return attn_launch(who, p, (int)H, ws_bytes, counter_bytes, (hipStream_t)stream);
 }
 
 extern "C" int tppx_keep_paged(void* cache, const void* table, const void* past, const void* path, const void* count, const void* cu,
