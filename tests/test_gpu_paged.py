@@ -324,6 +324,14 @@ def test_verify_long_chain_and_wide_tree():
     parents = [[-1] + [0] * 199]
     tokens = [0] + [int(x) for x in torch.randperm(500, generator=torch.Generator().manual_seed(1))[:199]]
     _check_verify([200], 500, torch.float32, 4, trees=True, given=(tokens, parents, target, None, u * 0 + 0.999, s))
+    # more children than the kernel keeps in LDS, none of which stands; then a tree of as many nodes
+    g = torch.Generator().manual_seed(8)
+    target = torch.randn((400, 3000), generator=g)
+    tokens = [0] + [int(x) for x in torch.randperm(3000, generator=g)[:399]]
+    for s in (0.0, 0.4, 0.9999):
+        _check_verify([400], 3000, torch.float32, 4, trees=True,
+                      given=(tokens, [[-1] + [0] * 399], target, None, torch.full((400,), 0.999), torch.tensor([s])))
+    _check_verify([400, 3, 270], 900, torch.bfloat16, 9, trees=True)
 
 
 def test_verify_of_infinities_and_nan():
