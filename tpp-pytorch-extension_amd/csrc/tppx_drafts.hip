@@ -22,6 +22,21 @@ namespace tppx {
 // to that maximum.  The second decides for all nodes at once what u M and u q are compared with, walks from node 0 down, and finds the
 // next token: the piece in which the border lies by the pieces' sums less the tried siblings' shares, then the token in it.  With draft
 // logits max(p - q, 0) of the last row is a pass of its own over pieces, the second launch, and the third one finds the token.
+struct Piece {
+  double sum;
+  float top;
+  int first;
+};
+typedef Piece RowSum;
+struct NodeShare { // of a node's token in its parent's row
+  double px, qx;
+  int up, token;
+  float u;
+};
+struct Walk {
+  RowSum p, q; // of the last node's row
+  int at, len, tried, pad;
+};
 struct DraftsParams {
   const int64_t* tokens;
   const void *target, *draft;
@@ -29,17 +44,14 @@ struct DraftsParams {
   const float *uniforms, *sample, *temps;
   int32_t *path, *count;
   int64_t* next;
-  struct Piece* pieces; // [sides][T][C]
-  double* sums;         // [B][C] of what is left of a sequence's last row
-  double *px, *qx;      // [T]
+  Piece* pieces;    // [sides][T][C]
+  double* sums;     // [B][C] of what is left of a sequence's last row
+  Walk* walks;      // [B]
+  RowSum* rows;     // [2][T], of sequences too long for LDS
+  NodeShare* nodes; // [T], of those
   int64_t t_ld, d_ld;
   int T, B, V, C, sides;
   float temperature;
-};
-struct Piece {
-  double sum;
-  float top;
-  int first;
 };
 constexpr double LOG2E_64 = 1.4426950408889634;
 
@@ -65,6 +77,23 @@ __device__ __forceinline__ double weight_of(float x, float top, double to2) {
   const double w = to2 == 0.0 ? 0.0 : exp2_64(((double)x - (double)top) * to2);
   return x == top ? 1.0 : w;
 }
+// The same for many: 2^(n / 256) from a table and 2^(f / 256), f in [-1/2, 1/2], by an interpolation of degree 3, 4e-14 relative: ten
+// instructions in 64 bits where the polynomial takes nineteen.  `lowest` stands for what lies below it (its weight is 2^-900).
+struct ManyWeights {
+  const double* table;
+  double top, k;
+  float lowest;
+  __device__ __forceinline__ ManyWeights(const double* t, float m, double to2) : table(t), top(m), k(to2 * 256.0), lowest(m - (float)(900.0 / to2)) {}
+  static __device__ __forceinline__ bool fits(float top, double to2) { return fabsf(top) < 1e5f && to2 < 64.0; }
+  __device__ __forceinline__ double operator()(float x) const {
+    constexpr double MAGIC = 0x1.8p52; // (a sum with it is rounded to a whole number, which its low bits are)
+    const double d = (double)fmaxf(x, lowest) - top, t = fma(d, k, MAGIC), f = fma(d, k, MAGIC - t);
+    const int n = __double2loint(t);
+    const double a = table[n & 255], s = __hiloint2double(__double2hiint(a) + ((n & ~255) << 12), __double2loint(a));
+    const double g = f * fma(f, fma(f, 3.3083029079191157e-09, 3.665566016796724e-06), 0.0027076061740622863);
+    return fma(s, g, s);
+  }
+};
 template <typename E>
 __device__ __forceinline__ float logit_of(E v) { // (what is no number is no token)
   float x;
@@ -135,6 +164,11 @@ draft_rows_kernel(const DraftsParams p) {
 #pragma unroll
   for (int i = 0; i < NV; i++)
     load_logits<E>(at, from + (i * DRAFT_THREADS + tid) * N, p.V, x[i]);
+  __shared__ double table[256];
+  if (NV > 1 && to2 != 0.0) {
+    table[tid] = exp2_64((double)tid * (1.0 / 256.0));
+    __syncthreads();
+  }
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NV; i++)
@@ -157,6 +191,14 @@ draft_rows_kernel(const DraftsParams p) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2)
       first = min(first, __shfl_xor(first, d));
+  } else if (NV > 1 && from + DRAFT_THREADS * NV * N <= p.V && ManyWeights::fits(top, to2)) { // (uniform in a wave)
+    const ManyWeights many(table, top, to2);
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int e = 0; e < N; e++)
+        sum += many(x[i][e]);
+    sum = reduce_lanes<64>(sum, [](double a, double z) { return a + z; });
   } else {
 #pragma unroll
     for (int i = 0; i < NV; i++)
@@ -186,32 +228,45 @@ draft_rows_kernel(const DraftsParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// The walk and the next token.  LAST: finds the token; otherwise sums what is left of the last row's piece blockIdx.y.
+// The walk and the next token, a workgroup of 1024 for a sequence: the state of its rows from their pieces, every node's token's p (and q)
+// in its parent's row, then down.  WALK, TOKEN: both without draft logits; with them the walk is done by every workgroup that sums
+// what is left of a piece (blockIdx.y) of the last row, the first of which leaves it to the launch that finds the token.
 // ---------------------------------------------------------------------------
 constexpr int DRAFT_NODES = 256; // nodes of a sequence that are held in LDS; more go through the workspace
-struct RowSum {
-  double sum;
-  float top;
-  int first;
-};
+constexpr int WALK_THREADS = 1024;
 
-template <typename E, int NV, bool LAST>
-__global__ void __launch_bounds__(DRAFT_THREADS)
+__device__ __forceinline__ double add64(double a, double z) { return a + z; }
+// sum over the lanes below, and this one's
+__device__ __forceinline__ double scan64(double v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const double t = __shfl_up(v, d);
+    v += lane >= d ? t : 0.0;
+  }
+  return v;
+}
+
+template <typename E, int NV, bool WALK, bool TOKEN>
+__global__ void __launch_bounds__(WALK_THREADS)
 draft_walk_kernel(const DraftsParams p) {
-  constexpr int N = per16<E>(), PIECE = DRAFT_THREADS * NV * N;
-  __shared__ double px_lds[DRAFT_NODES], qx_lds[DRAFT_NODES];
+  constexpr int N = per16<E>(), PIECE = DRAFT_THREADS * NV * N, WAVES = WALK_THREADS / 64;
+  constexpr int VECTORS = DRAFT_THREADS * NV; // of a piece; a thread takes at most one
+  static_assert(VECTORS <= WALK_THREADS);
+  __shared__ RowSum rows_lds[2][DRAFT_NODES];
+  __shared__ NodeShare nodes_lds[DRAFT_NODES];
   __shared__ double tried_px[DRAFT_NODES]; // the last node's children: shares, pieces that their tokens lie in
   __shared__ int tried_in[DRAFT_NODES];
   __shared__ uint32_t gone[PIECE / 32]; // tokens of a piece that were tried
-  __shared__ double red[DRAFT_THREADS];
-  __shared__ int found_at[4];
-  __shared__ int walk_at, walk_len, walk_tried, piece_at;
+  __shared__ double red[WAVES];
+  __shared__ int found_at[WAVES], last_at[WAVES];
+  __shared__ Walk walk;
+  __shared__ int piece_at;
   __shared__ double piece_before, piece_border;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = (int)blockIdx.x;
   const int first = p.cu ? min(max(p.cu[b], 0), p.T) : b, n = p.cu ? min(p.cu[b + 1], p.T) - first : 1;
   if (n < 1) {
-    if (LAST && tid == 0) {
+    if (TOKEN && tid == 0) {
       p.count[b] = 0;
       p.next[b] = 0;
     }
@@ -222,147 +277,183 @@ draft_walk_kernel(const DraftsParams p) {
   const int32_t* const parents = p.parents ? p.parents + first : nullptr;
   const int64_t* const tokens = p.tokens + first;
   auto parent = [&](int i) { return parents ? parents[i] : i - 1; };
-  // a row's state from its pieces: G lanes take them in turn
-  auto row_sum = [&](int side, int row, int u, auto G_) {
-    constexpr int G = decltype(G_)::value;
-    const Piece* const at = p.pieces + ((int64_t)side * p.T + row) * p.C;
-    RowSum r = {0.0, -INFINITY, p.V};
-    for (int i = u; i < p.C; i += G) {
-      const Piece z = at[i];
-      if (z.top > r.top) {
-        r.sum = r.sum > 0.0 ? r.sum * weight_of(r.top, z.top, to2) : 0.0;
-        r.top = z.top;
-        r.first = z.first;
-      } else if (z.top == r.top) {
-        r.first = min(r.first, z.first);
-      }
-      if (z.sum > 0.0) // (a piece of nothing but -inf counts where the row is nothing else)
-        r.sum += z.sum * weight_of(z.top, r.top, to2);
-    }
-#pragma unroll
-    for (int d = 1; d < G; d *= 2) {
-      const float top = __shfl_xor(r.top, d);
-      const int place = __shfl_xor(r.first, d);
-      const double sum = __shfl_xor(r.sum, d);
-      const float both = fmaxf(r.top, top);
-      r.first = top > r.top ? place : top == r.top ? min(r.first, place) : r.first;
-      // (the same order in both lanes: their sums must not differ)
-      const double a = r.sum * weight_of(r.top, both, to2), z = sum * weight_of(top, both, to2);
-      r.sum = a + z;
-      r.top = both;
-    }
-    return r;
-  };
-  auto share = [&](int side, int row, const RowSum& r, int64_t x) {
-    if (x < 0 || x >= p.V)
-      return 0.0;
-    if (to2 == 0.0)
-      return x == r.first ? 1.0 : 0.0;
-    const E* const at = (const E*)(side ? p.draft : p.target) + (int64_t)row * (side ? p.d_ld : p.t_ld);
-    return weight_of(logit_of(at[x]), r.top, to2) / r.sum;
-  };
-  // p (and q) of every node's token in its parent's row: 16 lanes a node
-  double* const px = n <= DRAFT_NODES ? px_lds : p.px + first;
-  double* const qx = n <= DRAFT_NODES ? qx_lds : p.qx + first;
-  for (int i0 = 0; i0 < n; i0 += DRAFT_THREADS / 16) {
-    const int i = i0 + tid / 16, u = tid % 16;
-    const int up = i < n ? parent(i) : -1;
-    if (up >= 0 && up < i) {
-      const double a = share(0, first + up, row_sum(0, first + up, u, std::integral_constant<int, 16>{}), tokens[i]);
-      const double z = drawn ? share(1, first + up, row_sum(1, first + up, u, std::integral_constant<int, 16>{}), tokens[i]) : 0.0;
-      if (u == 0) {
-        px[i] = a;
+  auto logits = [&](int side, int row) { return (const E*)(side ? p.draft : p.target) + (int64_t)row * (side ? p.d_ld : p.t_ld); };
+
+  if constexpr (WALK) {
+    const bool small = n <= DRAFT_NODES;
+    NodeShare* const nodes = small ? nodes_lds : p.nodes + first;
+    RowSum* const prows = small ? rows_lds[0] : p.rows + first;
+    RowSum* const qrows = small ? rows_lds[1] : p.rows + p.T + first;
+    // a node's token and its logits in its parent's row: asked for while the rows are summed up
+    auto own = [&](int i, NodeShare& z, float& x, float& y) {
+      z.up = parent(i);
+      z.up = z.up < i ? max(z.up, -1) : -1;
+      const int64_t t = tokens[i];
+      z.token = t >= 0 && t < p.V ? (int)t : -1;
+      z.u = p.uniforms && to2 != 0.0 ? p.uniforms[first + i] : 0.f;
+      x = y = 0.f;
+      if (z.up >= 0 && z.token >= 0) {
+        x = logit_of(logits(0, first + z.up)[z.token]);
         if (drawn)
-          qx[i] = z;
+          y = logit_of(logits(1, first + z.up)[z.token]);
       }
+    };
+    NodeShare z0;
+    float x0, y0;
+    if (tid < n)
+      own(tid, z0, x0, y0);
+    // 16 lanes a row: its pieces in turn
+    for (int i = tid / 16; i < (drawn ? 2 : 1) * n; i += WALK_THREADS / 16) {
+      const int side = i >= n, r = i - side * n, u = tid % 16;
+      const Piece* const at = p.pieces + ((int64_t)side * p.T + first + r) * p.C;
+      float top = -INFINITY;
+      int place = p.V;
+      for (int c = u; c < p.C; c += 16) {
+        const float t = at[c].top;
+        const int f = at[c].first;
+        place = t > top ? f : t == top ? min(place, f) : place;
+        top = fmaxf(top, t);
+      }
+#pragma unroll
+      for (int d = 1; d < 16; d *= 2) {
+        const float t = __shfl_xor(top, d);
+        const int f = __shfl_xor(place, d);
+        place = t > top ? f : t == top ? min(place, f) : place;
+        top = fmaxf(top, t);
+      }
+      double sum = 0.0;
+      if (to2 != 0.0)
+        for (int c = u; c < p.C; c += 16) {
+          const Piece z = at[c];
+          sum += z.sum > 0.0 ? z.sum * weight_of(z.top, top, to2) : 0.0;
+        }
+      sum = reduce_lanes<16>(sum, add64);
+      if (u == 0)
+        (side ? qrows : prows)[r] = RowSum{sum, top, place};
     }
-  }
-  __syncthreads();
-  if (wave == 0) { // down, all lanes alike
-    int at = 0, len = 0, tried;
-    for (;;) {
-      if (LAST && lane == 0)
-        p.path[first + len] = at;
-      len++;
-      int down = -1;
-      double left = 1.0;
-      tried = 0;
-      for (int c0 = at + 1; c0 < n && down < 0; c0 += 64) {
-        if (!parents && c0 > at + 1)
-          break; // (a chain: one child)
-        const int mine = c0 + lane;
-        uint64_t children = __builtin_amdgcn_ballot_w64(mine < n && parent(mine) == at);
-        while (children && down < 0) {
-          const int c = c0 + __builtin_ctzll(children);
-          children &= children - 1;
-          const double u = to2 == 0.0 ? 0.0 : (double)p.uniforms[first + c];
-          double x = px[c];
-          if (drawn) {
-            if (u * qx[c] < x)
-              down = c;
-          } else {
-            bool again = false; // (nothing is left of a token that was tried)
-            for (int e0 = at + 1; e0 < c; e0 += 64)
-              again |= __builtin_amdgcn_ballot_w64(e0 + lane < c && parent(e0 + lane) == at && tokens[e0 + lane] == tokens[c]) != 0;
-            x = again ? 0.0 : x;
-            if (u * left < x)
-              down = c;
-            left -= x;
-            if (tried < DRAFT_NODES && lane == 0) {
-              const bool inside = tokens[c] >= 0 && tokens[c] < p.V;
-              tried_px[tried] = x;
-              tried_in[tried] = inside ? (int)tokens[c] / PIECE : -1;
-            }
-          }
-          tried += down < 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += WALK_THREADS) {
+      if (i != tid)
+        own(i, z0, x0, y0);
+      z0.px = z0.qx = 0.0;
+      if (z0.up >= 0 && z0.token >= 0) {
+        const RowSum r = prows[z0.up];
+        z0.px = to2 == 0.0 ? (z0.token == r.first ? 1.0 : 0.0) : weight_of(x0, r.top, to2) / r.sum;
+        if (drawn) {
+          const RowSum s = qrows[z0.up];
+          z0.qx = weight_of(y0, s.top, to2) / s.sum;
         }
       }
-      if (down < 0)
-        break;
-      at = down;
+      nodes[i] = z0;
     }
-    if (lane == 0) {
-      walk_at = at;
-      walk_len = len;
-      walk_tried = tried;
+    __syncthreads();
+    if (parents) { // (nothing is left of a token that was tried before)
+      for (int i = tid; i < n; i += WALK_THREADS) {
+        const int up = nodes[i].up, token = nodes[i].token;
+        bool again = false;
+        for (int e = up + 1; e < i; e++)
+          again |= nodes[e].up == up && nodes[e].token == token;
+        if (again)
+          nodes[i].px = 0.0;
+      }
+      __syncthreads();
     }
-  }
-  __syncthreads();
-  const int at = walk_at, len = walk_len;
-  const int tried = walk_tried;
-  const int row = first + at;
-  if (LAST) {
-    for (int i = len + tid; i < n; i += DRAFT_THREADS)
-      p.path[first + i] = -1;
+    if (wave == 0) { // down, all lanes alike
+      int at = 0, len = 0, tried = 0;
+      if (!parents) { // a chain: the first node that does not stand ends it
+        int end = n;
+        for (int i0 = 0; i0 < n && end == n; i0 += 64) {
+          const int i = i0 + lane;
+          const NodeShare z = nodes[min(i, n - 1)];
+          const bool fails = i > 0 && i < n && !((double)z.u * (drawn ? z.qx : 1.0) < z.px);
+          const uint64_t bad = __builtin_amdgcn_ballot_w64(fails);
+          if (bad)
+            end = i0 + __builtin_ctzll(bad);
+          if (TOKEN || blockIdx.y == 0)
+            if (i < min(i0 + 64, n))
+              p.path[first + i] = i < end ? i : -1;
+        }
+        at = end - 1;
+        len = end;
+        if (end < n) {
+          tried = 1;
+          if (lane == 0) {
+            tried_px[0] = nodes[end].px;
+            tried_in[0] = nodes[end].token < 0 ? -1 : nodes[end].token / PIECE;
+          }
+          if (TOKEN || blockIdx.y == 0)
+            for (int i = end / 64 * 64 + 64 + lane; i < n; i += 64)
+              p.path[first + i] = -1;
+        }
+      } else {
+        for (;;) {
+          if (lane == 0)
+            p.path[first + len] = at;
+          len++;
+          int down = -1;
+          double left = 1.0;
+          tried = 0;
+          for (int c0 = at + 1; c0 < n && down < 0; c0 += 64) {
+            const int c = c0 + lane;
+            const NodeShare z = nodes[min(c, n - 1)];
+            const bool child = c < n && z.up == at;
+            const double x = child ? z.px : 0.0, upto = scan64(x, lane);
+            const uint64_t children = __builtin_amdgcn_ballot_w64(child);
+            const uint64_t stands = __builtin_amdgcn_ballot_w64(child && (double)z.u * (left - (upto - x)) < x);
+            if (stands)
+              down = c0 + __builtin_ctzll(stands);
+            const int place = tried + __popcll(children & ((1ull << lane) - 1));
+            if (!stands && child && place < DRAFT_NODES) {
+              tried_px[place] = x;
+              tried_in[place] = z.token < 0 ? -1 : z.token / PIECE;
+            }
+            tried += __popcll(children);
+            left -= __shfl(upto, 63);
+          }
+          if (down < 0)
+            break;
+          at = down;
+        }
+        for (int i = len + lane; i < n; i += 64)
+          p.path[first + i] = -1;
+      }
+      if (lane == 0)
+        walk = Walk{prows[at], drawn ? qrows[at] : RowSum{1.0, 0.f, 0}, at, len, tried, 0};
+    }
+    __syncthreads();
+    if (!TOKEN && blockIdx.y == 0 && tid == 0)
+      p.walks[b] = walk;
+  } else {
     if (tid == 0)
-      p.count[b] = len;
+      walk = p.walks[b];
+    __syncthreads();
   }
-  const RowSum ps = row_sum(0, row, lane, std::integral_constant<int, 64>{});
+  const int at = walk.at, tried = walk.tried, row = first + at;
+  if (TOKEN && tid == 0)
+    p.count[b] = walk.len;
+  const RowSum ps = walk.p, qs = walk.q;
   if (to2 == 0.0) {
-    if (LAST && tid == 0)
+    if (TOKEN && tid == 0)
       p.next[b] = ps.first;
     return;
   }
   const bool residual = drawn && tried;
-  RowSum qs = {1.0, 0.f, 0};
-  if (residual)
-    qs = row_sum(1, row, lane, std::integral_constant<int, 64>{});
-  const E* const prow = (const E*)p.target + (int64_t)row * p.t_ld;
-  const E* const qrow = (const E*)p.draft + (int64_t)row * p.d_ld;
-  // What is left of a vector of 16 bytes of the last row: p without the tokens that were tried, or max(p - q, 0).  all: p.
+  const E* const prow = logits(0, row);
+  const E* const qrow = logits(1, row);
   auto mark = [&](int piece) { // the tried tokens of a piece
     if (!tried || drawn)
       return;
-    for (int i = tid; i < PIECE / 32; i += DRAFT_THREADS)
+    for (int i = tid; i < PIECE / 32; i += WALK_THREADS)
       gone[i] = 0;
     __syncthreads();
-    for (int c = at + 1 + tid; c < n; c += DRAFT_THREADS) {
+    for (int c = at + 1 + tid; c < (parents ? n : min(at + 2, n)); c += WALK_THREADS) {
       const int64_t x = parent(c) == at ? tokens[c] : -1;
       if (x >= 0 && x < p.V && x / PIECE == piece)
         atomicOr(&gone[x % PIECE / 32], 1u << (x % 32));
     }
     __syncthreads();
   };
+  // What is left of a vector of 16 bytes of the last row: p without the tokens that were tried, or max(p - q, 0).  all: p.
   const double pn = 1.0 / ps.sum, qn = 1.0 / qs.sum;
   auto rest = [&](int from, bool all, double (&w)[N]) {
     float x[N], y[N];
@@ -380,31 +471,37 @@ draft_walk_kernel(const DraftsParams p) {
       w[e] = from + e < p.V ? w[e] : 0.0;
     }
   };
-  auto sum_of_piece = [&](int piece, bool all) { // in all threads; `gone` marked
+  // this thread's vector of a piece (-inf where the piece has fewer), and its sum
+  auto mine = [&](int piece, bool all, double (&w)[N]) {
     double s = 0.0;
-    for (int i = 0; i < NV; i++) {
-      double w[N];
-      rest(piece * PIECE + (i * DRAFT_THREADS + tid) * N, all, w);
+    if (tid < VECTORS) {
+      rest(piece * PIECE + tid * N, all, w);
 #pragma unroll
       for (int e = 0; e < N; e++)
         s += w[e];
     }
-    s = reduce_lanes<64>(s, [](double a, double z) { return a + z; });
+    return s;
+  };
+  auto sum_of_piece = [&](int piece) { // in all threads; `gone` marked
+    double w[N];
+    const double s = reduce_lanes<64>(mine(piece, false, w), add64);
     __syncthreads();
     if (lane == 0)
       red[wave] = s;
     __syncthreads();
-    s = (red[0] + red[1]) + (red[2] + red[3]);
-    return s;
+    double whole = 0.0;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++)
+      whole += red[i];
+    return whole;
   };
   double* const sums = p.sums + (int64_t)b * p.C;
-  if constexpr (!LAST) {
+  if constexpr (!TOKEN) {
     if (residual) {
-      const double s = sum_of_piece((int)blockIdx.y, false);
+      const double s = sum_of_piece((int)blockIdx.y);
       if (tid == 0)
         sums[blockIdx.y] = s;
     }
-    return;
   } else {
     // The pieces' sums: from the first launch less the tried tokens' shares (a difference of sums near 1, so a rest that small is
     // summed anew, as it is where more were tried than are kept), from the second one, or, where nothing is left, p.
@@ -426,28 +523,20 @@ draft_walk_kernel(const DraftsParams p) {
         const double head = of_piece(lane);
         double whole = 0.0;
         for (int i0 = 0; i0 < p.C; i0 += 64)
-          whole += reduce_lanes<64>(i0 ? of_piece(i0 + lane) : head, [](double a, double z) { return a + z; });
+          whole += reduce_lanes<64>(i0 ? of_piece(i0 + lane) : head, add64);
         const double border = (double)p.sample[b] * whole;
         double before = 0.0, start = 0.0;
         int piece = -1, last = 0;
         for (int i0 = 0; i0 < p.C && piece < 0; i0 += 64) {
-          const double s = i0 ? of_piece(i0 + lane) : head;
-          double run = s;
-#pragma unroll
-          for (int d = 1; d < 64; d *= 2) {
-            const double t = __shfl_up(run, d);
-            run += lane >= d ? t : 0.0;
-          }
+          const double s = i0 ? of_piece(i0 + lane) : head, run = scan64(s, lane);
           const uint64_t beyond = __builtin_amdgcn_ballot_w64(s > 0.0 && before + run > border);
           const uint64_t some = __builtin_amdgcn_ballot_w64(s > 0.0);
           if (beyond) {
-            const int j = __builtin_ctzll(beyond);
-            piece = i0 + j;
-            start = before + __shfl(run - s, j);
+            piece = i0 + __builtin_ctzll(beyond);
+            start = before + __shfl(run - s, __builtin_ctzll(beyond));
           } else if (some) { // (where the border is rounded past the last one)
-            const int j = 63 - __builtin_clzll(some);
-            last = i0 + j;
-            start = before + __shfl(run - s, j);
+            last = i0 + 63 - __builtin_clzll(some);
+            start = before + __shfl(run - s, 63 - __builtin_clzll(some));
           }
           before += __shfl(run, 63);
         }
@@ -461,41 +550,25 @@ draft_walk_kernel(const DraftsParams p) {
       __syncthreads();
       const bool fine = piece_border >= 0.0;
       __syncthreads();
-      if (fine)
+      if (fine || all)
         break;
-      if (all || drawn || round > 0) {
-        if (all)
-          break; // (does not happen: p sums to 1)
+      if (drawn || round > 0) {
         all = true;
         continue;
       }
       for (int i = 0; i < p.C; i++) { // too little for differences
         mark(i);
-        const double s = sum_of_piece(i, false);
+        const double s = sum_of_piece(i);
         if (tid == 0)
           sums[i] = s;
       }
       __syncthreads();
     }
-    // the token: a thread takes a run of the piece
     const int piece = piece_at;
     const double border = piece_border;
     mark(piece);
-    constexpr int RUN = NV * N;
-    double w[NV][N], s = 0.0;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      rest(piece * PIECE + tid * RUN + i * N, all, w[i]);
-#pragma unroll
-      for (int e = 0; e < N; e++)
-        s += w[i][e];
-    }
-    double run = s;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double t = __shfl_up(run, d);
-      run += lane >= d ? t : 0.0;
-    }
+    double w[N];
+    const double s = mine(piece, all, w), run = scan64(s, lane);
     if (lane == 63)
       red[wave] = run;
     __syncthreads();
@@ -504,32 +577,34 @@ draft_walk_kernel(const DraftsParams p) {
       before += red[i];
     before += run - s;
     int found = p.V, last = -1;
-#pragma unroll
-    for (int i = 0; i < NV; i++)
+    if (tid < VECTORS) {
 #pragma unroll
       for (int e = 0; e < N; e++) {
-        before += w[i][e];
-        const int x = piece * PIECE + tid * RUN + i * N + e;
-        if (w[i][e] > 0.0) {
+        before += w[e];
+        const int x = piece * PIECE + tid * N + e;
+        if (w[e] > 0.0) {
           last = x;
           found = before > border && found == p.V ? x : found;
         }
       }
+    }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       found = min(found, __shfl_xor(found, d));
       last = max(last, __shfl_xor(last, d));
     }
-    if (lane == 0)
+    if (lane == 0) {
       found_at[wave] = found;
+      last_at[wave] = last;
+    }
     __syncthreads();
-    found = min(min(found_at[0], found_at[1]), min(found_at[2], found_at[3]));
-    __syncthreads();
-    if (lane == 0)
-      found_at[wave] = last;
-    __syncthreads();
-    if (tid == 0) // (a border that is rounded past the piece's last token: that one)
-      p.next[b] = found < p.V ? found : max(max(max(found_at[0], found_at[1]), max(found_at[2], found_at[3])), 0);
+    if (tid == 0) {
+      for (int i = 1; i < WAVES; i++) {
+        found = min(found, found_at[i]);
+        last = max(last, last_at[i]);
+      }
+      p.next[b] = found < p.V ? found : max(last, 0); // (a border that is rounded past the piece's last token: that one)
+    }
   }
 }
 
@@ -576,16 +651,20 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
   TPPX_REQUIRE(aligned16(ws), TPPX_EINVAL, "%s: workspace not 16-byte aligned", who);
   p.pieces = (Piece*)ws;
   p.sums = (double*)(p.pieces + p.sides * T * p.C);
-  p.px = p.sums + B * p.C;
-  p.qx = p.px + T;
+  p.walks = (Walk*)(p.sums + (B * p.C + 1) / 2 * 2);
+  p.rows = (RowSum*)(p.walks + B);
+  p.nodes = (NodeShare*)(p.rows + 2 * T);
   auto go = [&](auto e, auto nv_) {
     using E = decltype(e);
     constexpr int NV = decltype(nv_)::value;
     if (T > 0)
       draft_rows_kernel<E, NV><<<dim3((unsigned)(T * p.C), (unsigned)p.sides), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
-    if (T > 0 && draft)
-      draft_walk_kernel<E, NV, false><<<dim3((unsigned)B, (unsigned)p.C), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
-    draft_walk_kernel<E, NV, true><<<dim3((unsigned)B), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
+    if (draft) {
+      draft_walk_kernel<E, NV, true, false><<<dim3((unsigned)B, (unsigned)p.C), dim3(WALK_THREADS), 0, (hipStream_t)stream>>>(p);
+      draft_walk_kernel<E, NV, false, true><<<dim3((unsigned)B), dim3(WALK_THREADS), 0, (hipStream_t)stream>>>(p);
+    } else {
+      draft_walk_kernel<E, NV, true, true><<<dim3((unsigned)B), dim3(WALK_THREADS), 0, (hipStream_t)stream>>>(p);
+    }
   };
   auto typed = [&](auto e) {
     if (nv == 4)
@@ -605,5 +684,5 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
 extern "C" int64_t tppx_verify_drafts_bytes(int64_t T, int64_t B, int64_t V, int drafts) {
   // (of the type with the most pieces, in the form with the most)
   const int64_t C = draft_pieces(V, 4, 1);
-  return (drafts ? 2 : 1) * T * C * (int64_t)sizeof(Piece) + B * C * 8 + 2 * T * 8 + 256;
+  return (drafts ? 2 : 1) * T * C * (int64_t)sizeof(Piece) + (B * C + 1) / 2 * 16 + B * (int64_t)sizeof(Walk) + T * (int64_t)(2 * sizeof(RowSum) + sizeof(NodeShare)) + 256;
 }
