@@ -77,21 +77,56 @@ __device__ __forceinline__ double weight_of(float x, float top, double to2) {
   const double w = to2 == 0.0 ? 0.0 : exp2_64(((double)x - (double)top) * to2);
   return x == top ? 1.0 : w;
 }
-// The same for many: 2^(n / 256) from a table and 2^(f / 256), f in [-1/2, 1/2], by an interpolation of degree 3, 4e-14 relative: ten
-// instructions in 64 bits where the polynomial takes nineteen.  `lowest` stands for what lies below it (its weight is 2^-900).
+// The same for many: 2^(x k) = 2^(n / 256) 2^(f / 256), n whole, f in [-1/2, 1/2]; the first from a table, the second by an
+// interpolation of degree 3, 4e-14 relative.  Eight instructions in 64 bits where the polynomial takes nineteen.  The sum is relative to
+// 2^(r / 256), r the whole number next to that of the maximum, so that no difference is taken.  `lowest` stands for what lies below
+// it (its weight is 2^-900).  A NaN may come out for one that comes in.
+struct Powers { // 2^(j / 256), less the bits that n << 12 adds to it
+  double v[256];
+  constexpr Powers() : v() {
+    constexpr double f[8] = {1.0027112750502025, 1.0054299011128027, 1.0108892860517005, 1.0218971486541166, 1.0442737824274138, 1.0905077326652577, 1.189207115002721, 1.4142135623730951};
+    for (int j = 0; j < 256; j++) {
+      double x = 1.0;
+      for (int i = 0; i < 8; i++)
+        x *= j >> i & 1 ? f[i] : 1.0;
+      v[j] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, x) - ((uint64_t)j << 44));
+    }
+  }
+};
+__device__ constexpr Powers POWERS;
 struct ManyWeights {
   const double* table;
-  double top, k;
+  double k, magic;
   float lowest;
-  __device__ __forceinline__ ManyWeights(const double* t, float m, double to2) : table(t), top(m), k(to2 * 256.0), lowest(m - (float)(900.0 / to2)) {}
-  static __device__ __forceinline__ bool fits(float top, double to2) { return fabsf(top) < 1e5f && to2 < 64.0; }
-  __device__ __forceinline__ double operator()(float x) const {
-    constexpr double MAGIC = 0x1.8p52; // (a sum with it is rounded to a whole number, which its low bits are)
-    const double d = (double)fmaxf(x, lowest) - top, t = fma(d, k, MAGIC), f = fma(d, k, MAGIC - t);
+  __device__ __forceinline__ ManyWeights(const double* t, float top, double to2)
+      : table(t), k(to2 * 256.0), magic(0x1.8p52 - __builtin_rint((double)top * (to2 * 256.0))), lowest(top - 900.0f / (float)to2) {}
+  static __device__ __forceinline__ bool fits(float top, double to2) { return fabsf(top) < 1e5f && to2 < 64.0 && to2 > 1e-6 && fabsf(top) * (float)to2 < 1e6f; }
+  // what the sum of the weights relative to the maximum is that of these times
+  __device__ __forceinline__ double off(float top) const { return exp2_64(((0x1.8p52 - magic) - (double)top * k) * (1.0 / 256.0)); }
+  // 2^(n / 256), and what is left
+  __device__ __forceinline__ double parts(float x, double& g) const {
+    float c;
+    asm("v_max_f32 %0, %1, %2" : "=v"(c) : "v"(x), "v"(lowest));
+    const double d = (double)c, t = fma(d, k, magic), f = fma(d, k, magic - t); // (t is rounded to a whole number, which its low bits are)
     const int n = __double2loint(t);
-    const double a = table[n & 255], s = __hiloint2double(__double2hiint(a) + ((n & ~255) << 12), __double2loint(a));
-    const double g = f * fma(f, fma(f, 3.3083029079191157e-09, 3.665566016796724e-06), 0.0027076061740622863);
-    return fma(s, g, s);
+    const double a = table[n & 255];
+    g = fma(f, fma(f, fma(f, 3.3083029079191157e-09, 3.665566016796724e-06), 0.0027076061740622863), 1.0);
+    return __hiloint2double(__double2hiint(a) + (n << 12), __double2loint(a));
+  }
+  template <int N>
+  __device__ __forceinline__ double sum(const float (&x)[N], double s) const {
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      double g;
+      const double w = parts(x[e], g);
+      s = fma(w, g, s);
+    }
+    return s;
+  }
+  __device__ __forceinline__ double operator()(float x) const {
+    double g;
+    const double w = parts(x, g);
+    return w * g;
   }
 };
 template <typename E>
@@ -113,7 +148,47 @@ constexpr int DRAFT_THREADS = 256;
 // logits per 16 bytes
 template <typename E>
 constexpr int per16() { return 16 / (int)sizeof(E); }
-// `n` logits of a row from `at` on, -inf behind its end (rows need no more than their type's alignment)
+// logits as they lie in 16 bytes
+template <typename E>
+__device__ __forceinline__ void raw_logits(const uint4& v, float (&x)[per16<E>()]) {
+  const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (std::is_same_v<E, float>) {
+      x[i] = __uint_as_float(d[i]);
+    } else if constexpr (std::is_same_v<E, uint16_t>) {
+      x[2 * i] = __uint_as_float(d[i] << 16);
+      x[2 * i + 1] = __uint_as_float(d[i] & 0xffff0000u);
+    } else {
+      x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)d[i]);
+      x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(d[i] >> 16));
+    }
+  }
+}
+// 16 bytes of a row from logit `at` on, -inf behind its end (rows need no more than their type's alignment)
+template <typename E>
+__device__ __forceinline__ uint4 load_raw(const E* row, int at, int V) {
+  constexpr int N = per16<E>();
+  constexpr uint32_t none = std::is_same_v<E, float> ? 0xff800000u : std::is_same_v<E, uint16_t> ? 0xff80ff80u : 0xfc00fc00u;
+  uint4 v = make_uint4(none, none, none, none);
+  if (at + N <= V) {
+    __builtin_memcpy(&v, row + at, 16);
+  } else if (at < V) {
+    uint32_t d[4] = {none, none, none, none};
+#pragma unroll
+    for (int e = 0; e < N; e++)
+      if (at + e < V) {
+        if constexpr (N == 4)
+          d[e] = __builtin_bit_cast(uint32_t, row[at + e]);
+        else
+          d[e / 2] = e & 1 ? (d[e / 2] & 0xffffu) | (uint32_t)__builtin_bit_cast(uint16_t, row[at + e]) << 16
+                           : (d[e / 2] & 0xffff0000u) | __builtin_bit_cast(uint16_t, row[at + e]);
+      }
+    v = make_uint4(d[0], d[1], d[2], d[3]);
+  }
+  return v;
+}
+// N logits from `at` on
 template <typename E>
 __device__ __forceinline__ void load_logits(const E* row, int at, int V, float (&x)[per16<E>()]) {
   constexpr int N = per16<E>();
@@ -160,54 +235,79 @@ draft_rows_kernel(const DraftsParams p) {
   const double to2 = to2_of(p, b);
   const E* const at = (const E*)(side ? p.draft : p.target) + (int64_t)row * (side ? p.d_ld : p.t_ld);
   const int from = piece * (DRAFT_THREADS * NV * N);
-  float x[NV][N];
-#pragma unroll
-  for (int i = 0; i < NV; i++)
-    load_logits<E>(at, from + (i * DRAFT_THREADS + tid) * N, p.V, x[i]);
-  __shared__ double table[256];
-  if (NV > 1 && to2 != 0.0) {
-    table[tid] = exp2_64((double)tid * (1.0 / 256.0));
-    __syncthreads();
-  }
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < NV; i++)
-#pragma unroll
-    for (int e = 0; e < N; e++)
-      top = fmaxf(top, x[i][e]);
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2)
-    top = fmaxf(top, __shfl_xor(top, d));
   int first = p.V;
   double sum = 0.0;
-  if (to2 == 0.0) {
+  float top = -INFINITY;
+  bool done = false; // (uniform in a wave)
+  if (NV > 1 && to2 != 0.0) {
+    __shared__ double table[256];
+    uint4 v[NV];
 #pragma unroll
-    for (int i = NV - 1; i >= 0; i--)
+    for (int i = 0; i < NV; i++)
+      v[i] = load_raw<E>(at, from + (i * DRAFT_THREADS + tid) * N, p.V);
+    table[tid] = POWERS.v[tid];
+    __syncthreads();
 #pragma unroll
-      for (int e = N - 1; e >= 0; e--) {
-        const int j = from + (i * DRAFT_THREADS + tid) * N + e;
-        first = x[i][e] == top && j < p.V ? j : first;
-      }
+    for (int i = 0; i < NV; i++) {
+      float x[N];
+      raw_logits<E>(v[i], x);
+#pragma unroll
+      for (int e = 0; e < N; e += 2)
+        asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top) : "v"(x[e]), "v"(x[e + 1]));
+    }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2)
-      first = min(first, __shfl_xor(first, d));
-  } else if (NV > 1 && from + DRAFT_THREADS * NV * N <= p.V && ManyWeights::fits(top, to2)) { // (uniform in a wave)
-    const ManyWeights many(table, top, to2);
+      top = fmaxf(top, __shfl_xor(top, d));
+    if (from + wave * (64 * N) >= p.V) { // (behind the end)
+      done = true;
+    } else if (ManyWeights::fits(top, to2)) {
+      const ManyWeights many(table, top, to2);
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        float x[N];
+        raw_logits<E>(v[i], x);
+        sum = many.sum(x, sum);
+      }
+      sum = reduce_lanes<64>(sum, [](double a, double z) { return a + z; }) * many.off(top);
+      done = sum > 0.0; // (and no NaN)
+    }
+  }
+  if (!done) {
+    float x[NV][N];
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+      load_logits<E>(at, from + (i * DRAFT_THREADS + tid) * N, p.V, x[i]);
+    top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
       for (int e = 0; e < N; e++)
-        sum += many(x[i][e]);
-    sum = reduce_lanes<64>(sum, [](double a, double z) { return a + z; });
-  } else {
+        top = fmaxf(top, x[i][e]);
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+    for (int d = 1; d < 64; d *= 2)
+      top = fmaxf(top, __shfl_xor(top, d));
+    sum = 0.0;
+    if (to2 == 0.0) {
 #pragma unroll
-      for (int e = 0; e < N; e++) { // (behind the end: -inf, which counts where the row is nothing else)
-        const double w = weight_of(x[i][e], top, to2);
-        sum += from + (i * DRAFT_THREADS + tid) * N + e < p.V ? w : 0.0;
-      }
-    sum = reduce_lanes<64>(sum, [](double a, double z) { return a + z; });
+      for (int i = NV - 1; i >= 0; i--)
+#pragma unroll
+        for (int e = N - 1; e >= 0; e--) {
+          const int j = from + (i * DRAFT_THREADS + tid) * N + e;
+          first = x[i][e] == top && j < p.V ? j : first;
+        }
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2)
+        first = min(first, __shfl_xor(first, d));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int e = 0; e < N; e++) { // (behind the end: -inf, which counts where the row is nothing else)
+          const double w = weight_of(x[i][e], top, to2);
+          sum += from + (i * DRAFT_THREADS + tid) * N + e < p.V ? w : 0.0;
+        }
+      sum = reduce_lanes<64>(sum, [](double a, double z) { return a + z; });
+    }
   }
   if (lane == 0) {
     tops[wave] = top;
@@ -236,13 +336,20 @@ constexpr int DRAFT_NODES = 256; // nodes of a sequence that are held in LDS; mo
 constexpr int WALK_THREADS = 1024;
 
 __device__ __forceinline__ double add64(double a, double z) { return a + z; }
-// sum over the lanes below, and this one's
-__device__ __forceinline__ double scan64(double v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const double t = __shfl_up(v, d);
-    v += lane >= d ? t : 0.0;
-  }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lane(double v) { // (0 where there is no such lane)
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, ROWS == 0xf);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, ROWS == 0xf);
+  return __hiloint2double(hi, lo);
+}
+// sum over the lanes below, and this one's; all lanes take part
+__device__ __forceinline__ double scan64(double v) {
+  v += from_lane<0x111, 0xf>(v); // row_shr:1
+  v += from_lane<0x112, 0xf>(v);
+  v += from_lane<0x114, 0xf>(v);
+  v += from_lane<0x118, 0xf>(v);
+  v += from_lane<0x142, 0xa>(v); // row_bcast:15 into the second and the last row
+  v += from_lane<0x143, 0xc>(v); // row_bcast:31 into the upper rows
   return v;
 }
 
@@ -348,12 +455,12 @@ draft_walk_kernel(const DraftsParams p) {
     }
     __syncthreads();
     if (parents) { // (nothing is left of a token that was tried before)
-      for (int i = tid; i < n; i += WALK_THREADS) {
+      for (int i = wave; i < n; i += WAVES) {
         const int up = nodes[i].up, token = nodes[i].token;
         bool again = false;
-        for (int e = up + 1; e < i; e++)
+        for (int e = up + 1 + lane; e < i; e += 64)
           again |= nodes[e].up == up && nodes[e].token == token;
-        if (again)
+        if (__builtin_amdgcn_ballot_w64(again) != 0 && lane == 0)
           nodes[i].px = 0.0;
       }
       __syncthreads();
@@ -397,7 +504,7 @@ draft_walk_kernel(const DraftsParams p) {
             const int c = c0 + lane;
             const NodeShare z = nodes[min(c, n - 1)];
             const bool child = c < n && z.up == at;
-            const double x = child ? z.px : 0.0, upto = scan64(x, lane);
+            const double x = child ? z.px : 0.0, upto = scan64(x);
             const uint64_t children = __builtin_amdgcn_ballot_w64(child);
             const uint64_t stands = __builtin_amdgcn_ballot_w64(child && (double)z.u * (left - (upto - x)) < x);
             if (stands)
@@ -497,11 +604,40 @@ draft_walk_kernel(const DraftsParams p) {
   };
   double* const sums = p.sums + (int64_t)b * p.C;
   if constexpr (!TOKEN) {
-    if (residual) {
-      const double s = sum_of_piece((int)blockIdx.y);
-      if (tid == 0)
-        sums[blockIdx.y] = s;
+    if (!residual)
+      return;
+    __shared__ double table[256];
+    double s = 0.0;
+    if (ManyWeights::fits(ps.top, to2) && ManyWeights::fits(qs.top, to2)) { // (uniform)
+      const int from = (int)blockIdx.y * PIECE + tid * N;
+      float x[N], y[N];
+      if (tid < VECTORS) {
+        load_logits<E>(prow, from, p.V, x);
+        load_logits<E>(qrow, from, p.V, y);
+      }
+      if (tid < 256)
+        table[tid] = POWERS.v[tid];
+      __syncthreads();
+      if (tid < VECTORS) {
+        const ManyWeights mp(table, ps.top, to2), mq(table, qs.top, to2);
+        const double a = pn * mp.off(ps.top), z = qn * mq.off(qs.top);
+#pragma unroll
+        for (int e = 0; e < N; e++)
+          s += fmax(mp(x[e]) * a - mq(y[e]) * z, 0.0);
+      }
+      s = reduce_lanes<64>(s, add64);
+      if (lane == 0)
+        red[wave] = s;
+      __syncthreads();
+      s = 0.0;
+#pragma unroll
+      for (int i = 0; i < WAVES; i++)
+        s += red[i];
+    } else {
+      s = sum_of_piece((int)blockIdx.y);
     }
+    if (tid == 0)
+      sums[blockIdx.y] = s;
   } else {
     // The pieces' sums: from the first launch less the tried tokens' shares (a difference of sums near 1, so a rest that small is
     // summed anew, as it is where more were tried than are kept), from the second one, or, where nothing is left, p.
@@ -516,6 +652,7 @@ draft_walk_kernel(const DraftsParams p) {
           const Piece z = p.pieces[(int64_t)row * p.C + i];
           double s = z.sum > 0.0 ? z.sum * weight_of(z.top, ps.top, to2) * pn : 0.0;
           if (!all)
+#pragma unroll 8
             for (int c = 0; c < min(tried, DRAFT_NODES); c++)
               s -= tried_in[c] == i ? tried_px[c] : 0.0;
           return fmax(s, 0.0);
@@ -528,7 +665,7 @@ draft_walk_kernel(const DraftsParams p) {
         double before = 0.0, start = 0.0;
         int piece = -1, last = 0;
         for (int i0 = 0; i0 < p.C && piece < 0; i0 += 64) {
-          const double s = i0 ? of_piece(i0 + lane) : head, run = scan64(s, lane);
+          const double s = i0 ? of_piece(i0 + lane) : head, run = scan64(s);
           const uint64_t beyond = __builtin_amdgcn_ballot_w64(s > 0.0 && before + run > border);
           const uint64_t some = __builtin_amdgcn_ballot_w64(s > 0.0);
           if (beyond) {
@@ -568,7 +705,7 @@ draft_walk_kernel(const DraftsParams p) {
     const double border = piece_border;
     mark(piece);
     double w[N];
-    const double s = mine(piece, all, w), run = scan64(s, lane);
+    const double s = mine(piece, all, w), run = scan64(s);
     if (lane == 63)
       red[wave] = run;
     __syncthreads();
