@@ -167,17 +167,30 @@ struct PagedAttnParams {
   int T, B, Nq, Nkv, R, splits, chunk; // chunk: tiles of a split
   float scale;
 };
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t* ConstantInts; // (scalar loads)
 
-template <int NJ, int CW, int TW, int KEYS>
-__global__ void __launch_bounds__(64 * CW * TW, CW == 8 ? 4 : CW * TW == 4 && CW > 1 ? 2 : 1)
+constexpr int MAX_SPLITS = 64;
+// keys that nodes 0 .. last of sequence b see, of which the last sees most; splits of so many tiles
+__device__ __forceinline__ int paged_past(const PagedAttnParams& p, int b) { return min(p.past[b], (int)(p.g.table_ld << p.g.shift)); }
+__device__ __forceinline__ int paged_keys(const PagedAttnParams& p, int b, int last) {
+  const int past = paged_past(p, b);
+  return past < 0 ? 0 : (int)min((int64_t)past + last + 1, p.g.table_ld << p.g.shift);
+}
+__device__ __forceinline__ int paged_splits(const PagedAttnParams& p, int tiles) { return max((tiles + p.chunk - 1) / p.chunk, 1); }
+constexpr int PAGED_NODES = 256;
+
+template <int NJ, int CG, int CW, int TW, int KEYS>
+__global__ void __launch_bounds__(64 * CW * TW, CG == 1 && CW == 8 ? 4 : CW > 1 ? 2 : 1)
 paged_attn_kernel(const PagedAttnParams p) {
-  constexpr int H = 32 * NJ, ROW = 64 * NJ, PER = 4 * NJ, SIDE = KEYS * ROW, COLS = 16 * CW, TH = 64 * CW * TW, NA = H / 16, NT = KEYS / 16;
+  constexpr int H = 32 * NJ, ROW = 64 * NJ, PER = 4 * NJ, SIDE = KEYS * ROW, WCOLS = 16 * CG, COLS = WCOLS * CW, TH = 64 * CW * TW, NA = H / 16, NT = KEYS / 16;
   constexpr int XK = NJ % 4 == 0 ? 4 : NJ % 2 == 0 ? 2 : 1, XV = NJ % 4 == 0 ? 8 : NJ % 2 == 0 ? 4 : 2, NR = NJ == 3 ? 6 : XV;
-  constexpr int RUNS = 2 * NT, MINE = RUNS / CW; // runs of 16 rows of a tile, K then V; of a wave
-  static_assert(RUNS % CW == 0 && (KEYS == 32 || KEYS == 64));
+  constexpr int RUNS = 2 * NT, MINE = RUNS >= CW ? RUNS / CW : 1; // runs of 16 rows of a tile, K then V; of a wave
+  static_assert((RUNS % CW == 0 || CW > RUNS) && (KEYS == 32 || KEYS == 64));
   extern __shared__ __align__(16) uint8_t lds[]; // V [team][stage], K [team][stage]
   __shared__ int arrived_last;
+  __shared__ int tree[PAGED_NODES]; // parents, of a sequence that has no more (a load from memory waits for the tile under way)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % CW, team = __builtin_amdgcn_readfirstlane(tid >> 6) / CW;
   const int g = lane >> 4, c = lane & 15;
@@ -187,23 +200,22 @@ paged_attn_kernel(const PagedAttnParams p) {
     return;
   const int ncol = min(COLS, o.n * p.R - o.at * COLS); // of this workgroup
   const int col0 = o.at * COLS;
-  const int capacity = (int)(p.g.table_ld << p.g.shift);
-  const int past = min(p.past[o.b], capacity);
-  const int keys = past < 0 ? 0 : (int)min((int64_t)past + (col0 + ncol - 1) / p.R + 1, (int64_t)capacity); // that some column sees
-  const int tiles = (keys + KEYS - 1) / KEYS;
-  const int S = max((tiles + p.chunk - 1) / p.chunk, 1); // splits that have tiles; the others take no part
+  const int past = paged_past(p, o.b), keys = paged_keys(p, o.b, (col0 + ncol - 1) / p.R); // that some column sees
+  const int tiles = (keys + KEYS - 1) / KEYS, S = paged_splits(p, tiles); // splits that have tiles; the others take no part
   if ((int)blockIdx.y >= S)
     return;
-  const bool idle = wave * 16 >= ncol;
-  const int col = col0 + min(wave * 16 + c, ncol - 1), node = col / p.R, r0 = col - node * p.R;
+  const bool idle = wave * WCOLS >= ncol;
   const int32_t* const parents = p.parents ? p.parents + o.start : nullptr;
-
-  bf16x8 q[NJ];
-  {
-    const uint16_t* qrow = p.q + (int64_t)(o.start + node) * p.q_ld + (hk * p.R + r0) * H + g * 8;
+  int node[CG], up[CG]; // of this lane's columns; where their ways up have come to
+  bf16x8 q[CG][NJ];
+#pragma unroll
+  for (int k = 0; k < CG; k++) {
+    const int col = col0 + min(wave * WCOLS + k * 16 + c, ncol - 1);
+    node[k] = up[k] = col / p.R;
+    const uint16_t* qrow = p.q + (int64_t)(o.start + node[k]) * p.q_ld + (hk * p.R + col - node[k] * p.R) * H + g * 8;
 #pragma unroll
     for (int j = 0; j < NJ; j++)
-      q[j] = *reinterpret_cast<const bf16x8*>(qrow + j * 32);
+      q[k][j] = *reinterpret_cast<const bf16x8*>(qrow + j * 32);
   }
   // Tiles top, top - TW, .. of this team, down to the split's last one.
   const int low = (S - 1 - (int)blockIdx.y) * tiles / S, top = (S - (int)blockIdx.y) * tiles / S - 1 - team, most = (top + team - low) / TW + 1;
@@ -214,7 +226,7 @@ paged_attn_kernel(const PagedAttnParams p) {
     if (t >= low) {
 #pragma unroll
       for (int i = 0; i < MINE; i++) {
-        const int run = (i * CW + wave) % NT;
+        const int run = (i * CW + wave) % NT; // (more waves than runs: the last ones bring nothing)
         ids[i] = table[min(t * KEYS + run * 16, keys - 1) >> p.g.shift];
       }
     }
@@ -231,6 +243,8 @@ paged_attn_kernel(const PagedAttnParams p) {
 #pragma unroll
     for (int i = 0; i < MINE; i++) {
       const int run = (i * CW + wave) % NT, side = (i * CW + wave) / NT;
+      if (CW > RUNS && side > 1)
+        continue;
       const int key = min(t * KEYS + run * 16, keys - 1), rows = min(keys - key, 16);
       // (a page that does not exist: the first one)
       const int id = (unsigned)ids[i] < (unsigned)p.g.pages ? ids[i] : 0;
@@ -260,21 +274,32 @@ paged_attn_kernel(const PagedAttnParams p) {
                  (uint32_t)(team * 2 * SIDE + r * ROW + ((d * 2 + ((c >> 1) & 1)) ^ packed_v_turn(NJ, r)) * 16 + (c & 1) * 8);
   }
 
-  float m = LOWEST, l = 0.f;
-  f32x4 acc[NA];
+  float m[CG], l[CG];
+  f32x4 acc[CG][NA];
 #pragma unroll
-  for (int dt = 0; dt < NA; dt++)
-    acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k = 0; k < CG; k++) {
+    m[k] = LOWEST;
+    l[k] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < NA; dt++)
+      acc[k][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   const float unit = p.scale * LOG2E;
-  int up = node; // where this column's way up has come to
+  const bool small = o.n <= PAGED_NODES;
+  if (parents && small)
+    for (int i = tid; i < o.n; i += TH)
+      tree[i] = parent_of(parents, i);
+  auto parent = [&](int i) { return small ? tree[i] : parent_of(parents, i); };
   auto tile = [&](auto S_, int t, int highest) { // highest: the tile of the first team, at the same time
     constexpr int stage = decltype(S_)::value;
     const int kb = t * KEYS;
-    // this tile has landed and the other stage has been read, for this wave and then for every wave that shares them
-    if constexpr (CW == 1)
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
-    else
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory");
+    // this tile has landed and the other stage has been read, for this wave and then for every wave that shares them (the wait as a
+    // builtin, which the compiler counts: behind one in asm it waits for q once more in every tile, and so for the loads under way)
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070); // vmcnt(0) lgkmcnt(0)
+    if constexpr (CW > 1)
+      __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
     const bool mine = t >= low; // (uniform in a team)
     bool odd = false;
     if ((CW == 1 ? kb : highest * KEYS) + KEYS > past) { // some column may not see some key
@@ -296,61 +321,77 @@ paged_attn_kernel(const PagedAttnParams p) {
       request(t - TW, stage ^ 1); // in flight during the arithmetic below
       look_up(t - 2 * TW);
     }
-    bf16x8 pb[NT / 2];
-    uint64_t seen = ~0ull;
+    bf16x8 pb[CG][NT / 2];
+    uint64_t seen[CG];
+#pragma unroll
+    for (int k = 0; k < CG; k++)
+      seen[k] = ~0ull; // (a tile below the step's slots beside one that holds some)
     const bool busy = mine && !idle;
     if (busy) {
       const uint8_t* const st = lds + stage * SIDE;
-      f32x4 sc[NT];
+      f32x4 sc[CG][NT];
 #pragma unroll
       for (int u = 0; u < NT; u++) {
-        sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
-          sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<const bf16x8*>(st + kaddr[j % XK] + u * (16 * ROW) + j / XK * (XK * 64)), q[j], sc[u], 0, 0, 0);
+        for (int k = 0; k < CG; k++)
+          sc[k][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+          const bf16x8 w = *reinterpret_cast<const bf16x8*>(st + kaddr[j % XK] + u * (16 * ROW) + j / XK * (XK * 64));
+#pragma unroll
+          for (int k = 0; k < CG; k++)
+            sc[k][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, q[k][j], sc[k][u], 0, 0, 0);
+        }
       }
       if (kb + KEYS > past) { // (uniform in a team)
         const int lo = kb - past; // the node whose slot is the tile's first key
-        seen = lo < 0 ? (1ull << -lo) - 1 : 0ull; // (above -KEYS)
-        if (!parents) {
-          const int last = node - lo; // (the capacity ends the keys: what lies behind is not asked about)
-          seen = last >= 63 ? ~0ull : last < 0 ? 0ull : (2ull << last) - 1;
-        } else {
-          while (up >= max(lo + KEYS, 0))
-            up = parent_of(parents, up);
-          while (up >= max(lo, 0)) {
-            seen |= 1ull << (up - lo);
-            up = parent_of(parents, up);
+#pragma unroll
+        for (int k = 0; k < CG; k++) {
+          uint64_t s = lo < 0 ? (1ull << -lo) - 1 : 0ull; // (above -KEYS)
+          if (!parents) {
+            const int last = node[k] - lo; // (the capacity ends the keys: what lies behind is not asked about)
+            s = last >= 63 ? ~0ull : last < 0 ? 0ull : (2ull << last) - 1;
+          } else {
+            while (up[k] >= max(lo + KEYS, 0))
+              up[k] = parent(up[k]);
+            while (up[k] >= max(lo, 0)) {
+              s |= 1ull << (up[k] - lo);
+              up[k] = parent(up[k]);
+            }
           }
+          const int behind = keys - kb;
+          if (behind < 64)
+            s &= (1ull << behind) - 1;
+          seen[k] = s;
+          const uint64_t bits = s >> (g * 4);
+#pragma unroll
+          for (int i = 0; i < 4 * NT; i++)
+            sc[k][i >> 2][i & 3] = bits >> ((i >> 2) * 16 + (i & 3)) & 1 ? sc[k][i >> 2][i & 3] : -INFINITY;
         }
-        const int behind = keys - kb;
-        if (behind < 64)
-          seen &= (1ull << behind) - 1;
-        const uint64_t bits = seen >> (g * 4);
+      }
+#pragma unroll
+      for (int k = 0; k < CG; k++) {
+        float mx = m[k];
 #pragma unroll
         for (int i = 0; i < 4 * NT; i++)
-          sc[i >> 2][i & 3] = bits >> ((i >> 2) * 16 + (i & 3)) & 1 ? sc[i >> 2][i & 3] : -INFINITY;
-      }
-      float mx = m;
+          mx = fmaxf(mx, sc[k][i >> 2][i & 3]);
+        if (__builtin_amdgcn_ballot_w64((mx - m[k]) * unit > 8.f) != 0) {
+          mx = max_of_groups(mx);
+          const float alpha = __builtin_amdgcn_exp2f((m[k] - mx) * unit);
 #pragma unroll
-      for (int i = 0; i < 4 * NT; i++)
-        mx = fmaxf(mx, sc[i >> 2][i & 3]);
-      if (__builtin_amdgcn_ballot_w64((mx - m) * unit > 8.f) != 0) {
-        mx = max_of_groups(mx);
-        const float alpha = __builtin_amdgcn_exp2f((m - mx) * unit);
+          for (int dt = 0; dt < NA; dt++)
+            acc[k][dt] *= alpha;
+          l[k] *= alpha;
+          m[k] = mx;
+        }
+        const float off = -m[k] * unit;
 #pragma unroll
-        for (int dt = 0; dt < NA; dt++)
-          acc[dt] *= alpha;
-        l *= alpha;
-        m = mx;
-      }
-      const float off = -m * unit;
-#pragma unroll
-      for (int i = 0; i < 4 * NT; i += 2) {
-        const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(sc[i >> 2][(i & 3) + 1], unit, off))};
-        l = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l, false);
-        pb[i >> 3][i & 7] = pr[0];
-        pb[i >> 3][(i & 7) + 1] = pr[1];
+        for (int i = 0; i < 4 * NT; i += 2) {
+          const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(sc[k][i >> 2][i & 3], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(sc[k][i >> 2][(i & 3) + 1], unit, off))};
+          l[k] = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l[k], false);
+          pb[k][i >> 3][i & 7] = pr[0];
+          pb[k][i >> 3][(i & 7) + 1] = pr[1];
+        }
       }
     }
     if (__builtin_expect(odd, 0)) { // values that are not finite: to the columns that see them, then zeros
@@ -358,16 +399,17 @@ paged_attn_kernel(const PagedAttnParams p) {
       if (busy) {
 #pragma unroll 1
         for (int key = 0; key < KEYS; key++)
-          if (seen >> key & 1)
 #pragma unroll
-            for (int dt = 0; dt < NA; dt++)
+          for (int dt = 0; dt < NA; dt++)
 #pragma unroll
-              for (int e = 0; e < 4; e++) {
-                const int ch = dt * 16 + g * 4 + e;
-                const uint32_t w = *reinterpret_cast<const uint16_t*>(vt + key * ROW + ((ch >> 3) ^ packed_v_turn(NJ, key)) * 16 + (ch & 7) * 2);
-                if ((w & 0x7f80u) == 0x7f80u)
-                  acc[dt][e] += bf16_bits_to_f32(w);
-              }
+            for (int e = 0; e < 4; e++) {
+              const int ch = dt * 16 + g * 4 + e;
+              const uint32_t w = *reinterpret_cast<const uint16_t*>(vt + key * ROW + ((ch >> 3) ^ packed_v_turn(NJ, key)) * 16 + (ch & 7) * 2);
+#pragma unroll
+              for (int k = 0; k < CG; k++)
+                if ((w & 0x7f80u) == 0x7f80u && (seen[k] >> key & 1))
+                  acc[k][dt][e] += bf16_bits_to_f32(w);
+            }
       }
       if constexpr (CW > 1)
         __syncthreads();
@@ -391,7 +433,9 @@ paged_attn_kernel(const PagedAttnParams p) {
 #pragma unroll
         for (int d = 0; d < NR; d++) {
           const i32x4 w = {vv[d][0][0], vv[d][0][1], vv[d][1][0], vv[d][1][1]};
-          acc[d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pb[u], acc[d0 + d], 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < CG; k++)
+            acc[k][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pb[k][u], acc[k][d0 + d], 0, 0, 0);
         }
       });
     }
@@ -401,58 +445,56 @@ paged_attn_kernel(const PagedAttnParams p) {
     request(top, 0);
     look_up(top - TW);
   }
+  if (parents)
+    __syncthreads();
   for (int k = 0; k < most; k += 2) {
     tile(std::integral_constant<int, 0>{}, top - k * TW, top + team - k * TW);
     if (k + 1 < most)
       tile(std::integral_constant<int, 1>{}, top - (k + 1) * TW, top + team - (k + 1) * TW);
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  m = m == LOWEST ? LOWEST : m * unit; // in powers of two
+#pragma unroll
+  for (int k = 0; k < CG; k++) {
+    l[k] += __shfl_xor(l[k], 16);
+    l[k] += __shfl_xor(l[k], 32);
+    m[k] = m[k] == LOWEST ? LOWEST : m[k] * unit; // in powers of two
+  }
 
-  float* const part_ml = p.part + (int64_t)gridDim.x * p.splits * COLS * H;
   auto store4 = [&](int cc, int ch, f32x4 v, float sum) { // (nothing seen: zeros)
     const int cl = col0 + cc, nd = cl / p.R, rr = cl - nd * p.R;
     const float inv = sum != 0.f ? 1.0f / sum : 0.f;
     *reinterpret_cast<uint2*>(p.out + ((int64_t)(o.start + nd) * p.Nq + hk * p.R + rr) * H + ch) =
         make_uint2(f32x2_to_bf16_bits(v[0] * inv, v[1] * inv), f32x2_to_bf16_bits(v[2] * inv, v[3] * inv));
   };
-  // a split's result for the merge: device-scope stores, written through to the level that all XCDs share
-  const int64_t part_at = ((int64_t)blockIdx.x * p.splits + blockIdx.y) * COLS;
-  auto leave4 = [&](int cc, int ch, f32x4 v) {
-    uint64_t* const dst = reinterpret_cast<uint64_t*>(p.part + (part_at + cc) * H + ch);
-    __hip_atomic_store(dst, __builtin_bit_cast(uint64_t, make_float2(v[0], v[1])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(dst + 1, __builtin_bit_cast(uint64_t, make_float2(v[2], v[3])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  };
-  auto leave_state = [&](int cc, float mm, float ll) {
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(part_ml + (part_at + cc) * 2), __builtin_bit_cast(uint64_t, make_float2(mm, ll)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  };
-  if constexpr (TW == 1) {
-    const int cc = wave * 16 + c;
-    if (cc < ncol) {
+  // A split's results for the merge: stores and loads at the scope of the device, written through to the level that all XCDs share.
+  constexpr int SHARED = 16; // (sc1)
+  const auto part = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)blockIdx.x * p.splits * COLS * H, 0, (int)(p.splits * COLS * H * 4), 0x00020000);
+  const auto part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)gridDim.x * p.splits * COLS * H + (int64_t)blockIdx.x * p.splits * COLS * 2, 0,
+                                                         (int)(p.splits * COLS * 8), 0x00020000);
+  if (TW == 1 && S == 1) {
 #pragma unroll
-      for (int dt = 0; dt < NA; dt++) {
-        if (S == 1)
-          store4(cc, dt * 16 + g * 4, acc[dt], l);
-        else
-          leave4(cc, dt * 16 + g * 4, acc[dt]);
-      }
-      if (S > 1 && g == 0)
-        leave_state(cc, m, l);
+    for (int k = 0; k < CG; k++) {
+      const int cc = wave * WCOLS + k * 16 + c;
+      if (cc < ncol)
+#pragma unroll
+        for (int dt = 0; dt < NA; dt++)
+          store4(cc, dt * 16 + g * 4, acc[k][dt], l[k]);
     }
   } else { // the teams' states through LDS
     constexpr int OP = H + 4;
     float* const mo = reinterpret_cast<float*>(lds); // [team][col][OP]
     float* const sm = mo + TW * COLS * OP;           // [team][col] maximum, then sum
     __syncthreads();
-    const int cc = wave * 16 + c;
 #pragma unroll
-    for (int dt = 0; dt < NA; dt++)
-      if (cc < ncol)
-        *reinterpret_cast<f32x4*>(mo + (team * COLS + cc) * OP + dt * 16 + g * 4) = acc[dt];
-    if (g == 0) {
-      sm[team * COLS + cc] = m;
-      sm[TW * COLS + team * COLS + cc] = l;
+    for (int k = 0; k < CG; k++) {
+      const int cc = wave * WCOLS + k * 16 + c;
+#pragma unroll
+      for (int dt = 0; dt < NA; dt++)
+        if (cc < ncol)
+          *reinterpret_cast<f32x4*>(mo + (team * COLS + cc) * OP + dt * 16 + g * 4) = acc[k][dt];
+      if (g == 0) {
+        sm[team * COLS + cc] = m[k];
+        sm[TW * COLS + team * COLS + cc] = l[k];
+      }
     }
     __syncthreads();
     for (int i = tid; i < ncol * (H / 4); i += TH) {
@@ -475,13 +517,20 @@ paged_attn_kernel(const PagedAttnParams p) {
       if (S == 1) {
         store4(cl, d4 * 4, v, Ls);
       } else {
-        leave4(cl, d4 * 4, v);
-        if (d4 == 0)
-          leave_state(cl, M, Ls);
+        const int at = (int)blockIdx.y * COLS + cl;
+        if (p.counters) {
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, (at * H + d4 * 4) * 4, 0, SHARED);
+          if (d4 == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, make_float2(M, Ls)), part_ml, at * 8, 0, SHARED);
+        } else {
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, (at * H + d4 * 4) * 4, 0, 0);
+          if (d4 == 0)
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, make_float2(M, Ls)), part_ml, at * 8, 0, 0);
+        }
       }
     }
   }
-  if (S == 1)
+  if (S == 1 || !p.counters)
     return;
   // The split that arrives last merges all of them, in split order (the same sums whichever that is).  Every thread waits until
   // its own stores are acknowledged, then the barrier, the arrival, and the device-scope loads; nobody waits for another workgroup.
@@ -492,54 +541,103 @@ paged_attn_kernel(const PagedAttnParams p) {
   __syncthreads();
   if (!arrived_last)
     return;
-  auto load2 = [](const float* src) {
-    return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(src), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  };
-  float* const merged = reinterpret_cast<float*>(lds); // [col][33]: weights of the splits, then the sum
-  const int64_t unit_at = (int64_t)blockIdx.x * p.splits * COLS;
-  for (int i = tid; i < ncol * 32; i += TH) { // 32 lanes per column, one split each
-    const int cc = i >> 5, s = i & 31;
-    float2 ml = {LOWEST, 0.f};
-    if (s < S)
-      ml = load2(part_ml + (unit_at + s * COLS + cc) * 2);
-    float M = ml.x;
+  // (A load at that scope takes more than a microsecond: as many under way as there are registers for.)
+  float* const merged = reinterpret_cast<float*>(lds); // [col][MAX_SPLITS + 1]: weights of the splits, then the sum
+  const int lp = S <= 2 ? 1 : 32 - __builtin_clz(S - 1), P = 1 << lp; // lanes per column
+  for (int i0 = tid; i0 < ncol << lp; i0 += 4 * TH) {
+    float2 ml[4];
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2)
-      M = fmaxf(M, __shfl_xor(M, d));
-    const float wt = __builtin_amdgcn_exp2f(ml.x - M);
-    float Ls = wt * ml.y;
+    for (int j = 0; j < 4; j++) {
+      const int i = i0 + j * TH, cc = i >> lp, s = i & (P - 1);
+      ml[j] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_ml, cc < ncol && s < S ? (s * COLS + cc) * 8 : 0x7ffffff0, 0, SHARED));
+      if (s >= S)
+        ml[j].x = LOWEST;
+    }
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2)
-      Ls += __shfl_xor(Ls, d);
-    merged[cc * 33 + s] = wt;
-    if (s == 0)
-      merged[cc * 33 + 32] = Ls;
+    for (int j = 0; j < 4; j++) {
+      const int i = i0 + j * TH, cc = i >> lp, s = i & (P - 1);
+      float M = ml[j].x;
+      for (int d = 1; d < P; d *= 2)
+        M = fmaxf(M, __shfl_xor(M, d));
+      const float wt = __builtin_amdgcn_exp2f(ml[j].x - M);
+      float Ls = wt * ml[j].y;
+      for (int d = 1; d < P; d *= 2)
+        Ls += __shfl_xor(Ls, d);
+      if (cc < ncol) {
+        merged[cc * (MAX_SPLITS + 1) + s] = wt;
+        if (s == 0)
+          merged[cc * (MAX_SPLITS + 1) + MAX_SPLITS] = Ls;
+      }
+    }
   }
   __syncthreads();
-  for (int i = tid; i < ncol * (H / 4); i += TH) {
-    const int cc = i / (H / 4), d4 = i % (H / 4);
-    const float* src = p.part + (unit_at + cc) * H + d4 * 4;
+  // 16 loads at a time: of 16 / P items of four channels, or of one item in turn
+  const int la = min(lp, 4), each = 16 >> la;
+  for (int i0 = tid; i0 < ncol * (H / 4); i0 += each * TH) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < S; s0 += 8) { // eight splits' loads in flight
-      float2 a[8][2];
+    for (int s0 = 0; s0 < S; s0 += 16) {
+      f32x4 a[16];
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const float* at = src + (int64_t)min(s0 + u, S - 1) * COLS * H;
-        a[u][0] = load2(at);
-        a[u][1] = load2(at + 2);
+      for (int j = 0; j < 16; j++) { // (past the last item or split: zeros)
+        const int i = i0 + (j >> la) * TH, s = s0 + (j & ((1 << la) - 1)), cc = i / (H / 4), d4 = i % (H / 4);
+        a[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, cc < ncol && s < S ? ((s * COLS + cc) * H + d4 * 4) * 4 : 0x7ffffff0, 0, SHARED));
       }
 #pragma unroll
-      for (int u = 0; u < 8; u++)
-        if (s0 + u < S) {
-          const float wt = merged[cc * 33 + s0 + u];
-          v[0] = fmaf(wt, a[u][0].x, v[0]);
-          v[1] = fmaf(wt, a[u][0].y, v[1]);
-          v[2] = fmaf(wt, a[u][1].x, v[2]);
-          v[3] = fmaf(wt, a[u][1].y, v[3]);
+      for (int j = 0; j < 16; j++) {
+        const int i = i0 + (j >> la) * TH, s = s0 + (j & ((1 << la) - 1)), cc = i / (H / 4), d4 = i % (H / 4);
+        if (cc < ncol && s < S) {
+          const float wt = merged[cc * (MAX_SPLITS + 1) + s];
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            v[e] = fmaf(wt, a[j][e], v[e]);
         }
+        if ((j & ((1 << la) - 1)) == (1 << la) - 1 && s0 + 16 >= S) {
+          if (cc < ncol)
+            store4(cc, d4 * 4, v, merged[cc * (MAX_SPLITS + 1) + MAX_SPLITS]);
+          v = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+      }
     }
-    store4(cc, d4 * 4, v, merged[cc * 33 + 32]);
   }
+}
+
+// The splits' results of launches with many columns: a thread takes four channels of a column, all splits.
+template <int NJ>
+__global__ void __launch_bounds__(256)
+paged_merge_kernel(const PagedAttnParams p, int cols, int keys_of_tile) {
+  constexpr int H = 32 * NJ, EACH = H / 4, PER = 256 / EACH; // threads of a column, columns of a workgroup
+  const int hk = (int)blockIdx.x % p.Nkv;
+  Block o;
+  if (!locate(p.cu, p.B, p.T, p.R, cols, (int)blockIdx.x / p.Nkv, o))
+    return;
+  const int col0 = o.at * cols, ncol = min(cols, o.n * p.R - col0);
+  const int cc = (int)blockIdx.y * PER + (int)threadIdx.x / EACH, d4 = (int)threadIdx.x % EACH;
+  const int keys = paged_keys(p, o.b, (col0 + ncol - 1) / p.R), S = paged_splits(p, (keys + keys_of_tile - 1) / keys_of_tile);
+  if (S == 1 || cc >= ncol || (int)threadIdx.x >= PER * EACH)
+    return;
+  const int64_t at = (int64_t)blockIdx.x * p.splits * cols + cc;
+  const float* const part = p.part + at * H + d4 * 4;
+  const float2* const ml = reinterpret_cast<const float2*>(p.part + (int64_t)gridDim.x * p.splits * cols * H) + at;
+  float M = LOWEST;
+#pragma unroll 8
+  for (int s = 0; s < S; s++)
+    M = fmaxf(M, ml[s * cols].x);
+  float L = 0.f;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < S; s++) {
+    const float2 z = ml[s * cols];
+    const f32x4 a = *reinterpret_cast<const f32x4*>(part + (int64_t)s * cols * H);
+    const float w = __builtin_amdgcn_exp2f(z.x - M);
+    L = fmaf(w, z.y, L);
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      v[e] = fmaf(w, a[e], v[e]);
+  }
+  const float inv = L != 0.f ? 1.0f / L : 0.f;
+  const int cl = col0 + cc, nd = cl / p.R;
+  *reinterpret_cast<uint2*>(p.out + ((int64_t)(o.start + nd) * p.Nq + hk * p.R + cl - nd * p.R) * H + d4 * 4) =
+      make_uint2(f32x2_to_bf16_bits(v[0] * inv, v[1] * inv), f32x2_to_bf16_bits(v[2] * inv, v[3] * inv));
 }
 
 // ---------------------------------------------------------------------------
@@ -600,8 +698,8 @@ static int paged_checks(const char* who, const void* table, const void* past, co
 static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_bytes, int64_t counter_bytes, hipStream_t stream) {
   hipError_t e = hipSuccess;
   int rc = TPPX_OK;
-  auto go = [&](auto nj, auto cw, auto tw, auto kt) {
-    constexpr int NJ = decltype(nj)::value, CW = decltype(cw)::value, TW = decltype(tw)::value, KEYS = decltype(kt)::value, COLS = 16 * CW;
+  auto go = [&](auto nj, auto cg, auto cw, auto tw, auto kt) {
+    constexpr int NJ = decltype(nj)::value, CG = decltype(cg)::value, CW = decltype(cw)::value, TW = decltype(tw)::value, KEYS = decltype(kt)::value, COLS = 16 * CG * CW;
     const int64_t blocks = p.cu ? ((int64_t)p.T * p.R + (int64_t)p.B * (COLS - 1)) / COLS : (int64_t)p.B * ((p.R + COLS - 1) / COLS);
     const int64_t units = blocks * p.Nkv;
     if (units >= ((int64_t)1 << 31)) {
@@ -612,47 +710,71 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     int64_t chunk = env_int("TPPX_PAGED_CHUNK", 0) / KEYS;
     if (chunk <= 0)
       chunk = std::max<int64_t>(tiles * units / 1024, 256 / KEYS);
-    chunk = std::max<int64_t>(chunk, (tiles + 31) / 32);
-    int64_t S = (tiles + chunk - 1) / chunk;
-    if (units * S * COLS * (32 * NJ + 2) * (int64_t)sizeof(float) > ws_bytes || units * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) > counter_bytes) {
-      S = 1;
-      chunk = tiles;
-    }
+    chunk = std::max<int64_t>(chunk, (tiles + MAX_SPLITS - 1) / MAX_SPLITS);
+    const int64_t room = ws_bytes / (units * COLS * (32 * NJ + 2) * (int64_t)sizeof(float));
+    chunk = room < 2 ? tiles : std::max(chunk, (tiles + room - 1) / room);
+    const int64_t S = (tiles + chunk - 1) / chunk;
     p.splits = (int)S;
     p.chunk = (int)chunk;
-    const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ, teams = TW > 1 ? TW * COLS * (32 * NJ + 6) * sizeof(float) : 0;
+    const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ, teams = TW > 1 || S > 1 ? TW * COLS * (32 * NJ + 6) * sizeof(float) : 0; // (the merge's weights take less)
     const size_t lds = std::max(stages, teams);
-    auto kern = paged_attn_kernel<NJ, CW, TW, KEYS>;
+    auto kern = paged_attn_kernel<NJ, CG, CW, TW, KEYS>;
     e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
-    if (e == hipSuccess)
-      kern<<<dim3((unsigned)units, (unsigned)S), dim3(64 * CW * TW), lds, stream>>>(p);
+    if (e != hipSuccess)
+      return;
+    const bool here = COLS == 16 && p.R <= 16 && !p.cu && S <= 16 && units * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) <= counter_bytes;
+    if (!here)
+      p.counters = nullptr;
+    kern<<<dim3((unsigned)units, (unsigned)S), dim3(64 * CW * TW), lds, stream>>>(p);
+    constexpr int PER = 256 / (8 * NJ);
+    if (S > 1 && !here)
+      paged_merge_kernel<NJ><<<dim3((unsigned)units, (COLS + PER - 1) / PER), dim3(256), 0, stream>>>(p, COLS, KEYS);
   };
   const int64_t cols = (p.cu ? (p.T + p.B - 1) / p.B : 1) * (int64_t)p.R; // of a sequence's K/V head, on average
-  constexpr std::integral_constant<int, 1> one{};
-  constexpr std::integral_constant<int, 2> two{};
-  constexpr std::integral_constant<int, 4> four{};
-  constexpr std::integral_constant<int, 8> eight{};
+  constexpr std::integral_constant<int, 1> n1{};
+  constexpr std::integral_constant<int, 2> n2{};
+  constexpr std::integral_constant<int, 4> n4{};
+  constexpr std::integral_constant<int, 8> n8{};
   constexpr std::integral_constant<int, 32> k32{};
   constexpr std::integral_constant<int, 64> k64{};
   const int form = env_int("TPPX_PAGED_FORM", 0);
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
     const int f = form ? form : cols <= 16 ? 1 : cols <= 64 ? 2 : 3;
-    if (f == 1) {
-      if constexpr (NJ > 4)
-        go(nj, one, two, k32);
+    if constexpr (NJ > 4) {
+      if (f == 1)
+        go(nj, n1, n1, n2, k32);
       else
-        go(nj, one, four, k32);
-    } else if (f == 2) {
-      if constexpr (NJ > 4)
-        go(nj, four, one, k32);
-      else
-        go(nj, four, one, k64);
+        go(nj, n1, n4, n1, k32);
     } else {
-      if constexpr (NJ > 4)
-        go(nj, four, one, k32);
+      if (f == 1)
+        go(nj, n1, n1, n4, k32);
+      else if (f == 2)
+        go(nj, n1, n4, n1, k64);
+      else if (f == 3)
+        go(nj, n1, n8, n1, k64);
+      else if (f == 4)
+        go(nj, n2, n1, n4, k32);
+      else if (f == 5)
+        go(nj, n2, n2, n2, k32);
+      else if (f == 6)
+        go(nj, n2, n2, n4, k32);
+      else if (f == 7)
+        go(nj, n2, n4, n1, k64);
+      else if (f == 8)
+        go(nj, n2, n4, n2, k32);
+      else if (f == 9)
+        go(nj, n1, n2, n4, k32);
+      else if (f == 10)
+        go(nj, n1, n4, n1, k32);
+      else if (f == 11)
+        go(nj, n1, n8, n1, k32);
+      else if (f == 12)
+        go(nj, n2, n2, n1, k32);
+      else if (f == 13)
+        go(nj, n2, n4, n1, k32);
       else
-        go(nj, eight, one, k64);
+        go(nj, n1, n4, n2, k32);
     }
   });
   if (rc)
