@@ -145,8 +145,8 @@ def test_attention_of_trees(H, Nq, Nkv, page, form, monkeypatch):
 @pytest.mark.parametrize("new,past", [([70, 1, 200], [0, 500, 33]), ([130], [1000]), ([3, 2, 2], [15, -1, 0])])
 @pytest.mark.parametrize("chunk", ["", "64"])
 def test_attention_of_pieces_of_prompts(H, Nq, Nkv, new, past, chunk, monkeypatch):
-    if chunk:  # (splits of 64 keys)
-        monkeypatch.setenv("TPPX_PAGED_CHUNK", chunk)
+    if chunk:  # (parts of 64 keys)
+        monkeypatch.setenv("TPPX_PAGED_LEAST", chunk)
     _check_attention(new, past, 32, Nq, Nkv, H, None, seed=H + len(new), spare_rows=2)
 
 

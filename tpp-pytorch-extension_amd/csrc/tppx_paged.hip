@@ -160,11 +160,13 @@ struct PagedAttnParams {
   const uint16_t *q, *layer;
   const int32_t *past, *cu, *parents;
   uint16_t* out; // [T][Nq][H]
-  float* part;   // [unit][split][cols][H], then [unit][split][cols][2]
+  float* part;   // [item][cols][H], then, behind `items` of those, [item][cols][2]
+  int items;     // at most
   unsigned int* counters;
   Pages g;
   int64_t q_ld;
-  int T, B, Nq, Nkv, R, splits, chunk; // chunk: tiles of a split
+  int T, B, Nq, Nkv, R;
+  int target, least; // items of a launch (0: units are not split), tiles of one at least
   float scale;
 };
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
@@ -172,14 +174,101 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t* ConstantInts; // (scalar loads)
 
 constexpr int MAX_SPLITS = 64;
-// keys that nodes 0 .. last of sequence b see, of which the last sees most; splits of so many tiles
+constexpr int PAGED_NODES = 256;
+
+// The work of a launch, laid out on the device, where the lengths are: an item is a part of a unit's keys, a unit a block of a sequence's
+// columns for one K/V head.  The parts are of so many tiles that there are about `target` items in all, so that long sequences are split
+// where short ones are not.  Items of a sequence: [split][block][K/V head]; its first one, and its first unit, behind those of the
+// sequences before it.
+struct Item {
+  Block o;           // sequence, its first row and nodes, block
+  int hk, split, S;  // of S splits
+  int first, stride; // item of the unit's first split, from one split's to the next one's
+};
+// keys that the nodes of sequence b up to `last` see, of which that one sees most
 __device__ __forceinline__ int paged_past(const PagedAttnParams& p, int b) { return min(p.past[b], (int)(p.g.table_ld << p.g.shift)); }
-__device__ __forceinline__ int paged_keys(const PagedAttnParams& p, int b, int last) {
-  const int past = paged_past(p, b);
+__device__ __forceinline__ int paged_keys(const PagedAttnParams& p, int past, int last) {
   return past < 0 ? 0 : (int)min((int64_t)past + last + 1, p.g.table_ld << p.g.shift);
 }
-__device__ __forceinline__ int paged_splits(const PagedAttnParams& p, int tiles) { return max((tiles + p.chunk - 1) / p.chunk, 1); }
-constexpr int PAGED_NODES = 256;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int from_lane(int v) { // (0 where there is no such lane)
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, ROWS == 0xf);
+}
+// sum over the lanes below, and this one's; all lanes take part
+__device__ __forceinline__ int scan_wave(int v) {
+  v += from_lane<0x111, 0xf>(v); // row_shr:1
+  v += from_lane<0x112, 0xf>(v);
+  v += from_lane<0x114, 0xf>(v);
+  v += from_lane<0x118, 0xf>(v);
+  v += from_lane<0x142, 0xa>(v); // row_bcast:15 into the second and the last row
+  v += from_lane<0x143, 0xc>(v); // row_bcast:31 into the upper rows
+  return v;
+}
+__device__ __forceinline__ int sum_of_wave(int v) { return __builtin_amdgcn_readlane(scan_wave(v), 63); }
+// Item blockIdx.x (units: unit blockIdx.x, its split 0); false past the last one.  All lanes of a wave take part.
+template <int COLS, int KEYS>
+__device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, bool units, Item& it) {
+  const int lane = threadIdx.x & 63;
+  it.hk = id % p.Nkv;
+  id /= p.Nkv;
+  struct Seq {
+    int s, n, blocks, tiles;
+  };
+  auto seq = [&](int b) {
+    Seq q = {0, 0, 0, 0};
+    if (b < p.B) {
+      const int s = p.cu ? min(max(p.cu[b], 0), p.T) : b, e = p.cu ? min(max(p.cu[b + 1], 0), p.T) : b + 1;
+      q.s = s;
+      q.n = max(e - s, 0);
+      q.blocks = (int)(((int64_t)q.n * p.R + COLS - 1) / COLS);
+      q.tiles = q.n ? (paged_keys(p, paged_past(p, b), q.n - 1) + KEYS - 1) / KEYS : 0;
+    }
+    return q;
+  };
+  Seq q = seq(lane);
+  int chunk = 1 << 30;
+  if (p.target > 0) {
+    int blocks = 0;
+    float tiles = 0.f; // of all units
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+      const Seq z = b0 ? seq(b0 + lane) : q;
+      blocks += sum_of_wave(z.blocks);
+      tiles += wave_sum((float)z.blocks * (float)z.tiles);
+    }
+    const int room = p.target / p.Nkv; // items of a K/V head
+    if (p.B <= 64) { // the smallest parts that are no more items
+      chunk = max(p.least, (int)(tiles / (float)room));
+      while (__builtin_amdgcn_ballot_w64(q.tiles > chunk) != 0 && sum_of_wave(q.blocks * max((q.tiles + chunk - 1) / chunk, 1)) > room)
+        chunk += chunk / 8 + 1;
+    } else if (room > blocks) { // (no more than tiles / chunk and one for each block; the sum is within 1 % of the true one)
+      chunk = max(p.least, (int)(tiles * 1.01f / (float)(room - blocks)) + 1);
+    }
+  }
+  int before = 0, items_before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    if (b0)
+      q = seq(b0 + lane);
+    const int S = min(max((q.tiles + chunk - 1) / chunk, 1), MAX_SPLITS), items = q.blocks * S, c = units ? q.blocks : items;
+    const int sum = scan_wave(c), all = units ? scan_wave(items) : sum;
+    const int total = __builtin_amdgcn_readlane(sum, 63);
+    if (id < before + total) {
+      const int j = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + sum > id));
+      const int blocks = __builtin_amdgcn_readlane(q.blocks, j), in = id - before - (__builtin_amdgcn_readlane(sum, j) - __builtin_amdgcn_readlane(c, j));
+      it.o.b = b0 + j;
+      it.o.start = __builtin_amdgcn_readlane(q.s, j);
+      it.o.n = __builtin_amdgcn_readlane(q.n, j);
+      it.S = __builtin_amdgcn_readlane(S, j);
+      it.split = in / blocks;
+      it.o.at = in - it.split * blocks;
+      it.first = (items_before + __builtin_amdgcn_readlane(all, j) - __builtin_amdgcn_readlane(items, j) + it.o.at) * p.Nkv + it.hk;
+      it.stride = blocks * p.Nkv;
+      return true;
+    }
+    before += total;
+    items_before += __builtin_amdgcn_readlane(all, 63);
+  }
+  return false;
+}
 
 template <int NJ, int CG, int CW, int TW, int KEYS>
 __global__ void __launch_bounds__(64 * CW * TW, CG == 1 && CW == 8 ? 4 : CW > 1 ? 2 : 1)
@@ -194,16 +283,13 @@ paged_attn_kernel(const PagedAttnParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % CW, team = __builtin_amdgcn_readfirstlane(tid >> 6) / CW;
   const int g = lane >> 4, c = lane & 15;
-  const int hk = (int)blockIdx.x % p.Nkv;
-  Block o;
-  if (!locate(p.cu, p.B, p.T, p.R, COLS, (int)blockIdx.x / p.Nkv, o))
+  Item it;
+  if (!locate_item<COLS, KEYS>(p, (int)blockIdx.x, false, it))
     return;
-  const int ncol = min(COLS, o.n * p.R - o.at * COLS); // of this workgroup
-  const int col0 = o.at * COLS;
-  const int past = paged_past(p, o.b), keys = paged_keys(p, o.b, (col0 + ncol - 1) / p.R); // that some column sees
-  const int tiles = (keys + KEYS - 1) / KEYS, S = paged_splits(p, tiles); // splits that have tiles; the others take no part
-  if ((int)blockIdx.y >= S)
-    return;
+  const Block& o = it.o;
+  const int hk = it.hk, col0 = o.at * COLS, ncol = min(COLS, o.n * p.R - col0); // of this workgroup
+  const int past = paged_past(p, o.b), keys = paged_keys(p, past, (col0 + ncol - 1) / p.R); // that some column sees
+  const int tiles = (keys + KEYS - 1) / KEYS, S = it.S;
   const bool idle = wave * WCOLS >= ncol;
   const int32_t* const parents = p.parents ? p.parents + o.start : nullptr;
   int node[CG], up[CG]; // of this lane's columns; where their ways up have come to
@@ -218,7 +304,7 @@ paged_attn_kernel(const PagedAttnParams p) {
       q[k][j] = *reinterpret_cast<const bf16x8*>(qrow + j * 32);
   }
   // Tiles top, top - TW, .. of this team, down to the split's last one.
-  const int low = (S - 1 - (int)blockIdx.y) * tiles / S, top = (S - (int)blockIdx.y) * tiles / S - 1 - team, most = (top + team - low) / TW + 1;
+  const int low = (int)((int64_t)(S - 1 - it.split) * tiles / S), top = (int)((int64_t)(S - it.split) * tiles / S) - 1 - team, most = (top + team - low) / TW + 1;
   const ConstantInts table = (ConstantInts)(uintptr_t)(p.g.table + (int64_t)o.b * p.g.table_ld);
   const int64_t values = (((int64_t)p.g.pages * p.Nkv) << p.g.shift) * H;
   int ids[MINE]; // pages of this wave's runs of the tile that is asked for next
@@ -467,9 +553,8 @@ paged_attn_kernel(const PagedAttnParams p) {
   };
   // A split's results for the merge: stores and loads at the scope of the device, written through to the level that all XCDs share.
   constexpr int SHARED = 16; // (sc1)
-  const auto part = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)blockIdx.x * p.splits * COLS * H, 0, (int)(p.splits * COLS * H * 4), 0x00020000);
-  const auto part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)gridDim.x * p.splits * COLS * H + (int64_t)blockIdx.x * p.splits * COLS * 2, 0,
-                                                         (int)(p.splits * COLS * 8), 0x00020000);
+  const auto part = __builtin_amdgcn_make_buffer_rsrc(p.part, 0, p.items * (COLS * H * 4), 0x00020000);
+  const auto part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)p.items * COLS * H, 0, p.items * (COLS * 8), 0x00020000);
   if (TW == 1 && S == 1) {
 #pragma unroll
     for (int k = 0; k < CG; k++) {
@@ -517,7 +602,7 @@ paged_attn_kernel(const PagedAttnParams p) {
       if (S == 1) {
         store4(cl, d4 * 4, v, Ls);
       } else {
-        const int at = (int)blockIdx.y * COLS + cl;
+        const int at = (int)blockIdx.x * COLS + cl;
         if (p.counters) {
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, (at * H + d4 * 4) * 4, 0, SHARED);
           if (d4 == 0)
@@ -537,7 +622,7 @@ paged_attn_kernel(const PagedAttnParams p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0)
-    arrived_last = atomicInc(p.counters + (int64_t)blockIdx.x * MX4_COUNTER_STRIDE, (unsigned)S - 1) == (unsigned)S - 1;
+    arrived_last = atomicInc(p.counters + (int64_t)it.first * MX4_COUNTER_STRIDE, (unsigned)S - 1) == (unsigned)S - 1;
   __syncthreads();
   if (!arrived_last)
     return;
@@ -549,7 +634,7 @@ paged_attn_kernel(const PagedAttnParams p) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int i = i0 + j * TH, cc = i >> lp, s = i & (P - 1);
-      ml[j] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_ml, cc < ncol && s < S ? (s * COLS + cc) * 8 : 0x7ffffff0, 0, SHARED));
+      ml[j] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_ml, cc < ncol && s < S ? ((it.first + s * it.stride) * COLS + cc) * 8 : 0x7ffffff0, 0, SHARED));
       if (s >= S)
         ml[j].x = LOWEST;
     }
@@ -580,7 +665,7 @@ paged_attn_kernel(const PagedAttnParams p) {
 #pragma unroll
       for (int j = 0; j < 16; j++) { // (past the last item or split: zeros)
         const int i = i0 + (j >> la) * TH, s = s0 + (j & ((1 << la) - 1)), cc = i / (H / 4), d4 = i % (H / 4);
-        a[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, cc < ncol && s < S ? ((s * COLS + cc) * H + d4 * 4) * 4 : 0x7ffffff0, 0, SHARED));
+        a[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, cc < ncol && s < S ? (((it.first + s * it.stride) * COLS + cc) * H + d4 * 4) * 4 : 0x7ffffff0, 0, SHARED));
       }
 #pragma unroll
       for (int j = 0; j < 16; j++) {
@@ -602,32 +687,30 @@ paged_attn_kernel(const PagedAttnParams p) {
 }
 
 // The splits' results of launches with many columns: a thread takes four channels of a column, all splits.
-template <int NJ>
+template <int NJ, int COLS, int KEYS>
 __global__ void __launch_bounds__(256)
-paged_merge_kernel(const PagedAttnParams p, int cols, int keys_of_tile) {
+paged_merge_kernel(const PagedAttnParams p) {
   constexpr int H = 32 * NJ, EACH = H / 4, PER = 256 / EACH; // threads of a column, columns of a workgroup
-  const int hk = (int)blockIdx.x % p.Nkv;
-  Block o;
-  if (!locate(p.cu, p.B, p.T, p.R, cols, (int)blockIdx.x / p.Nkv, o))
+  Item it;
+  if (!locate_item<COLS, KEYS>(p, (int)blockIdx.x, true, it) || it.S == 1)
     return;
-  const int col0 = o.at * cols, ncol = min(cols, o.n * p.R - col0);
+  const int S = it.S, col0 = it.o.at * COLS, ncol = min(COLS, it.o.n * p.R - col0);
   const int cc = (int)blockIdx.y * PER + (int)threadIdx.x / EACH, d4 = (int)threadIdx.x % EACH;
-  const int keys = paged_keys(p, o.b, (col0 + ncol - 1) / p.R), S = paged_splits(p, (keys + keys_of_tile - 1) / keys_of_tile);
-  if (S == 1 || cc >= ncol || (int)threadIdx.x >= PER * EACH)
+  if (cc >= ncol || (int)threadIdx.x >= PER * EACH)
     return;
-  const int64_t at = (int64_t)blockIdx.x * p.splits * cols + cc;
+  const int64_t at = (int64_t)it.first * COLS + cc, step = (int64_t)it.stride * COLS;
   const float* const part = p.part + at * H + d4 * 4;
-  const float2* const ml = reinterpret_cast<const float2*>(p.part + (int64_t)gridDim.x * p.splits * cols * H) + at;
+  const float2* const ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.items * COLS * H) + at;
   float M = LOWEST;
 #pragma unroll 8
   for (int s = 0; s < S; s++)
-    M = fmaxf(M, ml[s * cols].x);
+    M = fmaxf(M, ml[s * step].x);
   float L = 0.f;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int s = 0; s < S; s++) {
-    const float2 z = ml[s * cols];
-    const f32x4 a = *reinterpret_cast<const f32x4*>(part + (int64_t)s * cols * H);
+    const float2 z = ml[s * step];
+    const f32x4 a = *reinterpret_cast<const f32x4*>(part + s * step * H);
     const float w = __builtin_amdgcn_exp2f(z.x - M);
     L = fmaf(w, z.y, L);
 #pragma unroll
@@ -636,7 +719,7 @@ paged_merge_kernel(const PagedAttnParams p, int cols, int keys_of_tile) {
   }
   const float inv = L != 0.f ? 1.0f / L : 0.f;
   const int cl = col0 + cc, nd = cl / p.R;
-  *reinterpret_cast<uint2*>(p.out + ((int64_t)(o.start + nd) * p.Nq + hk * p.R + cl - nd * p.R) * H + d4 * 4) =
+  *reinterpret_cast<uint2*>(p.out + ((int64_t)(it.o.start + nd) * p.Nq + it.hk * p.R + cl - nd * p.R) * H + d4 * 4) =
       make_uint2(f32x2_to_bf16_bits(v[0] * inv, v[1] * inv), f32x2_to_bf16_bits(v[2] * inv, v[3] * inv));
 }
 
@@ -706,29 +789,30 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
       rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
       return;
     }
-    const int64_t tiles = ((p.g.table_ld << p.g.shift) + KEYS - 1) / KEYS;
-    int64_t chunk = env_int("TPPX_PAGED_CHUNK", 0) / KEYS;
-    if (chunk <= 0)
-      chunk = std::max<int64_t>(tiles * units / 1024, 256 / KEYS);
-    chunk = std::max<int64_t>(chunk, (tiles + MAX_SPLITS - 1) / MAX_SPLITS);
-    const int64_t room = ws_bytes / (units * COLS * (32 * NJ + 2) * (int64_t)sizeof(float));
-    chunk = room < 2 ? tiles : std::max(chunk, (tiles + room - 1) / room);
-    const int64_t S = (tiles + chunk - 1) / chunk;
-    p.splits = (int)S;
-    p.chunk = (int)chunk;
-    const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ, teams = TW > 1 || S > 1 ? TW * COLS * (32 * NJ + 6) * sizeof(float) : 0; // (the merge's weights take less)
+    // items: some more than `target`, as the last part of every unit is one of its own
+    const int64_t room = std::min<int64_t>(ws_bytes / (COLS * (32 * NJ + 2) * (int64_t)sizeof(float)), (((int64_t)1 << 31) - 1) / (COLS * 32 * NJ * 4));
+    int64_t target = env_int("TPPX_PAGED_ITEMS", 0);
+    if (target <= 0)
+      target = COLS <= 32 ? std::max<int64_t>(1024, 2 * units) : 512;
+    target = std::min<int64_t>(std::min<int64_t>(target, room), p.B <= 64 ? room : room - units);
+    if (target < units + p.Nkv)
+      target = 0;
+    p.target = (int)target;
+    p.least = std::max(env_int("TPPX_PAGED_LEAST", 256) / KEYS, 1);
+    p.items = (int)std::max<int64_t>(target, units);
+    const bool here = COLS == 16 && p.R <= 16 && !p.cu && p.items * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) <= counter_bytes;
+    if (!here)
+      p.counters = nullptr;
+    const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ, teams = TW > 1 || target ? TW * COLS * (32 * NJ + 6) * sizeof(float) : 0; // (the merge's weights take less)
     const size_t lds = std::max(stages, teams);
     auto kern = paged_attn_kernel<NJ, CG, CW, TW, KEYS>;
     e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
     if (e != hipSuccess)
       return;
-    const bool here = COLS == 16 && p.R <= 16 && !p.cu && S <= 16 && units * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) <= counter_bytes;
-    if (!here)
-      p.counters = nullptr;
-    kern<<<dim3((unsigned)units, (unsigned)S), dim3(64 * CW * TW), lds, stream>>>(p);
+    kern<<<dim3((unsigned)p.items), dim3(64 * CW * TW), lds, stream>>>(p);
     constexpr int PER = 256 / (8 * NJ);
-    if (S > 1 && !here)
-      paged_merge_kernel<NJ><<<dim3((unsigned)units, (COLS + PER - 1) / PER), dim3(256), 0, stream>>>(p, COLS, KEYS);
+    if (target && !here)
+      paged_merge_kernel<NJ, COLS, KEYS><<<dim3((unsigned)units, (COLS + PER - 1) / PER), dim3(256), 0, stream>>>(p);
   };
   const int64_t cols = (p.cu ? (p.T + p.B - 1) / p.B : 1) * (int64_t)p.R; // of a sequence's K/V head, on average
   constexpr std::integral_constant<int, 1> n1{};
