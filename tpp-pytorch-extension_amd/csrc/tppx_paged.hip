@@ -626,63 +626,48 @@ paged_attn_kernel(const PagedAttnParams p) {
   __syncthreads();
   if (!arrived_last)
     return;
-  // (A load at that scope takes more than a microsecond: as many under way as there are registers for.)
+  // A load at that scope takes more than a microsecond: those of the first eight parts are under way while the weights are found.
+  const int lane_ = tid & 63, wave_ = tid >> 6;
+  f32x4 a[8];
+  auto fetch = [&](int i, int s0) {
+    const int cc = i / (H / 4), d4 = i % (H / 4);
+#pragma unroll
+    for (int u = 0; u < 8; u++) // (past the last one: that again)
+      a[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, ((it.first + min(s0 + u, S - 1) * it.stride) * COLS + cc) * (H * 4) + d4 * 16, 0, SHARED));
+  };
+  if (tid < ncol * (H / 4))
+    fetch(tid, 0);
   float* const merged = reinterpret_cast<float*>(lds); // [col][MAX_SPLITS + 1]: weights of the splits, then the sum
-  const int lp = S <= 2 ? 1 : 32 - __builtin_clz(S - 1), P = 1 << lp; // lanes per column
-  for (int i0 = tid; i0 < ncol << lp; i0 += 4 * TH) {
-    float2 ml[4];
+  for (int cc = wave_; cc < ncol; cc += TH / 64) { // a lane per split
+    float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_ml, ((it.first + min(lane_, S - 1) * it.stride) * COLS + cc) * 8, 0, SHARED));
+    if (lane_ >= S)
+      ml = float2{LOWEST, 0.f};
+    float M = ml.x;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int i = i0 + j * TH, cc = i >> lp, s = i & (P - 1);
-      ml[j] = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_ml, cc < ncol && s < S ? ((it.first + s * it.stride) * COLS + cc) * 8 : 0x7ffffff0, 0, SHARED));
-      if (s >= S)
-        ml[j].x = LOWEST;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const int i = i0 + j * TH, cc = i >> lp, s = i & (P - 1);
-      float M = ml[j].x;
-      for (int d = 1; d < P; d *= 2)
-        M = fmaxf(M, __shfl_xor(M, d));
-      const float wt = __builtin_amdgcn_exp2f(ml[j].x - M);
-      float Ls = wt * ml[j].y;
-      for (int d = 1; d < P; d *= 2)
-        Ls += __shfl_xor(Ls, d);
-      if (cc < ncol) {
-        merged[cc * (MAX_SPLITS + 1) + s] = wt;
-        if (s == 0)
-          merged[cc * (MAX_SPLITS + 1) + MAX_SPLITS] = Ls;
-      }
-    }
+    for (int d = 1; d < 64; d *= 2)
+      M = fmaxf(M, __shfl_xor(M, d));
+    const float wt = __builtin_amdgcn_exp2f(ml.x - M), Ls = wave_sum(wt * ml.y);
+    merged[cc * (MAX_SPLITS + 1) + lane_] = wt;
+    if (lane_ == 0)
+      merged[cc * (MAX_SPLITS + 1) + MAX_SPLITS] = Ls;
   }
   __syncthreads();
-  // 16 loads at a time: of 16 / P items of four channels, or of one item in turn
-  const int la = min(lp, 4), each = 16 >> la;
-  for (int i0 = tid; i0 < ncol * (H / 4); i0 += each * TH) {
+  for (int i = tid; i < ncol * (H / 4); i += TH) {
+    const int cc = i / (H / 4), d4 = i % (H / 4);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s0 = 0; s0 < S; s0 += 16) {
-      f32x4 a[16];
+    for (int s0 = 0; s0 < S; s0 += 8) {
+      if (i != tid || s0)
+        fetch(i, s0);
 #pragma unroll
-      for (int j = 0; j < 16; j++) { // (past the last item or split: zeros)
-        const int i = i0 + (j >> la) * TH, s = s0 + (j & ((1 << la) - 1)), cc = i / (H / 4), d4 = i % (H / 4);
-        a[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, cc < ncol && s < S ? (((it.first + s * it.stride) * COLS + cc) * H + d4 * 4) * 4 : 0x7ffffff0, 0, SHARED));
-      }
-#pragma unroll
-      for (int j = 0; j < 16; j++) {
-        const int i = i0 + (j >> la) * TH, s = s0 + (j & ((1 << la) - 1)), cc = i / (H / 4), d4 = i % (H / 4);
-        if (cc < ncol && s < S) {
-          const float wt = merged[cc * (MAX_SPLITS + 1) + s];
+      for (int u = 0; u < 8; u++)
+        if (s0 + u < S) {
+          const float wt = merged[cc * (MAX_SPLITS + 1) + s0 + u];
 #pragma unroll
           for (int e = 0; e < 4; e++)
-            v[e] = fmaf(wt, a[j][e], v[e]);
+            v[e] = fmaf(wt, a[u][e], v[e]);
         }
-        if ((j & ((1 << la) - 1)) == (1 << la) - 1 && s0 + 16 >= S) {
-          if (cc < ncol)
-            store4(cc, d4 * 4, v, merged[cc * (MAX_SPLITS + 1) + MAX_SPLITS]);
-          v = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-      }
     }
+    store4(cc, d4 * 4, v, merged[cc * (MAX_SPLITS + 1) + MAX_SPLITS]);
   }
 }
 
@@ -695,32 +680,34 @@ paged_merge_kernel(const PagedAttnParams p) {
   if (!locate_item<COLS, KEYS>(p, (int)blockIdx.x, true, it) || it.S == 1)
     return;
   const int S = it.S, col0 = it.o.at * COLS, ncol = min(COLS, it.o.n * p.R - col0);
-  const int cc = (int)blockIdx.y * PER + (int)threadIdx.x / EACH, d4 = (int)threadIdx.x % EACH;
-  if (cc >= ncol || (int)threadIdx.x >= PER * EACH)
+  const int d4 = (int)threadIdx.x % EACH;
+  if ((int)threadIdx.x >= PER * EACH)
     return;
-  const int64_t at = (int64_t)it.first * COLS + cc, step = (int64_t)it.stride * COLS;
-  const float* const part = p.part + at * H + d4 * 4;
-  const float2* const ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.items * COLS * H) + at;
-  float M = LOWEST;
+  for (int cc = (int)blockIdx.y * PER + (int)threadIdx.x / EACH; cc < ncol; cc += (int)gridDim.y * PER) {
+    const int64_t at = (int64_t)it.first * COLS + cc, step = (int64_t)it.stride * COLS;
+    const float* const part = p.part + at * H + d4 * 4;
+    const float2* const ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.items * COLS * H) + at;
+    float M = LOWEST;
 #pragma unroll 8
-  for (int s = 0; s < S; s++)
-    M = fmaxf(M, ml[s * step].x);
-  float L = 0.f;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < S; s++)
+      M = fmaxf(M, ml[s * step].x);
+    float L = 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int s = 0; s < S; s++) {
-    const float2 z = ml[s * step];
-    const f32x4 a = *reinterpret_cast<const f32x4*>(part + s * step * H);
-    const float w = __builtin_amdgcn_exp2f(z.x - M);
-    L = fmaf(w, z.y, L);
+    for (int s = 0; s < S; s++) {
+      const float2 z = ml[s * step];
+      const f32x4 a = *reinterpret_cast<const f32x4*>(part + s * step * H);
+      const float w = __builtin_amdgcn_exp2f(z.x - M);
+      L = fmaf(w, z.y, L);
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-      v[e] = fmaf(w, a[e], v[e]);
+      for (int e = 0; e < 4; e++)
+        v[e] = fmaf(w, a[e], v[e]);
+    }
+    const float inv = L != 0.f ? 1.0f / L : 0.f;
+    const int cl = col0 + cc, nd = cl / p.R;
+    *reinterpret_cast<uint2*>(p.out + ((int64_t)(it.o.start + nd) * p.Nq + it.hk * p.R + cl - nd * p.R) * H + d4 * 4) =
+        make_uint2(f32x2_to_bf16_bits(v[0] * inv, v[1] * inv), f32x2_to_bf16_bits(v[2] * inv, v[3] * inv));
   }
-  const float inv = L != 0.f ? 1.0f / L : 0.f;
-  const int cl = col0 + cc, nd = cl / p.R;
-  *reinterpret_cast<uint2*>(p.out + ((int64_t)(it.o.start + nd) * p.Nq + it.hk * p.R + cl - nd * p.R) * H + d4 * 4) =
-      make_uint2(f32x2_to_bf16_bits(v[0] * inv, v[1] * inv), f32x2_to_bf16_bits(v[2] * inv, v[3] * inv));
 }
 
 // ---------------------------------------------------------------------------
@@ -793,9 +780,10 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     const int64_t room = std::min<int64_t>(ws_bytes / (COLS * (32 * NJ + 2) * (int64_t)sizeof(float)), (((int64_t)1 << 31) - 1) / (COLS * 32 * NJ * 4));
     int64_t target = env_int("TPPX_PAGED_ITEMS", 0);
     if (target <= 0)
-      target = COLS <= 32 ? std::max<int64_t>(1024, 2 * units) : 512;
+      target = COLS == 16 ? std::max<int64_t>(1024, 2 * units) : TW == 1 ? 512 : 256;
     target = std::min<int64_t>(std::min<int64_t>(target, room), p.B <= 64 ? room : room - units);
-    if (target < units + p.Nkv)
+    // A few pages hold no more than a part would: not worth the look at the lengths and the merge.
+    if (target < units + p.Nkv || (p.g.table_ld << p.g.shift) <= 384)
       target = 0;
     p.target = (int)target;
     p.least = std::max(env_int("TPPX_PAGED_LEAST", 256) / KEYS, 1);
@@ -811,54 +799,39 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
       return;
     kern<<<dim3((unsigned)p.items), dim3(64 * CW * TW), lds, stream>>>(p);
     constexpr int PER = 256 / (8 * NJ);
-    if (target && !here)
-      paged_merge_kernel<NJ, COLS, KEYS><<<dim3((unsigned)units, (COLS + PER - 1) / PER), dim3(256), 0, stream>>>(p);
+    if (target && !here) // (units that were not split end at once: not too many of those)
+      paged_merge_kernel<NJ, COLS, KEYS><<<dim3((unsigned)units, (unsigned)std::min<int64_t>((COLS + PER - 1) / PER, std::max<int64_t>(2048 / units, 1))), dim3(256), 0, stream>>>(p);
   };
   const int64_t cols = (p.cu ? (p.T + p.B - 1) / p.B : 1) * (int64_t)p.R; // of a sequence's K/V head, on average
+  // units of c columns, about: pieces of prompts as if they were equally long, the last block of a tree half empty
+  auto units_of = [&](int64_t c) { return (p.parents ? ((int64_t)p.T * p.R + (int64_t)p.B * (c / 2)) / c : (cols + c - 1) / c * (int64_t)p.B) * p.Nkv; };
   constexpr std::integral_constant<int, 1> n1{};
   constexpr std::integral_constant<int, 2> n2{};
   constexpr std::integral_constant<int, 4> n4{};
-  constexpr std::integral_constant<int, 8> n8{};
   constexpr std::integral_constant<int, 32> k32{};
   constexpr std::integral_constant<int, 64> k64{};
   const int form = env_int("TPPX_PAGED_FORM", 0);
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
-    const int f = form ? form : cols <= 16 ? 1 : cols <= 64 ? 2 : 3;
+    const int f = form ? form : cols <= 16 ? 1 : cols <= 32 ? 2 : units_of(64) <= 280 ? 3 : cols >= 512 && units_of(128) <= 280 ? 5 : 4;
     if constexpr (NJ > 4) {
-      if (f == 1)
+      if (f == 1 || f == 2)
         go(nj, n1, n1, n2, k32);
+      else if (f == 3)
+        go(nj, n1, n4, n2, k32);
       else
         go(nj, n1, n4, n1, k32);
     } else {
       if (f == 1)
         go(nj, n1, n1, n4, k32);
       else if (f == 2)
-        go(nj, n1, n4, n1, k64);
-      else if (f == 3)
-        go(nj, n1, n8, n1, k64);
-      else if (f == 4)
         go(nj, n2, n1, n4, k32);
-      else if (f == 5)
-        go(nj, n2, n2, n2, k32);
-      else if (f == 6)
+      else if (f == 3)
         go(nj, n2, n2, n4, k32);
-      else if (f == 7)
+      else if (f == 4)
         go(nj, n2, n4, n1, k64);
-      else if (f == 8)
-        go(nj, n2, n4, n2, k32);
-      else if (f == 9)
-        go(nj, n1, n2, n4, k32);
-      else if (f == 10)
-        go(nj, n1, n4, n1, k32);
-      else if (f == 11)
-        go(nj, n1, n8, n1, k32);
-      else if (f == 12)
-        go(nj, n2, n2, n1, k32);
-      else if (f == 13)
-        go(nj, n2, n4, n1, k32);
       else
-        go(nj, n1, n4, n2, k32);
+        go(nj, n2, n4, n2, k32);
     }
   });
   if (rc)
