@@ -687,21 +687,33 @@ paged_merge_kernel(const PagedAttnParams p) {
     const int64_t at = (int64_t)it.first * COLS + cc, step = (int64_t)it.stride * COLS;
     const float* const part = p.part + at * H + d4 * 4;
     const float2* const ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.items * COLS * H) + at;
-    float M = LOWEST;
-#pragma unroll 8
-    for (int s = 0; s < S; s++)
-      M = fmaxf(M, ml[s * step].x);
-    float L = 0.f;
+    float M = LOWEST, L = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int s = 0; s < S; s++) {
-      const float2 z = ml[s * step];
-      const f32x4 a = *reinterpret_cast<const f32x4*>(part + s * step * H);
-      const float w = __builtin_amdgcn_exp2f(z.x - M);
-      L = fmaf(w, z.y, L);
+    for (int s0 = 0; s0 < S; s0 += 8) { // eight parts' loads at a time
+      float2 z[8];
+      f32x4 a[8];
 #pragma unroll
-      for (int e = 0; e < 4; e++)
-        v[e] = fmaf(w, a[e], v[e]);
+      for (int u = 0; u < 8; u++) {
+        const int64_t i = min(s0 + u, S - 1) * step;
+        z[u] = ml[i];
+        a[u] = *reinterpret_cast<const f32x4*>(part + i * H);
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        top = fmaxf(top, z[u].x);
+      const float alpha = __builtin_amdgcn_exp2f(M - top);
+      M = top;
+      L *= alpha;
+      v *= alpha;
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const float w = s0 + u < S ? __builtin_amdgcn_exp2f(z[u].x - M) : 0.f;
+        L = fmaf(w, z[u].y, L);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          v[e] = s0 + u < S ? fmaf(w, a[u][e], v[e]) : v[e];
+      }
     }
     const float inv = L != 0.f ? 1.0f / L : 0.f;
     const int cl = col0 + cc, nd = cl / p.R;
@@ -800,7 +812,7 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     kern<<<dim3((unsigned)p.items), dim3(64 * CW * TW), lds, stream>>>(p);
     constexpr int PER = 256 / (8 * NJ);
     if (target && !here) // (units that were not split end at once: not too many of those)
-      paged_merge_kernel<NJ, COLS, KEYS><<<dim3((unsigned)units, (unsigned)std::min<int64_t>((COLS + PER - 1) / PER, std::max<int64_t>(2048 / units, 1))), dim3(256), 0, stream>>>(p);
+      paged_merge_kernel<NJ, COLS, KEYS><<<dim3((unsigned)units, (unsigned)std::min<int64_t>((COLS + PER - 1) / PER, std::max<int64_t>(4096 / units, 1))), dim3(256), 0, stream>>>(p);
   };
   const int64_t cols = (p.cu ? (p.T + p.B - 1) / p.B : 1) * (int64_t)p.R; // of a sequence's K/V head, on average
   // units of c columns, about: pieces of prompts as if they were equally long, the last block of a tree half empty
