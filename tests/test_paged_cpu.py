@@ -94,3 +94,61 @@ def test_plain_forms():
     assert R.verify(one, None, half, drawn, [0.0, 0.4], 0.8, 0.0) == ([0], 0)
     assert R.verify([0, 0], None, half, None, None, None, 0.0) == ([0, 1], 1)
     assert R.verify([0, 1, 2], [-1, 0, 0], half[[0, 1, 1]], None, [0.0, 0.3, 0.3], 0.1, 1.0) == ([0, 2], 0)  # 0.3 * 0.75 < 0.25
+
+
+def test_lookup_drafts():
+    from tpp_pytorch_extension.llm.paged_cache import lookup_drafts
+    assert lookup_drafts([1, 2, 3, 4, 1, 2, 3]) == ([4, 1, 2, 3], [-1, 0, 1, 2])
+    assert lookup_drafts([7, 1, 2, 9, 8, 7, 5, 1, 2], most=2) == ([9, 8], [-1, 0])
+    assert lookup_drafts([1]) == lookup_drafts([5, 6, 7]) == lookup_drafts([]) == ([], [])
+
+
+def test_pages_of_a_cache():
+    """What a PagedCache keeps on the host: pages taken and given back, lengths, announced passes, refusals that change nothing."""
+    _lib, _, at = _mods()
+    cache = at.PagedCache(100, 2, page=16, pages=10)
+    assert cache.get_capacity() == 112 and cache.get_seq_length() == 0 and cache.room_for(112) and not cache.room_for(113)
+    bounds = cache.nodes([20, 0, 33], device="cpu")
+    assert bounds.tolist() == [0, 20, 20, 53] and cache.next_positions(53, "cpu")[0].tolist() == list(range(20)) + list(range(33))
+    assert (cache.table >= 0).sum(1).tolist() == [2, 0, 3] and len(set(cache.table[cache.table >= 0].tolist())) == 5
+    assert cache.room_for(53)
+
+    def refuses(call, code=_lib.ESHAPE):
+        before = (list(cache.lengths), cache.table.clone(), len(cache._free))
+        with pytest.raises(_lib.TppxError) as e:
+            call()
+        assert e.value.code == code
+        assert cache.lengths == before[0] and torch.equal(cache.table, before[1]) and len(cache._free) == before[2]
+
+    refuses(lambda: cache.room_for(7), _lib.EINVAL)
+    refuses(lambda: cache.nodes([1, 1, 1], device="cpu"), _lib.EINVAL)
+    refuses(lambda: cache.release(0), _lib.EINVAL)
+    refuses(lambda: cache.advance(9), _lib.EINVAL)
+    cache.advance(53)
+    assert cache.lengths == cache.seq_len_dev.tolist() == [20, 0, 33] and cache.get_seq_length() == 33
+    refuses(lambda: cache.nodes([3, 3], device="cpu"))
+    refuses(lambda: cache.nodes([0, 0, 80], device="cpu"))      # past the capacity
+    refuses(lambda: cache.nodes([60, 60, 0], device="cpu"))     # past the pool
+    refuses(lambda: cache.nodes([1, -1, 0], device="cpu"))
+    refuses(lambda: cache.nodes([1, 2, 0], [[-1], [-1], []], device="cpu"))
+    refuses(lambda: cache.reorder_cache(torch.tensor([0, 1, 2])), _lib.EUNSUPPORTED)
+    refuses(lambda: cache.keep(None, None), _lib.EINVAL)
+    cache.nodes([4, 1, 3], [[-1, 0, 0, 2], [-1], [-1, 0, 0]], device="cpu")
+    assert cache.next_positions(8, "cpu")[0].tolist() == [20, 21, 21, 22, 0, 33, 34, 34]
+    refuses(lambda: cache.advance(), _lib.EINVAL)               # (a tree: which of its nodes?)
+    path = torch.tensor([0, 2, 3, -1, 0, 0, 1, -1], dtype=torch.int32)
+    assert cache.keep(path, torch.tensor([3, 1, 2], dtype=torch.int32)) == [3, 1, 2]  # (no layer has been written: nothing to move)
+    assert cache.lengths == cache.seq_len_dev.tolist() == [23, 1, 35]
+    cache.nodes([30, 0, 0], device="cpu")
+    cache.cancel_nodes()
+    assert cache.lengths == [23, 1, 35]
+    cache.release(2)
+    assert cache.lengths == cache.seq_len_dev.tolist() == [23, 1, 0] and (cache.table >= 0).sum(1).tolist() == [4, 1, 0]
+    cache.crop(10)
+    assert cache.lengths == cache.seq_len_dev.tolist() == [10, 1, 0] and (cache.table >= 0).sum(1).tolist() == [1, 1, 0] and len(cache._free) == 8
+    cache.reserve(16)
+    assert (cache.table >= 0).sum(1).tolist() == [2, 2, 1]
+    with pytest.raises(_lib.TppxError):
+        at.PagedCache(0, 2)
+    with pytest.raises(_lib.TppxError):
+        at.PagedCache(10, 0)

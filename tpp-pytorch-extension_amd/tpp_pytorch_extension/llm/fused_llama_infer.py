@@ -21,7 +21,7 @@ import torch
 
 from .. import _lib, _ops
 from .._lib import TppxError
-from . import mx4_cache
+from . import mx4_cache, paged_cache
 
 
 # ---------------------------------------------------------------------------
@@ -497,6 +497,247 @@ class Mx4Cache(TppCache):
         return out.view(B, Sq, Nkv, R, H).permute(0, 2, 1, 3, 4).contiguous()
 
 
+class PagedCache(TppCache):
+    """A TppCache in bf16 whose slots lie in pages (`paged_cache`), which a sequence gets as it grows, and whose sequences have lengths of
+    their own (`seq_len_dev` is int32 [B], `lengths` the same on the host).  capacity: slots of a sequence at most; page: slots of a
+    page; pages: of the pool, None: enough for all sequences at their capacity.  The decoder blocks take it wherever they take a
+    TppCache, without padding masks; `nodes()` makes their next pass one over packed nodes, drafted trees among them."""
+
+    kv_dtype = "paged"
+
+    def __init__(self, capacity, n_layers, page=64, pages=None):
+        super().__init__(-(-int(capacity) // int(page)) * int(page))
+        if self.capacity <= 0 or n_layers <= 0:
+            raise TppxError(_lib.EINVAL, f"PagedCache: a capacity of {capacity} slots and {n_layers} layers")
+        self.n_layers, self.page, self.pages = int(n_layers), int(page), pages
+        self.storage = None    # [layers][2][pages][Nkv][page][H]
+        self.table = None      # int32 [B][pages of a sequence], device
+        self.lengths = None    # host
+        self._held = None      # pages of every sequence, host
+        self._free = None      # of the pool
+        self._nodes = None     # (bounds, parents or None, lengths, positions) of an announced pass
+        self._bounds = {}
+
+    def _sequences(self, B, device):
+        if self.lengths is None:
+            width = self.capacity // self.page
+            if self.pages is None:
+                self.pages = B * width
+            self.lengths, self._held, self._free = [0] * B, [[] for _ in range(B)], list(range(self.pages))[::-1]
+            self.table = torch.full((B, width), -1, dtype=torch.int32, device=device)
+            self.seq_len_dev = torch.zeros(B, dtype=torch.int32, device=device)
+        if len(self.lengths) != B:
+            raise TppxError(_lib.ESHAPE, f"PagedCache: {B} sequences in a cache of {len(self.lengths)}")
+
+    def _take(self, more):
+        """Pages for more[b] slots behind what sequence b holds."""
+        need = [-(-(n + m) // self.page) for n, m in zip(self.lengths, more)]
+        if max(need) > self.table.shape[1]:
+            raise TppxError(_lib.ESHAPE, f"PagedCache: {self.lengths} cached + {more} new keys exceed the capacity {self.capacity}")
+        new = [max(w - len(h), 0) for w, h in zip(need, self._held)]
+        if not any(new):
+            return
+        if sum(new) > len(self._free):
+            raise TppxError(_lib.ESHAPE, f"PagedCache: {sum(new)} pages wanted, {len(self._free)} of the pool's {self.pages} are free")
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise TppxError(_lib.EINVAL, "PagedCache: a capture takes no pages: reserve() them before")
+        for h, n in zip(self._held, new):
+            h.extend(self._free.pop() for _ in range(n))
+        self._write_table()
+
+    def _write_table(self):
+        width = self.table.shape[1]
+        self.table.copy_(torch.tensor([h + [-1] * (width - len(h)) for h in self._held], dtype=torch.int32))
+
+    def reserve(self, n):
+        """Pages for n more slots of every sequence, so that its next steps take none (a step that is replayed as a graph cannot)."""
+        self._take([n] * len(self.lengths))
+
+    def release(self, b):
+        """Sequence b is done: its pages go back to the pool, it holds nothing."""
+        self._refuse_while_announced("a release")
+        self._set_length(b, 0)
+        self._write_table()
+        self.seq_len_dev[b] = 0
+
+    def _set_length(self, b, n):
+        self.lengths[b] = n
+        keep = -(-n // self.page)
+        self._free.extend(self._held[b][keep:][::-1])
+        del self._held[b][keep:]
+
+    def _ensure(self, layer_idx, B, Nkv, H, device):
+        self._sequences(B, device)
+        if self.storage is None:
+            if H not in mx4_cache.HEAD_SIZES:
+                raise TppxError(_lib.EUNSUPPORTED, f"PagedCache: head size {H} ({', '.join(map(str, mx4_cache.HEAD_SIZES))} are built)")
+            self.storage = torch.zeros((self.n_layers, 2, self.pages, Nkv, self.page, H), dtype=torch.bfloat16, device=device)
+        if not 0 <= layer_idx < self.n_layers or self.storage.shape[3:] != (Nkv, self.page, H):
+            raise TppxError(_lib.ESHAPE, f"PagedCache: layer {layer_idx}, {Nkv} heads of {H} do not fit {tuple(self.storage.shape)}")
+        return self.storage[layer_idx]
+
+    def _refuse_while_announced(self, what):
+        if self._nodes is not None:
+            raise TppxError(_lib.EINVAL, f"PagedCache: {what} while a pass over nodes of {self._nodes[2]} is announced (advance() or keep() ends "
+                                         "it, cancel_nodes() drops it)")
+
+    def nodes(self, lengths, parents=None, device="cuda"):
+        """The next pass of the blocks runs over packed nodes: hidden states [1][sum(lengths)][..], sequence b's behind sequence b - 1's,
+        positions [1][sum(lengths)] (`next_positions`).  parents: of every sequence the list of its nodes' parents (`paged_cache`), or None:
+        chains.  `keep()` ends the pass with an accepted path, `advance()` with all of a chain's nodes; `cancel_nodes()` where it failed.
+        Until then other passes are refused.  Returns the bounds int32 [B + 1]."""
+        lengths = [int(n) for n in lengths]
+        if not lengths or min(lengths) < 0 or (parents is not None and [len(p) for p in parents] != lengths):
+            raise TppxError(_lib.ESHAPE, f"PagedCache.nodes: lengths {lengths}" + ("" if parents is None else f", parents of {[len(p) for p in parents]}"))
+        self._refuse_while_announced("a pass over other nodes")
+        self._sequences(len(lengths), device)
+        self._take(lengths)
+        bounds, flat, pos = [0], [], []
+        for b, n in enumerate(lengths):
+            bounds.append(bounds[-1] + n)
+            depth = []
+            for i in range(n):
+                up = i - 1 if parents is None else int(parents[b][i])
+                up = up if 0 <= up < i else -1
+                depth.append(0 if up < 0 else depth[up] + 1)
+                flat.append(up)
+            pos += [self.lengths[b] + d for d in depth]
+        made = torch.tensor(bounds + flat, dtype=torch.int32, device=device)
+        self._nodes = (made[:len(bounds)], None if parents is None else made[len(bounds):], lengths,
+                       torch.tensor(pos, dtype=torch.int64, device=device).unsqueeze(0))
+        return self._nodes[0]
+
+    def prompts(self, lengths, device="cuda"):
+        """`nodes()` of prompts: chains."""
+        return self.nodes(lengths, None, device)
+
+    def cancel_nodes(self):
+        """The pass that `nodes()` announced does not take place: the sequences hold what they held before."""
+        self._nodes = None
+
+    cancel_prompts = cancel_nodes
+
+    def keep(self, path, count):
+        """Ends an announced pass: of sequence b the first count[b] nodes of its part of `path` stay (`verify_drafts`), in all layers.
+        Returns the counts as a list (they are copied to the host)."""
+        if self._nodes is None:
+            raise TppxError(_lib.EINVAL, "PagedCache.keep: no pass over nodes was announced")
+        bounds, parents, lengths, _ = self._nodes
+        if parents is not None and self.storage is not None:
+            paged_cache.keep_paged(self.storage, self.table, self.seq_len_dev, path, count, bounds)
+        self.seq_len_dev.add_(count)
+        counts = count.tolist()
+        self._nodes = None
+        for b, n in enumerate(counts):
+            self._set_length(b, self.lengths[b] + n)
+        return counts
+
+    def room_for(self, S):
+        if self._nodes is None:
+            return self.get_seq_length() + S <= self.capacity
+        if S != sum(self._nodes[2]):
+            self._refuse_while_announced(f"a pass of {S} tokens a row")
+        return True  # (nodes() has seen to it)
+
+    def get_seq_length(self, layer_idx=0):
+        return max(self.lengths) if self.lengths else 0
+
+    def size(self):
+        return 0 if self.storage is None else self.n_layers
+
+    def positions(self, B, device):
+        self._sequences(B, device)
+        return self.seq_len_dev.to(torch.int64).view(B, 1)
+
+    def next_positions(self, S, device):
+        if self._nodes is not None:
+            return self._nodes[3]
+        if self.lengths is None:
+            return torch.arange(S, dtype=torch.int64, device=device).unsqueeze(0)
+        return self.positions(len(self.lengths), device) + torch.arange(S, dtype=torch.int64, device=device)
+
+    def advance(self, n=None):
+        """Every sequence holds n more keys (default 1); after an announced pass, each its nodes (n, if it is given, is the number of all
+        of them)."""
+        if self._nodes is None:
+            n = 1 if n is None else n
+            self.seq_len_dev.add_(n)
+            return self._advance_host(n)
+        bounds, parents, lengths, _ = self._nodes
+        if (n is not None and n != sum(lengths)) or parents is not None:
+            self._refuse_while_announced("advance() over a tree" if parents is not None else f"advance({n})")
+        self._nodes = None
+        self.seq_len_dev.add_(bounds.diff())
+        self.lengths = [h + k for h, k in zip(self.lengths, lengths)]
+
+    def _advance_host(self, n=1):
+        self.lengths = [h + n for h in self.lengths]
+
+    def crop(self, max_length):
+        self._nodes = None
+        if self.lengths is None:
+            return
+        for b, n in enumerate(self.lengths):
+            self._set_length(b, min(n, int(max_length)))
+        self._write_table()
+        self.seq_len_dev.clamp_(max=int(max_length))
+
+    def reorder_cache(self, beam_idx):
+        raise TppxError(_lib.EUNSUPPORTED, "PagedCache: the sequences of a cache in pages are not reordered")
+
+    def get(self, layer_idx):
+        """[keys, values] [B][Nkv][longest length][H]; what lies behind a shorter sequence is whatever is there."""
+        n = max(self.lengths)
+        pages = self.table[:, :-(-n // self.page)].clamp(min=0).to(torch.int64)
+        return [side[pages].permute(0, 2, 1, 3, 4).flatten(2, 3)[:, :, :n] for side in self.storage[layer_idx]]
+
+    def update(self, key_states, value_states, layer_idx):
+        raise TppxError(_lib.EUNSUPPORTED, "PagedCache: keys and values go to pages by append_paged")
+
+    def attend(self, t_QL, t_KL, t_VL, t_AM, layer_idx):
+        raise TppxError(_lib.EUNSUPPORTED, "PagedCache: attention over pages is append_paged and attn_paged")
+
+    def fill_(self, layer_idx, keys, values):
+        B, Nkv, S, H = keys.shape
+        if values.shape != keys.shape:
+            raise TppxError(_lib.ESHAPE, "PagedCache: keys and values differ in shape")
+        self._refuse_while_announced("a fill")
+        self._sequences(B, keys.device)
+        for b in range(B):
+            self._set_length(b, 0)
+        self._take([S] * B)
+        self._write_table()
+        layer = self._ensure(layer_idx, B, Nkv, H, keys.device)
+        rows = [t.to(torch.bfloat16).transpose(1, 2).reshape(B * S, Nkv, H) for t in (keys, values)]
+        bounds = torch.arange(B + 1, dtype=torch.int32, device=keys.device) * S
+        paged_cache.append_paged(None, *rows, layer, self.table, torch.zeros_like(self.seq_len_dev), bounds, style=None)
+        self.lengths = [S] * B
+        self.seq_len_dev.fill_(S)
+        return self
+
+    def rotate_append_attend(self, q, k, v, t_am, t_pid, layer_idx, B, S, Nq, Nkv, H, t_EP, style, qk_norm=None):
+        """What the function of that name does for a contiguous cache, in two launches: norm, rotation and append, then attention."""
+        T = B * S
+        if t_am is not None and t_am.numel():
+            raise TppxError(_lib.EUNSUPPORTED, "PagedCache: sequences of different lengths are packed, there is no padding mask")
+        parents = None
+        if self._nodes is not None:
+            bounds, parents, lengths, _ = self._nodes
+            if B != 1 or S != sum(lengths):
+                raise TppxError(_lib.ESHAPE, f"PagedCache: a pass of [{B}][{S}] tokens over nodes of [1][{sum(lengths)}]")
+            B = len(lengths)
+        else:
+            bounds = None if S == 1 else torch.arange(B + 1, dtype=torch.int32, device=q.device) * S
+            self._sequences(B, q.device)
+            self._take([S] * B)
+        layer = self._ensure(layer_idx, B, Nkv, H, q.device)
+        wq, wk, eps = qk_norm or (None, None, 0.0)
+        pos = _token_positions(t_pid, T, S) if style else None
+        rows = paged_cache.append_paged(q.view(T, Nq, H), k.view(T, Nkv, H), v.view(T, Nkv, H), layer, self.table, self.seq_len_dev, bounds, parents,
+                                        wq, wk, eps, t_EP, pos, style)
+        return paged_cache.attn_paged(rows, layer, self.table, self.seq_len_dev, bounds, parents).view(q.shape)
+
+
 def kv_cache(capacity=0, kv_dtype="bfloat16"):
     """A cache by the type that holds its keys and values: "bfloat16" (TppCache) or "mxfp4" (Mx4Cache)."""
     if kv_dtype not in ("bfloat16", "mxfp4"):
@@ -774,9 +1015,12 @@ class LlamaDecoder:
         self.n_kv_heads = n_kv_heads
         self._graph = None
 
+    def _empty_cache(self, capacity):
+        return PagedCache(capacity, self.n_layers) if self.kv_dtype == "paged" else kv_cache(capacity, self.kv_dtype)
+
     def new_cache(self, B, context, capacity, seed=1):
         """Cache pre-filled with `context` positions of N(0,1) keys / values in every layer."""
-        cache = kv_cache(capacity, self.kv_dtype)
+        cache = self._empty_cache(capacity)
         g = torch.Generator(device=self.device).manual_seed(seed)
         for i in range(self.n_layers):
             shape = (B, self.n_kv_heads, context, self.H)
@@ -833,10 +1077,13 @@ class LlamaDecoder:
         return logits.view(B, -1).argmax(dim=-1)
 
     def prefill_packed(self, prompts, cache):
-        """Prompts of different lengths (a list of i64 [n], n > 0) in one pass on top of whatever an Mx4Cache holds of each sequence,
-        laid one after the other without padding -> next tokens i64 [B]; advances the cache by every prompt's length."""
-        if cache.kv_dtype != "mxfp4":
-            raise TppxError(_lib.EINVAL, "prefill_packed: sequences of different lengths need an Mx4Cache (kv_dtype=\"mxfp4\")")
+        """Prompts of different lengths (a list of i64 [n], n > 0) in one pass on top of whatever an Mx4Cache or a PagedCache holds of each
+        sequence, laid one after the other without padding -> next tokens i64 [B]; advances the cache by every prompt's length."""
+        return self._logits_packed(prompts, cache).argmax(dim=-1)
+
+    def _logits_packed(self, prompts, cache):
+        if cache.kv_dtype not in ("mxfp4", "paged"):
+            raise TppxError(_lib.EINVAL, "prefill_packed: sequences of different lengths need an Mx4Cache (kv_dtype=\"mxfp4\") or a PagedCache (\"paged\")")
         lengths = [int(p.numel()) for p in prompts]
         if not lengths or min(lengths) < 1:
             raise TppxError(_lib.ESHAPE, f"prefill_packed: prompts of {lengths} tokens")
@@ -852,16 +1099,16 @@ class LlamaDecoder:
             raise
         cache.advance()
         h = rms_norm(h[0].index_select(0, bounds[1:].to(torch.int64) - 1), self.norm_w, self.eps)
-        return _ops.fc_plain(h, self.lm_head, None).argmax(dim=-1)
+        return _ops.fc_plain(h, self.lm_head, None)
 
     def generate_packed(self, prompts, n_new, capacity=None, use_graph=True):
         """`generate` for prompts of different lengths (a list of i64 [n]): one packed pass, then one token per sequence and step, on an
-        MXFP4 cache: for a decoder with kv_dtype="mxfp4".  Returns i64 [B][n_new]."""
+        MXFP4 cache or one in pages: for a decoder with kv_dtype="mxfp4" or "paged".  Returns i64 [B][n_new]."""
         if not prompts:
             raise TppxError(_lib.ESHAPE, "generate_packed: no prompts")
-        if self.kv_dtype != "mxfp4":  # (not four bits in the place of sixteen unasked)
-            raise TppxError(_lib.EINVAL, f"generate_packed: sequences of different lengths need an MXFP4 cache, the decoder's kv_dtype is {self.kv_dtype!r}")
-        cache = Mx4Cache(capacity or max(int(p.numel()) for p in prompts) + n_new + 32)
+        if self.kv_dtype not in ("mxfp4", "paged"):  # (not four bits in the place of sixteen unasked)
+            raise TppxError(_lib.EINVAL, f"generate_packed: sequences of different lengths need an MXFP4 cache or one in pages, the decoder's kv_dtype is {self.kv_dtype!r}")
+        cache = self._empty_cache(capacity or max(int(p.numel()) for p in prompts) + n_new + 32)
         first = self.prefill_packed(prompts, cache).view(-1, 1)
         if n_new == 1:
             return first
@@ -871,7 +1118,7 @@ class LlamaDecoder:
         """Greedy generation as run_generation.py drives it: the prompt in one pass, then one token per step.
         Returns i64 [B][n_new]."""
         B, S = prompt.shape
-        cache = kv_cache(capacity or S + n_new + 32, self.kv_dtype)
+        cache = self._empty_cache(capacity or S + n_new + 32)
         first = self.prefill(prompt, cache)
         if n_new == 1:
             return first.view(B, 1)
@@ -888,6 +1135,59 @@ class LlamaDecoder:
         if start + n_new > self.EP.shape[1]:
             raise TppxError(_lib.ESHAPE, f"decoding {n_new} tokens from position {start} overruns the rotary table "
                                          f"({self.EP.shape[1]} positions)")
+        if cache.kv_dtype == "paged":
+            cache.reserve(n_new)
+
+    def generate_drafted(self, prompts, n_new, propose=None, temperature=0.0, generator=None, capacity=None):
+        """`generate_packed` with drafted tokens, for a decoder with kv_dtype="paged": in every step `propose(tokens)` of a sequence's tokens
+        so far (a list) gives (drafted tokens, their parents: -1 for what follows the last token, otherwise the number of an earlier
+        drafted one), by default `paged_cache.lookup_drafts`; one pass runs over all sequences' trees, and those stand that
+        `verify_drafts` lets stand at `temperature` (0: greedy; random numbers from `generator`).  The tokens are distributed as without
+        drafts, at temperature 0 they are the same but for roundings of the passes.  Returns a list of i64 [n_new], and the number of passes."""
+        if not prompts or n_new < 1 or self.kv_dtype != "paged":
+            raise TppxError(_lib.EINVAL, f"generate_drafted: {len(prompts)} prompts, {n_new} tokens, a decoder with kv_dtype {self.kv_dtype!r} (\"paged\" is wanted)")
+        propose = propose or paged_cache.lookup_drafts
+        B = len(prompts)
+        texts = [p.reshape(-1).tolist() for p in prompts]
+        ends = [len(t) + n_new for t in texts]
+        cache = PagedCache(capacity or max(ends) + 128, self.n_layers)
+
+        def numbers(n):
+            return torch.rand(n, generator=generator, device=self.device) if temperature else None
+
+        logits = self._logits_packed(prompts, cache)
+        _, _, last = paged_cache.verify_drafts(torch.zeros(B, dtype=torch.int64, device=self.device), logits, uniforms=numbers(B), sample=numbers(B),
+                                               temperature=temperature)
+        for t, x in zip(texts, last.tolist()):
+            t.append(x)
+        passes = 1
+        while any(len(t) < e for t, e in zip(texts, ends)):
+            tokens, parents = [], []
+            for t, e in zip(texts, ends):
+                drafted, up = propose(t) if len(t) < e else ((), ())
+                room = min(self.EP.shape[1], cache.capacity) - len(t)  # (every node has a slot, and a position below it)
+                drafted, up = list(drafted)[:max(room, 0)], list(up)[:max(room, 0)]
+                tokens.append([t[-1]] + drafted if len(t) < e else [])
+                parents.append([-1] + [u + 1 for u in up] if len(t) < e else [])
+            flat = torch.tensor([x for t in tokens for x in t], dtype=torch.int64, device=self.device)
+            bounds = cache.nodes([len(t) for t in tokens], parents, self.device)
+            try:
+                h = self.embed.index_select(0, flat).unsqueeze(0)
+                for layer in self.layers:
+                    h = layer.forward([h, None, cache.next_positions(flat.numel(), self.device)], cache)[0]
+            except BaseException:
+                cache.cancel_nodes()
+                raise
+            logits = _ops.fc_plain(rms_norm(h[0].contiguous(), self.norm_w, self.eps), self.lm_head, None)
+            path, count, last = paged_cache.verify_drafts(flat, logits, bounds, cache._nodes[1], uniforms=numbers(flat.numel()), sample=numbers(B),
+                                                          temperature=temperature)
+            counts, stood, then, at = cache.keep(path, count), path.tolist(), last.tolist(), 0
+            for b, n in enumerate(counts):
+                if n:
+                    texts[b] += [tokens[b][i] for i in stood[at + 1:at + n]] + [then[b]]
+                at += len(tokens[b])
+            passes += 1
+        return [torch.tensor(t[e - n_new:e], dtype=torch.int64, device=self.device) for t, e in zip(texts, ends)], passes
 
     def time_decode_steps(self, tokens, cache, n_new):
         """Seconds spent in n_new replays of the captured decode step (capture excluded)."""

@@ -161,3 +161,15 @@ def keep_paged(cache, table, past, path, count, cu_seqlens=None):
     at, pages, page, table_at, table_ld = _pages(whole, table, None, None, B, dev, 6)
     _run(dev, _lib.lib().tppx_keep_paged, at, table_at, past_at, _index(path, "path", T, dev), _index(count, "count", B, dev), cu_at,
          whole.shape[0], T, B, whole.shape[3], whole.shape[5], pages, page, table_ld)
+
+
+def lookup_drafts(tokens, most=8, longest=3):
+    """Drafts from the text itself: what followed the last earlier occurrence of its last `longest` (or fewer) tokens, at most `most`
+    of them, as a chain (tokens, parents)."""
+    for n in range(min(longest, len(tokens) - 1), 0, -1):
+        tail = tokens[-n:]
+        for at in range(len(tokens) - n - 1, -1, -1):
+            if tokens[at:at + n] == tail:
+                found = tokens[at + n:at + n + most]
+                return found, list(range(-1, len(found) - 1))
+    return [], []
