@@ -798,8 +798,11 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     // A few pages hold no more than a part would: not worth the look at the lengths and the merge.
     if (target < units + p.Nkv || (p.g.table_ld << p.g.shift) <= 384)
       target = 0;
-    p.target = (int)target;
     p.least = std::max(env_int("TPPX_PAGED_LEAST", 256) / KEYS, 1);
+    // no more than the capacity would make: a workgroup without work waits for room on a CU like any other
+    const int64_t most = ((p.g.table_ld << p.g.shift) / KEYS + p.least) / p.least;
+    target = std::min<int64_t>(target, units * most);
+    p.target = (int)target;
     p.items = (int)std::max<int64_t>(target, units);
     const bool here = COLS == 16 && p.R <= 16 && !p.cu && p.items * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) <= counter_bytes;
     if (!here)
