@@ -123,10 +123,10 @@ struct ManyWeights {
     }
     return s;
   }
-  __device__ __forceinline__ double operator()(float x) const {
+  __device__ __forceinline__ double operator()(float x) const { // (below `lowest` nothing: no token of that weight is drawn)
     double g;
     const double w = parts(x, g);
-    return w * g;
+    return x > lowest ? w * g : 0.0;
   }
 };
 template <typename E>
@@ -226,11 +226,11 @@ draft_rows_kernel(const DraftsParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = (int)(blockIdx.x / (unsigned)p.C), piece = (int)(blockIdx.x % (unsigned)p.C), side = (int)blockIdx.y;
   int b = 0;
-  if (p.temps) {
-    if (p.cu)
-      b = min(sequence_of(p.cu, p.B, row), p.B - 1);
-    else
-      b = row;
+  if (p.temps || side) {
+    b = p.cu ? sequence_of(p.cu, p.B, row) : row;
+    if (side && (!p.cu || b >= p.B || p.cu[b + 1] == row + 1))
+      return; // (nothing was drawn from the last node's)
+    b = min(b, p.B - 1);
   }
   const double to2 = to2_of(p, b);
   const E* const at = (const E*)(side ? p.draft : p.target) + (int64_t)row * (side ? p.d_ld : p.t_ld);
@@ -328,12 +328,13 @@ draft_rows_kernel(const DraftsParams p) {
 }
 
 // ---------------------------------------------------------------------------
-// The walk and the next token, a workgroup of 1024 for a sequence: the state of its rows from their pieces, every node's token's p (and q)
+// The walk and the next token, a workgroup for a sequence: the state of its rows from their pieces, every node's token's p (and q)
 // in its parent's row, then down.  WALK, TOKEN: both without draft logits; with them the walk is done by every workgroup that sums
 // what is left of a piece (blockIdx.y) of the last row, the first of which leaves it to the launch that finds the token.
 // ---------------------------------------------------------------------------
 constexpr int DRAFT_NODES = 256; // nodes of a sequence that are held in LDS; more go through the workspace
-constexpr int WALK_THREADS = 1024;
+// threads of a workgroup: where there is one for each piece, few enough that all of them run at once
+constexpr int walk_threads(bool token) { return token ? 1024 : 512; }
 
 __device__ __forceinline__ double add64(double a, double z) { return a + z; }
 template <int CTRL, int ROWS>
@@ -354,11 +355,11 @@ __device__ __forceinline__ double scan64(double v) {
 }
 
 template <typename E, int NV, bool WALK, bool TOKEN>
-__global__ void __launch_bounds__(WALK_THREADS)
+__global__ void __launch_bounds__(walk_threads(TOKEN), 4)
 draft_walk_kernel(const DraftsParams p) {
-  constexpr int N = per16<E>(), PIECE = DRAFT_THREADS * NV * N, WAVES = WALK_THREADS / 64;
-  constexpr int VECTORS = DRAFT_THREADS * NV; // of a piece; a thread takes at most one
-  static_assert(VECTORS <= WALK_THREADS);
+  constexpr int THREADS = walk_threads(TOKEN), N = per16<E>(), PIECE = DRAFT_THREADS * NV * N, WAVES = THREADS / 64;
+  constexpr int VECTORS = DRAFT_THREADS * NV, EACH = VECTORS > THREADS ? VECTORS / THREADS : 1; // of a piece, of a thread
+  static_assert(EACH == 1 || !TOKEN);
   __shared__ RowSum rows_lds[2][DRAFT_NODES];
   __shared__ NodeShare nodes_lds[DRAFT_NODES];
   __shared__ double tried_px[DRAFT_NODES]; // the last node's children: shares, pieces that their tokens lie in
@@ -366,6 +367,7 @@ draft_walk_kernel(const DraftsParams p) {
   __shared__ uint32_t gone[PIECE / 32]; // tokens of a piece that were tried
   __shared__ double red[WAVES];
   __shared__ int found_at[WAVES], last_at[WAVES];
+  __shared__ double table[256];
   __shared__ Walk walk;
   __shared__ int piece_at;
   __shared__ double piece_before, piece_border;
@@ -381,6 +383,9 @@ draft_walk_kernel(const DraftsParams p) {
   }
   const double to2 = to2_of(p, b);
   const bool drawn = p.draft && to2 != 0.0;
+  const float sample = TOKEN && to2 != 0.0 ? p.sample[b] : 0.f;
+  if (tid < 256)
+    table[tid] = POWERS.v[tid]; // (read behind a barrier)
   const int32_t* const parents = p.parents ? p.parents + first : nullptr;
   const int64_t* const tokens = p.tokens + first;
   auto parent = [&](int i) { return parents ? parents[i] : i - 1; };
@@ -405,17 +410,25 @@ draft_walk_kernel(const DraftsParams p) {
           y = logit_of(logits(1, first + z.up)[z.token]);
       }
     };
+    // (the first piece of the first row, too: the loads from memory are what this launch waits for)
+    const int sides = drawn ? 2 : 1, u = tid % 16;
+    auto pieces_of = [&](int i) { return p.pieces + ((int64_t)(i >= n) * p.T + first + (i >= n ? i - n : i)) * p.C; };
+    Piece ahead = {0.0, -INFINITY, p.V};
+    if (tid / 16 < sides * n && u < p.C)
+      ahead = pieces_of(tid / 16)[u];
     NodeShare z0;
     float x0, y0;
     if (tid < n)
       own(tid, z0, x0, y0);
     // 16 lanes a row: its pieces in turn
-    for (int i = tid / 16; i < (drawn ? 2 : 1) * n; i += WALK_THREADS / 16) {
-      const int side = i >= n, r = i - side * n, u = tid % 16;
-      const Piece* const at = p.pieces + ((int64_t)side * p.T + first + r) * p.C;
-      float top = -INFINITY;
-      int place = p.V;
-      for (int c = u; c < p.C; c += 16) {
+    for (int i = tid / 16; i < sides * n; i += THREADS / 16) {
+      const int side = i >= n, r = i - side * n;
+      const Piece* const at = pieces_of(i);
+      if (i != tid / 16)
+        ahead = u < p.C ? at[u] : Piece{0.0, -INFINITY, p.V};
+      float top = ahead.top;
+      int place = ahead.first;
+      for (int c = u + 16; c < p.C; c += 16) {
         const float t = at[c].top;
         const int f = at[c].first;
         place = t > top ? f : t == top ? min(place, f) : place;
@@ -429,17 +442,19 @@ draft_walk_kernel(const DraftsParams p) {
         top = fmaxf(top, t);
       }
       double sum = 0.0;
-      if (to2 != 0.0)
-        for (int c = u; c < p.C; c += 16) {
+      if (to2 != 0.0) {
+        sum = ahead.sum > 0.0 ? ahead.sum * weight_of(ahead.top, top, to2) : 0.0;
+        for (int c = u + 16; c < p.C; c += 16) {
           const Piece z = at[c];
           sum += z.sum > 0.0 ? z.sum * weight_of(z.top, top, to2) : 0.0;
         }
+      }
       sum = reduce_lanes<16>(sum, add64);
       if (u == 0)
         (side ? qrows : prows)[r] = RowSum{sum, top, place};
     }
     __syncthreads();
-    for (int i = tid; i < n; i += WALK_THREADS) {
+    for (int i = tid; i < n; i += THREADS) {
       if (i != tid)
         own(i, z0, x0, y0);
       z0.px = z0.qx = 0.0;
@@ -550,10 +565,10 @@ draft_walk_kernel(const DraftsParams p) {
   auto mark = [&](int piece) { // the tried tokens of a piece
     if (!tried || drawn)
       return;
-    for (int i = tid; i < PIECE / 32; i += WALK_THREADS)
+    for (int i = tid; i < PIECE / 32; i += THREADS)
       gone[i] = 0;
     __syncthreads();
-    for (int c = at + 1 + tid; c < (parents ? n : min(at + 2, n)); c += WALK_THREADS) {
+    for (int c = at + 1 + tid; c < (parents ? n : min(at + 2, n)); c += THREADS) {
       const int64_t x = parent(c) == at ? tokens[c] : -1;
       if (x >= 0 && x < p.V && x / PIECE == piece)
         atomicOr(&gone[x % PIECE / 32], 1u << (x % 32));
@@ -562,27 +577,37 @@ draft_walk_kernel(const DraftsParams p) {
   };
   // What is left of a vector of 16 bytes of the last row: p without the tokens that were tried, or max(p - q, 0).  all: p.
   const double pn = 1.0 / ps.sum, qn = 1.0 / qs.sum;
-  auto rest = [&](int from, bool all, double (&w)[N]) {
+  const bool fits = ManyWeights::fits(ps.top, to2) && (!residual || ManyWeights::fits(qs.top, to2)); // (uniform)
+  const ManyWeights mp(table, ps.top, to2), mq(table, qs.top, to2);
+  const double pm = fits ? pn * mp.off(ps.top) : 0.0, qm = fits && residual ? qn * mq.off(qs.top) : 0.0;
+  struct Vector {
+    uint4 p, q;
+  };
+  auto ask = [&](int piece, int i) { // vector i of a piece, where there is one
+    const int from = piece * PIECE + i * N;
+    return i < VECTORS ? Vector{load_raw<E>(prow, from, p.V), residual ? load_raw<E>(qrow, from, p.V) : uint4{}} : Vector{};
+  };
+  auto rest = [&](const Vector& v, int piece, int i, bool all, double (&w)[N]) {
+    const int from = piece * PIECE + i * N;
     float x[N], y[N];
-    load_logits<E>(prow, from, p.V, x);
-    if (residual && !all)
-      load_logits<E>(qrow, from, p.V, y);
+    raw_logits<E>(v.p, x);
+    raw_logits<E>(v.q, y);
     const bool without = tried && !drawn && !all;
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      w[e] = weight_of(x[e], ps.top, to2) * pn;
+      const float a = x[e] == x[e] ? x[e] : -INFINITY, z = y[e] == y[e] ? y[e] : -INFINITY;
+      w[e] = fits ? mp(a) * pm : weight_of(a, ps.top, to2) * pn;
       if (residual && !all)
-        w[e] = fmax(w[e] - weight_of(y[e], qs.top, to2) * qn, 0.0);
+        w[e] = fmax(w[e] - (fits ? mq(z) * qm : weight_of(z, qs.top, to2) * qn), 0.0);
       if (without && gone[(from + e) % PIECE / 32] >> ((from + e) % 32) & 1)
         w[e] = 0.0;
       w[e] = from + e < p.V ? w[e] : 0.0;
     }
   };
-  // this thread's vector of a piece (-inf where the piece has fewer), and its sum
-  auto mine = [&](int piece, bool all, double (&w)[N]) {
+  auto mine = [&](const Vector& v, int piece, int i, bool all, double (&w)[N]) { // and their sum
     double s = 0.0;
-    if (tid < VECTORS) {
-      rest(piece * PIECE + tid * N, all, w);
+    if (i < VECTORS) {
+      rest(v, piece, i, all, w);
 #pragma unroll
       for (int e = 0; e < N; e++)
         s += w[e];
@@ -590,8 +615,17 @@ draft_walk_kernel(const DraftsParams p) {
     return s;
   };
   auto sum_of_piece = [&](int piece) { // in all threads; `gone` marked
-    double w[N];
-    const double s = reduce_lanes<64>(mine(piece, false, w), add64);
+    Vector v[EACH];
+    double s = 0.0;
+#pragma unroll
+    for (int h = 0; h < EACH; h++)
+      v[h] = ask(piece, h * THREADS + tid);
+#pragma unroll
+    for (int h = 0; h < EACH; h++) {
+      double w[N];
+      s += mine(v[h], piece, h * THREADS + tid, false, w);
+    }
+    s = reduce_lanes<64>(s, add64);
     __syncthreads();
     if (lane == 0)
       red[wave] = s;
@@ -606,36 +640,7 @@ draft_walk_kernel(const DraftsParams p) {
   if constexpr (!TOKEN) {
     if (!residual)
       return;
-    __shared__ double table[256];
-    double s = 0.0;
-    if (ManyWeights::fits(ps.top, to2) && ManyWeights::fits(qs.top, to2)) { // (uniform)
-      const int from = (int)blockIdx.y * PIECE + tid * N;
-      float x[N], y[N];
-      if (tid < VECTORS) {
-        load_logits<E>(prow, from, p.V, x);
-        load_logits<E>(qrow, from, p.V, y);
-      }
-      if (tid < 256)
-        table[tid] = POWERS.v[tid];
-      __syncthreads();
-      if (tid < VECTORS) {
-        const ManyWeights mp(table, ps.top, to2), mq(table, qs.top, to2);
-        const double a = pn * mp.off(ps.top), z = qn * mq.off(qs.top);
-#pragma unroll
-        for (int e = 0; e < N; e++)
-          s += fmax(mp(x[e]) * a - mq(y[e]) * z, 0.0);
-      }
-      s = reduce_lanes<64>(s, add64);
-      if (lane == 0)
-        red[wave] = s;
-      __syncthreads();
-      s = 0.0;
-#pragma unroll
-      for (int i = 0; i < WAVES; i++)
-        s += red[i];
-    } else {
-      s = sum_of_piece((int)blockIdx.y);
-    }
+    const double s = sum_of_piece((int)blockIdx.y);
     if (tid == 0)
       sums[blockIdx.y] = s;
   } else {
@@ -658,14 +663,15 @@ draft_walk_kernel(const DraftsParams p) {
           return fmax(s, 0.0);
         };
         const double head = of_piece(lane);
-        double whole = 0.0;
-        for (int i0 = 0; i0 < p.C; i0 += 64)
-          whole += reduce_lanes<64>(i0 ? of_piece(i0 + lane) : head, add64);
-        const double border = (double)p.sample[b] * whole;
+        const double head_run = scan64(head);
+        double whole = __shfl(head_run, 63);
+        for (int i0 = 64; i0 < p.C; i0 += 64)
+          whole += reduce_lanes<64>(of_piece(i0 + lane), add64);
+        const double border = (double)sample * whole;
         double before = 0.0, start = 0.0;
         int piece = -1, last = 0;
         for (int i0 = 0; i0 < p.C && piece < 0; i0 += 64) {
-          const double s = i0 ? of_piece(i0 + lane) : head, run = scan64(s);
+          const double s = i0 ? of_piece(i0 + lane) : head, run = i0 ? scan64(s) : head_run;
           const uint64_t beyond = __builtin_amdgcn_ballot_w64(s > 0.0 && before + run > border);
           const uint64_t some = __builtin_amdgcn_ballot_w64(s > 0.0);
           if (beyond) {
@@ -703,15 +709,17 @@ draft_walk_kernel(const DraftsParams p) {
     }
     const int piece = piece_at;
     const double border = piece_border;
+    const Vector own = ask(piece, tid);
     mark(piece);
     double w[N];
-    const double s = mine(piece, all, w), run = scan64(s);
+    const double s = mine(own, piece, tid, all, w), run = scan64(s);
     if (lane == 63)
       red[wave] = run;
     __syncthreads();
     double before = piece_before;
-    for (int i = 0; i < wave; i++)
-      before += red[i];
+#pragma unroll
+    for (int i = 0; i < WAVES - 1; i++)
+      before += i < wave ? red[i] : 0.0;
     before += run - s;
     int found = p.V, last = -1;
     if (tid < VECTORS) {
@@ -725,22 +733,29 @@ draft_walk_kernel(const DraftsParams p) {
         }
       }
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      found = min(found, __shfl_xor(found, d));
-      last = max(last, __shfl_xor(last, d));
-    }
+    // the first lane and the first wave that found one; a border that is rounded past the piece's last token: that one
+    const uint64_t lanes = __builtin_amdgcn_ballot_w64(found < p.V), some = __builtin_amdgcn_ballot_w64(last >= 0);
     if (lane == 0) {
-      found_at[wave] = found;
-      last_at[wave] = last;
+      found_at[wave] = p.V;
+      last_at[wave] = -1;
     }
+    if (lanes && lane == __builtin_ctzll(lanes))
+      found_at[wave] = found;
+    if (some && lane == 63 - __builtin_clzll(some))
+      last_at[wave] = last;
     __syncthreads();
-    if (tid == 0) {
-      for (int i = 1; i < WAVES; i++) {
-        found = min(found, found_at[i]);
-        last = max(last, last_at[i]);
+    if (wave == 0) {
+      const int f = found_at[min(lane, WAVES - 1)], z = last_at[min(lane, WAVES - 1)];
+      const uint64_t first_wave = __builtin_amdgcn_ballot_w64(f < p.V), last_wave = __builtin_amdgcn_ballot_w64(z >= 0 && lane < WAVES);
+      if (first_wave) {
+        if (lane == __builtin_ctzll(first_wave))
+          p.next[b] = f;
+      } else if (last_wave) {
+        if (lane == 63 - __builtin_clzll(last_wave))
+          p.next[b] = z;
+      } else if (lane == 0) {
+        p.next[b] = 0;
       }
-      p.next[b] = found < p.V ? found : max(last, 0); // (a border that is rounded past the piece's last token: that one)
     }
   }
 }
@@ -797,10 +812,10 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
     if (T > 0)
       draft_rows_kernel<E, NV><<<dim3((unsigned)(T * p.C), (unsigned)p.sides), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
     if (draft) {
-      draft_walk_kernel<E, NV, true, false><<<dim3((unsigned)B, (unsigned)p.C), dim3(WALK_THREADS), 0, (hipStream_t)stream>>>(p);
-      draft_walk_kernel<E, NV, false, true><<<dim3((unsigned)B), dim3(WALK_THREADS), 0, (hipStream_t)stream>>>(p);
+      draft_walk_kernel<E, NV, true, false><<<dim3((unsigned)B, (unsigned)p.C), dim3(walk_threads(false)), 0, (hipStream_t)stream>>>(p);
+      draft_walk_kernel<E, NV, false, true><<<dim3((unsigned)B), dim3(walk_threads(true)), 0, (hipStream_t)stream>>>(p);
     } else {
-      draft_walk_kernel<E, NV, true, true><<<dim3((unsigned)B), dim3(WALK_THREADS), 0, (hipStream_t)stream>>>(p);
+      draft_walk_kernel<E, NV, true, true><<<dim3((unsigned)B), dim3(walk_threads(true)), 0, (hipStream_t)stream>>>(p);
     }
   };
   auto typed = [&](auto e) {
