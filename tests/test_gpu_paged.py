@@ -150,6 +150,22 @@ def test_attention_of_pieces_of_prompts(H, Nq, Nkv, new, past, chunk, monkeypatc
     _check_attention(new, past, 32, Nq, Nkv, H, None, seed=H + len(new), spare_rows=2)
 
 
+@pytest.mark.parametrize("B", [65, 150, 400])
+@pytest.mark.parametrize("form", ["", "1", "2", "3", "4", "5"])
+@pytest.mark.parametrize("kind", ["single", "chains", "trees"])
+def test_attention_of_many_sequences(B, form, kind, monkeypatch):
+    """More sequences than a wave has lanes, some long enough to be split, some empty, some that take no part."""
+    if form:
+        monkeypatch.setenv("TPPX_PAGED_FORM", form)
+    monkeypatch.setenv("TPPX_PAGED_LEAST", "64")
+    monkeypatch.setenv("TPPX_PAGED_ITEMS", "6000")
+    new = [1] * B if kind == "single" else [(0, 3, 1, 8, 21)[i * 7 % 5] for i in range(B)]
+    past = [(0, 5, 130, -1, 33)[i * 3 % 5] for i in range(B)]
+    past[1], past[63], past[64], past[B - 1] = 900, 2100, 1200, 700
+    trees = [R.tree(n, i) if n else [] for i, n in enumerate(new)] if kind == "trees" else None
+    _check_attention(new, past, 16, 4, 2, 64, trees, seed=B)
+
+
 def test_attention_of_a_deep_tree_and_of_one_that_is_a_chain():
     n = 300
     _check_attention([n], [20], 16, 4, 2, 128, [R.tree(n, 5, deep=0.97)])
@@ -496,6 +512,42 @@ def test_steps_in_a_replayed_graph():
         for got, w in zip(outs, want):
             assert torch.equal(got, w)
         assert torch.equal(cache, again)
+
+
+def test_two_graphs_replayed_at_once():
+    """Steps of drafted tokens keep what they leave for their later launches apart: replays of two graphs need no order."""
+    at = _at()
+    jobs, want, graphs, outs = [], [], [], []
+    for i in range(2):
+        new, past = [20, 9], [2000 + 300 * i, 900]
+        table, pool = R.table_for([p + n for p, n in zip(past, new)], 32, seed=i)
+        parents = _i32([x for n in new for x in R.tree(n, n + i)])
+        tokens, _, target, _, u, s = _verify_case(new, 4000, torch.bfloat16, i, True, False, [1.0, 1.0])
+        jobs.append([t.cuda() for t in (M.randn((29, 16, 128), 1.0, i), _layer(pool, 2, 32, 128, 90 + i), table, _i32(past), _i32([0, 20, 29]), parents,
+                                        torch.tensor(tokens), target, u, s)])
+
+    def work(j):
+        q, layer, table, past, cu, parents, tokens, target, u, s = j
+        return (at.attn_paged(q, layer, table, past, cu, parents), *at.verify_drafts(tokens, target, cu, parents, None, u, s))
+
+    for j in jobs:
+        want.append(work(j))
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(work(j))
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, z) for a, z in zip(outs[i], want[i]))
+            for t in outs[i]:
+                t.zero_()
+        torch.cuda.synchronize()
 
 
 def test_two_streams_at_once():

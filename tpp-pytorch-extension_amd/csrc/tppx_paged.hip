@@ -554,8 +554,9 @@ paged_attn_kernel(const PagedAttnParams p) {
   };
   // A split's results for the merge: stores and loads at the scope of the device, written through to the level that all XCDs share.
   constexpr int SHARED = 16; // (sc1)
-  const auto part = __builtin_amdgcn_make_buffer_rsrc(p.part, 0, p.items * (COLS * H * 4), 0x00020000);
-  const auto part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)p.items * COLS * H, 0, p.items * (COLS * 8), 0x00020000);
+  const int split_items = p.target > 0 ? p.items : 0; // (those fit into 31 bits)
+  const auto part = __builtin_amdgcn_make_buffer_rsrc(p.part, 0, split_items * (COLS * H * 4), 0x00020000);
+  const auto part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)split_items * COLS * H, 0, split_items * (COLS * 8), 0x00020000);
   if (TW == 1 && S == 1) {
 #pragma unroll
     for (int k = 0; k < CG; k++) {
@@ -680,6 +681,8 @@ paged_merge_kernel(const PagedAttnParams p) {
   Item it;
   if (!locate_item<COLS, KEYS>(p, (int)blockIdx.x, true, it) || it.S == 1)
     return;
+  if ((int64_t)it.first + (int64_t)(it.S - 1) * it.stride >= p.items || it.first < 0)
+    return; // (bounds that do not ascend: more items than were launched)
   const int S = it.S, col0 = it.o.at * COLS, ncol = min(COLS, it.o.n * p.R - col0);
   const int d4 = (int)threadIdx.x % EACH;
   if ((int)threadIdx.x >= PER * EACH)
@@ -785,16 +788,15 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     constexpr int NJ = decltype(nj)::value, CG = decltype(cg)::value, CW = decltype(cw)::value, TW = decltype(tw)::value, KEYS = decltype(kt)::value, COLS = 16 * CG * CW;
     const int64_t blocks = p.cu ? ((int64_t)p.T * p.R + (int64_t)p.B * (COLS - 1)) / COLS : (int64_t)p.B * ((p.R + COLS - 1) / COLS);
     const int64_t units = blocks * p.Nkv;
-    if (units >= ((int64_t)1 << 31)) {
+    if (units > (((int64_t)1 << 32) - 1) / (64 * CW * TW)) { // (threads of a grid)
       rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
       return;
     }
-    // items: some more than `target`, as the last part of every unit is one of its own
     const int64_t room = std::min<int64_t>(ws_bytes / (COLS * (32 * NJ + 2) * (int64_t)sizeof(float)), (((int64_t)1 << 31) - 1) / (COLS * 32 * NJ * 4));
     int64_t target = env_int("TPPX_PAGED_ITEMS", 0);
     if (target <= 0)
       target = COLS == 16 ? std::max<int64_t>(1024, 2 * units) : TW == 1 ? 512 : 256;
-    target = std::min<int64_t>(std::min<int64_t>(target, room), p.B <= 64 ? room : room - units);
+    target = std::min<int64_t>({target, room, (((int64_t)1 << 32) - 1) / (64 * CW * TW)});
     // A few pages hold no more than a part would: not worth the look at the lengths and the merge.
     if (target < units + p.Nkv || (p.g.table_ld << p.g.shift) <= 384)
       target = 0;

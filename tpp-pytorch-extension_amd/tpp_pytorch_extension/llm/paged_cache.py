@@ -78,8 +78,10 @@ def attn_paged(q, layer, table, past, cu_seqlens=None, parents=None):
     at, pages, page, table_at, table_ld = _pages(layer, table, Nkv, H, B, dev)
     up = _index(parents, "parents", T, dev) if parents is not None else None
     out = q.new_empty(T, Nq, H)
+    # (single tokens merge their parts in the launch itself, by counters that only the shared workspace has)
+    ws = _lib.workspace(q, own=cu_at is not None)
     _run(dev, _lib.lib().tppx_attn_paged, q_at, at, table_at, past_at, cu_at, up, out.data_ptr(), T, B, Nq, Nkv, H, pages, page, table_ld, q_ld,
-         *_lib.with_counters(_lib.workspace(q)))
+         *(_lib.with_counters(ws) if cu_at is None else (ws.data_ptr(), _lib.WORKSPACE_BYTES, None, 0)))
     return out
 
 
@@ -144,9 +146,9 @@ def verify_drafts(tokens, target, cu_seqlens=None, parents=None, draft=None, uni
     count = tokens.new_empty(B, dtype=I32)
     following = tokens.new_empty(B)
     need = _lib.lib().tppx_verify_drafts_bytes(T, B, V, draft is not None)
-    ws = torch.empty(need, dtype=torch.uint8, device=tokens.device) if need > _lib.WORKSPACE_BYTES else _lib.workspace(target)
+    ws = torch.empty(need, dtype=torch.uint8, device=tokens.device) if need > _lib.WORKSPACE_BYTES else _lib.workspace(target, own=True)
     _run(dev, _lib.lib().tppx_verify_drafts, tok, t_at, d_at, code, cu, up, u_at, s_at, temps, number, path.data_ptr(), count.data_ptr(),
-         following.data_ptr(), T, B, V, t_ld, d_ld, ws.data_ptr(), ws.numel())
+         following.data_ptr(), T, B, V, t_ld, d_ld, ws.data_ptr(), max(need, _lib.WORKSPACE_BYTES))
     return path, count, following
 
 
