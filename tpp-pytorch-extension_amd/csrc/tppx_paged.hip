@@ -6,6 +6,7 @@
 // a step ("nodes") are packed: sequence b owns rows cu[b] .. cu[b + 1] - 1 and held past[b] keys before them; cu null: one each.  Node i
 // goes to slot past + i.  parents[i] is the node of the same sequence that node i continues; without parents that is node i - 1.  All of
 // these arrays live on the device and are clamped there, so that no value in them leads out of a buffer.
+#include <limits.h>
 #include <math.h>
 #include <string.h>
 
@@ -160,15 +161,24 @@ struct PagedAttnParams {
   const uint16_t *q, *layer;
   const int32_t *past, *cu, *parents;
   uint16_t* out; // [T][Nq][H]
-  float* part;   // [item][cols][H], then, behind `items` of those, [item][cols][2]
-  int items;     // at most
+  float* part;   // [part][cols][H], then, behind `parts` of those, [part][cols][2], then the units to merge
+  int parts;     // at most
   unsigned int* counters;
   Pages g;
   int64_t q_ld;
   int T, B, Nq, Nkv, R;
-  int target, least; // items of a launch (0: units are not split), tiles of one at least
+  int target, least; // items of a launch that run at once (0: units are not split), tiles of one at least
+  int spare;         // there may be more of them
   float scale;
 };
+// what the merge has to know of a unit: parts (1: nothing to do), the first one's place, from one to the next, the last one's; its
+// K/V head, first row, columns in front of it and in it
+struct Merge {
+  int S, first, stride, last, hk, start, col0, ncol;
+};
+// [0].S: how many follow
+template <int COLS, int H>
+__device__ __forceinline__ Merge* merges_of(const PagedAttnParams& p) { return reinterpret_cast<Merge*>(p.part + (int64_t)p.parts * (COLS * (H + 2))); }
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef const __attribute__((address_space(4))) int32_t* ConstantInts; // (scalar loads)
@@ -177,13 +187,19 @@ constexpr int MAX_SPLITS = 64;
 constexpr int PAGED_NODES = 256;
 
 // The work of a launch, laid out on the device, where the lengths are: an item is a part of a unit's keys, a unit a block of a sequence's
-// columns for one K/V head.  The parts are of so many tiles that there are about `target` items in all, so that long sequences are split
-// where short ones are not.  Items of a sequence: [split][block][K/V head]; its first one, and its first unit, behind those of the
-// sequences before it.
+// columns for one K/V head.  Parts are of about `chunk` tiles: long sequences are split where short ones are not, and in all there are
+// no more than run at once.  Items of a sequence: [split][block][K/V head].
+// ROUNDS: as many units as fill whole rounds of what runs at once are not split and come first, then the parts of the others: all that
+// are of `chunk` tiles, of a sequence [split][block][K/V head], then the last ones, of the first keys, [block][K/V head].  If those are
+// short enough a few of them run one after another beside the others.  Blocks go down, the longest first.
 struct Item {
   Block o;           // sequence, its first row and nodes, block
-  int hk, split, S;  // of S splits
-  int first, stride; // item of the unit's first split, from one split's to the next one's
+  int hk, S;         // of S parts
+  int low, high;     // tiles
+  int first, stride; // the unit's first part, from one's to the next one's
+  int last, mine;    // its last part, this item's
+  int unit, units;   // its place among those that may be split, where this is the last part (else -1); how many there are, all told
+  __device__ __forceinline__ int part(int s) const { return s < S - 1 ? first + s * stride : last; }
 };
 // keys that the nodes of sequence b up to `last` see, of which that one sees most
 __device__ __forceinline__ int paged_past(const PagedAttnParams& p, int b) { return min(p.past[b], (int)(p.g.table_ld << p.g.shift)); }
@@ -204,15 +220,22 @@ __device__ __forceinline__ int scan_wave(int v) {
   v += from_lane<0x143, 0xc>(v); // row_bcast:31 into the upper rows
   return v;
 }
+__device__ __forceinline__ int max_of_wave(int v) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2)
+    v = max(v, __shfl_xor(v, d));
+  return v;
+}
 __device__ __forceinline__ int sum_of_wave(int v) { return __builtin_amdgcn_readlane(scan_wave(v), 63); }
-// Item blockIdx.x (units: unit blockIdx.x, its split 0); false past the last one.  All lanes of a wave take part.
-template <int COLS, int KEYS>
-__device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, bool units, Item& it) {
+// Item `id`; false past the last one.  All lanes of a wave take part.
+template <int COLS, int KEYS, bool ROUNDS>
+__device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, Item& it) {
   const int lane = threadIdx.x & 63;
   it.hk = id % p.Nkv;
+  it.units = 0;
   id /= p.Nkv;
   struct Seq {
-    int s, n, blocks, tiles;
+    int s, n, blocks, past;
   };
   auto seq = [&](int b) {
     Seq q = {0, 0, 0, 0};
@@ -221,51 +244,133 @@ __device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, bo
       q.s = s;
       q.n = max(e - s, 0);
       q.blocks = (int)(((int64_t)q.n * p.R + COLS - 1) / COLS);
-      q.tiles = q.n ? (paged_keys(p, paged_past(p, b), q.n - 1) + KEYS - 1) / KEYS : 0;
+      q.past = paged_past(p, b);
     }
     return q;
   };
+  auto tiles_of = [&](const Seq& z, int tail) { // of its first `tail` blocks, at most
+    return tail ? (paged_keys(p, z.past, !ROUNDS || tail == z.blocks ? z.n - 1 : (tail * COLS - 1) / p.R) + KEYS - 1) / KEYS : 0;
+  };
   Seq q = seq(lane);
-  int chunk = 1 << 30;
+  int chunk = 1 << 30, wholes = 0, full = 0; // whole parts, units of full rounds
+  bool even = true;                          // a sequence's parts as long as each other, no longer than `chunk`
+  auto parts_of = [&](int tiles) { return min(max((tiles + chunk - 1) / chunk, 1), MAX_SPLITS); };
   if (p.target > 0) {
-    int blocks = 0;
-    float tiles = 0.f; // of all units
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-      const Seq z = b0 ? seq(b0 + lane) : q;
-      blocks += sum_of_wave(z.blocks);
-      tiles += wave_sum((float)z.blocks * (float)z.tiles);
+    const int room = p.target / p.Nkv; // items of a K/V head that run at once
+    if (p.B <= 64) { // the smallest parts that all run at once, or whose rests run beside the whole ones one after another
+      int tail = q.blocks, blocks;
+      if constexpr (ROUNDS) {
+        const int upto = scan_wave(q.blocks);
+        blocks = __builtin_amdgcn_readlane(upto, 63);
+        if (p.spare) {
+          full = blocks / room * room;
+          blocks -= full;
+          tail = min(tail, max(upto - full, 0));
+        }
+      }
+      const int tiles = tiles_of(q, tail), longest = ROUNDS ? max_of_wave(tiles) : 0;
+      for (chunk = max(p.least, (int)(wave_sum((float)tail * (float)tiles) / (float)room)); __builtin_amdgcn_ballot_w64(tiles > chunk) != 0;
+           chunk += ROUNDS ? chunk / 16 + 1 : chunk / 8 + 1) {
+        const int S = parts_of(tiles);
+        if constexpr (ROUNDS) {
+          wholes = sum_of_wave(tail * (S - 1));
+          it.units = blocks;
+          if (wholes + blocks <= room)
+            break;
+          if (p.spare && wholes < room && chunk < longest - longest / 8) { // (less is not worth the merge)
+            const int rest = tail ? tiles - (S - 1) * chunk : 0;
+            even = wave_sum((float)tail * (float)rest) / (float)(room - wholes) + (float)max_of_wave(rest) > (float)chunk;
+            if (!even)
+              break;
+          }
+          wholes = it.units = 0;
+        } else if (sum_of_wave(tail * S) <= room) {
+          it.units = 1;
+          break;
+        }
+      }
+    } else {
+      int blocks = 0;
+      float tiles = 0.f; // of all units
+      for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const Seq z = b0 ? seq(b0 + lane) : q;
+        blocks += sum_of_wave(z.blocks);
+        tiles += wave_sum((float)z.blocks * (float)tiles_of(z, z.blocks));
+      }
+      if (room > blocks) { // (no more than tiles / chunk and one for each block; the sum is within 1 % of the true one)
+        chunk = max(p.least, (int)(tiles * 1.01f / (float)(room - blocks)) + 1);
+        it.units = blocks;
+        if constexpr (ROUNDS)
+          for (int b0 = 0; b0 < p.B; b0 += 64) {
+            const Seq z = b0 ? seq(b0 + lane) : q;
+            wholes += sum_of_wave(z.blocks * (parts_of(tiles_of(z, z.blocks)) - 1));
+          }
+      }
     }
-    const int room = p.target / p.Nkv; // items of a K/V head
-    if (p.B <= 64) { // the smallest parts that are no more items
-      chunk = max(p.least, (int)(tiles / (float)room));
-      while (__builtin_amdgcn_ballot_w64(q.tiles > chunk) != 0 && sum_of_wave(q.blocks * max((q.tiles + chunk - 1) / chunk, 1)) > room)
-        chunk += chunk / 8 + 1;
-    } else if (room > blocks) { // (no more than tiles / chunk and one for each block; the sum is within 1 % of the true one)
-      chunk = max(p.least, (int)(tiles * 1.01f / (float)(room - blocks)) + 1);
-    }
+    // what these come from is the same in all lanes, which the compiler does not see (without: up to 20 % more time of the kernel)
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+    wholes = __builtin_amdgcn_readfirstlane(wholes);
+    even = __builtin_amdgcn_readfirstlane(even) != 0;
+    it.units = __builtin_amdgcn_readfirstlane(it.units);
+    if (!ROUNDS && p.B <= 64 && it.units)
+      it.units = sum_of_wave(q.blocks);
+    it.units *= p.Nkv;
+    if ((full + wholes) * p.Nkv + it.units > (int)gridDim.x || it.units < 0) // (bounds that do not ascend)
+      it.units = 0;
   }
-  int before = 0, items_before = 0;
+  const bool whole = ROUNDS && id >= full && id < full + wholes;
+  if constexpr (ROUNDS)
+    id = whole ? id - full : id < full ? id : id - wholes;
+  int before = 0, other = 0; // of the counts that id is looked for in, and of the others: units, and whole parts or (not ROUNDS) all
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (b0)
       q = seq(b0 + lane);
-    const int S = min(max((q.tiles + chunk - 1) / chunk, 1), MAX_SPLITS), items = q.blocks * S, c = units ? q.blocks : items;
-    const int sum = scan_wave(c), all = units ? scan_wave(items) : sum;
+    const int upto = scan_wave(q.blocks);
+    int tail = q.blocks;
+    if constexpr (ROUNDS)
+      tail = min(q.blocks, max(upto - full, 0)); // (full: up to 64 sequences)
+    const int of_tail = tiles_of(q, tail), S = parts_of(of_tail), more = ROUNDS ? tail * (S - 1) : q.blocks * S, upto_more = scan_wave(more);
+    const bool by_more = whole || !ROUNDS;
+    const int sum = by_more ? upto_more : upto, sum_z = by_more ? upto : upto_more, c = by_more ? more : q.blocks, z = by_more ? q.blocks : more;
     const int total = __builtin_amdgcn_readlane(sum, 63);
     if (id < before + total) {
       const int j = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + sum > id));
-      const int blocks = __builtin_amdgcn_readlane(q.blocks, j), in = id - before - (__builtin_amdgcn_readlane(sum, j) - __builtin_amdgcn_readlane(c, j));
+      const int blocks = __builtin_amdgcn_readlane(q.blocks, j), tiles = __builtin_amdgcn_readlane(of_tail, j);
+      const int mine = before + __builtin_amdgcn_readlane(sum, j) - __builtin_amdgcn_readlane(c, j), in = id - mine;
+      const int its = other + __builtin_amdgcn_readlane(sum_z, j) - __builtin_amdgcn_readlane(z, j);
       it.o.b = b0 + j;
       it.o.start = __builtin_amdgcn_readlane(q.s, j);
       it.o.n = __builtin_amdgcn_readlane(q.n, j);
       it.S = __builtin_amdgcn_readlane(S, j);
-      it.split = in / blocks;
-      it.o.at = in - it.split * blocks;
-      it.first = (items_before + __builtin_amdgcn_readlane(all, j) - __builtin_amdgcn_readlane(items, j) + it.o.at) * p.Nkv + it.hk;
-      it.stride = blocks * p.Nkv;
+      if constexpr (ROUNDS) {
+        const int split_blocks = __builtin_amdgcn_readlane(tail, j), units_before = whole ? its : mine, wholes_before = whole ? mine : its;
+        const int split = whole ? in / split_blocks : 0, unit = whole ? blocks - split_blocks + in - split * split_blocks : in; // of the sequence
+        if (unit < blocks - split_blocks)
+          it.S = 1;
+        const int part = even ? (tiles + it.S - 1) / it.S : chunk;
+        it.o.at = blocks - 1 - unit;
+        it.low = whole ? max(tiles - (split + 1) * part, 0) : 0;
+        it.high = whole ? tiles - split * part : it.S > 1 ? tiles - (it.S - 1) * part : INT_MAX;
+        it.first = (wholes_before + unit - (blocks - split_blocks)) * p.Nkv + it.hk;
+        it.stride = split_blocks * p.Nkv;
+        it.last = (wholes + units_before + unit - full) * p.Nkv + it.hk;
+        it.mine = whole ? it.first + split * it.stride : it.last;
+        it.unit = whole ? -1 : (units_before + unit - full) * p.Nkv + it.hk;
+      } else {
+        const int split = in / blocks;
+        it.o.at = in - split * blocks;
+        it.low = (int)((int64_t)(it.S - 1 - split) * tiles / it.S);
+        it.high = (int)((int64_t)(it.S - split) * tiles / it.S);
+        it.first = (mine + it.o.at) * p.Nkv + it.hk;
+        it.stride = blocks * p.Nkv;
+        it.last = it.first + (it.S - 1) * it.stride;
+        it.mine = it.first + split * it.stride;
+        it.unit = split < it.S - 1 ? -1 : (its + it.o.at) * p.Nkv + it.hk;
+      }
       return true;
     }
     before += total;
-    items_before += __builtin_amdgcn_readlane(all, 63);
+    other += __builtin_amdgcn_readlane(sum_z, 63);
   }
   return false;
 }
@@ -284,13 +389,18 @@ paged_attn_kernel(const PagedAttnParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % CW, team = __builtin_amdgcn_readfirstlane(tid >> 6) / CW;
   const int g = lane >> 4, c = lane & 15;
   Item it;
-  if (!locate_item<COLS, KEYS>(p, (int)blockIdx.x, false, it))
+  const bool any = locate_item<COLS, KEYS, TW == 1>(p, (int)blockIdx.x, it);
+  if (p.target > 0 && !p.counters && tid == 0 && blockIdx.x == 0)
+    merges_of<COLS, H>(p)->S = it.units;
+  if (!any)
     return;
   const Block& o = it.o;
   const int hk = it.hk, col0 = o.at * COLS, ncol = min(COLS, o.n * p.R - col0); // of this workgroup
   const int past = paged_past(p, o.b), keys = paged_keys(p, past, (col0 + ncol - 1) / p.R); // that some column sees
   const int tiles = (keys + KEYS - 1) / KEYS, S = it.S;
   const bool idle = wave * WCOLS >= ncol;
+  if (tid == 0 && !p.counters && it.unit >= 0 && it.unit < it.units)
+    merges_of<COLS, H>(p)[1 + it.unit] = Merge{S, it.first, it.stride, it.last, hk, o.start, col0, ncol};
   const int32_t* const parents = p.parents ? p.parents + o.start : nullptr;
   int node[CG], up[CG]; // of this lane's columns; where their ways up have come to
   bf16x8 q[CG][NJ];
@@ -303,8 +413,8 @@ paged_attn_kernel(const PagedAttnParams p) {
     for (int j = 0; j < NJ; j++)
       q[k][j] = *reinterpret_cast<const bf16x8*>(qrow + j * 32);
   }
-  // Tiles top, top - TW, .. of this team, down to the split's last one.
-  const int low = (int)((int64_t)(S - 1 - it.split) * tiles / S), top = (int)((int64_t)(S - it.split) * tiles / S) - 1 - team, most = (top + team - low) / TW + 1;
+  // Tiles top, top - TW, .. of this team, down to the part's last one.
+  const int low = it.low, top = min(it.high, tiles) - 1 - team, most = (top + team - low) / TW + 1;
   const ConstantInts table = (ConstantInts)(uintptr_t)(p.g.table + (int64_t)o.b * p.g.table_ld);
   const int64_t values = (((int64_t)p.g.pages * p.Nkv) << p.g.shift) * H;
   int ids[MINE]; // pages of this wave's runs of the tile that is asked for next
@@ -554,9 +664,8 @@ paged_attn_kernel(const PagedAttnParams p) {
   };
   // A split's results for the merge: stores and loads at the scope of the device, written through to the level that all XCDs share.
   constexpr int SHARED = 16; // (sc1)
-  const int split_items = p.target > 0 ? p.items : 0; // (those fit into 31 bits)
-  const auto part = __builtin_amdgcn_make_buffer_rsrc(p.part, 0, split_items * (COLS * H * 4), 0x00020000);
-  const auto part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)split_items * COLS * H, 0, split_items * (COLS * 8), 0x00020000);
+  const auto part = __builtin_amdgcn_make_buffer_rsrc(p.part, 0, p.parts * (COLS * H * 4), 0x00020000);
+  const auto part_ml = __builtin_amdgcn_make_buffer_rsrc(p.part + (int64_t)p.parts * COLS * H, 0, p.parts * (COLS * 8), 0x00020000);
   if (TW == 1 && S == 1) {
 #pragma unroll
     for (int k = 0; k < CG; k++) {
@@ -604,7 +713,7 @@ paged_attn_kernel(const PagedAttnParams p) {
       if (S == 1) {
         store4(cl, d4 * 4, v, Ls);
       } else {
-        const int at = (int)blockIdx.x * COLS + cl;
+        const int at = it.mine * COLS + cl;
         if (p.counters) {
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), part, (at * H + d4 * 4) * 4, 0, SHARED);
           if (d4 == 0)
@@ -624,7 +733,7 @@ paged_attn_kernel(const PagedAttnParams p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0)
-    arrived_last = atomicInc(p.counters + (int64_t)it.first * MX4_COUNTER_STRIDE, (unsigned)S - 1) == (unsigned)S - 1;
+    arrived_last = atomicInc(p.counters + (int64_t)it.last * MX4_COUNTER_STRIDE, (unsigned)S - 1) == (unsigned)S - 1;
   __syncthreads();
   if (!arrived_last)
     return;
@@ -635,13 +744,13 @@ paged_attn_kernel(const PagedAttnParams p) {
     const int cc = i / (H / 4), d4 = i % (H / 4);
 #pragma unroll
     for (int u = 0; u < 8; u++) // (past the last one: that again)
-      a[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, ((it.first + min(s0 + u, S - 1) * it.stride) * COLS + cc) * (H * 4) + d4 * 16, 0, SHARED));
+      a[u] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(part, (it.part(min(s0 + u, S - 1)) * COLS + cc) * (H * 4) + d4 * 16, 0, SHARED));
   };
   if (tid < ncol * (H / 4))
     fetch(tid, 0);
   float* const merged = reinterpret_cast<float*>(lds); // [col][MAX_SPLITS + 1]: weights of the splits, then the sum
   for (int cc = wave_; cc < ncol; cc += TH / 64) { // a lane per split
-    float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_ml, ((it.first + min(lane_, S - 1) * it.stride) * COLS + cc) * 8, 0, SHARED));
+    float2 ml = __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(part_ml, (it.part(min(lane_, S - 1)) * COLS + cc) * 8, 0, SHARED));
     if (lane_ >= S)
       ml = float2{LOWEST, 0.f};
     float M = ml.x;
@@ -674,23 +783,22 @@ paged_attn_kernel(const PagedAttnParams p) {
 }
 
 // The splits' results of launches with many columns: a thread takes four channels of a column, all splits.
-template <int NJ, int COLS, int KEYS>
+template <int NJ, int COLS>
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(const PagedAttnParams p) {
   constexpr int H = 32 * NJ, EACH = H / 4, PER = 256 / EACH; // threads of a column, columns of a workgroup
-  Item it;
-  if (!locate_item<COLS, KEYS>(p, (int)blockIdx.x, true, it) || it.S == 1)
+  const Merge* const all = merges_of<COLS, H>(p);
+  const int units = all->S;
+  const Merge it = all[1 + blockIdx.x];
+  if ((int)blockIdx.x >= units || it.S == 1)
     return;
-  if ((int64_t)it.first + (int64_t)(it.S - 1) * it.stride >= p.items || it.first < 0)
-    return; // (bounds that do not ascend: more items than were launched)
-  const int S = it.S, col0 = it.o.at * COLS, ncol = min(COLS, it.o.n * p.R - col0);
+  const int S = it.S;
   const int d4 = (int)threadIdx.x % EACH;
   if ((int)threadIdx.x >= PER * EACH)
     return;
-  for (int cc = (int)blockIdx.y * PER + (int)threadIdx.x / EACH; cc < ncol; cc += (int)gridDim.y * PER) {
-    const int64_t at = (int64_t)it.first * COLS + cc, step = (int64_t)it.stride * COLS;
-    const float* const part = p.part + at * H + d4 * 4;
-    const float2* const ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.items * COLS * H) + at;
+  for (int cc = (int)blockIdx.y * PER + (int)threadIdx.x / EACH; cc < it.ncol; cc += (int)gridDim.y * PER) {
+    const float* const part = p.part + cc * H + d4 * 4;
+    const float2* const ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.parts * COLS * H) + cc;
     float M = LOWEST, L = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < S; s0 += 8) { // eight parts' loads at a time
@@ -698,7 +806,7 @@ paged_merge_kernel(const PagedAttnParams p) {
       f32x4 a[8];
 #pragma unroll
       for (int u = 0; u < 8; u++) {
-        const int64_t i = min(s0 + u, S - 1) * step;
+        const int64_t i = (int64_t)(s0 + u < S - 1 ? it.first + (s0 + u) * it.stride : it.last) * COLS;
         z[u] = ml[i];
         a[u] = *reinterpret_cast<const f32x4*>(part + i * H);
       }
@@ -720,8 +828,8 @@ paged_merge_kernel(const PagedAttnParams p) {
       }
     }
     const float inv = L != 0.f ? 1.0f / L : 0.f;
-    const int cl = col0 + cc, nd = cl / p.R;
-    *reinterpret_cast<uint2*>(p.out + ((int64_t)(it.o.start + nd) * p.Nq + it.hk * p.R + cl - nd * p.R) * H + d4 * 4) =
+    const int cl = it.col0 + cc, nd = cl / p.R;
+    *reinterpret_cast<uint2*>(p.out + ((int64_t)(it.start + nd) * p.Nq + it.hk * p.R + cl - nd * p.R) * H + d4 * 4) =
         make_uint2(f32x2_to_bf16_bits(v[0] * inv, v[1] * inv), f32x2_to_bf16_bits(v[2] * inv, v[3] * inv));
   }
 }
@@ -788,25 +896,27 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     constexpr int NJ = decltype(nj)::value, CG = decltype(cg)::value, CW = decltype(cw)::value, TW = decltype(tw)::value, KEYS = decltype(kt)::value, COLS = 16 * CG * CW;
     const int64_t blocks = p.cu ? ((int64_t)p.T * p.R + (int64_t)p.B * (COLS - 1)) / COLS : (int64_t)p.B * ((p.R + COLS - 1) / COLS);
     const int64_t units = blocks * p.Nkv;
-    if (units > (((int64_t)1 << 32) - 1) / (64 * CW * TW)) { // (threads of a grid)
+    if (units > ((int64_t)1 << 31) / (64 * CW * TW)) { // (threads of a grid)
       rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
       return;
     }
-    const int64_t room = std::min<int64_t>(ws_bytes / (COLS * (32 * NJ + 2) * (int64_t)sizeof(float)), (((int64_t)1 << 31) - 1) / (COLS * 32 * NJ * 4));
+    const int64_t room = std::min<int64_t>(std::max<int64_t>(ws_bytes - (int64_t)sizeof(Merge), 0) / (COLS * (32 * NJ + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(Merge)), (((int64_t)1 << 31) - 1) / (COLS * 32 * NJ * 4));
     int64_t target = env_int("TPPX_PAGED_ITEMS", 0);
     if (target <= 0)
       target = COLS == 16 ? std::max<int64_t>(1024, 2 * units) : TW == 1 ? 512 : 256;
-    target = std::min<int64_t>({target, room, (((int64_t)1 << 32) - 1) / (64 * CW * TW)});
+    target = std::min<int64_t>({target, room, ((int64_t)1 << 31) / (64 * CW * TW)});
     // A few pages hold no more than a part would: not worth the look at the lengths and the merge.
-    if (target < units + p.Nkv || (p.g.table_ld << p.g.shift) <= 384)
+    p.spare = TW == 1 && p.B <= 64 && 2 * target <= room;
+    if ((!p.spare && target < units + p.Nkv) || target < p.Nkv || (p.g.table_ld << p.g.shift) <= 384)
       target = 0;
     p.least = std::max(env_int("TPPX_PAGED_LEAST", 256) / KEYS, 1);
     // no more than the capacity would make: a workgroup without work waits for room on a CU like any other
     const int64_t most = ((p.g.table_ld << p.g.shift) / KEYS + p.least) / p.least;
     target = std::min<int64_t>(target, units * most);
     p.target = (int)target;
-    p.items = (int)std::max<int64_t>(target, units);
-    const bool here = COLS == 16 && p.R <= 16 && !p.cu && p.items * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) <= counter_bytes;
+    p.parts = (int)(p.spare ? 2 * target : target); // (whole ones are fewer than `target`, and so are the units that are split)
+    const int64_t items = p.spare ? target + units : std::max<int64_t>(target, units);
+    const bool here = COLS == 16 && p.R <= 16 && !p.cu && p.parts * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) <= counter_bytes;
     if (!here)
       p.counters = nullptr;
     const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ, teams = TW > 1 || target ? TW * COLS * (32 * NJ + 6) * sizeof(float) : 0; // (the merge's weights take less)
@@ -815,10 +925,12 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
     if (e != hipSuccess)
       return;
-    kern<<<dim3((unsigned)p.items), dim3(64 * CW * TW), lds, stream>>>(p);
+    kern<<<dim3((unsigned)items), dim3(64 * CW * TW), lds, stream>>>(p);
     constexpr int PER = 256 / (8 * NJ);
-    if (target && !here) // (units that were not split end at once: not too many of those)
-      paged_merge_kernel<NJ, COLS, KEYS><<<dim3((unsigned)units, (unsigned)std::min<int64_t>((COLS + PER - 1) / PER, std::max<int64_t>(4096 / units, 1))), dim3(256), 0, stream>>>(p);
+    if (target && !here) { // (units that were not split end at once: not too many of those)
+      const int64_t split = p.spare ? std::min(target, units) : units;
+      paged_merge_kernel<NJ, COLS><<<dim3((unsigned)split, (unsigned)std::min<int64_t>((COLS + PER - 1) / PER, std::max<int64_t>(4096 / split, 1))), dim3(256), 0, stream>>>(p);
+    }
   };
   const int64_t cols = (p.cu ? (p.T + p.B - 1) / p.B : 1) * (int64_t)p.R; // of a sequence's K/V head, on average
   // units of c columns, about: pieces of prompts as if they were equally long, the last block of a tree half empty
@@ -831,7 +943,7 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
   const int form = env_int("TPPX_PAGED_FORM", 0);
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
-    const int f = form ? form : cols <= 16 ? 1 : cols <= 32 ? 2 : units_of(64) <= 280 ? 3 : cols >= 512 && units_of(128) <= 280 ? 5 : 4;
+    const int f = form ? form : cols <= 16 ? 1 : cols <= 32 ? 2 : units_of(64) <= 280 && units_of(64) * (p.g.table_ld << p.g.shift) < 800000 ? 3 : 4;
     if constexpr (NJ > 4) {
       if (f == 1 || f == 2)
         go(nj, n1, n1, n2, k32);
@@ -846,10 +958,8 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
         go(nj, n2, n1, n4, k32);
       else if (f == 3)
         go(nj, n2, n2, n4, k32);
-      else if (f == 4)
-        go(nj, n2, n4, n1, k64);
       else
-        go(nj, n2, n4, n2, k32);
+        go(nj, n2, n4, n1, k64);
     }
   });
   if (rc)

@@ -78,10 +78,11 @@ def attn_paged(q, layer, table, past, cu_seqlens=None, parents=None):
     at, pages, page, table_at, table_ld = _pages(layer, table, Nkv, H, B, dev)
     up = _index(parents, "parents", T, dev) if parents is not None else None
     out = q.new_empty(T, Nq, H)
-    # (single tokens merge their parts in the launch itself, by counters that only the shared workspace has)
-    ws = _lib.workspace(q, own=cu_at is not None)
+    # Single tokens merge their parts in the launch itself, by counters that only the shared workspace has.  Two parts of 128 columns for
+    # every workgroup that can run, 66 KB each, do not fit in there.
+    ws = _lib.workspace(q, own=cu_at is not None) if T * Nq * H < 1 << 20 or cu_at is None else torch.empty(72 << 20, dtype=torch.uint8, device=q.device)
     _run(dev, _lib.lib().tppx_attn_paged, q_at, at, table_at, past_at, cu_at, up, out.data_ptr(), T, B, Nq, Nkv, H, pages, page, table_ld, q_ld,
-         *(_lib.with_counters(ws) if cu_at is None else (ws.data_ptr(), _lib.WORKSPACE_BYTES, None, 0)))
+         *(_lib.with_counters(ws) if cu_at is None else (ws.data_ptr(), ws.numel(), None, 0)))
     return out
 
 
