@@ -167,8 +167,8 @@ struct PagedAttnParams {
   Pages g;
   int64_t q_ld;
   int T, B, Nq, Nkv, R;
-  int target, least; // items of a launch that run at once (0: units are not split), tiles of one at least
-  int spare;         // there may be more of them
+  int target, most;  // items of a launch that run at once (0: units are not split), that there may be
+  int least;         // tiles of one at least
   float scale;
 };
 // what the merge has to know of a unit: parts (1: nothing to do), the first one's place, from one to the next, the last one's; its
@@ -220,13 +220,27 @@ __device__ __forceinline__ int scan_wave(int v) {
   v += from_lane<0x143, 0xc>(v); // row_bcast:31 into the upper rows
   return v;
 }
-__device__ __forceinline__ int max_of_wave(int v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2)
-    v = max(v, __shfl_xor(v, d));
-  return v;
-}
 __device__ __forceinline__ int sum_of_wave(int v) { return __builtin_amdgcn_readlane(scan_wave(v), 63); }
+__device__ __forceinline__ int max_of_wave(int v) { // of none below 0
+  v = max(v, from_lane<0x111, 0xf>(v));
+  v = max(v, from_lane<0x112, 0xf>(v));
+  v = max(v, from_lane<0x114, 0xf>(v));
+  v = max(v, from_lane<0x118, 0xf>(v));
+  v = max(v, from_lane<0x142, 0xa>(v));
+  v = max(v, from_lane<0x143, 0xc>(v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ float sum_of_wave(float v) {
+  auto add = [&](auto c, auto r) { v += __int_as_float(from_lane<decltype(c)::value, decltype(r)::value>(__float_as_int(v))); };
+  constexpr std::integral_constant<int, 15> all{};
+  add(std::integral_constant<int, 0x111>{}, all);
+  add(std::integral_constant<int, 0x112>{}, all);
+  add(std::integral_constant<int, 0x114>{}, all);
+  add(std::integral_constant<int, 0x118>{}, all);
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 10>{});
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 12>{});
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
 // Item `id`; false past the last one.  All lanes of a wave take part.
 template <int COLS, int KEYS, bool ROUNDS>
 __device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, Item& it) {
@@ -256,49 +270,52 @@ __device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, It
   bool even = true;                          // a sequence's parts as long as each other, no longer than `chunk`
   auto parts_of = [&](int tiles) { return min(max((tiles + chunk - 1) / chunk, 1), MAX_SPLITS); };
   if (p.target > 0) {
-    const int room = p.target / p.Nkv; // items of a K/V head that run at once
-    if (p.B <= 64) { // the smallest parts that all run at once, or whose rests run beside the whole ones one after another
-      int tail = q.blocks, blocks;
-      if constexpr (ROUNDS) {
-        const int upto = scan_wave(q.blocks);
-        blocks = __builtin_amdgcn_readlane(upto, 63);
-        if (p.spare) {
-          full = blocks / room * room;
-          blocks -= full;
-          tail = min(tail, max(upto - full, 0));
-        }
-      }
-      const int tiles = tiles_of(q, tail), longest = ROUNDS ? max_of_wave(tiles) : 0;
-      for (chunk = max(p.least, (int)(wave_sum((float)tail * (float)tiles) / (float)room)); __builtin_amdgcn_ballot_w64(tiles > chunk) != 0;
-           chunk += ROUNDS ? chunk / 16 + 1 : chunk / 8 + 1) {
+    const int room = p.target / p.Nkv, room_most = p.most / p.Nkv; // items of a K/V head
+    if (ROUNDS && p.B <= 64) { // the smallest parts that all run at once, or whose rests run beside the whole ones one after another
+      const int upto = scan_wave(q.blocks);
+      int blocks = __builtin_amdgcn_readlane(upto, 63);
+      full = blocks / room * room;
+      blocks -= full;
+      const int tail = min(q.blocks, max(upto - full, 0));
+      const int tiles = tiles_of(q, tail), longest = max_of_wave(tiles);
+      for (chunk = max(p.least, (int)(sum_of_wave((float)tail * (float)tiles) / (float)room)); longest > chunk; chunk += chunk / 16 + 1) {
         const int S = parts_of(tiles);
-        if constexpr (ROUNDS) {
-          wholes = sum_of_wave(tail * (S - 1));
-          it.units = blocks;
-          if (wholes + blocks <= room)
-            break;
-          if (p.spare && wholes < room && chunk < longest - longest / 8) { // (less is not worth the merge)
-            const int rest = tail ? tiles - (S - 1) * chunk : 0;
-            even = wave_sum((float)tail * (float)rest) / (float)(room - wholes) + (float)max_of_wave(rest) > (float)chunk;
-            if (!even)
-              break;
-          }
-          wholes = it.units = 0;
-        } else if (sum_of_wave(tail * S) <= room) {
-          it.units = 1;
+        wholes = sum_of_wave(tail * (S - 1));
+        it.units = blocks;
+        if (wholes + blocks <= room)
           break;
+        if (wholes < room && chunk < longest - longest / 8) { // (less is not worth the merge)
+          const int rest = tail ? tiles - (S - 1) * chunk : 0;
+          even = sum_of_wave((float)tail * (float)rest) / (float)(room - wholes) + (float)max_of_wave(rest) > (float)chunk;
+          if (!even)
+            break;
         }
+        wholes = it.units = 0;
       }
     } else {
-      int blocks = 0;
-      float tiles = 0.f; // of all units
-      for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const Seq z = b0 ? seq(b0 + lane) : q;
+      int tiles = tiles_of(q, q.blocks), blocks = sum_of_wave(q.blocks);
+      float sum = sum_of_wave((float)q.blocks * (float)tiles); // of all units' tiles
+      for (int b0 = 64; b0 < p.B; b0 += 64) {
+        const Seq z = seq(b0 + lane);
+        const int more = tiles_of(z, z.blocks);
         blocks += sum_of_wave(z.blocks);
-        tiles += wave_sum((float)z.blocks * (float)tiles_of(z, z.blocks));
+        sum += sum_of_wave((float)z.blocks * (float)more);
+        tiles = max(tiles, more); // (of this lane's, the longest)
       }
-      if (room > blocks) { // (no more than tiles / chunk and one for each block; the sum is within 1 % of the true one)
-        chunk = max(p.least, (int)(tiles * 1.01f / (float)(room - blocks)) + 1);
+      const float each = sum / (float)room; // of what runs at once
+      if (blocks > room && __builtin_amdgcn_ballot_w64((float)tiles > each * 1.2f) == 0) {
+        // more units than that, none of them long: as they are
+      } else if (p.B <= 64) { // the smallest parts that all run at once; if that leaves too much idle, more of them
+        for (int items = blocks > room ? room_most : room;; items = room_most) {
+          for (chunk = max(p.least, (int)(sum / (float)items)); __builtin_amdgcn_ballot_w64(tiles > chunk) != 0; chunk += chunk / 8 + 1)
+            if (sum_of_wave(q.blocks * parts_of(tiles)) <= items)
+              break;
+          if (items == room_most || (float)chunk <= fmaxf(each * 1.4f, 2048.f / KEYS))
+            break;
+        }
+        it.units = __builtin_amdgcn_ballot_w64(tiles > chunk) != 0 ? blocks : 0;
+      } else if (room_most > blocks) { // (no more than tiles / chunk and one for each block; the sum is within 1 % of the true one)
+        chunk = max(p.least, (int)(sum * 1.01f / (float)(room_most - blocks)) + 1);
         it.units = blocks;
         if constexpr (ROUNDS)
           for (int b0 = 0; b0 < p.B; b0 += 64) {
@@ -312,8 +329,6 @@ __device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, It
     wholes = __builtin_amdgcn_readfirstlane(wholes);
     even = __builtin_amdgcn_readfirstlane(even) != 0;
     it.units = __builtin_amdgcn_readfirstlane(it.units);
-    if (!ROUNDS && p.B <= 64 && it.units)
-      it.units = sum_of_wave(q.blocks);
     it.units *= p.Nkv;
     if ((full + wholes) * p.Nkv + it.units > (int)gridDim.x || it.units < 0) // (bounds that do not ascend)
       it.units = 0;
@@ -325,7 +340,7 @@ __device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, It
   for (int b0 = 0; b0 < p.B; b0 += 64) {
     if (b0)
       q = seq(b0 + lane);
-    const int upto = scan_wave(q.blocks);
+    const int upto = ROUNDS || !p.counters ? scan_wave(q.blocks) : 0; // (with counters nobody asks for units)
     int tail = q.blocks;
     if constexpr (ROUNDS)
       tail = min(q.blocks, max(upto - full, 0)); // (full: up to 64 sequences)
@@ -900,26 +915,34 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
       rc = set_error(TPPX_ESHAPE, "%s: problem too large", who);
       return;
     }
+    const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ;
     const int64_t room = std::min<int64_t>(std::max<int64_t>(ws_bytes - (int64_t)sizeof(Merge), 0) / (COLS * (32 * NJ + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(Merge)), (((int64_t)1 << 31) - 1) / (COLS * 32 * NJ * 4));
+    // what runs at once: two workgroups on a CU where the LDS has room for them
     int64_t target = env_int("TPPX_PAGED_ITEMS", 0);
     if (target <= 0)
-      target = COLS == 16 ? std::max<int64_t>(1024, 2 * units) : TW == 1 ? 512 : 256;
-    target = std::min<int64_t>({target, room, ((int64_t)1 << 31) / (64 * CW * TW)});
-    // A few pages hold no more than a part would: not worth the look at the lengths and the merge.
-    p.spare = TW == 1 && p.B <= 64 && 2 * target <= room;
-    if ((!p.spare && target < units + p.Nkv) || target < p.Nkv || (p.g.table_ld << p.g.shift) <= 384)
-      target = 0;
-    p.least = std::max(env_int("TPPX_PAGED_LEAST", 256) / KEYS, 1);
+      target = 256 * (TW == 1 || stages <= 80 * 1024 ? 2 : 1);
     // no more than the capacity would make: a workgroup without work waits for room on a CU like any other
-    const int64_t most = ((p.g.table_ld << p.g.shift) / KEYS + p.least) / p.least;
-    target = std::min<int64_t>(target, units * most);
+    const int64_t capacity = p.g.table_ld << p.g.shift, limit = std::min<int64_t>(room, ((int64_t)1 << 31) / (64 * CW * TW));
+    p.least = std::max(env_int("TPPX_PAGED_LEAST", COLS == 16 ? 512 : 256) / KEYS, 1);
+    target = std::min<int64_t>({target, limit, units * ((capacity / KEYS + p.least) / p.least)});
+    const bool rounds = TW == 1 && p.B <= 64;
+    int64_t most; // (rounds: whole parts are fewer than `target`, and so are the units that are split)
+    if (rounds) {
+      target = std::min(target, room / 2);
+      most = 2 * target;
+    } else { // (few units: parts of equal lengths come near enough to the same)
+      most = std::min<int64_t>({4 * units <= target || capacity < 4096 ? std::max(target, units + p.Nkv) : (units / target + 2) * target, limit, units * ((capacity / KEYS + p.least) / p.least)});
+    }
+    // A few pages hold no more than a part would: not worth the look at the lengths and the merge.
+    if (target < p.Nkv || (!rounds && most < units + p.Nkv) || capacity <= 384)
+      target = most = 0;
     p.target = (int)target;
-    p.parts = (int)(p.spare ? 2 * target : target); // (whole ones are fewer than `target`, and so are the units that are split)
-    const int64_t items = p.spare ? target + units : std::max<int64_t>(target, units);
+    p.most = p.parts = (int)most;
+    const int64_t items = rounds ? target + units : std::max<int64_t>(most, units);
     const bool here = COLS == 16 && p.R <= 16 && !p.cu && p.parts * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) <= counter_bytes;
     if (!here)
       p.counters = nullptr;
-    const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ, teams = TW > 1 || target ? TW * COLS * (32 * NJ + 6) * sizeof(float) : 0; // (the merge's weights take less)
+    const size_t teams = TW > 1 || target ? TW * COLS * (32 * NJ + 6) * sizeof(float) : 0; // (the merge's weights take less)
     const size_t lds = std::max(stages, teams);
     auto kern = paged_attn_kernel<NJ, CG, CW, TW, KEYS>;
     e = allow_dynamic_lds(reinterpret_cast<const void*>(kern), lds);
@@ -928,7 +951,7 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     kern<<<dim3((unsigned)items), dim3(64 * CW * TW), lds, stream>>>(p);
     constexpr int PER = 256 / (8 * NJ);
     if (target && !here) { // (units that were not split end at once: not too many of those)
-      const int64_t split = p.spare ? std::min(target, units) : units;
+      const int64_t split = rounds ? std::min(target, units) : units;
       paged_merge_kernel<NJ, COLS><<<dim3((unsigned)split, (unsigned)std::min<int64_t>((COLS + PER - 1) / PER, std::max<int64_t>(4096 / split, 1))), dim3(256), 0, stream>>>(p);
     }
   };
