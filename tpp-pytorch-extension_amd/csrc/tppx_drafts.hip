@@ -51,7 +51,7 @@ struct DraftsParams {
   NodeShare* nodes; // [T], of those
   int64_t t_ld, d_ld;
   int T, B, V, C, sides;
-  float temperature;
+  double to2; // of the temperature, where that is a number
 };
 constexpr double LOG2E_64 = 1.4426950408889634;
 
@@ -99,10 +99,11 @@ struct ManyWeights {
   double k, magic;
   float lowest;
   __device__ __forceinline__ ManyWeights(const double* t, float top, double to2)
-      : table(t), k(to2 * 256.0), magic(0x1.8p52 - __builtin_rint((double)top * (to2 * 256.0))), lowest(top - 900.0f / (float)to2) {}
+      : table(t), k(to2 * 256.0), magic(0x1.8p52 - __builtin_rint((double)top * (to2 * 256.0))), lowest(top - 900.0f * __builtin_amdgcn_rcpf((float)to2)) {}
   static __device__ __forceinline__ bool fits(float top, double to2) { return fabsf(top) < 1e5f && to2 < 64.0 && to2 > 1e-6 && fabsf(top) * (float)to2 < 1e6f; }
-  // what the sum of the weights relative to the maximum is that of these times
-  __device__ __forceinline__ double off(float top) const { return exp2_64(((0x1.8p52 - magic) - (double)top * k) * (1.0 / 256.0)); }
+  // what the sum of the weights relative to the maximum is that of these times, and its logarithm
+  __device__ __forceinline__ double log_off(float top) const { return ((0x1.8p52 - magic) - (double)top * k) * (1.0 / 256.0); }
+  __device__ __forceinline__ double off(float top) const { return exp2_64(log_off(top)); }
   // 2^(n / 256), and what is left
   __device__ __forceinline__ double parts(float x, double& g) const {
     float c;
@@ -140,7 +141,9 @@ __device__ __forceinline__ float logit_of(E v) { // (what is no number is no tok
 }
 // 0: the first maximum alone (for what is no positive finite temperature, too)
 __device__ __forceinline__ double to2_of(const DraftsParams& p, int b) {
-  const float t = p.temps ? p.temps[b] : p.temperature;
+  if (!p.temps)
+    return p.to2;
+  const float t = p.temps[b];
   return t > 0.f && t < INFINITY ? LOG2E_64 / (double)t : 0.0;
 }
 
@@ -205,6 +208,38 @@ __device__ __forceinline__ void load_logits(const E* row, int at, int V, float (
   }
 }
 
+__device__ __forceinline__ double add64(double a, double z) { return a + z; }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from_lane(double v) { // (0 where there is no such lane)
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, ROWS == 0xf);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, ROWS == 0xf);
+  return __hiloint2double(hi, lo);
+}
+// sum over the lanes below, and this one's; all lanes take part
+__device__ __forceinline__ double scan64(double v) {
+  v += from_lane<0x111, 0xf>(v); // row_shr:1
+  v += from_lane<0x112, 0xf>(v);
+  v += from_lane<0x114, 0xf>(v);
+  v += from_lane<0x118, 0xf>(v);
+  v += from_lane<0x142, 0xa>(v); // row_bcast:15 into the second and the last row
+  v += from_lane<0x143, 0xc>(v); // row_bcast:31 into the upper rows
+  return v;
+}
+
+// the largest of a wave, in all lanes
+__device__ __forceinline__ float top_of_wave(float v) {
+  auto step = [&](auto c, auto r) {
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), decltype(c)::value, decltype(r)::value, 0xf, false)));
+  };
+  constexpr std::integral_constant<int, 15> all{};
+  step(std::integral_constant<int, 0x111>{}, all);
+  step(std::integral_constant<int, 0x112>{}, all);
+  step(std::integral_constant<int, 0x114>{}, all);
+  step(std::integral_constant<int, 0x118>{}, all);
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 10>{});
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 12>{});
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
 template <int N, typename F>
 __device__ __forceinline__ double reduce_lanes(double v, F&& f) {
 #pragma unroll
@@ -222,9 +257,9 @@ draft_rows_kernel(const DraftsParams p) {
   constexpr int N = per16<E>();
   __shared__ float tops[4];
   __shared__ int firsts[4];
-  __shared__ double sums[4];
+  __shared__ double sums[4], offs[4]; // of a wave, relative to 2^off times the weight of its maximum
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = (int)(blockIdx.x / (unsigned)p.C), piece = (int)(blockIdx.x % (unsigned)p.C), side = (int)blockIdx.y;
+  const int row = (int)blockIdx.x, piece = (int)blockIdx.y, side = (int)blockIdx.z;
   int b = 0;
   if (p.temps || side) {
     b = p.cu ? sequence_of(p.cu, p.B, row) : row;
@@ -236,7 +271,7 @@ draft_rows_kernel(const DraftsParams p) {
   const E* const at = (const E*)(side ? p.draft : p.target) + (int64_t)row * (side ? p.d_ld : p.t_ld);
   const int from = piece * (DRAFT_THREADS * NV * N);
   int first = p.V;
-  double sum = 0.0;
+  double sum = 0.0, off = 0.0;
   float top = -INFINITY;
   bool done = false; // (uniform in a wave)
   if (NV > 1 && to2 != 0.0) {
@@ -255,9 +290,7 @@ draft_rows_kernel(const DraftsParams p) {
       for (int e = 0; e < N; e += 2)
         asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top) : "v"(x[e]), "v"(x[e + 1]));
     }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2)
-      top = fmaxf(top, __shfl_xor(top, d));
+    top = top_of_wave(top);
     if (from + wave * (64 * N) >= p.V) { // (behind the end)
       done = true;
     } else if (ManyWeights::fits(top, to2)) {
@@ -268,7 +301,8 @@ draft_rows_kernel(const DraftsParams p) {
         raw_logits<E>(v[i], x);
         sum = many.sum(x, sum);
       }
-      sum = reduce_lanes<64>(sum, [](double a, double z) { return a + z; }) * many.off(top);
+      sum = __shfl(scan64(sum), 63);
+      off = many.log_off(top);
       done = sum > 0.0; // (and no NaN)
     }
   }
@@ -283,10 +317,8 @@ draft_rows_kernel(const DraftsParams p) {
 #pragma unroll
       for (int e = 0; e < N; e++)
         top = fmaxf(top, x[i][e]);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2)
-      top = fmaxf(top, __shfl_xor(top, d));
-    sum = 0.0;
+    top = top_of_wave(top);
+    sum = off = 0.0;
     if (to2 == 0.0) {
 #pragma unroll
       for (int i = NV - 1; i >= 0; i--)
@@ -306,24 +338,30 @@ draft_rows_kernel(const DraftsParams p) {
           const double w = weight_of(x[i][e], top, to2);
           sum += from + (i * DRAFT_THREADS + tid) * N + e < p.V ? w : 0.0;
         }
-      sum = reduce_lanes<64>(sum, [](double a, double z) { return a + z; });
+      sum = __shfl(scan64(sum), 63);
     }
   }
   if (lane == 0) {
     tops[wave] = top;
     firsts[wave] = first;
     sums[wave] = sum;
+    offs[wave] = off;
   }
   __syncthreads();
-  if (tid == 0) {
-    Piece r = {0.0, fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), p.V};
-    for (int w = 3; w >= 0; w--) {
-      if (sums[w] > 0.0)
-        r.sum += sums[w] * weight_of(tops[w], r.top, to2);
-      if (firsts[w] < p.V && tops[w] == r.top)
-        r.first = firsts[w];
+  if (tid < 64) { // lanes 0 to 3: a wave's each
+    const int w = tid & 3;
+    const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), mine = tops[w];
+    double v = sums[w];
+    if (to2 != 0.0)
+      v = v > 0.0 ? v * exp2_64(mine == most ? offs[w] : ((double)mine - (double)most) * to2 + offs[w]) : 0.0;
+    int at = firsts[w] < p.V && mine == most ? firsts[w] : p.V;
+#pragma unroll
+    for (int d = 1; d < 4; d *= 2) {
+      v += __shfl_xor(v, d);
+      at = min(at, __shfl_xor(at, d));
     }
-    p.pieces[((int64_t)side * p.T + row) * p.C + piece] = r;
+    if (tid == 0)
+      p.pieces[((int64_t)side * p.T + row) * p.C + piece] = Piece{v, most, at};
   }
 }
 
@@ -335,24 +373,6 @@ draft_rows_kernel(const DraftsParams p) {
 constexpr int DRAFT_NODES = 256; // nodes of a sequence that are held in LDS; more go through the workspace
 // threads of a workgroup: where there is one for each piece, few enough that all of them run at once
 constexpr int walk_threads(bool token) { return token ? 1024 : 512; }
-
-__device__ __forceinline__ double add64(double a, double z) { return a + z; }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double from_lane(double v) { // (0 where there is no such lane)
-  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, ROWS == 0xf);
-  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, ROWS == 0xf);
-  return __hiloint2double(hi, lo);
-}
-// sum over the lanes below, and this one's; all lanes take part
-__device__ __forceinline__ double scan64(double v) {
-  v += from_lane<0x111, 0xf>(v); // row_shr:1
-  v += from_lane<0x112, 0xf>(v);
-  v += from_lane<0x114, 0xf>(v);
-  v += from_lane<0x118, 0xf>(v);
-  v += from_lane<0x142, 0xa>(v); // row_bcast:15 into the second and the last row
-  v += from_lane<0x143, 0xc>(v); // row_bcast:31 into the upper rows
-  return v;
-}
 
 template <typename E, int NV, bool WALK, bool TOKEN>
 __global__ void __launch_bounds__(walk_threads(TOKEN), 4)
@@ -792,7 +812,7 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
   DraftsParams p;
   memset(&p, 0, sizeof(p));
   p.tokens = (const int64_t*)tokens; p.target = target; p.draft = draft; p.cu = (const int32_t*)cu; p.parents = (const int32_t*)parents;
-  p.uniforms = (const float*)uniforms; p.sample = (const float*)sample; p.temps = (const float*)temperatures; p.temperature = temperature;
+  p.uniforms = (const float*)uniforms; p.sample = (const float*)sample; p.temps = (const float*)temperatures; p.to2 = temperature > 0.f ? LOG2E_64 / (double)temperature : 0.0;
   p.path = (int32_t*)path; p.count = (int32_t*)count; p.next = (int64_t*)next;
   p.t_ld = t_ld; p.d_ld = d_ld; p.T = (int)T; p.B = (int)B; p.V = (int)V; p.sides = draft ? 2 : 1;
   const int nv = draft_vectors(T * p.sides, V, size);
@@ -810,7 +830,7 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
     using E = decltype(e);
     constexpr int NV = decltype(nv_)::value;
     if (T > 0)
-      draft_rows_kernel<E, NV><<<dim3((unsigned)(T * p.C), (unsigned)p.sides), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
+      draft_rows_kernel<E, NV><<<dim3((unsigned)T, (unsigned)p.C, (unsigned)p.sides), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
     if (draft) {
       draft_walk_kernel<E, NV, true, false><<<dim3((unsigned)B, (unsigned)p.C), dim3(walk_threads(false)), 0, (hipStream_t)stream>>>(p);
       draft_walk_kernel<E, NV, false, true><<<dim3((unsigned)B), dim3(walk_threads(true)), 0, (hipStream_t)stream>>>(p);
