@@ -462,14 +462,16 @@ paged_attn_kernel(const PagedAttnParams p) {
       const uint16_t* const at = p.layer + (side ? values : 0) + slot_at(p.g, id, p.Nkv, hk, key, H);
       const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(at), 0, rows * ROW, 0x00020000);
       uint8_t* const dst = lds + (((side ? 0 : TW) + team) * 2 + stage) * SIDE + run * (NJ * 1024);
+      if (rows == 16) {
 #pragma unroll
-      for (int j = 0; j < NJ; j++) { // (rows past the keys repeat the last one)
-        uint32_t off = side ? from[1][j] : from[0][j];
-        if (rows < 16) {
-          const int item = j * 64 + lane, row = item / PER;
-          off -= (uint32_t)(max(row - (rows - 1), 0) * ROW);
+        for (int j = 0; j < NJ; j++)
+          load_to_lds(src, dst + j * 1024, side ? from[1][j] : from[0][j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) { // (rows past the keys repeat the last one)
+          const int row = (j * 64 + lane) / PER;
+          load_to_lds(src, dst + j * 1024, (side ? from[1][j] : from[0][j]) - (uint32_t)(max(row - (rows - 1), 0) * ROW));
         }
-        load_to_lds(src, dst + j * 1024, off);
       }
     }
   };
@@ -532,7 +534,7 @@ paged_attn_kernel(const PagedAttnParams p) {
       request(t - TW, stage ^ 1); // in flight during the arithmetic below
       look_up(t - 2 * TW);
     }
-    bf16x8 pb[CG][NT / 2];
+    f32x4 sc[CG][NT];
     uint64_t seen[CG];
 #pragma unroll
     for (int k = 0; k < CG; k++)
@@ -540,7 +542,6 @@ paged_attn_kernel(const PagedAttnParams p) {
     const bool busy = mine && !idle;
     if (busy) {
       const uint8_t* const st = lds + stage * SIDE;
-      f32x4 sc[CG][NT];
 #pragma unroll
       for (int u = 0; u < NT; u++) {
 #pragma unroll
@@ -596,14 +597,6 @@ paged_attn_kernel(const PagedAttnParams p) {
           l[k] *= alpha;
           m[k] = mx;
         }
-        const float off = -m[k] * unit;
-#pragma unroll
-        for (int i = 0; i < 4 * NT; i += 2) {
-          const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(sc[k][i >> 2][i & 3], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(sc[k][i >> 2][(i & 3) + 1], unit, off))};
-          l[k] = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l[k], false);
-          pb[k][i >> 3][i & 7] = pr[0];
-          pb[k][i >> 3][(i & 7) + 1] = pr[1];
-        }
       }
     }
     if (__builtin_expect(odd, 0)) { // values that are not finite: to the columns that see them, then zeros
@@ -638,17 +631,38 @@ paged_attn_kernel(const PagedAttnParams p) {
         asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     }
     if (busy) {
-      static_for<0, KEYS / 32 * (NA / NR)>([&](auto I) { // 32 keys, NR pieces of channels
-        constexpr int u = decltype(I)::value / (NA / NR), d0 = decltype(I)::value % (NA / NR) * NR;
-        i32x2 vv[NR][2];
-        packed_v_operands<stage * SIDE + u * 32 * ROW + d0 * 32, 16 * ROW>(vv, vaddr);
+      bf16x8 pb[CG][NT / 2];
+      auto weights = [&](int u) { // of 32 keys
 #pragma unroll
-        for (int d = 0; d < NR; d++) {
-          const i32x4 w = {vv[d][0][0], vv[d][0][1], vv[d][1][0], vv[d][1][1]};
+        for (int k = 0; k < CG; k++) {
+          const float off = -m[k] * unit;
 #pragma unroll
-          for (int k = 0; k < CG; k++)
-            acc[k][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pb[k][u], acc[k][d0 + d], 0, 0, 0);
+          for (int i = 0; i < 8; i += 2) {
+            const f32x4 v = sc[k][u * 2 + (i >> 2)];
+            const bf16x2 pr = {(__bf16)__builtin_amdgcn_exp2f(fmaf(v[i & 3], unit, off)), (__bf16)__builtin_amdgcn_exp2f(fmaf(v[(i & 3) + 1], unit, off))};
+            l[k] = __builtin_amdgcn_fdot2_f32_bf16(pr, bf16x2{(__bf16)1.f, (__bf16)1.f}, l[k], false);
+            pb[k][u][i] = pr[0];
+            pb[k][u][i + 1] = pr[1];
+          }
         }
+      };
+      weights(0);
+      static_for<0, KEYS / 32>([&](auto U) {
+        constexpr int u = decltype(U)::value;
+        static_for<0, NA / NR>([&](auto D) { // NR pieces of channels
+          constexpr int d0 = decltype(D)::value * NR;
+          i32x2 vv[NR][2];
+          packed_v_operands<stage * SIDE + u * 32 * ROW + d0 * 32, 16 * ROW>(vv, vaddr);
+          if constexpr (d0 == 0 && u + 1 < KEYS / 32)
+            weights(u + 1); // (the compiler lets them run beside the MFMAs)
+#pragma unroll
+          for (int d = 0; d < NR; d++) {
+            const i32x4 w = {vv[d][0][0], vv[d][0][1], vv[d][1][0], vv[d][1][1]};
+#pragma unroll
+            for (int k = 0; k < CG; k++)
+              acc[k][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pb[k][u], acc[k][d0 + d], 0, 0, 0);
+          }
+        });
       });
     }
   };
