@@ -783,7 +783,7 @@ draft_walk_kernel(const DraftsParams p) {
 static int64_t draft_pieces(int64_t V, int64_t size, int nv) { return (V * size + DRAFT_THREADS * 16 * nv - 1) / (DRAFT_THREADS * 16 * nv); }
 // vectors of 16 bytes that a thread takes of a row
 static int draft_vectors(int64_t rows, int64_t V, int64_t size) {
-  return rows * draft_pieces(V, size, 4) >= 512 ? 4 : 1;
+  return rows * draft_pieces(V, size, 4) >= 128 ? 4 : 1;
 }
 
 } // namespace tppx

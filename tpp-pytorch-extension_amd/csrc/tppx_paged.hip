@@ -450,30 +450,35 @@ paged_attn_kernel(const PagedAttnParams p) {
       const int item = i * 64 + lane, row = item / PER, ch = item % PER;
       from[s][i] = (uint32_t)(row * ROW + (ch ^ (s ? packed_v_turn(NJ, row) : packed_k_turn(NJ, row))) * 16);
     }
-  auto request = [&](int t, int stage) {
-#pragma unroll
-    for (int i = 0; i < MINE; i++) {
-      const int run = (i * CW + wave) % NT, side = (i * CW + wave) / NT;
-      if (CW > RUNS && side > 1)
-        continue;
-      const int key = min(t * KEYS + run * 16, keys - 1), rows = min(keys - key, 16);
-      // (a page that does not exist: the first one)
-      const int id = (unsigned)ids[i] < (unsigned)p.g.pages ? ids[i] : 0;
-      const uint16_t* const at = p.layer + (side ? values : 0) + slot_at(p.g, id, p.Nkv, hk, key, H);
-      const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(at), 0, rows * ROW, 0x00020000);
-      uint8_t* const dst = lds + (((side ? 0 : TW) + team) * 2 + stage) * SIDE + run * (NJ * 1024);
-      if (rows == 16) {
-#pragma unroll
-        for (int j = 0; j < NJ; j++)
-          load_to_lds(src, dst + j * 1024, side ? from[1][j] : from[0][j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) { // (rows past the keys repeat the last one)
-          const int row = (j * 64 + lane) / PER;
-          load_to_lds(src, dst + j * 1024, (side ? from[1][j] : from[0][j]) - (uint32_t)(max(row - (rows - 1), 0) * ROW));
-        }
-      }
-    }
+  auto request = [&](int t, int stage) __attribute__((always_inline)) {
+    const bool whole = (t + 1) * KEYS <= keys; // (rows past the keys repeat the last one)
+    auto runs = [&](auto whole_) __attribute__((always_inline)) {
+      constexpr bool WHOLE = decltype(whole_)::value;
+      static_for<0, MINE>([&](auto I) {
+        constexpr int i = decltype(I)::value;
+        const int run = (i * CW + wave) % NT, side = (i * CW + wave) / NT;
+        if (CW > RUNS && side > 1)
+          return;
+        const int key = WHOLE ? t * KEYS + run * 16 : min(t * KEYS + run * 16, keys - 1), rows = WHOLE ? 16 : min(keys - key, 16);
+        // (a page that does not exist: the first one)
+        const int id = (unsigned)ids[i] < (unsigned)p.g.pages ? ids[i] : 0;
+        const uint16_t* const at = p.layer + (side ? values : 0) + slot_at(p.g, id, p.Nkv, hk, key, H);
+        const auto src = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(at), 0, rows * ROW, 0x00020000);
+        uint8_t* const dst = lds + (((side ? 0 : TW) + team) * 2 + stage) * SIDE + run * (NJ * 1024);
+        static_for<0, NJ>([&](auto J) {
+          constexpr int j = decltype(J)::value;
+          const uint32_t k_off = from[0][j], v_off = from[1][j];
+          uint32_t off = side ? v_off : k_off;
+          if constexpr (!WHOLE)
+            off -= (uint32_t)(max((j * 64 + lane) / PER - (rows - 1), 0) * ROW);
+          load_to_lds(src, dst + j * 1024, off);
+        });
+      });
+    };
+    if (whole)
+      runs(std::true_type{});
+    else
+      runs(std::false_type{});
   };
   uint32_t kaddr[XK], vaddr[XV];
 #pragma unroll
@@ -503,7 +508,7 @@ paged_attn_kernel(const PagedAttnParams p) {
     for (int i = tid; i < o.n; i += TH)
       tree[i] = parent_of(parents, i);
   auto parent = [&](int i) { return small ? tree[i] : parent_of(parents, i); };
-  auto tile = [&](auto S_, int t, int highest) { // highest: the tile of the first team, at the same time
+  auto tile = [&](auto S_, int t, int highest) __attribute__((always_inline)) { // highest: the tile of the first team, at the same time
     constexpr int stage = decltype(S_)::value;
     const int kb = t * KEYS;
     // this tile has landed and the other stage has been read, for this wave and then for every wave that shares them (the wait as a
@@ -632,7 +637,7 @@ paged_attn_kernel(const PagedAttnParams p) {
     }
     if (busy) {
       bf16x8 pb[CG][NT / 2];
-      auto weights = [&](int u) { // of 32 keys
+      auto weights = [&](int u) __attribute__((always_inline)) { // of 32 keys
 #pragma unroll
         for (int k = 0; k < CG; k++) {
           const float off = -m[k] * unit;
@@ -937,7 +942,7 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
       target = 256 * (TW == 1 || stages <= 80 * 1024 ? 2 : 1);
     // no more than the capacity would make: a workgroup without work waits for room on a CU like any other
     const int64_t capacity = p.g.table_ld << p.g.shift, limit = std::min<int64_t>(room, ((int64_t)1 << 31) / (64 * CW * TW));
-    p.least = std::max(env_int("TPPX_PAGED_LEAST", COLS == 16 ? 512 : 256) / KEYS, 1);
+    p.least = std::max(env_int("TPPX_PAGED_LEAST", COLS == 16 && !p.cu ? 512 : 256) / KEYS, 1);
     target = std::min<int64_t>({target, limit, units * ((capacity / KEYS + p.least) / p.least)});
     const bool rounds = TW == 1 && p.B <= 64;
     int64_t most; // (rounds: whole parts are fewer than `target`, and so are the units that are split)
@@ -980,14 +985,16 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
   const int form = env_int("TPPX_PAGED_FORM", 0);
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
-    const int f = form ? form : cols <= 16 ? 1 : cols <= 32 ? 2 : units_of(64) <= 280 && units_of(64) * (p.g.table_ld << p.g.shift) < 800000 ? 3 : 4;
+    const int64_t capacity = p.g.table_ld << p.g.shift;
+    const bool few = cols <= 16 || (NJ <= 4 && units_of(16) * capacity < 400000);
+    const int f = form ? form : few ? 1 : NJ <= 4 && cols <= 32 ? 2 : units_of(64) <= 280 && units_of(64) * capacity < 800000 ? 3 : 4;
     if constexpr (NJ > 4) {
-      if (f == 1 || f == 2)
+      if (f == 1)
         go(nj, n1, n1, n2, k32);
-      else if (f == 3)
-        go(nj, n1, n4, n2, k32);
-      else
+      else if (f == 4)
         go(nj, n1, n4, n1, k32);
+      else
+        go(nj, n1, n4, n2, k32);
     } else {
       if (f == 1)
         go(nj, n1, n1, n4, k32);
