@@ -59,7 +59,8 @@ __device__ __forceinline__ bool sequence_at(const int32_t* cu, int B, int T, int
 
 // ---------------------------------------------------------------------------
 // Norm, rotation and append, as the MXFP4 cache's: a thread keeps its token, the heads go by.  Everything in fp32, one rounding.  A node's
-// position, where none is given, is past + the number of nodes that it continues.
+// position, where none is given, is past + the number of nodes that it continues.  Copy work: 24 trees of 20 to 61 nodes, 64 + 16 heads
+// of 128 (36.7 MB) 10.2 us, 3.6 TB/s; one token 3.1 us, a launch and one way to memory and back.
 // ---------------------------------------------------------------------------
 struct PagedRowsParams {
   const uint16_t *q, *k, *v; // [T][heads][H], rows *_ld elements apart; q may be null
@@ -156,6 +157,14 @@ paged_rows_kernel(const PagedRowsParams p) {
 // tile above ended.
 // A key that a column does not see adds nothing whatever it holds: its score is replaced, and in those tiles values that are infinite
 // or NaN are added one by one to the columns that see them and become zeros in LDS.
+// Scores, maxima, sums and outputs in fp32; rounded to bf16 are the probabilities (the second product's operand; their sum is taken over the
+// rounded ones, so that the weights add up to one) and the result.
+// What bounds it: of single tokens the cache's bytes (48 sequences of up to 9000 keys, 64 heads on 8 of 128: 752 MB in 140 us, 5.4 TB/s,
+// above a large copy's 4.9).  Of long pieces of prompts the clock: 1024 tokens behind 8000 keys 282 us, 1010 TFLOP/s, at 1.8 of 2.4 GHz with
+// the matrix instructions busy in half of the cycles, the others' issue in 0.4 of them, LDS in a quarter (a library product of 8192^3
+// reaches 1560).  Of small steps the way through it: 8 nodes behind 50 keys 7.1 us, 60 behind 5000 (28 heads on 4) 19.5 + 4 for the merge, of
+// which tiles are 7.  Not faster: the scores of the next tile under the weights of this one (registers), 64 columns a wave at one wave
+// per SIMD (282 -> 361 us), s_setprio around the products.
 // ---------------------------------------------------------------------------
 struct PagedAttnParams {
   const uint16_t *q, *layer;
@@ -188,10 +197,14 @@ constexpr int PAGED_NODES = 256;
 
 // The work of a launch, laid out on the device, where the lengths are: an item is a part of a unit's keys, a unit a block of a sequence's
 // columns for one K/V head.  Parts are of about `chunk` tiles: long sequences are split where short ones are not, and in all there are
-// no more than run at once.  Items of a sequence: [split][block][K/V head].
+// no more than run at once, or, where that leaves parts 1.4 times the mean and longer than 2048 keys, some rounds of them (30 single
+// tokens behind up to 9000 keys 105 -> 93 us).  More units than run at once, none longer than 1.2 of the mean share: not split (64 of up
+// to 2000 50 us, split 60).  Items of a sequence: [split][block][K/V head].
 // ROUNDS: as many units as fill whole rounds of what runs at once are not split and come first, then the parts of the others: all that
 // are of `chunk` tiles, of a sequence [split][block][K/V head], then the last ones, of the first keys, [block][K/V head].  If those are
-// short enough a few of them run one after another beside the others.  Blocks go down, the longest first.
+// short enough a few of them run one after another beside the others (700 tokens behind 9000 keys, 352 units where 512 run: 309 us
+// unsplit, 266 so).  Blocks go down, the longest first (8000 tokens without a past 1516 -> 1418 us).
+// A K/V head is an item's last index: its workgroups lie on one XCD where there are eight, and share that one's L2.
 struct Item {
   Block o;           // sequence, its first row and nodes, block
   int hk, S;         // of S parts
@@ -816,7 +829,8 @@ paged_attn_kernel(const PagedAttnParams p) {
   }
 }
 
-// The splits' results of launches with many columns: a thread takes four channels of a column, all splits.
+// The parts' results, where the launch itself does not merge them: a thread takes four channels of a column, all parts.  Bound by their bytes,
+// 8 H fp32 a column and part there and back, and a launch: 4 us for 28 units of nine parts, 7.5 for 248 of two or three (128 columns each).
 template <int NJ, int COLS>
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(const PagedAttnParams p) {
@@ -870,7 +884,8 @@ paged_merge_kernel(const PagedAttnParams p) {
 
 // ---------------------------------------------------------------------------
 // The keys and values of an accepted path to the slots from past on, in all layers.  A thread takes 16 bytes of a head's row through the
-// whole path: node path[i] goes to slot past + i, and as path ascends no row is read after another was written over it.
+// whole path: node path[i] goes to slot past + i, and as path ascends no row is read after another was written over it.  Launch and one way
+// through table, path and rows: one sequence, 4 layers 2.1 us; 12 sequences, 28 layers (5.5 MB) 4.2.
 // ---------------------------------------------------------------------------
 struct PagedKeepParams {
   uint16_t* cache; // [sides][pages][Nkv][page][H], sides = 2 layers
@@ -936,12 +951,15 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     }
     const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ;
     const int64_t room = std::min<int64_t>(std::max<int64_t>(ws_bytes - (int64_t)sizeof(Merge), 0) / (COLS * (32 * NJ + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(Merge)), (((int64_t)1 << 31) - 1) / (COLS * 32 * NJ * 4));
-    // what runs at once: two workgroups on a CU where the LDS has room for them
+    // What runs at once: two workgroups on a CU where the LDS has room for them.  Twice that, and the merge has more to do than it gives: one
+    // token behind 30000 keys 36.4 us, so 30.5; 8 behind up to 8000 22.1 and 17.3.
     int64_t target = env_int("TPPX_PAGED_ITEMS", 0);
     if (target <= 0)
       target = 256 * (TW == 1 || stages <= 80 * 1024 ? 2 : 1);
     // no more than the capacity would make: a workgroup without work waits for room on a CU like any other
     const int64_t capacity = p.g.table_ld << p.g.shift, limit = std::min<int64_t>(room, ((int64_t)1 << 31) / (64 * CW * TW));
+    // Parts of 512 keys at least where the launch merges them (one token behind 400 keys 8.6 us, of 256 10.0; behind 1900 12.3 and 12.0), of
+    // 256 else (8 nodes behind 1000 keys 11.4 us, of 512 13.2).
     p.least = std::max(env_int("TPPX_PAGED_LEAST", COLS == 16 && !p.cu ? 512 : 256) / KEYS, 1);
     target = std::min<int64_t>({target, limit, units * ((capacity / KEYS + p.least) / p.least)});
     const bool rounds = TW == 1 && p.B <= 64;
@@ -952,12 +970,15 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     } else { // (few units: parts of equal lengths come near enough to the same)
       most = std::min<int64_t>({4 * units <= target || capacity < 4096 ? std::max(target, units + p.Nkv) : (units / target + 2) * target, limit, units * ((capacity / KEYS + p.least) / p.least)});
     }
-    // A few pages hold no more than a part would: not worth the look at the lengths and the merge.
+    // A few pages hold no more than a part would: not worth the look at the lengths and the merge (8 nodes behind 300 keys 8.7 us; 440 keys
+    // in parts of 256 11.3, whole 9.8).
     if (target < p.Nkv || (!rounds && most < units + p.Nkv) || capacity <= 384)
       target = most = 0;
     p.target = (int)target;
     p.most = p.parts = (int)most;
     const int64_t items = rounds ? target + units : std::max<int64_t>(most, units);
+    // Merged in the launch, by the part that arrives last (counters), where a unit is a few rows: single tokens (1 behind 1900 keys 12.3 us, by a
+    // second launch 13.3; 8 behind up to 8000 17.2 and 18.3)
     const bool here = COLS == 16 && p.R <= 16 && !p.cu && p.parts * MX4_COUNTER_STRIDE * (int64_t)sizeof(unsigned) <= counter_bytes;
     if (!here)
       p.counters = nullptr;
@@ -982,6 +1003,12 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
   constexpr std::integral_constant<int, 4> n4{};
   constexpr std::integral_constant<int, 32> k32{};
   constexpr std::integral_constant<int, 64> k64{};
+  // Forms (columns of a workgroup; teams).  1 (16; 4): little work altogether, or single tokens: 8 nodes behind 50, 2000, 8000 keys of 64 heads
+  // on 8 7.1, 11.4, 18.4 us (3: 10.5, 15.2, 21.8); 12 x 4 behind 3000 23.8 (2: 22.0); 60 behind 5000 of 28 on 4 over 25.8 (3: 22.3).
+  // 2 (32; 4): 12 x 4 behind 3000 22.0 (1: 23.8, 4: 26.8).  3 (64; 4): few units, as teams share their tiles: 64 behind 8000 36.6 (4: 39.5), 4 x 128 behind
+  // 1000 of 32 on 32 26 (4: 30).  4 (128; 1): an operand read feeds 32 columns and nothing is merged in LDS: 128 behind 8000 53.5
+  // (3: 60), 1024 282 (3: 392).  Heads of 192 and 256 have registers for 16 columns a wave: no form 2 (2 x 20 behind 1500 of 16 on
+  // 16: 3 17.8, 1 22.5).
   const int form = env_int("TPPX_PAGED_FORM", 0);
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
@@ -1045,6 +1072,7 @@ extern "C" int tppx_append_paged(const void* q, const void* k, const void* v, co
   p.T = (int)T; p.B = (int)B; p.Nq = (int)Nq; p.Nkv = (int)Nkv; p.H = (int)H; p.MP = (int)MP; p.HR = emb_pos ? (int)HR : 0;
   const int G = H <= 64 ? 4 : H <= 128 ? 8 : 16;
   const int64_t rows = (q ? Nq : 0) + 2 * Nkv, blocks = (T * G + 255) / 256;
+  // heads over up to 1024 workgroups (24 trees 10.2 us; 256 13.3, 4096 12.3)
   const int64_t per_block = std::max<int64_t>(1, std::min<int64_t>({rows, 65535, 1024 / blocks}));
   const dim3 grid((unsigned)blocks, (unsigned)per_block);
   if (G == 4)
