@@ -764,8 +764,8 @@ int tppx_append_paged(const void* q, const void* k, const void* v,
 /* Attention of nodes over the cache, after their own keys went to it: node i of sequence b sees the slots 0 .. past[b] - 1, its own and
  * those of the nodes that it continues.  softmax(q K^T / sqrt(H)) V, q and out bf16 [T][Nq][H]; a node that sees nothing gets zeros.  A
  * slot without a page within what a node sees makes that sequence's results arbitrary.  ws: 256-byte aligned scratch (no state) and
- * counters (u32 words 256 bytes apart, zero before the first launch, left zero): with enough of both, keys split over workgroups
- * where nodes are few; launches that share either must be ordered. */
+ * counters (u32 words 256 bytes apart, zero before the first launch, left zero; single tokens only): with scratch, keys split over
+ * workgroups where nodes are few, 72 MiB serve any launch; launches that share either must be ordered. */
 int tppx_attn_paged(const void* q, const void* layer, const void* table,
                     const void* past, const void* cu, const void* parents,
                     void* out, int64_t T, int64_t B, int64_t Nq, int64_t Nkv,

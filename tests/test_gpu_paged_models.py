@@ -183,3 +183,11 @@ def test_a_decoder_without_pages_refuses_drafts():
     for call in (lambda: dec.generate_drafted(_prompts([3]), 4), lambda: dec.generate_packed(_prompts([3]), 4)):
         with pytest.raises(F.TppxError):
             call()
+
+
+def test_drafted_tokens_outside_of_the_vocabulary():
+    F, dec = _decoder()
+    for bad in (-1, 1 << 20):
+        with pytest.raises(F.TppxError, match="vocabulary"):
+            dec.generate_drafted(_prompts([5], 6), 4, lambda t: ([3, bad], [-1, 0]))
+    assert dec.generate_drafted(_prompts([5], 6), 4)[0][0].numel() == 4

@@ -1169,7 +1169,10 @@ class LlamaDecoder:
                 drafted, up = list(drafted)[:max(room, 0)], list(up)[:max(room, 0)]
                 tokens.append([t[-1]] + drafted if len(t) < e else [])
                 parents.append([-1] + [u + 1 for u in up] if len(t) < e else [])
-            flat = torch.tensor([x for t in tokens for x in t], dtype=torch.int64, device=self.device)
+            flat = [int(x) for t in tokens for x in t]
+            if min(flat) < 0 or max(flat) >= self.embed.shape[0]:
+                raise TppxError(_lib.EINVAL, f"generate_drafted: drafted tokens outside of the vocabulary of {self.embed.shape[0]}")
+            flat = torch.tensor(flat, dtype=torch.int64, device=self.device)
             bounds = cache.nodes([len(t) for t in tokens], parents, self.device)
             try:
                 h = self.embed.index_select(0, flat).unsqueeze(0)
