@@ -527,6 +527,33 @@ def test_steps_in_a_replayed_graph():
         assert torch.equal(cache, again)
 
 
+def test_drawn_chains_in_a_replayed_graph():
+    at = _at()
+    new, V = [6, 1, 0, 3, 8], 30000
+
+    def inputs(i):
+        tokens, _, target, draft, u, s = _verify_case(new, V, torch.bfloat16, 80 + i, False, True, [1.0] * 5)
+        return [t.cuda() for t in (torch.tensor(tokens), target, draft, u, s, torch.tensor([1.0, 0.7, 1.0, 0.0, 1.2]))]
+
+    def check(a):
+        return at.verify_drafts(a[0], a[1], cu, None, a[2], a[3], a[4], a[5])
+
+    cu, fixed = _i32(_starts(new)), inputs(0)
+    check(fixed)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = check(fixed)
+    for i in (1, 2, 3, 1, 4):
+        a = inputs(i)
+        for to, t in zip(fixed, a):
+            to.copy_(t)
+        graph.replay()
+        want = check(a)
+        torch.cuda.synchronize()
+        assert all(torch.equal(got, w) for got, w in zip(outs, want))
+
+
 def test_two_graphs_replayed_at_once():
     """Steps of drafted tokens keep what they leave for their later launches apart: replays of two graphs need no order."""
     at = _at()

@@ -18,10 +18,10 @@
 
 namespace tppx {
 
-// Two launches, three with draft logits.  The first goes over all logits, in pieces: maximum, its place, and the sum of the weights relative
-// to that maximum.  The second decides for all nodes at once what u M and u q are compared with, walks from node 0 down, and finds the
-// next token: the piece in which the border lies by the pieces' sums less the tried siblings' shares, then the token in it.  With draft
-// logits max(p - q, 0) of the last row is a pass of its own over pieces, the second launch, and the third one finds the token.
+// Two launches.  The first goes over all logits, in pieces: maximum, its place, and the sum of the weights relative to that maximum.  The
+// second decides for all nodes at once what u M and u q are compared with, walks from node 0 down, and finds the next token: the piece in
+// which the border lies by the pieces' sums less the tried siblings' shares, then the token in it.  With draft logits max(p - q, 0) of the
+// last row is summed by a workgroup for each piece, and the one that ends last finds the token.
 struct Piece {
   double sum;
   float top;
@@ -35,7 +35,7 @@ struct NodeShare { // of a node's token in its parent's row
 };
 struct Walk {
   RowSum p, q; // of the last node's row
-  int at, len, tried, pad;
+  int at, len, tried;
 };
 struct DraftsParams {
   const int64_t* tokens;
@@ -46,7 +46,7 @@ struct DraftsParams {
   int64_t* next;
   Piece* pieces;    // [sides][T][C]
   double* sums;     // [B][C] of what is left of a sequence's last row
-  Walk* walks;      // [B]
+  unsigned int* ended; // [B] workgroups that have summed their piece of it, from 0 in the first launch
   RowSum* rows;     // [2][T], of sequences too long for LDS
   NodeShare* nodes; // [T], of those
   int64_t t_ld, d_ld;
@@ -272,6 +272,9 @@ draft_rows_kernel(const DraftsParams p) {
   const double to2 = to2_of(p, b);
   const E* const at = (const E*)(side ? p.draft : p.target) + (int64_t)row * (side ? p.d_ld : p.t_ld);
   const int from = piece * (DRAFT_THREADS * NV * N);
+  if (side == 0 && row == 0 && piece == 0 && p.sides == 2)
+    for (int i = tid; i < p.B; i += DRAFT_THREADS)
+      p.ended[i] = 0;
   int first = p.V;
   double sum = 0.0, off = 0.0;
   float top = -INFINITY;
@@ -369,22 +372,22 @@ draft_rows_kernel(const DraftsParams p) {
 
 // ---------------------------------------------------------------------------
 // The walk and the next token, a workgroup for a sequence: the state of its rows from their pieces, every node's token's p (and q)
-// in its parent's row, then down.  WALK, TOKEN: both without draft logits; with them the walk is done by every workgroup that sums
-// what is left of a piece (blockIdx.y) of the last row, the first of which leaves it to the launch that finds the token.
+// in its parent's row, then down.  DRAFTS: a workgroup for each piece (blockIdx.y) walks down, sums what is left of its piece of the last
+// row, and the one that ends last goes on to the token (nobody waits for another one).
 // What they spend is waiting: row sums, nodes, the way down, the pieces and the token are five trips to memory or LDS one after another.
-// 5 nodes, greedy 3.2 us; 10 trees of up to 60 nodes 12.2; 24 drawn chains 13.3 for the sums and 8.4 for the token.
+// 5 nodes, greedy 3.2 us; 10 trees of up to 60 nodes 12.2; 24 drawn chains 20, of which the token is
+// 7 (with a launch of its own for that 13.3 + 8.5).
 // ---------------------------------------------------------------------------
 constexpr int DRAFT_NODES = 256; // nodes of a sequence that are held in LDS; more go through the workspace
-// threads of a workgroup: where there is one for each piece, few enough that all of them run at once (24 chains' sums of 128000 logits 13.3 us, with 1024
-// 17.4)
-constexpr int walk_threads(bool token) { return token ? 1024 : 512; }
+// threads of a workgroup: where there is one for each piece, few enough that all of them run at once (24 chains' sums of 128000 logits alone
+// 13.3 us, with 1024 threads 17.4)
+constexpr int walk_threads(bool drafts) { return drafts ? 512 : 1024; }
 
-template <typename E, int NV, bool WALK, bool TOKEN>
-__global__ void __launch_bounds__(walk_threads(TOKEN), 4)
+template <typename E, int NV, bool DRAFTS>
+__global__ void __launch_bounds__(walk_threads(DRAFTS), 4)
 draft_walk_kernel(const DraftsParams p) {
-  constexpr int THREADS = walk_threads(TOKEN), N = per16<E>(), PIECE = DRAFT_THREADS * NV * N, WAVES = THREADS / 64;
+  constexpr int THREADS = walk_threads(DRAFTS), N = per16<E>(), PIECE = DRAFT_THREADS * NV * N, WAVES = THREADS / 64;
   constexpr int VECTORS = DRAFT_THREADS * NV, EACH = VECTORS > THREADS ? VECTORS / THREADS : 1; // of a piece, of a thread
-  static_assert(EACH == 1 || !TOKEN);
   __shared__ RowSum rows_lds[2][DRAFT_NODES];
   __shared__ NodeShare nodes_lds[DRAFT_NODES];
   __shared__ double tried_px[DRAFT_NODES]; // the last node's children: shares, pieces that their tokens lie in
@@ -394,21 +397,21 @@ draft_walk_kernel(const DraftsParams p) {
   __shared__ int found_at[WAVES], last_at[WAVES];
   __shared__ double table[256];
   __shared__ Walk walk;
-  __shared__ int piece_at;
+  __shared__ int piece_at, ended_last;
   __shared__ double piece_before, piece_border;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int b = (int)blockIdx.x;
   const int first = p.cu ? min(max(p.cu[b], 0), p.T) : b, n = p.cu ? min(p.cu[b + 1], p.T) - first : 1;
   if (n < 1) {
-    if (TOKEN && tid == 0) {
+    if (blockIdx.y == 0 && tid == 0) {
       p.count[b] = 0;
       p.next[b] = 0;
     }
     return;
   }
   const double to2 = to2_of(p, b);
-  const bool drawn = p.draft && to2 != 0.0;
-  const float sample = TOKEN && to2 != 0.0 ? p.sample[b] : 0.f;
+  const bool drawn = DRAFTS && to2 != 0.0;
+  const float sample = to2 != 0.0 ? p.sample[b] : 0.f;
   if (tid < 256)
     table[tid] = POWERS.v[tid]; // (read behind a barrier)
   const int32_t* const parents = p.parents ? p.parents + first : nullptr;
@@ -416,7 +419,7 @@ draft_walk_kernel(const DraftsParams p) {
   auto parent = [&](int i) { return parents ? parents[i] : i - 1; };
   auto logits = [&](int side, int row) { return (const E*)(side ? p.draft : p.target) + (int64_t)row * (side ? p.d_ld : p.t_ld); };
 
-  if constexpr (WALK) {
+  {
     const bool small = n <= DRAFT_NODES;
     NodeShare* const nodes = small ? nodes_lds : p.nodes + first;
     RowSum* const prows = small ? rows_lds[0] : p.rows + first;
@@ -516,7 +519,7 @@ draft_walk_kernel(const DraftsParams p) {
           const uint64_t bad = __builtin_amdgcn_ballot_w64(fails);
           if (bad)
             end = i0 + __builtin_ctzll(bad);
-          if (TOKEN || blockIdx.y == 0)
+          if (!DRAFTS || blockIdx.y == 0)
             if (i < min(i0 + 64, n))
               p.path[first + i] = i < end ? i : -1;
         }
@@ -528,7 +531,7 @@ draft_walk_kernel(const DraftsParams p) {
             tried_px[0] = nodes[end].px;
             tried_in[0] = nodes[end].token < 0 ? -1 : nodes[end].token / PIECE;
           }
-          if (TOKEN || blockIdx.y == 0)
+          if (!DRAFTS || blockIdx.y == 0)
             for (int i = end / 64 * 64 + 64 + lane; i < n; i += 64)
               p.path[first + i] = -1;
         }
@@ -565,22 +568,16 @@ draft_walk_kernel(const DraftsParams p) {
           p.path[first + i] = -1;
       }
       if (lane == 0)
-        walk = Walk{prows[at], drawn ? qrows[at] : RowSum{1.0, 0.f, 0}, at, len, tried, 0};
+        walk = Walk{prows[at], drawn ? qrows[at] : RowSum{1.0, 0.f, 0}, at, len, tried};
     }
-    __syncthreads();
-    if (!TOKEN && blockIdx.y == 0 && tid == 0)
-      p.walks[b] = walk;
-  } else {
-    if (tid == 0)
-      walk = p.walks[b];
     __syncthreads();
   }
   const int at = walk.at, tried = walk.tried, row = first + at;
-  if (TOKEN && tid == 0)
+  if (blockIdx.y == 0 && tid == 0)
     p.count[b] = walk.len;
   const RowSum ps = walk.p, qs = walk.q;
   if (to2 == 0.0) {
-    if (TOKEN && tid == 0)
+    if (blockIdx.y == 0 && tid == 0)
       p.next[b] = ps.first;
     return;
   }
@@ -662,13 +659,23 @@ draft_walk_kernel(const DraftsParams p) {
     return whole;
   };
   double* const sums = p.sums + (int64_t)b * p.C;
-  if constexpr (!TOKEN) {
-    if (!residual)
+  if constexpr (DRAFTS) {
+    if (residual) {
+      const double s = sum_of_piece((int)blockIdx.y);
+      if (tid == 0) { // (written through to the level that all XCDs share, and there before it counts)
+        __hip_atomic_store(&sums[blockIdx.y], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        ended_last = __hip_atomic_fetch_add(&p.ended[b], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)p.C - 1;
+      }
+      __syncthreads();
+      if (!ended_last)
+        return;
+    } else if (blockIdx.y) {
       return;
-    const double s = sum_of_piece((int)blockIdx.y);
-    if (tid == 0)
-      sums[blockIdx.y] = s;
-  } else {
+    }
+  }
+  auto sum_at = [&](int i) { return DRAFTS ? __hip_atomic_load(&sums[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : sums[i]; };
+  {
     // The pieces' sums: from the first launch less the tried tokens' shares (a difference of sums near 1, so a rest that small is
     // summed anew, as it is where more were tried than are kept), from the second one, or, where nothing is left, p.
     bool all = !tried;
@@ -678,7 +685,7 @@ draft_walk_kernel(const DraftsParams p) {
           if (i >= p.C)
             return 0.0;
           if (!all && (drawn || round > 0))
-            return sums[i];
+            return sum_at(i);
           const Piece z = p.pieces[(int64_t)row * p.C + i];
           double s = z.sum > 0.0 ? z.sum * weight_of(z.top, ps.top, to2) * pn : 0.0;
           if (!all)
@@ -734,10 +741,16 @@ draft_walk_kernel(const DraftsParams p) {
     }
     const int piece = piece_at;
     const double border = piece_border;
-    const Vector own = ask(piece, tid);
+    Vector own[EACH]; // (one after the other in order)
+    double w[EACH][N], s = 0.0;
+#pragma unroll
+    for (int h = 0; h < EACH; h++)
+      own[h] = ask(piece, tid * EACH + h);
     mark(piece);
-    double w[N];
-    const double s = mine(own, piece, tid, all, w), run = scan64(s);
+#pragma unroll
+    for (int h = 0; h < EACH; h++)
+      s += mine(own[h], piece, tid * EACH + h, all, w[h]);
+    const double run = scan64(s);
     if (lane == 63)
       red[wave] = run;
     __syncthreads();
@@ -747,16 +760,18 @@ draft_walk_kernel(const DraftsParams p) {
       before += i < wave ? red[i] : 0.0;
     before += run - s;
     int found = p.V, last = -1;
-    if (tid < VECTORS) {
+    if (tid * EACH < VECTORS) {
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        before += w[e];
-        const int x = piece * PIECE + tid * N + e;
-        if (w[e] > 0.0) {
-          last = x;
-          found = before > border && found == p.V ? x : found;
+      for (int h = 0; h < EACH; h++)
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+          before += w[h][e];
+          const int x = piece * PIECE + (tid * EACH + h) * N + e;
+          if (w[h][e] > 0.0) {
+            last = x;
+            found = before > border && found == p.V ? x : found;
+          }
         }
-      }
     }
     // the first lane and the first wave that found one; a border that is rounded past the piece's last token: that one
     const uint64_t lanes = __builtin_amdgcn_ballot_w64(found < p.V), some = __builtin_amdgcn_ballot_w64(last >= 0);
@@ -829,20 +844,18 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
   TPPX_REQUIRE(aligned16(ws), TPPX_EINVAL, "%s: workspace not 16-byte aligned", who);
   p.pieces = (Piece*)ws;
   p.sums = (double*)(p.pieces + p.sides * T * p.C);
-  p.walks = (Walk*)(p.sums + (B * p.C + 1) / 2 * 2);
-  p.rows = (RowSum*)(p.walks + B);
+  p.ended = (unsigned int*)(p.sums + (B * p.C + 1) / 2 * 2);
+  p.rows = (RowSum*)(p.ended + (B + 3) / 4 * 4);
   p.nodes = (NodeShare*)(p.rows + 2 * T);
   auto go = [&](auto e, auto nv_) {
     using E = decltype(e);
     constexpr int NV = decltype(nv_)::value;
     if (T > 0)
       draft_rows_kernel<E, NV><<<dim3((unsigned)T, (unsigned)p.C, (unsigned)p.sides), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
-    if (draft) {
-      draft_walk_kernel<E, NV, true, false><<<dim3((unsigned)B, (unsigned)p.C), dim3(walk_threads(false)), 0, (hipStream_t)stream>>>(p);
-      draft_walk_kernel<E, NV, false, true><<<dim3((unsigned)B), dim3(walk_threads(true)), 0, (hipStream_t)stream>>>(p);
-    } else {
-      draft_walk_kernel<E, NV, true, true><<<dim3((unsigned)B), dim3(walk_threads(true)), 0, (hipStream_t)stream>>>(p);
-    }
+    if (draft)
+      draft_walk_kernel<E, NV, true><<<dim3((unsigned)B, (unsigned)p.C), dim3(walk_threads(true)), 0, (hipStream_t)stream>>>(p);
+    else
+      draft_walk_kernel<E, NV, false><<<dim3((unsigned)B), dim3(walk_threads(false)), 0, (hipStream_t)stream>>>(p);
   };
   auto typed = [&](auto e) {
     if (nv == 4)
@@ -862,5 +875,5 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
 extern "C" int64_t tppx_verify_drafts_bytes(int64_t T, int64_t B, int64_t V, int drafts) {
   // (of the type with the most pieces, in the form with the most)
   const int64_t C = draft_pieces(V, 4, 1);
-  return (drafts ? 2 : 1) * T * C * (int64_t)sizeof(Piece) + (B * C + 1) / 2 * 16 + B * (int64_t)sizeof(Walk) + T * (int64_t)(2 * sizeof(RowSum) + sizeof(NodeShare)) + 256;
+  return (drafts ? 2 : 1) * T * C * (int64_t)sizeof(Piece) + (B * C + 1) / 2 * 16 + (B + 3) / 4 * 16 + T * (int64_t)(2 * sizeof(RowSum) + sizeof(NodeShare)) + 256;
 }
