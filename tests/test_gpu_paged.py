@@ -133,7 +133,7 @@ def test_attention_of_single_tokens(H, Nq, Nkv, page):
 
 @pytest.mark.parametrize("H,Nq,Nkv", [(64, 12, 4), (96, 10, 2), (128, 8, 8), (128, 16, 2), (192, 3, 1), (256, 4, 2)])
 @pytest.mark.parametrize("page", [16, 32, 256])
-@pytest.mark.parametrize("form", ["", "1", "2", "3", "4"])
+@pytest.mark.parametrize("form", ["", "1", "2", "3", "4", "5", "6"])
 def test_attention_of_trees(H, Nq, Nkv, page, form, monkeypatch):
     if form:  # (one of the kernel's forms instead of the one that the sizes give)
         monkeypatch.setenv("TPPX_PAGED_FORM", form)
@@ -151,7 +151,7 @@ def test_attention_of_pieces_of_prompts(H, Nq, Nkv, new, past, chunk, monkeypatc
 
 
 @pytest.mark.parametrize("B", [65, 150, 400])
-@pytest.mark.parametrize("form", ["", "1", "2", "3", "4"])
+@pytest.mark.parametrize("form", ["", "1", "2", "3", "4", "5", "6"])
 @pytest.mark.parametrize("kind", ["single", "chains", "trees"])
 def test_attention_of_many_sequences(B, form, kind, monkeypatch):
     """More sequences than a wave has lanes, some long enough to be split, some empty, some that take no part."""
@@ -166,7 +166,7 @@ def test_attention_of_many_sequences(B, form, kind, monkeypatch):
     _check_attention(new, past, 16, 4, 2, 64, trees, seed=B)
 
 
-@pytest.mark.parametrize("form", ["1", "2", "3", "4"])
+@pytest.mark.parametrize("form", ["1", "2", "3", "4", "5", "6"])
 @pytest.mark.parametrize("items", ["4", "10", "24", "100"])
 @pytest.mark.parametrize("kind", ["one", "fresh", "trees", "single"])
 def test_attention_in_rounds(form, items, kind, monkeypatch):
@@ -213,7 +213,7 @@ def test_attention_past_the_table():
 
 @pytest.mark.parametrize("H,Nq,Nkv", [(64, 4, 2), (96, 4, 2), (128, 16, 2), (256, 4, 2)])
 @pytest.mark.parametrize("new", [4, 40])
-@pytest.mark.parametrize("form", ["1", "2", "3", "4"])
+@pytest.mark.parametrize("form", ["1", "2", "3", "4", "5", "6"])
 def test_what_a_node_does_not_see_may_be_anything(H, Nq, Nkv, new, form, monkeypatch):
     """Infinities and NaN in the keys and values of nodes that another does not continue, and behind the last one, stay there."""
     at = _at()

@@ -404,7 +404,7 @@ __device__ __forceinline__ bool locate_item(const PagedAttnParams& p, int id, It
 }
 
 template <int NJ, int CG, int CW, int TW, int KEYS>
-__global__ void __launch_bounds__(64 * CW * TW, CG == 1 && CW == 8 ? 4 : CW > 1 ? 2 : 1)
+__global__ void __launch_bounds__(64 * CW * TW, CW > 1 ? 2 : 1)
 paged_attn_kernel(const PagedAttnParams p) {
   constexpr int H = 32 * NJ, ROW = 64 * NJ, PER = 4 * NJ, SIDE = KEYS * ROW, WCOLS = 16 * CG, COLS = WCOLS * CW, TH = 64 * CW * TW, NA = H / 16, NT = KEYS / 16;
   constexpr int XK = NJ % 4 == 0 ? 4 : NJ % 2 == 0 ? 2 : 1, XV = NJ % 4 == 0 ? 8 : NJ % 2 == 0 ? 4 : 2, NR = NJ == 3 ? 6 : XV;
@@ -417,7 +417,7 @@ paged_attn_kernel(const PagedAttnParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6) % CW, team = __builtin_amdgcn_readfirstlane(tid >> 6) / CW;
   const int g = lane >> 4, c = lane & 15;
   Item it;
-  const bool any = locate_item<COLS, KEYS, TW == 1>(p, (int)blockIdx.x, it);
+  const bool any = locate_item<COLS, KEYS, (TW == 1 && CW > 1)>(p, (int)blockIdx.x, it);
   if (p.target > 0 && !p.counters && tid == 0 && blockIdx.x == 0)
     merges_of<COLS, H>(p)->S = it.units;
   if (!any)
@@ -941,6 +941,7 @@ static int paged_checks(const char* who, const void* table, const void* past, co
 static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_bytes, int64_t counter_bytes, hipStream_t stream) {
   hipError_t e = hipSuccess;
   int rc = TPPX_OK;
+  auto at_once = [](size_t lds) { return (int64_t)256 * std::min<int64_t>(160 * 1024 / lds, 8); }; // workgroups of one wave a team
   auto go = [&](auto nj, auto cg, auto cw, auto tw, auto kt) {
     constexpr int NJ = decltype(nj)::value, CG = decltype(cg)::value, CW = decltype(cw)::value, TW = decltype(tw)::value, KEYS = decltype(kt)::value, COLS = 16 * CG * CW;
     const int64_t blocks = p.cu ? ((int64_t)p.T * p.R + (int64_t)p.B * (COLS - 1)) / COLS : (int64_t)p.B * ((p.R + COLS - 1) / COLS);
@@ -951,18 +952,18 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     }
     const size_t stages = 4 * TW * KEYS * 64 * (size_t)NJ;
     const int64_t room = std::min<int64_t>(std::max<int64_t>(ws_bytes - (int64_t)sizeof(Merge), 0) / (COLS * (32 * NJ + 2) * (int64_t)sizeof(float) + (int64_t)sizeof(Merge)), (((int64_t)1 << 31) - 1) / (COLS * 32 * NJ * 4));
-    // What runs at once: two workgroups on a CU where the LDS has room for them.  Twice that, and the merge has more to do than it gives: one
-    // token behind 30000 keys 36.4 us, so 30.5; 8 behind up to 8000 22.1 and 17.3.
+    // What runs at once, by the LDS.  Twice that, and the merge has more to do than it gives: one token behind 30000 keys 36.4 us, so 30.5; 8
+    // behind up to 8000 22.1 and 17.3.
     int64_t target = env_int("TPPX_PAGED_ITEMS", 0);
     if (target <= 0)
-      target = 256 * (TW == 1 || stages <= 80 * 1024 ? 2 : 1);
+      target = CW > 1 ? 256 * (TW == 1 || stages <= 80 * 1024 ? 2 : 1) : at_once(stages);
     // no more than the capacity would make: a workgroup without work waits for room on a CU like any other
     const int64_t capacity = p.g.table_ld << p.g.shift, limit = std::min<int64_t>(room, ((int64_t)1 << 31) / (64 * CW * TW));
     // Parts of 512 keys at least where the launch merges them (one token behind 400 keys 8.6 us, of 256 10.0; behind 1900 12.3 and 12.0), of
     // 256 else (8 nodes behind 1000 keys 11.4 us, of 512 13.2).
     p.least = std::max(env_int("TPPX_PAGED_LEAST", COLS == 16 && !p.cu ? 512 : 256) / KEYS, 1);
     target = std::min<int64_t>({target, limit, units * ((capacity / KEYS + p.least) / p.least)});
-    const bool rounds = TW == 1 && p.B <= 64;
+    const bool rounds = TW == 1 && CW > 1 && p.B <= 64;
     int64_t most; // (rounds: whole parts are fewer than `target`, and so are the units that are split)
     if (rounds) {
       target = std::min(target, room / 2);
@@ -1003,20 +1004,44 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
   constexpr std::integral_constant<int, 4> n4{};
   constexpr std::integral_constant<int, 32> k32{};
   constexpr std::integral_constant<int, 64> k64{};
-  // Forms (columns of a workgroup; teams).  1 (16; 4): little work altogether, or single tokens: 8 nodes behind 50, 2000, 8000 keys of 64 heads
-  // on 8 7.1, 11.4, 18.4 us (3: 10.5, 15.2, 21.8); 12 x 4 behind 3000 23.8 (2: 22.0); 60 behind 5000 of 28 on 4 over 25.8 (3: 22.3).
-  // 2 (32; 4): 12 x 4 behind 3000 22.0 (1: 23.8, 4: 26.8).  3 (64; 4): few units, as teams share their tiles: 64 behind 8000 36.6 (4: 39.5), 4 x 128 behind
-  // 1000 of 32 on 32 26 (4: 30).  4 (128; 1): an operand read feeds 32 columns and nothing is merged in LDS: 128 behind 8000 53.5
-  // (3: 60), 1024 282 (3: 392).  Heads of 192 and 256 have registers for 16 columns a wave: no form 2 (2 x 20 behind 1500 of 16 on
-  // 16: 3 17.8, 1 22.5).
+  // Forms (columns of a workgroup; teams).  2 (32; 4): 12 x 4 nodes behind 3000 keys of 64 heads on 8 22.0 us (1: 23.8, 4: 26.8).  3 (64; 4): few
+  // units, as teams share their tiles: 64 behind 8000 36.6 (4: 39.5), 4 x 128 behind 1000 of 32 on 32 26 (4: 30).  4 (128; 1): an operand
+  // read feeds 32 columns and nothing is merged in LDS: 128 behind 8000 53.5 (3: 60), 1024 282 (3: 392).  Heads of 192 and 256 have
+  // registers for 16 columns a wave: no form 2 (2 x 20 behind 1500 of 16 on 16: 3 17.8, 1 22.5).
+  // 16 columns: single tokens, and little work altogether.  1 (four teams, two at heads of 192 and 256): 8 nodes behind 50, 2000, 8000 keys 7.1, 11.4,
+  // 18.4 (3: 10.5, 15.2, 21.8); 60 behind 5000 of 28 on 4 over 25.8 (3: 22.3).  5 (two), 6 (one): more units than workgroups with more
+  // teams run at once, and short ones: 24 x 3 behind 300 5 10.9 (1: 13.3, 3: 11.4), 18 single tokens without a past of 32 on 32 6 5.8 (5: 9.6, 1: 14),
+  // 3 x 69 without a past 6 9.4 (1: 16, 3: 10.1), 64 single tokens behind 500 5 15.5 (1: 17.9, 6: 18.8), behind 2000 1 49.8 (5: 53.6).
   const int form = env_int("TPPX_PAGED_FORM", 0);
   mx4_for_head(H, [&](auto nj) {
     constexpr int NJ = decltype(nj)::value;
     const int64_t capacity = p.g.table_ld << p.g.shift;
-    const bool few = cols <= 16 || (NJ <= 4 && units_of(16) * capacity < 400000);
-    const int f = form ? form : few ? 1 : NJ <= 4 && cols <= 32 ? 2 : units_of(64) <= 280 && units_of(64) * capacity < 800000 ? 3 : 4;
+    const int64_t u16 = units_of(16);
+    auto room = [&](int teams) { return at_once(teams * 8192 * NJ); };
+    int f = form;
+    if (!f && cols <= 16) {
+      f = 1;
+      if (u16 > room(NJ > 4 ? 2 : 4) && capacity <= 1024) { // rounds of: start and end, tiles (us, as measured)
+        auto cost = [&](int teams) { return (double)((u16 + room(teams) - 1) / room(teams)) * ((teams > 1 ? 5.5 : 4.5) + 0.0034 * NJ * (double)capacity / teams); };
+        const double one = cost(1), two = cost(2), four = NJ > 4 ? two : cost(4);
+        f = one < two && one < four ? 6 : two < four ? 5 : 1;
+      }
+    } else if (!f && NJ <= 4) {
+      if (u16 <= room(4) && u16 * capacity * NJ < 1600000)
+        f = 1;
+      else if (u16 <= room(2) && capacity > 128 && capacity <= 512)
+        f = 5;
+      else if (u16 <= room(1) && capacity <= 128)
+        f = 6;
+      else if (cols <= 32)
+        f = 2;
+    }
+    if (!f)
+      f = units_of(64) <= 280 && units_of(64) * capacity < 800000 ? 3 : 4;
     if constexpr (NJ > 4) {
-      if (f == 1)
+      if (f == 6)
+        go(nj, n1, n1, n1, k32);
+      else if (f == 1 || f == 5)
         go(nj, n1, n1, n2, k32);
       else if (f == 4)
         go(nj, n1, n4, n1, k32);
@@ -1025,6 +1050,10 @@ static int attn_launch(const char* who, PagedAttnParams& p, int H, int64_t ws_by
     } else {
       if (f == 1)
         go(nj, n1, n1, n4, k32);
+      else if (f == 5)
+        go(nj, n1, n1, n2, k32);
+      else if (f == 6)
+        go(nj, n1, n1, n1, k32);
       else if (f == 2)
         go(nj, n2, n1, n4, k32);
       else if (f == 3)
