@@ -783,14 +783,15 @@ int tppx_attn_paged(const void* q, const void* layer, const void* table,
  * logit is -inf; infinite ones share the row; a token outside of 0 .. V - 1 never stands.  Results: path i32 [T] (the numbers of
  * the nodes that stand, node 0 first, then -1), count i32 [B] (how many, node 0 with them), next i64 [B].  A sequence without
  * nodes has count 0 and next 0.  ws: 256-byte aligned scratch of tppx_verify_drafts_bytes(T, B, V, draft != NULL) bytes, no state;
- * launches that share it must be ordered. */
+ * counters (u32 words 256 bytes apart, zero before the first launch, left zero; may be NULL): with one for each sequence small problems
+ * are a single launch, of the same results.  Launches that share either must be ordered. */
 int tppx_verify_drafts(const void* tokens, const void* target, const void* draft,
                        int dtype, const void* cu, const void* parents,
                        const void* uniforms, const void* sample,
                        const void* temperatures, float temperature, void* path,
                        void* count, void* next, int64_t T, int64_t B, int64_t V,
                        int64_t t_ld, int64_t d_ld, void* ws, int64_t ws_bytes,
-                       tppx_stream_t stream);
+                       void* counters, int64_t counter_bytes, tppx_stream_t stream);
 int64_t tppx_verify_drafts_bytes(int64_t T, int64_t B, int64_t V, int drafts);
 
 /* The keys and values of accepted paths to the slots from past[b] on, in all layers of cache [layers][2][pages][Nkv][page][H]: for i <

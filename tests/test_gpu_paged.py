@@ -338,13 +338,27 @@ def _check_verify(new, V, dtype, seed, trees=False, drafts=False, temps=None, as
 
 @pytest.mark.parametrize("V,dtype", [(1, torch.float32), (7, torch.bfloat16), (1000, torch.float16), (4099, torch.bfloat16), (32000, torch.bfloat16),
                                      (50401, torch.float32), (9000, torch.float32), (128000, torch.float16)])
-@pytest.mark.parametrize("kind", ["single", "chain", "drawn", "tree"])
+@pytest.mark.parametrize("kind", ["single", "chain", "drawn", "tree", "small tree"])
 def test_verify(V, dtype, kind):
-    new = {"single": [1, 1, 1, 1], "chain": [5, 0, 1, 9], "drawn": [6, 1, 0, 3, 8], "tree": [20, 1, 0, 66, 7]}[kind]
-    args = dict(trees=kind == "tree", drafts=kind == "drawn")
+    new = {"single": [1, 1, 1, 1], "chain": [5, 0, 1, 9], "drawn": [6, 1, 0, 3, 8], "tree": [20, 1, 0, 66, 7], "small tree": [0, 12, 1, 9, 8]}[kind]
+    args = dict(trees="tree" in kind, drafts=kind == "drawn")
     _check_verify(new, V, dtype, V + len(new), temps=[0.8] * len(new), **args)
     _check_verify(new, V, dtype, V + 1, temps=[0.0, 1.0, 0.7, 1.3, 0.05][:len(new)], as_tensor=True, **args)
     _check_verify(new, V, dtype, V + 2, temps=[0.0] * len(new), **args)
+
+
+def test_verify_of_bounds_that_do_not_ascend():
+    """Sequences that share rows, end before they begin or lie outside: every call ends, and the ones after it are right."""
+    at = _at()
+    V = 4099
+    tokens, parents, target, _, u, s = _verify_case([12, 8], V, torch.bfloat16, 3, True, False, [1.0, 1.0])
+    args = [torch.tensor(tokens, device="cuda"), target.cuda(), _i32([0, 12, 20]), _i32([p for of in parents for p in of]), None, u.cuda(), s.cuda()]
+    want = at.verify_drafts(*args)
+    for cu in ([0, 20, 0], [20, 5, 12], [-7, 30, 9], [12, 0, 20], [0, 2 ** 31 - 1, -2 ** 31], [9, 9, 9], [0, 0, 20], [3, 15, 18]):
+        path, count, following = at.verify_drafts(args[0], args[1], _i32(cu), *args[3:])
+        assert 0 <= int(count.min()) and int(count.max()) <= 20 and 0 <= int(following.min()) and int(following.max()) < V
+        for got, w in zip(at.verify_drafts(*args), want):
+            assert torch.equal(got, w)
 
 
 def test_verify_long_chain_and_wide_tree():

@@ -46,7 +46,7 @@ def test_c_refusals():
 
     def verify(tok=A, target=A, draft=None, dt=1, cu=A, parents=None, u=A, s=A, temps=None, t=1.0, path=A, count=A, nxt=A, T=3, B=2, V=100, t_ld=100,
                d_ld=100, ws=A, wb=1 << 30):
-        return L.tppx_verify_drafts(tok, target, draft, dt, cu, parents, u, s, temps, t, path, count, nxt, T, B, V, t_ld, d_ld, ws, wb, None)
+        return L.tppx_verify_drafts(tok, target, draft, dt, cu, parents, u, s, temps, t, path, count, nxt, T, B, V, t_ld, d_ld, ws, wb, None, 0, None)
 
     for name in ("tok", "target", "path", "count", "nxt", "u", "s"):
         assert verify(**{name: None}) == _lib.EINVAL

@@ -21,7 +21,8 @@ namespace tppx {
 // Two launches.  The first goes over all logits, in pieces: maximum, its place, and the sum of the weights relative to that maximum.  The
 // second decides for all nodes at once what u M and u q are compared with, walks from node 0 down, and finds the next token: the piece in
 // which the border lies by the pieces' sums less the tried siblings' shares, then the token in it.  With draft logits max(p - q, 0) of the
-// last row is summed by a workgroup for each piece, and the one that ends last finds the token.
+// last row is summed by a workgroup for each piece, and the one that ends last finds the token.  Small problems without draft logits are one
+// launch, in which the workgroup that leaves a sequence's last piece goes on with the walk.
 struct Piece {
   double sum;
   float top;
@@ -47,12 +48,14 @@ struct DraftsParams {
   Piece* pieces;    // [sides][T][C]
   double* sums;     // [B][C] of what is left of a sequence's last row
   unsigned int* ended; // [B] workgroups that have summed their piece of it, from 0 in the first launch
+  unsigned int* left;  // pieces that a sequence has, DRAFT_STRIDE apart; 0 between launches.  Null: two launches
   RowSum* rows;     // [2][T], of sequences too long for LDS
   NodeShare* nodes; // [T], of those
   int64_t t_ld, d_ld;
   int T, B, V, C, sides;
   double to2; // of the temperature, where that is a number
 };
+constexpr int DRAFT_STRIDE = 64;
 constexpr double LOG2E_64 = 1.4426950408889634;
 
 // 2^y for y <= 0, 1e-15 relative: 2^f, f in [-1/2, 1/2], by its interpolation at the Chebyshev points of degree 10
@@ -253,28 +256,17 @@ __device__ __forceinline__ double reduce_lanes(double v, F&& f) {
 // 3.6 TB/s, of which 26 are the 531 vector instructions for 32 logits of every thread (12.5 a logit, 8 of those in 64 bits).  At a temperature
 // 0, without sums, 26 us, 4.6 TB/s.
 // ---------------------------------------------------------------------------
+// The piece, in thread 0.
 template <typename E, int NV>
-__global__ void __launch_bounds__(DRAFT_THREADS)
-draft_rows_kernel(const DraftsParams p) {
+__device__ __forceinline__ Piece piece_of_row(const DraftsParams& p, int b, int row, int piece, int side) {
   constexpr int N = per16<E>();
   __shared__ float tops[4];
   __shared__ int firsts[4];
   __shared__ double sums[4], offs[4]; // of a wave, relative to 2^off times the weight of its maximum
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row = (int)blockIdx.x, piece = (int)blockIdx.y, side = (int)blockIdx.z;
-  int b = 0;
-  if (p.temps || side) {
-    b = p.cu ? sequence_of(p.cu, p.B, row) : row;
-    if (side && (!p.cu || b >= p.B || p.cu[b + 1] == row + 1))
-      return; // (nothing was drawn from the last node's)
-    b = min(b, p.B - 1);
-  }
   const double to2 = to2_of(p, b);
   const E* const at = (const E*)(side ? p.draft : p.target) + (int64_t)row * (side ? p.d_ld : p.t_ld);
   const int from = piece * (DRAFT_THREADS * NV * N);
-  if (side == 0 && row == 0 && piece == 0 && p.sides == 2)
-    for (int i = tid; i < p.B; i += DRAFT_THREADS)
-      p.ended[i] = 0;
   int first = p.V;
   double sum = 0.0, off = 0.0;
   float top = -INFINITY;
@@ -353,21 +345,38 @@ draft_rows_kernel(const DraftsParams p) {
     offs[wave] = off;
   }
   __syncthreads();
-  if (tid < 64) { // lanes 0 to 3: a wave's each
-    const int w = tid & 3;
-    const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), mine = tops[w];
-    double v = sums[w];
-    if (to2 != 0.0)
-      v = v > 0.0 ? v * exp2_64(mine == most ? offs[w] : ((double)mine - (double)most) * to2 + offs[w]) : 0.0;
-    int at = firsts[w] < p.V && mine == most ? firsts[w] : p.V;
+  // lanes 0 to 3: a wave's each
+  const int w = tid & 3;
+  const float most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), mine = tops[w];
+  double v = sums[w];
+  if (tid < 64 && to2 != 0.0)
+    v = v > 0.0 ? v * exp2_64(mine == most ? offs[w] : ((double)mine - (double)most) * to2 + offs[w]) : 0.0;
+  int place = firsts[w] < p.V && mine == most ? firsts[w] : p.V;
 #pragma unroll
-    for (int d = 1; d < 4; d *= 2) {
-      v += __shfl_xor(v, d);
-      at = min(at, __shfl_xor(at, d));
-    }
-    if (tid == 0)
-      p.pieces[((int64_t)side * p.T + row) * p.C + piece] = Piece{v, most, at};
+  for (int d = 1; d < 4; d *= 2) {
+    v += __shfl_xor(v, d);
+    place = min(place, __shfl_xor(place, d));
   }
+  return Piece{v, most, place};
+}
+
+template <typename E, int NV>
+__global__ void __launch_bounds__(DRAFT_THREADS)
+draft_rows_kernel(const DraftsParams p) {
+  const int tid = threadIdx.x, row = (int)blockIdx.x, piece = (int)blockIdx.y, side = (int)blockIdx.z;
+  int b = 0;
+  if (p.temps || side) {
+    b = p.cu ? sequence_of(p.cu, p.B, row) : row;
+    if (side && (!p.cu || b >= p.B || p.cu[b + 1] == row + 1))
+      return; // (nothing was drawn from the last node's)
+    b = min(b, p.B - 1);
+  }
+  if (side == 0 && row == 0 && piece == 0 && p.sides == 2)
+    for (int i = tid; i < p.B; i += DRAFT_THREADS)
+      p.ended[i] = 0;
+  const Piece r = piece_of_row<E, NV>(p, b, row, piece, side);
+  if (tid == 0)
+    p.pieces[((int64_t)side * p.T + row) * p.C + piece] = r;
 }
 
 // ---------------------------------------------------------------------------
@@ -383,10 +392,23 @@ constexpr int DRAFT_NODES = 256; // nodes of a sequence that are held in LDS; mo
 // 13.3 us, with 1024 threads 17.4)
 constexpr int walk_threads(bool drafts) { return drafts ? 512 : 1024; }
 
-template <typename E, int NV, bool DRAFTS>
-__global__ void __launch_bounds__(walk_threads(DRAFTS), 4)
-draft_walk_kernel(const DraftsParams p) {
-  constexpr int THREADS = walk_threads(DRAFTS), N = per16<E>(), PIECE = DRAFT_THREADS * NV * N, WAVES = THREADS / 64;
+template <bool SHARED>
+__device__ __forceinline__ Piece load_piece(const Piece* at) {
+  if constexpr (!SHARED)
+    return *at;
+  const uint64_t* const w = reinterpret_cast<const uint64_t*>(at);
+  const uint64_t s = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), z = __hip_atomic_load(w + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return Piece{__builtin_bit_cast(double, s), __uint_as_float((uint32_t)z), (int)(z >> 32)};
+}
+// first row and nodes of a sequence (fewer than 1: none)
+__device__ __forceinline__ void bounds_of(const DraftsParams& p, int b, int& first, int& n) {
+  first = p.cu ? min(max(p.cu[b], 0), p.T) : b;
+  n = p.cu ? min(p.cu[b + 1], p.T) - first : 1;
+}
+// SHARED: pieces of the same launch, from the level that all XCDs share
+template <typename E, int NV, bool DRAFTS, int THREADS, bool SHARED>
+__device__ __forceinline__ void walk_sequence(const DraftsParams& p, int b) {
+  constexpr int N = per16<E>(), PIECE = DRAFT_THREADS * NV * N, WAVES = THREADS / 64;
   constexpr int VECTORS = DRAFT_THREADS * NV, EACH = VECTORS > THREADS ? VECTORS / THREADS : 1; // of a piece, of a thread
   __shared__ RowSum rows_lds[2][DRAFT_NODES];
   __shared__ NodeShare nodes_lds[DRAFT_NODES];
@@ -400,10 +422,11 @@ draft_walk_kernel(const DraftsParams p) {
   __shared__ int piece_at, ended_last;
   __shared__ double piece_before, piece_border;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = (int)blockIdx.x;
-  const int first = p.cu ? min(max(p.cu[b], 0), p.T) : b, n = p.cu ? min(p.cu[b + 1], p.T) - first : 1;
+  const bool lead = !DRAFTS || blockIdx.y == 0;
+  int first, n;
+  bounds_of(p, b, first, n);
   if (n < 1) {
-    if (blockIdx.y == 0 && tid == 0) {
+    if (lead && tid == 0) {
       p.count[b] = 0;
       p.next[b] = 0;
     }
@@ -443,7 +466,7 @@ draft_walk_kernel(const DraftsParams p) {
     auto pieces_of = [&](int i) { return p.pieces + ((int64_t)(i >= n) * p.T + first + (i >= n ? i - n : i)) * p.C; };
     Piece ahead = {0.0, -INFINITY, p.V};
     if (tid / 16 < sides * n && u < p.C)
-      ahead = pieces_of(tid / 16)[u];
+      ahead = load_piece<SHARED>(pieces_of(tid / 16) + u);
     NodeShare z0;
     float x0, y0;
     if (tid < n)
@@ -453,12 +476,13 @@ draft_walk_kernel(const DraftsParams p) {
       const int side = i >= n, r = i - side * n;
       const Piece* const at = pieces_of(i);
       if (i != tid / 16)
-        ahead = u < p.C ? at[u] : Piece{0.0, -INFINITY, p.V};
+        ahead = u < p.C ? load_piece<SHARED>(at + u) : Piece{0.0, -INFINITY, p.V};
       float top = ahead.top;
       int place = ahead.first;
       for (int c = u + 16; c < p.C; c += 16) {
-        const float t = at[c].top;
-        const int f = at[c].first;
+        const Piece z = load_piece<SHARED>(at + c);
+        const float t = z.top;
+        const int f = z.first;
         place = t > top ? f : t == top ? min(place, f) : place;
         top = fmaxf(top, t);
       }
@@ -473,7 +497,7 @@ draft_walk_kernel(const DraftsParams p) {
       if (to2 != 0.0) {
         sum = ahead.sum > 0.0 ? ahead.sum * weight_of(ahead.top, top, to2) : 0.0;
         for (int c = u + 16; c < p.C; c += 16) {
-          const Piece z = at[c];
+          const Piece z = load_piece<SHARED>(at + c);
           sum += z.sum > 0.0 ? z.sum * weight_of(z.top, top, to2) : 0.0;
         }
       }
@@ -519,7 +543,7 @@ draft_walk_kernel(const DraftsParams p) {
           const uint64_t bad = __builtin_amdgcn_ballot_w64(fails);
           if (bad)
             end = i0 + __builtin_ctzll(bad);
-          if (!DRAFTS || blockIdx.y == 0)
+          if (lead)
             if (i < min(i0 + 64, n))
               p.path[first + i] = i < end ? i : -1;
         }
@@ -531,7 +555,7 @@ draft_walk_kernel(const DraftsParams p) {
             tried_px[0] = nodes[end].px;
             tried_in[0] = nodes[end].token < 0 ? -1 : nodes[end].token / PIECE;
           }
-          if (!DRAFTS || blockIdx.y == 0)
+          if (lead)
             for (int i = end / 64 * 64 + 64 + lane; i < n; i += 64)
               p.path[first + i] = -1;
         }
@@ -573,11 +597,11 @@ draft_walk_kernel(const DraftsParams p) {
     __syncthreads();
   }
   const int at = walk.at, tried = walk.tried, row = first + at;
-  if (blockIdx.y == 0 && tid == 0)
+  if (lead && tid == 0)
     p.count[b] = walk.len;
   const RowSum ps = walk.p, qs = walk.q;
   if (to2 == 0.0) {
-    if (blockIdx.y == 0 && tid == 0)
+    if (lead && tid == 0)
       p.next[b] = ps.first;
     return;
   }
@@ -686,7 +710,7 @@ draft_walk_kernel(const DraftsParams p) {
             return 0.0;
           if (!all && (drawn || round > 0))
             return sum_at(i);
-          const Piece z = p.pieces[(int64_t)row * p.C + i];
+          const Piece z = load_piece<SHARED>(p.pieces + (int64_t)row * p.C + i);
           double s = z.sum > 0.0 ? z.sum * weight_of(z.top, ps.top, to2) * pn : 0.0;
           if (!all)
 #pragma unroll 8
@@ -800,6 +824,52 @@ draft_walk_kernel(const DraftsParams p) {
   }
 }
 
+template <typename E, int NV, bool DRAFTS>
+__global__ void __launch_bounds__(walk_threads(DRAFTS), 4)
+draft_walk_kernel(const DraftsParams p) {
+  walk_sequence<E, NV, DRAFTS, walk_threads(DRAFTS), false>(p, (int)blockIdx.x);
+}
+
+// Both in one launch, for up to 64 sequences: a piece counts for each sequence that has its row (so that every count is full in the end,
+// whatever the bounds hold), and the workgroup that completes one goes on with it; nobody waits.
+template <typename E>
+__global__ void __launch_bounds__(DRAFT_THREADS)
+draft_small_kernel(const DraftsParams p) {
+  __shared__ uint64_t complete;
+  const int tid = threadIdx.x, row = (int)blockIdx.x, piece = (int)blockIdx.y;
+  int first = 0, n = 0;
+  const bool some = (tid & 63) < p.B;
+  if (some)
+    bounds_of(p, tid & 63, first, n);
+  const uint64_t mine = __builtin_amdgcn_ballot_w64(some && row >= first && row < first + n);
+  const Piece r = piece_of_row<E, 1>(p, mine ? __builtin_ctzll(mine) : 0, row, piece, 0);
+  if (tid < 64) {
+    if (row == 0 && piece == 0 && some && n < 1) {
+      p.count[tid] = 0;
+      p.next[tid] = 0;
+    }
+    if (tid == 0) { // (there before it counts)
+      uint64_t* const to = reinterpret_cast<uint64_t*>(p.pieces + (int64_t)row * p.C + piece);
+      __hip_atomic_store(to, __builtin_bit_cast(uint64_t, r.sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(to + 1, (uint64_t)__float_as_uint(r.top) | (uint64_t)(uint32_t)r.first << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    bool last = false;
+    if (mine >> tid & 1) {
+      const unsigned most = (unsigned)(n * p.C) - 1;
+      last = atomicInc(p.left + tid * DRAFT_STRIDE, most) == most;
+    }
+    const uint64_t done = __builtin_amdgcn_ballot_w64(last);
+    if (tid == 0)
+      complete = done;
+  }
+  __syncthreads();
+  for (uint64_t todo = complete; todo; todo &= todo - 1) {
+    walk_sequence<E, 1, false, DRAFT_THREADS, true>(p, __builtin_ctzll(todo));
+    __syncthreads();
+  }
+}
+
 static int64_t draft_pieces(int64_t V, int64_t size, int nv) { return (V * size + DRAFT_THREADS * 16 * nv - 1) / (DRAFT_THREADS * 16 * nv); }
 // Vectors of 16 bytes that a thread takes of a row: four, which halves the instructions around the sums, or one where that leaves most of the
 // CUs idle (5 rows of 32000 3.0 us, with four 4.0; 24 rows of 152000 7.1 + 10.6 for the walk, with four 5.3 + 9.6).
@@ -814,7 +884,7 @@ using namespace tppx;
 extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const void* draft, int dtype, const void* cu, const void* parents,
                                   const void* uniforms, const void* sample, const void* temperatures, float temperature, void* path,
                                   void* count, void* next, int64_t T, int64_t B, int64_t V, int64_t t_ld, int64_t d_ld, void* ws,
-                                  int64_t ws_bytes, tppx_stream_t stream) {
+                                  int64_t ws_bytes, void* counters, int64_t counter_bytes, tppx_stream_t stream) {
   const char* who = "tppx_verify_drafts";
   TPPX_REQUIRE(tokens && target && path && count && next, TPPX_EINVAL, "%s: null pointer", who);
   TPPX_REQUIRE(dtype == TPPX_DT_F32 || dtype == TPPX_DT_BF16 || dtype == TPPX_DT_F16, TPPX_EINVAL, "%s: dtype %d", who, dtype);
@@ -829,7 +899,8 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
                "%s: bad shape T=%ld B=%ld V=%ld", who, (long)T, (long)B, (long)V);
   TPPX_REQUIRE(t_ld >= V && (!draft || d_ld >= V), TPPX_ESHAPE, "%s: row strides must hold a row", who);
   TPPX_REQUIRE(cu || T == B, TPPX_ESHAPE, "%s: %ld tokens of %ld sequences need their bounds", who, (long)T, (long)B);
-  TPPX_REQUIRE(ws_bytes >= 0 && (ws_bytes == 0 || ws), TPPX_EINVAL, "%s: size given with a null pointer", who);
+  TPPX_REQUIRE(ws_bytes >= 0 && (ws_bytes == 0 || ws) && counter_bytes >= 0 && (counter_bytes == 0 || counters), TPPX_EINVAL, "%s: size given with a null pointer", who);
+  TPPX_REQUIRE(((uintptr_t)counters & 3u) == 0, TPPX_EINVAL, "%s: counters not 4-byte aligned", who);
   DraftsParams p;
   memset(&p, 0, sizeof(p));
   p.tokens = (const int64_t*)tokens; p.target = target; p.draft = draft; p.cu = (const int32_t*)cu; p.parents = (const int32_t*)parents;
@@ -847,9 +918,16 @@ extern "C" int tppx_verify_drafts(const void* tokens, const void* target, const 
   p.ended = (unsigned int*)(p.sums + (B * p.C + 1) / 2 * 2);
   p.rows = (RowSum*)(p.ended + (B + 3) / 4 * 4);
   p.nodes = (NodeShare*)(p.rows + 2 * T);
+  // One launch: few rows, whose pieces 16 lanes look over in a few trips (5 rows of 32000 greedy 7.0 us, two launches 3.2 + 3.2, and with the
+  // call from a program 13.3 and 15.6).
+  p.left = nv == 1 && !draft && T > 0 && T <= 32 && B <= 64 && p.C <= 32 && B * DRAFT_STRIDE * 4 <= counter_bytes ? (unsigned int*)counters : nullptr;
   auto go = [&](auto e, auto nv_) {
     using E = decltype(e);
     constexpr int NV = decltype(nv_)::value;
+    if (p.left) {
+      draft_small_kernel<E><<<dim3((unsigned)T, (unsigned)p.C), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
+      return;
+    }
     if (T > 0)
       draft_rows_kernel<E, NV><<<dim3((unsigned)T, (unsigned)p.C, (unsigned)p.sides), dim3(DRAFT_THREADS), 0, (hipStream_t)stream>>>(p);
     if (draft)

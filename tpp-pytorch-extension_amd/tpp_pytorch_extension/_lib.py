@@ -126,7 +126,7 @@ SIGNATURES = {
     "tppx_attn_packed": [_vp] * 5 + [_i64, _vp] + [_i64] * 8 + [_vp],
     "tppx_append_paged": [_vp] * 5 + [_i32, _f32, _vp, _i32] + [_vp] * 7 + [_i64] * 13 + [_vp],
     "tppx_attn_paged": [_vp] * 7 + [_i64] * 9 + [_vp, _i64, _vp, _i64, _vp],
-    "tppx_verify_drafts": [_vp] * 3 + [_i32] + [_vp] * 5 + [_f32] + [_vp] * 3 + [_i64] * 5 + [_vp, _i64, _vp],
+    "tppx_verify_drafts": [_vp] * 3 + [_i32] + [_vp] * 5 + [_f32] + [_vp] * 3 + [_i64] * 5 + [_vp, _i64, _vp, _i64, _vp],
     "tppx_verify_drafts_bytes": [_i64, _i64, _i64, _i32],
     "tppx_keep_paged": [_vp] * 6 + [_i64] * 8 + [_vp],
     "tppx_plan_linear_mxfp4": [_i64, _i64, _i64, _i32, _i64, ctypes.c_char_p, _i64],

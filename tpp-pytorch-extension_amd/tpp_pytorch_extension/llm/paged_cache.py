@@ -147,9 +147,15 @@ def verify_drafts(tokens, target, cu_seqlens=None, parents=None, draft=None, uni
     count = tokens.new_empty(B, dtype=I32)
     following = tokens.new_empty(B)
     need = _lib.lib().tppx_verify_drafts_bytes(T, B, V, draft is not None)
-    ws = torch.empty(need, dtype=torch.uint8, device=tokens.device) if need > _lib.WORKSPACE_BYTES else _lib.workspace(target, own=True)
+    if need > _lib.WORKSPACE_BYTES:
+        ws = torch.empty(need, dtype=torch.uint8, device=tokens.device)
+        scratch = ws.data_ptr(), need, None, 0
+    else:
+        ws = _lib.workspace(target, own=True)
+        # (a capture's own scratch has no counters, which replays of two graphs would share)
+        scratch = (ws.data_ptr(), _lib.WORKSPACE_BYTES, None, 0) if torch._C._cuda_isCurrentStreamCapturing() else _lib.with_counters(ws)
     _run(dev, _lib.lib().tppx_verify_drafts, tok, t_at, d_at, code, cu, up, u_at, s_at, temps, number, path.data_ptr(), count.data_ptr(),
-         following.data_ptr(), T, B, V, t_ld, d_ld, ws.data_ptr(), max(need, _lib.WORKSPACE_BYTES))
+         following.data_ptr(), T, B, V, t_ld, d_ld, *scratch)
     return path, count, following
 
 
