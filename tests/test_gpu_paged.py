@@ -483,6 +483,10 @@ def test_keep_of_bad_paths():
     assert torch.equal(cache[:, 2:], before[:, 2:])
     at.keep_paged(cache, table, _i32([2 ** 31 - 1, -2 ** 31]), _i32([0, 2, 1, 0, 2, 1]), _i32([3, 3]), _i32([0, 3, 6]))
     assert torch.equal(cache[:, 2:], before[:, 2:])
+    now = cache.clone()
+    for cu in ([6, 3, 0], [2 ** 31 - 1, -2 ** 31, 3], [-2 ** 31, -1, -2 ** 31], [7, 2 ** 31 - 1, 7]):
+        at.keep_paged(cache, table, _i32([2, 2]), _i32([0, 2, 3, 0, 2, 3]), _i32([3, 3]), _i32(cu))
+    assert torch.equal(cache[:, 2:], now[:, 2:])
 
 
 # -- together ---------------------------------------------------------------------------------------------------------

@@ -403,7 +403,7 @@ __device__ __forceinline__ Piece load_piece(const Piece* at) {
 // first row and nodes of a sequence (fewer than 1: none)
 __device__ __forceinline__ void bounds_of(const DraftsParams& p, int b, int& first, int& n) {
   first = p.cu ? min(max(p.cu[b], 0), p.T) : b;
-  n = p.cu ? min(p.cu[b + 1], p.T) - first : 1;
+  n = p.cu ? min(max(p.cu[b + 1], 0), p.T) - first : 1;
 }
 // SHARED: pieces of the same launch, from the level that all XCDs share
 template <typename E, int NV, bool DRAFTS, int THREADS, bool SHARED>

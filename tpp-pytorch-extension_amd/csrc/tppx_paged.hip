@@ -901,7 +901,7 @@ paged_keep_kernel(const PagedKeepParams p) {
   if (item >= (int64_t)items * p.sides)
     return;
   const int side = (int)(item / items), in = (int)(item % items), head = in / per, ch = in % per;
-  const int first = p.cu ? p.cu[b] : b, n = p.cu ? min(p.cu[b + 1], p.T) - first : 1;
+  const int first = p.cu ? p.cu[b] : b, n = p.cu ? min(max(p.cu[b + 1], 0), p.T) - max(first, 0) : 1;
   const int past = p.past[b];
   if (first < 0 || n < 1 || past < 0 || past > (1 << 30))
     return;
