@@ -45,13 +45,13 @@ def test_c_refusals():
     assert attn(T=0) == _lib.OK
 
     def verify(tok=A, target=A, draft=None, dt=1, cu=A, parents=None, u=A, s=A, temps=None, t=1.0, path=A, count=A, nxt=A, T=3, B=2, V=100, t_ld=100,
-               d_ld=100, ws=A, wb=1 << 30):
-        return L.tppx_verify_drafts(tok, target, draft, dt, cu, parents, u, s, temps, t, path, count, nxt, T, B, V, t_ld, d_ld, ws, wb, None, 0, None)
+               d_ld=100, ws=A, wb=1 << 30, ct=None, cb=0):
+        return L.tppx_verify_drafts(tok, target, draft, dt, cu, parents, u, s, temps, t, path, count, nxt, T, B, V, t_ld, d_ld, ws, wb, ct, cb, None)
 
     for name in ("tok", "target", "path", "count", "nxt", "u", "s"):
         assert verify(**{name: None}) == _lib.EINVAL
     assert verify(dt=3) == verify(tok=A + 4) == verify(target=A + 1) == verify(u=A + 2) == verify(cu=A + 2) == verify(nxt=A + 4) == _lib.EINVAL
-    assert verify(t=-1.0) == verify(t=float("nan")) == verify(t=float("inf")) == verify(temps=A, u=None) == verify(ws=None) == _lib.EINVAL
+    assert verify(t=-1.0) == verify(t=float("nan")) == verify(t=float("inf")) == verify(temps=A, u=None) == verify(ws=None) == verify(cb=64) == verify(ct=A + 2, cb=64) == _lib.EINVAL
     assert verify(draft=A, parents=A) == _lib.EUNSUPPORTED
     assert verify(V=0) == verify(B=0) == verify(T=-1) == verify(cu=None) == verify(t_ld=99) == verify(draft=A, d_ld=99) == _lib.ESHAPE
 
